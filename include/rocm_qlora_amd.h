@@ -530,6 +530,100 @@ int rq_adamw_step(const rq_adamw_tensor* tensors, int64_t n_tensors, void* devic
                   int64_t device_table_bytes, int64_t chunk_begin, int64_t chunk_end,
                   float* exp_avg, float* exp_avg_sq, hipStream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Adapters of many requests beside a shared projection
+ * (no counterpart in the reference)
+ * ------------------------------------------------------------------------ */
+
+/* Groups the M rows of a batch by adapter: ids[m] in 0 .. n - 1, anything else
+ * for a row without one.  plan: 16-byte aligned device memory of
+ * rq_adapter_rows_size bytes, read by the entry points below for as many
+ * projections as the batch passes through.  n <= 1024, M <= 2^30. */
+int rq_adapter_rows_size(int64_t M, int64_t n, int64_t* bytes);
+int rq_adapter_rows(const int32_t* ids, int64_t M, int64_t n, void* plan, int64_t plan_bytes, hipStream_t stream);
+
+/* Row slots of a grouped batch (grouped = 0: of rows that all belong to adapter 0,
+ * whose plan is NULL): the rank-wide sums u below are [slots][rank rounded up to
+ * 16] fp32. */
+int rq_multi_lora_slots(int64_t M, int64_t n, int grouped, int64_t* slots);
+
+/* Scratch memory of one call (256-byte aligned, contents ignored). */
+int rq_multi_lora_scratch_size(int dtype, int64_t M, int64_t K, int64_t N, int64_t n, int64_t rank, int grouped,
+                               int backward, int64_t* bytes);
+
+/* out[m] = base[m] + scaling[a] (x[m] A[a]^T) B[a]^T with a the adapter of row m
+ * (rows without one: base[m]).
+ *   x [M, K] stride ldx, lora_a [n, rank, K], lora_b [n, N, rank], base [M, N]
+ *   stride ld_base or NULL (zeros), out [M, N] stride ld_out (may be base), all of
+ *   `dtype`; scaling [n] fp32; plan: rq_adapter_rows' of the same M and n, or NULL
+ *   with n = 1: every row adapter 0's.  u: NULL, or the sums x A^T for the backward
+ *   pass.  Sums are fp32, x A^T is passed on in 16 bits or more, the result is
+ *   rounded once.  rank <= 512, any sizes, strides and element alignment. */
+int rq_multi_lora(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* plan, int64_t plan_bytes,
+                  const void* lora_a, const void* lora_b, const float* scaling, int64_t n, int64_t rank, int64_t N,
+                  const void* base, int64_t ld_base, void* out, int64_t ld_out, float* u, void* scratch,
+                  int64_t scratch_bytes, hipStream_t stream);
+
+/* Its gradients, with g[m] = scaling[a] dY[m] B[a]:
+ *   dx[m] = dx_base[m] + g[m] A[a],  dA[a] = sum g[m]^T x[m],
+ *   dB[a] = sum scaling[a] dY[m]^T u[m]  (sums over the rows of adapter a, in fp32 and
+ *   in an order that the plan alone sets; zeros for an adapter without rows).
+ * x: rows of `dtype`, or with x_exponents != NULL rq_act8_quantize's codes, ldx
+ * their pitch (K rounded up to 32), 16-byte aligned.  dx_base: NULL (zeros) or
+ * [M, K], may be dx.  dx, da, db: each may be NULL.  M >= 1. */
+int rq_multi_lora_grads(const void* x, const uint8_t* x_exponents, int dtype, int64_t M, int64_t K, int64_t ldx,
+                        const void* dy, int64_t N, int64_t lddy, const void* plan, int64_t plan_bytes,
+                        const void* lora_a, const void* lora_b, const float* scaling, int64_t n, int64_t rank,
+                        const float* u, const void* dx_base, int64_t ld_dx_base, void* dx, int64_t lddx, void* da,
+                        void* db, void* scratch, int64_t scratch_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Activation checkpoints in 8 bits (no counterpart in the reference)
+ * ------------------------------------------------------------------------ */
+
+/* Blocks of 32 values along a row share a power-of-two scale (the OCP MX format
+ * MXINT8): with E = floor(log2 max |x|) of the block, q = clamp(rne(x 2^(6-E)),
+ * -127, 127) and the value q 2^(E-6).  codes: [rows][pitch] bytes, pitch = cols
+ * rounded up to 32, 16-byte aligned (zeros past cols); exponents: [rows][pitch / 32]
+ * bytes E + 127; 255 for a block with an infinity or a NaN, which stands for NaN. */
+int rq_act8_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* codes,
+                     uint8_t* exponents, hipStream_t stream);
+int rq_act8_dequantize(const uint8_t* codes, const uint8_t* exponents, int64_t rows, int64_t cols, void* out,
+                       int out_dtype, int64_t ldo, hipStream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Preference loss (no counterpart in the reference)
+ * ------------------------------------------------------------------------ */
+
+/* Log-probabilities of S labelled sequences and, with loss != NULL, the
+ * preference loss on the pairs (p, S/2 + p) of them.
+ *   logits: T rows of V values of `dtype`; row t at t * ld, or with period > 0 at
+ *   (t / period) * outer + (t % period) * ld.  labels [T]: row t predicts labels[t + 1]
+ *   when that is a row of its sequence and not ignore_index; a label outside 0 ..
+ *   V - 1 makes its row NaN.  offsets [S + 1] ascending (sequence i is rows
+ *   offsets[i] .. offsets[i + 1] - 1), or NULL: sequences of T / S rows.
+ *   logps[i] = sum of log softmax(logits[t])[label] over the labelled rows of i
+ *   (average: over their number; 0 without any).
+ *   D_p = beta ((logps[p] - ref[p]) - (logps[q] - ref[q])), q = S/2 + p, ref_logps [S]
+ *   or NULL (zeros); loss = mean over p of -(1 - e) log sigmoid(D_p) - e log sigmoid(-D_p),
+ *   e = label_smoothing.
+ * coef [S]: d loss / d (sum of sequence i) (without loss: d logps[i] / d sum).
+ * row_info: 16 bytes a row, 16-byte aligned, for the backward pass.  workspace:
+ * 256-byte aligned, contents ignored.  T >= 1. */
+int rq_preference_workspace_size(int dtype, int64_t T, int64_t V, int64_t S, int64_t* bytes);
+int rq_preference_forward(const void* logits, int dtype, int64_t T, int64_t V, int64_t ld, int64_t period,
+                          int64_t outer, const int64_t* labels, const int32_t* offsets, int64_t S,
+                          int64_t ignore_index, const float* ref_logps, float beta, float label_smoothing,
+                          int average, float* logps, float* loss, float* coef, void* row_info,
+                          void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* dlogits[t] = c ([v = label] - softmax(logits[t])) with c = coef[i] * grad[0], or
+ * coef[i] * grad[i] with grad_per_sequence (grad NULL: 1); zeros for rows without a
+ * label.  [T, V] of `dtype`, row stride lddz. */
+int rq_preference_backward(const void* logits, int dtype, int64_t T, int64_t V, int64_t ld, int64_t period,
+                           int64_t outer, const void* row_info, const float* coef, const float* grad,
+                           int grad_per_sequence, void* dlogits, int64_t lddz, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

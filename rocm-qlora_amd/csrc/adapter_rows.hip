@@ -1,0 +1,151 @@
+// Grouping a batch's rows by adapter (rq_rows.h): a counting sort in one
+// workgroup, stable and without an atomic whose order shows.  Each of eight waves
+// counts its own stretch of the rows, the counts are summed over waves and
+// adapters, and each wave then places its stretch 64 rows at a time, rows of the
+// same adapter ranked by a ballot.  Bound by latency: it runs once for a batch,
+// for all the projections of all its layers.
+#include "rq_launch.h"
+#include "rq_rows.h"
+
+namespace rq {
+namespace {
+
+constexpr int kArThreads = 512;
+constexpr int kArWaves = kArThreads / 64;
+
+__device__ __forceinline__ int adapter_of(const int32_t* ids, int64_t row, int n) {
+  const int a = ids[row];
+  return a >= 0 && a < n ? a : n;  // n: no adapter
+}
+
+// Exclusive sums of v over 64 lanes, carry in and out.
+__device__ __forceinline__ int wave_excl(int v, int& carry) {
+  int s = v;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(s, o);
+    if (int(threadIdx.x & 63) >= o) s += x;
+  }
+  const int e = carry + s - v;
+  carry += __shfl(s, 63);
+  return e;
+}
+
+__global__ __launch_bounds__(kArThreads) void adapter_rows_kernel(const int32_t* ids, RowsPlan P, int32_t* plan) {
+  __shared__ int hist[kArWaves][kMaxAdapters + 1];  // counts, then this wave's next place among the adapter's rows
+  __shared__ int first[kMaxAdapters + 2];           // first tile of each adapter
+  __shared__ int total[kMaxAdapters + 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = P.n;
+  const int64_t M = P.M;
+  for (int i = tid; i < kArWaves * (kMaxAdapters + 1); i += kArThreads) (&hist[0][0])[i] = 0;
+  __syncthreads();
+  const int64_t per = ceil_div(ceil_div(M, kArWaves), 64) * 64;
+  const int64_t r0 = per * wave < M ? per * wave : M, r1 = r0 + per < M ? r0 + per : M;
+  for (int64_t r = r0 + lane; r < r1; r += 64) atomicAdd(&hist[wave][adapter_of(ids, r, n)], 1);
+  __syncthreads();
+  for (int a = tid; a <= n; a += kArThreads) {
+    int s = 0;
+#pragma unroll
+    for (int w = 0; w < kArWaves; ++w) {
+      const int c = hist[w][a];
+      hist[w][a] = s;
+      s += c;
+    }
+    total[a] = s;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int carry = 0;
+    for (int a0 = 0; a0 <= n; a0 += 64) {
+      const int a = a0 + lane;
+      const int e = wave_excl(a <= n ? (total[a] + kTileRows - 1) / kTileRows : 0, carry);
+      if (a <= n) first[a] = e;
+    }
+    if (lane == 0) first[n + 1] = carry;
+    // chunks of the adapters' tiles (none for the rows without one), and the
+    // partial slots of adapters with several
+    const int per_chunk = RowsPlan::chunk_tiles(carry);
+    int chunks = 0, parts = 0;
+    int32_t* tab = plan + P.off_chunks();
+    int32_t* part = plan + P.off_part();
+    for (int a0 = 0; a0 < n; a0 += 64) {
+      const int a = a0 + lane;
+      const int tiles = a < n ? (total[a] + kTileRows - 1) / kTileRows : 0;
+      const int c = (tiles + per_chunk - 1) / per_chunk;
+      const int c0 = wave_excl(c, chunks), p0 = wave_excl(c > 1 ? c : 0, parts);
+      if (a < n) {
+        part[2 * a] = c;
+        part[2 * a + 1] = p0;
+      }
+      // the tiles' sums are not all in `first` for later adapters, but this one's is:
+      const int t0 = a < n ? first[a] : 0;
+      for (int k = 0; k < c; ++k) {
+        const int b = t0 + k * per_chunk, e = b + per_chunk < t0 + tiles ? b + per_chunk : t0 + tiles;
+        tab[4 * (c0 + k)] = a;
+        tab[4 * (c0 + k) + 1] = b;
+        tab[4 * (c0 + k) + 2] = e;
+        tab[4 * (c0 + k) + 3] = c > 1 ? p0 + k : -1;
+      }
+    }
+    if (lane < 16) plan[lane] = lane == 0 ? carry : lane == 1 ? chunks : 0;
+  }
+  __syncthreads();
+  const int tiles = first[n + 1];
+  for (int t = tid; t < tiles; t += kArThreads) {
+    int lo = 0, hi = n;  // the last adapter whose first tile is at most t
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (first[mid] <= t) lo = mid;
+      else hi = mid - 1;
+    }
+    const int left = total[lo] - kTileRows * (t - first[lo]);
+    plan[16 + t] = lo < n ? lo : -1;
+    plan[P.off_count() + t] = left < kTileRows ? left : kTileRows;
+    // the slots after the last row of an adapter
+    for (int s = left; s < kTileRows; ++s) plan[P.off_rows() + int64_t(kTileRows) * t + s] = -1;
+  }
+  for (int64_t b = r0; b < r1; b += 64) {
+    const int64_t r = b + lane;
+    const int a = r < r1 ? adapter_of(ids, r, n) : -1;
+    unsigned long long left = __ballot(r < r1);
+    while (left) {
+      const int la = __shfl(a, int(__ffsll(left)) - 1);
+      const unsigned long long same = __ballot(a == la);
+      const int base = hist[wave][la];
+      if (a == la) {
+        const int place = base + __popcll(same & ((1ull << lane) - 1));
+        plan[P.off_rows() + int64_t(kTileRows) * first[la] + place] = int32_t(r);
+      }
+      if (lane == 0) hist[wave][la] = base + __popcll(same);
+      __builtin_amdgcn_wave_barrier();
+      left &= ~same;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace rq
+
+extern "C" int rq_adapter_rows_size(int64_t M, int64_t n, int64_t* bytes) {
+  using namespace rq;
+  if (!bytes) return RQ_ERR_NULL_POINTER;
+  if (M < 0 || n < 1 || M > (int64_t(1) << 30)) return RQ_ERR_BAD_SHAPE;
+  if (n > kMaxAdapters) return RQ_ERR_UNSUPPORTED;
+  static const int32_t some = 0;  // any non-null plan: sizes alone are asked for
+  *bytes = 4 * rows_plan(&some, M, n).words();
+  return RQ_OK;
+}
+
+extern "C" int rq_adapter_rows(const int32_t* ids, int64_t M, int64_t n, void* plan, int64_t plan_bytes,
+                               hipStream_t stream) {
+  using namespace rq;
+  int64_t need = 0;
+  const int st = rq_adapter_rows_size(M, n, &need);
+  if (st != RQ_OK) return st;
+  if (!plan || (M > 0 && !ids)) return RQ_ERR_NULL_POINTER;
+  if (plan_bytes < need) return RQ_ERR_WORKSPACE;
+  if (!aligned(plan, 16) || !aligned(ids, 4)) return RQ_ERR_BAD_ALIGNMENT;
+  int32_t* p = static_cast<int32_t*>(plan);
+  adapter_rows_kernel<<<1, kArThreads, 0, stream>>>(ids, rows_plan(p, M, n), p);
+  return rq_check_launch();
+}

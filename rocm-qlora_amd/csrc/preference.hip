@@ -1,0 +1,416 @@
+// Log-probabilities of labelled sequences, the preference loss on pairs of them,
+// and the gradient of the logits.
+//
+//   lp[t] = z[t, y_t] - max z[t] - log sum_v exp(z[t, v] - max z[t]),  y_t = labels[t + 1]
+//   L_i   = sum of lp over the labelled positions of sequence i (their mean if asked)
+//   D_p   = beta ((L_p - R_p) - (L_{P+p} - R_{P+p}))
+//   loss  = mean_p (1 - eps) softplus(-D_p) + eps softplus(D_p)
+//   dz[t, v] = c_i ([v = y_t] - exp(z[t, v] - max z[t]) / sum),  c_i = d loss / d L_i
+//
+// Three launches.  The rows' maxima and sums are one pass over the labelled
+// rows: every thread keeps its own running maximum and rescales its sum when a
+// piece of the row raises it; a row is split over workgroups when there are few.
+// The second launch joins the splits and sums each sequence, in fp64 and in a
+// fixed order; the workgroup that ends last takes the pairs.  The gradient is a
+// second pass: a pair's coefficient depends on every row of the pair.
+// Bound by memory: the labelled rows read twice, every row of the gradient
+// written once.
+#include "rq_io.h"
+#include "rq_launch.h"
+#include "rq_linear_dev.h"
+
+#include <algorithm>
+
+namespace rq {
+namespace {
+
+constexpr int kPfThreads = 256;
+constexpr int kPfUnroll = 4;       // 16-byte loads of a thread in flight
+constexpr int kPfSeqThreads = 1024;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// Rows of logits: T of them, row t at z + (t / period) * outer + (t % period) * ld.
+struct Rows {
+  int64_t T, V, ld, period, outer;
+  __device__ __forceinline__ int64_t at(int64_t t) const {
+    return period ? (t / period) * outer + (t % period) * ld : t * ld;
+  }
+};
+
+struct Labels {
+  const int64_t* labels;   // [T]
+  const int32_t* offsets;  // [S + 1], or nullptr: sequences of T / S rows
+  int64_t S;
+  int64_t ignore;
+};
+
+// The row's sequence (-1: none) and target: its label, -1 when it has none, -2 when
+// the label is no index of the vocabulary (such a row counts as NaN).
+struct RowTarget {
+  int seq;
+  int64_t target;
+};
+
+template <int NT>
+__device__ __forceinline__ RowTarget row_target(const Labels& L, const Rows& r, int64_t t) {
+  int64_t end;
+  RowTarget o;
+  if (L.offsets) {
+    // offsets are ascending: the sequence is the number of starts up to t, less one
+    int n = 0;
+    for (int64_t i = threadIdx.x; i < ceil_div(L.S, NT) * NT; i += NT) n += __syncthreads_count(i < L.S && L.offsets[i] <= t);
+    o.seq = n - 1;
+    end = n > 0 ? int64_t(L.offsets[n]) : 0;
+    if (t >= end) o.seq = -1;
+  } else {
+    const int64_t len = r.T / L.S;
+    o.seq = int(t / len);
+    end = (o.seq + 1) * len;
+  }
+  o.target = -1;
+  if (o.seq >= 0 && t + 1 < end && t + 1 < r.T) {
+    const int64_t y = L.labels[t + 1];
+    if (y != L.ignore) o.target = y >= 0 && y < r.V ? y : -2;
+  }
+  return o;
+}
+
+// What the forward leaves for every row: its target (as above), sequence, maximum
+// and 1 / sum.
+struct RowInfo {
+  int32_t target;
+  int32_t seq;
+  float top;
+  float inv;
+};
+
+__device__ __forceinline__ float exp_diff(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * kLog2e); }
+
+// (m, s) joined with (m2, s2); an empty side has m = -inf, s = 0.
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  if (top == -__builtin_inff()) {
+    s += s2;  // 0, or the NaN of a side that holds one
+    return;
+  }
+  s = s * exp_diff(m, top) + s2 * exp_diff(m2, top);
+  m = top;
+}
+
+// Piece [v0, v1) of the row: 16-byte loads at the element alignment the row has,
+// `body(values, first column)` for each, elementwise at the end.
+template <int XT>
+struct Piece {
+  int64_t v0, v1;
+};
+
+template <int XT>
+__device__ __forceinline__ Piece<XT> piece_of(int64_t V, int split, int splits) {
+  constexpr int64_t W = Elem<XT>::kVec * 64;
+  const int64_t per = ceil_div(ceil_div(V, splits), W) * W;
+  const int64_t v0 = std::min<int64_t>(split * per, V);
+  return Piece<XT>{v0, std::min<int64_t>(v0 + per, V)};
+}
+
+template <int XT>
+__global__ __launch_bounds__(kPfThreads) void row_sums_kernel(Rows r, Labels L, const void* z, int splits, RowInfo* info,
+                                                              float* part, uint32_t* done) {
+  typedef typename Elem<XT>::T T;
+  constexpr int VW = Elem<XT>::kVec;
+  const int64_t t = blockIdx.x / unsigned(splits);
+  const int split = int(blockIdx.x % unsigned(splits));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *done = 0;
+  const RowTarget rt = row_target<kPfThreads>(L, r, t);
+  if (split == 0 && threadIdx.x == 0) {
+    info[t].target = int32_t(rt.target);
+    info[t].seq = rt.seq;
+  }
+  if (rt.target < 0) return;
+  const T* row = static_cast<const T*>(z) + r.at(t);
+  const Piece<XT> p = piece_of<XT>(r.V, split, splits);
+  float m = -__builtin_inff(), s = 0.0f;
+  auto take = [&](const float* f, int n) {
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < n; ++i) top = fmaxf(top, f[i]);
+    if (top == -__builtin_inff()) {  // nothing above -inf yet; a NaN still has to show
+#pragma unroll
+      for (int i = 0; i < n; ++i) s += f[i] != f[i] ? f[i] : 0.0f;
+      return;
+    }
+    s *= exp_diff(m, top);
+#pragma unroll
+    for (int i = 0; i < n; ++i) s += exp_diff(f[i], top);
+    m = top;
+  };
+  constexpr int64_t kSpan = int64_t(kPfThreads) * VW;
+  int64_t v = p.v0 + threadIdx.x * VW;
+  for (; v + (kPfUnroll - 1) * kSpan + VW <= p.v1; v += kPfUnroll * kSpan) {
+    u32x4 raw[kPfUnroll];
+#pragma unroll
+    for (int u = 0; u < kPfUnroll; ++u) raw[u] = load16_any(row + v + u * kSpan);
+#pragma unroll
+    for (int u = 0; u < kPfUnroll; ++u) {
+      float f[VW];
+      unpack16<XT>(raw[u], f);
+      take(f, VW);
+    }
+  }
+  for (; v < p.v1; v += kSpan) {
+    if (v + VW <= p.v1) {
+      float f[VW];
+      unpack16<XT>(load16_any(row + v), f);
+      take(f, VW);
+    } else {
+      for (int64_t i = v; i < p.v1; ++i) {
+        const float f = to_f32<XT>(row[i]);
+        take(&f, 1);
+      }
+    }
+  }
+  for (int o = 1; o < 64; o <<= 1) join(m, s, __shfl_xor(m, o), __shfl_xor(s, o));
+  __shared__ float wm[kPfThreads / 64], wsum[kPfThreads / 64];
+  if ((threadIdx.x & 63) == 0) {
+    wm[threadIdx.x >> 6] = m;
+    wsum[threadIdx.x >> 6] = s;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < kPfThreads / 64; ++w) join(m, s, wm[w], wsum[w]);
+    part[2 * (t * splits + split)] = m;
+    part[2 * (t * splits + split) + 1] = s;
+  }
+}
+
+__device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
+
+struct Pairs {
+  const float* ref;  // [S] or nullptr: zeros
+  float beta, eps;
+  bool average;
+  bool pairs;        // false: log-probabilities alone
+};
+
+// A workgroup per sequence: the sum of its rows' log-probabilities.  The last
+// workgroup to end takes the pairs: sums[i] and counts[i] of the others are read
+// past the L2 of its XCD, as they were written.
+template <int XT>
+__global__ __launch_bounds__(kPfSeqThreads) void sequences_kernel(Rows r, Labels L, const void* z, int splits, RowInfo* info,
+                                                                  const float* part, uint32_t* done, double* sums,
+                                                                  Pairs P, float* logps, float* loss, float* coef) {
+  typedef typename Elem<XT>::T T;
+  const int64_t i = blockIdx.x;
+  int64_t b, e;
+  if (L.offsets) {
+    b = std::min<int64_t>(std::max<int64_t>(L.offsets[i], 0), r.T);
+    e = std::min<int64_t>(std::max<int64_t>(L.offsets[i + 1], b), r.T);
+  } else {
+    b = i * (r.T / L.S);
+    e = b + r.T / L.S;
+  }
+  double sum = 0.0;
+  int64_t count = 0;
+  for (int64_t t = b + threadIdx.x; t < e; t += kPfSeqThreads) {
+    const int y = info[t].target;
+    if (y == -1 || info[t].seq != i) continue;
+    ++count;
+    float m = -__builtin_inff(), s = 0.0f;
+    if (y >= 0) {
+      for (int k = 0; k < splits; ++k) join(m, s, part[2 * (t * splits + k)], part[2 * (t * splits + k) + 1]);
+      const float x = to_f32<XT>(static_cast<const T*>(z)[r.at(t) + y]);
+      sum += double(x) - double(m) - log(double(s));
+    } else {
+      s = __builtin_nanf("");
+      sum = __builtin_nan("");
+    }
+    info[t].top = m;
+    info[t].inv = 1.0f / s;
+  }
+  __shared__ double wsum[kPfSeqThreads / 64];
+  __shared__ int64_t wcount[kPfSeqThreads / 64];
+  __shared__ bool last;
+  for (int o = 1; o < 64; o <<= 1) {
+    sum += __shfl_xor(sum, o);
+    count += __shfl_xor(count, o);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    wsum[threadIdx.x >> 6] = sum;
+    wcount[threadIdx.x >> 6] = count;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kPfSeqThreads / 64; ++w) {
+      sum += wsum[w];
+      count += wcount[w];
+    }
+    const double n = P.average ? double(count > 0 ? count : 1) : 1.0;
+    sum /= n;
+    logps[i] = float(sum);
+    if (!P.pairs) {
+      coef[i] = float(1.0 / n);
+    } else {
+      __hip_atomic_store(sums + 2 * i, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(sums + 2 * i + 1, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last = __hip_atomic_fetch_add(done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == unsigned(L.S - 1);
+    }
+  }
+  if (!P.pairs) return;
+  __syncthreads();
+  if (!last) return;
+  const int64_t pairs = L.S / 2;
+  double total = 0.0;
+  for (int64_t p = threadIdx.x; p < pairs; p += kPfSeqThreads) {
+    double v[2], n[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int64_t q = p + k * pairs;
+      v[k] = __hip_atomic_load(sums + 2 * q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) - (P.ref ? double(P.ref[q]) : 0.0);
+      n[k] = __hip_atomic_load(sums + 2 * q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    const double beta = P.beta, eps = P.eps, d = beta * (v[0] - v[1]);
+    total += (1.0 - eps) * softplus(-d) + eps * softplus(d);
+    const double up = exp(-softplus(-d)), down = exp(-softplus(d));  // sigmoids of d and -d
+    const double c = beta / double(pairs) * (eps * up - (1.0 - eps) * down);
+    coef[p] = float(c / n[0]);
+    coef[p + pairs] = float(-c / n[1]);
+  }
+  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+  __syncthreads();  // wsum's sequence sums are read
+  if ((threadIdx.x & 63) == 0) wsum[threadIdx.x >> 6] = total;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kPfSeqThreads / 64; ++w) total += wsum[w];
+    *loss = float(total / double(pairs));
+  }
+}
+
+// dz = c ([v = y] - softmax), c = coef[seq] * (grad, or grad[seq] per sequence).
+template <int XT>
+__global__ __launch_bounds__(kPfThreads) void logits_grad_kernel(Rows r, const void* z, int splits, const RowInfo* info,
+                                                                 const float* coef, const float* grad, bool per_seq,
+                                                                 void* dz, int64_t lddz) {
+  typedef typename Elem<XT>::T T;
+  constexpr int VW = Elem<XT>::kVec;
+  const int64_t t = blockIdx.x / unsigned(splits);
+  const int split = int(blockIdx.x % unsigned(splits));
+  const RowInfo I = info[t];
+  const T* row = static_cast<const T*>(z) + r.at(t);
+  T* out = static_cast<T*>(dz) + t * lddz;
+  const Piece<XT> p = piece_of<XT>(r.V, split, splits);
+  constexpr int64_t kSpan = int64_t(kPfThreads) * VW;
+  int64_t v = p.v0 + threadIdx.x * VW;
+  if (I.target == -1) {
+    const float zero[VW] = {};
+    for (; v < p.v1; v += kSpan) store16_part<XT>(out + v, zero, p.v1 - v);
+    return;
+  }
+  float c = coef[I.seq];
+  if (grad) c *= per_seq ? grad[I.seq] : grad[0];
+  const float k = -c * I.inv;
+  auto put = [&](float (&f)[VW], int64_t at, int64_t n) {
+#pragma unroll
+    for (int i = 0; i < VW; ++i) f[i] = k * exp_diff(f[i], I.top);
+    const int64_t y = I.target - at;
+    if (y >= 0 && y < VW) {
+#pragma unroll
+      for (int i = 0; i < VW; ++i) f[i] += i == y ? c : 0.0f;
+    }
+    store16_part<XT>(out + at, f, n);
+  };
+  for (; v + (kPfUnroll - 1) * kSpan + VW <= p.v1; v += kPfUnroll * kSpan) {
+    u32x4 raw[kPfUnroll];
+#pragma unroll
+    for (int u = 0; u < kPfUnroll; ++u) raw[u] = load16_any(row + v + u * kSpan);
+#pragma unroll
+    for (int u = 0; u < kPfUnroll; ++u) {
+      float f[VW];
+      unpack16<XT>(raw[u], f);
+      put(f, v + u * kSpan, VW);
+    }
+  }
+  for (; v < p.v1; v += kSpan) {
+    float f[VW];
+    unpack16<XT>(load16_part<XT>(row + v, p.v1 - v), f);
+    put(f, v, p.v1 - v);
+  }
+}
+
+// Workgroups of a row: enough rows fill the GPU by themselves; fewer are split
+// until there are about four workgroups a compute unit or pieces of 8 KiB.
+int row_splits(int64_t T, int64_t V, int es) {
+  const int64_t want = ceil_div(4 * int64_t(device_cus()), std::max<int64_t>(T, 1));
+  return int(std::max<int64_t>(1, std::min({want, ceil_div(V * es, int64_t(8192)), int64_t(64)})));
+}
+
+size_t up256(size_t b) { return (b + 255) & ~size_t(255); }
+
+int check_rows(int dtype, int64_t T, int64_t V, int64_t ld, int64_t period, int64_t outer, Rows* r) {
+  if (!valid_float_dtype(dtype)) return RQ_ERR_BAD_DTYPE;
+  if (T < 0 || V < 1 || V > INT32_MAX || ld < V || period < 0 || (period > 0 && outer < 0)) return RQ_ERR_BAD_SHAPE;
+  if (T > kMaxThreads1D / kPfThreads) return RQ_ERR_UNSUPPORTED;  // workgroups of one launch
+  *r = Rows{T, V, ld, period, outer};
+  return RQ_OK;
+}
+
+}  // namespace
+}  // namespace rq
+
+extern "C" int rq_preference_workspace_size(int dtype, int64_t T, int64_t V, int64_t S, int64_t* bytes) {
+  using namespace rq;
+  if (!bytes) return RQ_ERR_NULL_POINTER;
+  if (!valid_float_dtype(dtype)) return RQ_ERR_BAD_DTYPE;
+  if (T < 0 || V < 1 || S < 1) return RQ_ERR_BAD_SHAPE;
+  *bytes = int64_t(256 + up256(size_t(S) * 16) + up256(size_t(T) * row_splits(T, V, int(dtype_size(dtype))) * 8));
+  return RQ_OK;
+}
+
+extern "C" int rq_preference_forward(const void* logits, int dtype, int64_t T, int64_t V, int64_t ld, int64_t period,
+                                     int64_t outer, const int64_t* labels, const int32_t* offsets, int64_t S,
+                                     int64_t ignore_index, const float* ref_logps, float beta, float label_smoothing,
+                                     int average, float* logps, float* loss, float* coef, void* row_info,
+                                     void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  using namespace rq;
+  Rows r{};
+  int st = check_rows(dtype, T, V, ld, period, outer, &r);
+  if (st != RQ_OK) return st;
+  if (T < 1 || S < 1 || S > kMaxThreads1D / kPfSeqThreads || (loss && S % 2 != 0) || (!offsets && T % S != 0)) return RQ_ERR_BAD_SHAPE;
+  if (!logps || !coef || !workspace || !logits || !labels || !row_info) return RQ_ERR_NULL_POINTER;
+  const int es = int(dtype_size(dtype)), splits = row_splits(T, V, es);
+  int64_t need = 0;
+  if ((st = rq_preference_workspace_size(dtype, T, V, S, &need)) != RQ_OK) return st;
+  if (workspace_bytes < need) return RQ_ERR_WORKSPACE;
+  if (!aligned(workspace, 256) || !aligned(row_info, 16) || !aligned(logits, es)) return RQ_ERR_BAD_ALIGNMENT;
+  char* ws = static_cast<char*>(workspace);
+  uint32_t* done = reinterpret_cast<uint32_t*>(ws);
+  double* sums = reinterpret_cast<double*>(ws + 256);
+  float* part = reinterpret_cast<float*>(ws + 256 + up256(size_t(S) * 16));
+  RowInfo* info = static_cast<RowInfo*>(row_info);
+  const Labels L{labels, offsets, S, ignore_index};
+  const Pairs P{ref_logps, beta, label_smoothing, average != 0, loss != nullptr};
+  const unsigned grid = unsigned(T * splits);
+  RQ_DISPATCH_DT(dtype, XT, row_sums_kernel<XT><<<grid, kPfThreads, 0, stream>>>(r, L, logits, splits, info, part, done));
+  if ((st = rq_check_launch()) != RQ_OK) return st;
+  RQ_DISPATCH_DT(dtype, XT, sequences_kernel<XT><<<unsigned(S), kPfSeqThreads, 0, stream>>>(
+                                r, L, logits, splits, info, part, done, sums, P, logps, loss, coef));
+  return rq_check_launch();
+}
+
+extern "C" int rq_preference_backward(const void* logits, int dtype, int64_t T, int64_t V, int64_t ld, int64_t period,
+                                      int64_t outer, const void* row_info, const float* coef, const float* grad,
+                                      int grad_per_sequence, void* dlogits, int64_t lddz, hipStream_t stream) {
+  using namespace rq;
+  Rows r{};
+  const int st = check_rows(dtype, T, V, ld, period, outer, &r);
+  if (st != RQ_OK) return st;
+  if (lddz < V) return RQ_ERR_BAD_SHAPE;
+  if (T == 0) return RQ_OK;
+  if (!logits || !row_info || !coef || !dlogits) return RQ_ERR_NULL_POINTER;
+  const int es = int(dtype_size(dtype));
+  if (!aligned(row_info, 16) || !aligned(logits, es) || !aligned(dlogits, es)) return RQ_ERR_BAD_ALIGNMENT;
+  const int splits = row_splits(T, V, es);
+  RQ_DISPATCH_DT(dtype, XT, logits_grad_kernel<XT><<<unsigned(T * splits), kPfThreads, 0, stream>>>(
+                                r, logits, splits, static_cast<const RowInfo*>(row_info), coef, grad,
+                                grad_per_sequence != 0, dlogits, lddz));
+  return rq_check_launch();
+}

@@ -110,6 +110,28 @@ SIGNATURES = {
     "rq_int8_quantize_rows": [_P, _I32, _I64, _I64, _I64, _P, _P, _P],
     "rq_adamw_step": [_P, _I64, _P, _I64, _I64, _I64, _P, _P, _P],  # table, n, dev table, bytes,
                                                                   # chunks [b, e), m, v, stream
+    "rq_adapter_rows_size": [_I64, _I64, _P],
+    "rq_adapter_rows": [_P, _I64, _I64, _P, _I64, _P],       # ids, M, n, plan, bytes, stream
+    "rq_multi_lora_slots": [_I64, _I64, _I32, _P],
+    "rq_multi_lora_scratch_size": [_I32, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _P],
+    "rq_multi_lora": [_P, _I32, _I64, _I64, _I64, _P, _I64,  # x, dtype, M, K, ldx, plan, bytes
+                      _P, _P, _P, _I64, _I64, _I64,          # A, B, scaling, n, rank, N
+                      _P, _I64, _P, _I64, _P,                # base, ld, out, ld, u
+                      _P, _I64, _P],                         # scratch, bytes, stream
+    "rq_multi_lora_grads": [_P, _P, _I32, _I64, _I64, _I64,  # x, exponents, dtype, M, K, ldx
+                            _P, _I64, _I64, _P, _I64,        # dy, N, lddy, plan, bytes
+                            _P, _P, _P, _I64, _I64, _P,      # A, B, scaling, n, rank, u
+                            _P, _I64, _P, _I64, _P, _P,      # dx base, ld, dx, ld, dA, dB
+                            _P, _I64, _P],                   # scratch, bytes, stream
+    "rq_act8_quantize": [_P, _I32, _I64, _I64, _I64, _P, _P, _P],  # x, dtype, rows, cols, ldx, codes, exponents, stream
+    "rq_act8_dequantize": [_P, _P, _I64, _I64, _P, _I32, _I64, _P],  # codes, exponents, rows, cols, out, dtype, ld, stream
+    "rq_preference_workspace_size": [_I32, _I64, _I64, _I64, _P],
+    "rq_preference_forward": [_P, _I32, _I64, _I64, _I64, _I64, _I64,  # logits, dtype, T, V, ld, period, outer
+                              _P, _P, _I64, _I64,            # labels, offsets, S, ignore index
+                              _P, _F32, _F32, _I32,          # ref logps, beta, smoothing, average
+                              _P, _P, _P, _P, _P, _I64, _P],  # logps, loss, coef, row info, workspace, bytes, stream
+    "rq_preference_backward": [_P, _I32, _I64, _I64, _I64, _I64, _I64,  # logits, dtype, T, V, ld, period, outer
+                               _P, _P, _P, _I32, _P, _I64, _P],  # row info, coef, grad, per sequence, dlogits, ld, stream
     "rq_int8_linear_w8a8_workspace_size": [_I64, _I64, _P],
     "rq_int8_linear_w8a8": [_P, _I32, _I64, _I64, _I64,      # x, dtype, M, K, ldx
                             _P, _I64, _P, _I32, _P, _I32,    # w, N, w scales, dtype, bias, dtype

@@ -19,12 +19,17 @@ import math
 import torch
 import torch.nn as nn
 
+from rocm_qlora.checkpoint.act8 import inputs_saved_in_8_bits
 from rocm_qlora.quantization.quant_linear import QuantLinear
 
 
 class LoRALinear(nn.Module):
     """Wraps a QuantLinear with LoRA adapters; merge_lora folds them into an
-    fp16 copy of the weight for inference."""
+    fp16 copy of the weight for inference.  activation_bits = 8 holds the
+    adapter's input for the backward pass as an 8-bit checkpoint
+    (rocm_qlora.checkpoint): half its memory, dA and dB at the held values."""
+
+    activation_bits = 16
 
     def __init__(self, quant_linear: QuantLinear, r: int = 8, lora_alpha: int = 16, lora_dropout: float = 0.0):
         super().__init__()
@@ -54,6 +59,9 @@ class LoRALinear(nn.Module):
         base = self.base_layer
         if isinstance(base, QuantLinear) and not base.merged_mode:
             p = self.lora_dropout.p if self._dropout_active() else 0.0
+            if self.activation_bits == 8 and torch.is_grad_enabled():
+                with inputs_saved_in_8_bits():
+                    return base.fused_forward(x, self.lora_A, self.lora_B, self.scaling, p)
             return base.fused_forward(x, self.lora_A, self.lora_B, self.scaling, p)
         if hasattr(base, "weight"):
             base_out = base(x.to(base.weight.dtype))

@@ -1,0 +1,203 @@
+"""Adapters of many requests (or of many users' training batches) beside one
+shared, quantized projection (no counterpart in the reference).
+
+Every row of a batch names its adapter, or none: y[m] = base(x[m]) + s[a]
+(x[m] A[a]^T) B[a]^T.  A serving step and a training step group their rows by
+adapter once (AdapterRows) and pass that to every projection.  In preference
+tuning the policy's rows name their adapter and the reference model's none, so
+that both run as one batch.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Union
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from rocm_qlora import ops
+from rocm_qlora.lora.lora_layer import LoRALinear
+from rocm_qlora.quantization.quant_linear import QuantLinear
+
+
+class AdapterRows:
+    """The rows of a batch grouped by adapter, for every projection that the batch
+    passes through.  ids: [M] (or the batch's leading shape) int32 or int64 on the
+    GPU, 0 .. n - 1, or anything else for rows without an adapter; made on the
+    current stream, without a host synchronization."""
+    __slots__ = ("M", "n", "plan")
+
+    def __init__(self, ids: torch.Tensor, n: int):
+        self.M, self.n = ids.numel(), int(n)
+        self.plan = ops.adapter_rows(ids, self.n)
+
+    @classmethod
+    def single(cls, M: int) -> "AdapterRows":
+        """M rows that all belong to adapter 0 of one."""
+        rows = cls.__new__(cls)
+        rows.M, rows.n, rows.plan = int(M), 1, None
+        return rows
+
+
+def _check(x: torch.Tensor, lora_a: torch.Tensor, rows: AdapterRows, activation_bits: int) -> None:
+    if activation_bits not in (8, 16):
+        raise ValueError(f"activation_bits must be 8 or 16, got {activation_bits}")
+    if rows.n != lora_a.shape[0] or rows.M * x.shape[-1] != x.numel():
+        raise RuntimeError(f"rows of {rows.M} rows and {rows.n} adapters do not fit x {tuple(x.shape)} and "
+                           f"{lora_a.shape[0]} adapters")
+
+
+class _MultiLoRA(torch.autograd.Function):
+    """base(x) plus the adapters' term.  base: a tensor of the rows' results, None, or
+    a pair (forward, dx) of a quantized linear's functions, whose result the term is
+    added to in place, and likewise in the backward pass."""
+
+    @staticmethod
+    def forward(ctx, x, lora_a, lora_b, base, scaling, rows, bits, linear):
+        a, b = lora_a.to(x.dtype), lora_b.to(x.dtype)
+        N = b.shape[1]
+        need_x, need_a, need_b = ctx.needs_input_grad[:3]
+        x2 = x.reshape(-1, x.shape[-1])
+        if linear is not None:
+            y = linear[0](x2)
+            out = y
+        else:
+            y, out = (base.reshape(-1, N) if base is not None else None), None
+        res = ops.multi_lora(x2, a, b, scaling, rows.plan, y, out, need_u=need_b)
+        y, u = res if need_b else (res, None)
+        ctx.plan, ctx.linear, ctx.bits, ctx.shape = rows.plan, linear, bits, x.shape
+        ctx.dtypes = (lora_a.dtype, lora_b.dtype)
+        held = (None, None)
+        if need_a:
+            held = ops.act8_quantize(x2) if bits == 8 else (x2, None)
+        ctx.save_for_backward(*held, a, b, scaling, u)
+        return y.view(*x.shape[:-1], N)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, exps, a, b, scaling, u = ctx.saved_tensors
+        need_x, need_a, need_b, need_base = ctx.needs_input_grad[:4]
+        dy2 = dy.reshape(-1, dy.shape[-1])
+        dx = ctx.linear[1](dy2) if need_x and ctx.linear is not None else None
+        dx, da, db = ops.multi_lora_grads((x, exps) if exps is not None else x, dy2, a, b, scaling, ctx.plan, u,
+                                          need_x=need_x, need_a=need_a, need_b=need_b, dx=dx)
+        return (dx.view(ctx.shape) if need_x else None, da.to(ctx.dtypes[0]) if need_a else None,
+                db.to(ctx.dtypes[1]) if need_b else None, dy if need_base else None, None, None, None, None)
+
+
+def _scalings(scaling: Union[float, torch.Tensor], n: int, dev: torch.device) -> torch.Tensor:
+    if isinstance(scaling, torch.Tensor):
+        return scaling
+    return torch.full((n,), float(scaling), dtype=torch.float32, device=dev)
+
+
+def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: Union[float, torch.Tensor],
+               rows: AdapterRows, base: Optional[torch.Tensor] = None, activation_bits: int = 16) -> torch.Tensor:
+    """base[m] + scaling[a] (x[m] A[a]^T) B[a]^T for the adapter a of every row m.
+
+    x: [..., K] fp32, bf16 or fp16; lora_a [n, r, K] and lora_b [n, N, r] (rounded to
+    x's dtype when they have another); scaling: fp32 [n], or one number; base: [...,
+    N] in x's dtype (None: zeros).  Sums are fp32; x A^T is passed to the second
+    product in 16 bits or more and the result rounded once.  Differentiable by x,
+    lora_a, lora_b and base; activation_bits=8 holds x for dA as an 8-bit checkpoint
+    (rocm_qlora.checkpoint), which the gradient kernel reads as it is."""
+    _check(x, lora_a, rows, activation_bits)
+    if base is not None and (base.dtype != x.dtype or base.shape[:-1] != x.shape[:-1] or base.shape[-1] != lora_b.shape[1]):
+        raise RuntimeError(f"base {tuple(base.shape)} {base.dtype} does not fit x {tuple(x.shape)} {x.dtype} and "
+                           f"{lora_b.shape[1]} columns")
+    scaling = _scalings(scaling, rows.n, x.device)
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (x, lora_a, lora_b, base)):
+        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        N = lora_b.shape[1]
+        y = ops.multi_lora(x2, lora_a.to(x.dtype), lora_b.to(x.dtype), scaling, rows.plan,
+                           base if base is None or base.dim() == 2 else base.reshape(-1, N))
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+    return _MultiLoRA.apply(x, lora_a, lora_b, base, scaling, rows, activation_bits, None)
+
+
+class MultiLoRALinear(nn.Module):
+    """A QuantLinear with n adapters of rank r.  lora_A [n, r, in] and lora_B [n, out,
+    r] are parameters (A Kaiming-uniform, B zeros, as LoRALinear's), `scaling` [n] a
+    buffer.  The rows of a batch are given to forward, or set for all layers of a
+    model by set_adapter_rows."""
+
+    def __init__(self, quant_linear: QuantLinear, n: int, r: int = 8, lora_alpha: float = 16, activation_bits: int = 16):
+        super().__init__()
+        self.base_layer = quant_linear
+        self.n, self.r = n, r
+        self.activation_bits = activation_bits
+        self.rows: Optional[AdapterRows] = None
+        for p in quant_linear.parameters():
+            p.requires_grad_(False)
+        dev = quant_linear.weight_quant.device
+        a = torch.empty(n, r, quant_linear.in_features)
+        for i in range(n):
+            nn.init.kaiming_uniform_(a[i], a=math.sqrt(5))
+        self.lora_A = nn.Parameter(a.to(dev))
+        self.lora_B = nn.Parameter(torch.zeros(n, quant_linear.out_features, r, device=dev))
+        self.register_buffer("scaling", torch.full((n,), lora_alpha / r, device=dev))
+
+    @torch.no_grad()
+    def load_adapter(self, i: int, layer: LoRALinear) -> None:
+        """Adapter i from a LoRALinear of at most this rank (the ranks it lacks are zeros)."""
+        if layer.r > self.r:
+            raise ValueError(f"an adapter of rank {layer.r} does not fit rank {self.r}")
+        self.lora_A[i].zero_()
+        self.lora_B[i].zero_()
+        self.lora_A[i, :layer.r].copy_(layer.lora_A)
+        self.lora_B[i, :, :layer.r].copy_(layer.lora_B)
+        self.scaling[i] = layer.scaling
+
+    def _linear(self):
+        """The quantized linear and its input gradient as functions of 2-D rows."""
+        from rocm_qlora import torch_ops
+        from rocm_qlora.kernels import dequant_matmul as dm
+        base = self.base_layer
+        if base.bits == 4:
+            w = base.nf4_weight()
+            return (lambda x: ops.nf4_linear(x, w.packed, w.scales, w.N, w.block_size, base.bias, **w.dq_kwargs()),
+                    lambda dy: torch_ops.call_nf4_linear_dx(dy, w.packed, w.scales, w.K, w.block_size, **w.dq_kwargs()))
+        w = base.int8_weight()
+        return (lambda x: ops.int8_linear(x, w.q, w.scales, w.N, w.block_size, base.bias), lambda dy: dm.int8_dx(dy, w))
+
+    def forward(self, x: torch.Tensor, rows: Optional[AdapterRows] = None) -> torch.Tensor:
+        rows = rows if rows is not None else self.rows
+        if rows is None:
+            raise RuntimeError("no adapter rows: pass them, or set them with set_adapter_rows(model, rows)")
+        _check(x, self.lora_A, rows, self.activation_bits)
+        linear = self._linear()
+        if torch.is_grad_enabled() and (x.requires_grad or self.lora_A.requires_grad or self.lora_B.requires_grad):
+            return _MultiLoRA.apply(x, self.lora_A, self.lora_B, None, self.scaling, rows, self.activation_bits, linear)
+        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        y = linear[0](x2)
+        ops.multi_lora(x2, self.lora_A.to(x.dtype), self.lora_B.to(x.dtype), self.scaling, rows.plan, y, y)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[-1])
+
+    def extra_repr(self) -> str:
+        return f"adapters={self.n}, r={self.r}, activation_bits={self.activation_bits}"
+
+
+def set_adapter_rows(model: nn.Module, rows: Optional[AdapterRows]) -> int:
+    """Set the batch's rows by adapter on every MultiLoRALinear; returns how many."""
+    count = 0
+    for m in model.modules():
+        if isinstance(m, MultiLoRALinear):
+            m.rows = rows
+            count += 1
+    return count
+
+
+def attach_adapters(model: nn.Module, n: int, activation_bits: int = 16) -> nn.Module:
+    """Replace every LoRALinear (quantize_model's) by a MultiLoRALinear of n adapters of
+    its rank over the same quantized weight; adapter 0 is the layer's own."""
+    for name, m in list(model.named_modules()):
+        if isinstance(m, LoRALinear):
+            if m.merged:
+                raise RuntimeError(f"{name} is merged: unmerge it first")
+            new = MultiLoRALinear(m.base_layer, n, m.r, m.lora_alpha, activation_bits)
+            new.load_adapter(0, m)
+            parent = model.get_submodule(name.rpartition(".")[0])
+            setattr(parent, name.rpartition(".")[2], new)
+    return model

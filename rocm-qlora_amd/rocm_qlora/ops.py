@@ -723,3 +723,272 @@ def merge_lora(weight_quant: torch.Tensor, weight_scales: torch.Tensor, out_feat
                  nat.ptr(la), nat.ptr(lb), ldb, lcode, rank, float(scaling), MERGE_MODES[mode],
                  out.data_ptr(), nat.dtype_code(out_dtype), K, nat.stream_handle(dev))
     return out
+
+
+# ---- adapters of many requests, 8-bit activation checkpoints, preference loss -----------
+ACT8_BLOCK = 32     # values that share a checkpoint's scale (kAct8Block in csrc/rq_act8.h)
+MAX_ADAPTERS = 1024  # kMaxAdapters in csrc/rq_rows.h
+
+
+def adapter_rows(ids: torch.Tensor, n: int) -> torch.Tensor:
+    """The rows of a batch grouped by adapter: ids [M] int32 or int64 on the GPU, 0 ..
+    n - 1 or, for a row without an adapter, anything else.  The result is what
+    multi_lora takes as `plan`."""
+    dev = nat.require_gpu(ids)
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"adapter ids must be int32 or int64, got {ids.dtype}")
+    if not 1 <= n <= MAX_ADAPTERS:
+        raise RuntimeError(f"{n} adapters: 1 to {MAX_ADAPTERS} are taken at once")
+    ids = ids.reshape(-1)
+    if ids.dtype == torch.int64:
+        ids = ids.clamp(-1, n)  # whatever int32 cannot hold has no adapter either
+    ids = ids.to(torch.int32).contiguous()
+    with on(dev):
+        plan = _scratch("rq_adapter_rows_size", dev, ids.numel(), n)
+        nat.call("rq_adapter_rows", ids.data_ptr(), ids.numel(), n, plan.data_ptr(), plan.numel(), nat.stream_handle(dev))
+    return plan
+
+
+def _adapter_operands(dtype, K: int, lora_a, lora_b, scaling) -> Tuple[int, int, int, torch.Tensor, torch.Tensor]:
+    """n, rank and N of stacked factors, and the factors as the kernels take them."""
+    if lora_a.dim() != 3 or lora_b.dim() != 3:
+        raise RuntimeError(f"stacked factors are [n, rank, K] and [n, N, rank], got {tuple(lora_a.shape)} and "
+                           f"{tuple(lora_b.shape)}")
+    n, rank, N = lora_a.shape[0], lora_a.shape[1], lora_b.shape[1]
+    if lora_a.shape[2] != K or lora_b.shape[0] != n or lora_b.shape[2] != rank or rank < 1 or N < 1:
+        raise RuntimeError(f"LoRA shapes {tuple(lora_a.shape)} / {tuple(lora_b.shape)} do not fit rows of {K}")
+    if lora_a.dtype != dtype or lora_b.dtype != dtype:
+        raise TypeError(f"stacked factors must have the rows' dtype {dtype}, got {lora_a.dtype} and {lora_b.dtype}")
+    if scaling.dtype != torch.float32 or scaling.shape != (n,) or not scaling.is_contiguous():
+        raise RuntimeError(f"scaling must be {n} contiguous fp32 values, got {tuple(scaling.shape)} {scaling.dtype}")
+    return n, rank, N, lora_a.contiguous(), lora_b.contiguous()
+
+
+def _check_rows(t: torch.Tensor, M: int, cols: int, dtype: torch.dtype, name: str) -> None:
+    if t.dtype != dtype or t.shape != (M, cols) or (t.stride(1) != 1 and cols > 1) or (M > 1 and t.stride(0) < cols):
+        raise RuntimeError(f"{name} must be [{M}, {cols}] {dtype} with adjacent columns, got {tuple(t.shape)} {t.dtype} "
+                           f"of strides {t.stride()}")
+
+
+def _ld(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: torch.Tensor,
+               plan: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None, need_u: bool = False):
+    """out[m] = base[m] + scaling[a] (x[m] A[a]^T) B[a]^T, a the adapter of row m in
+    `plan` (None: adapter 0 of one).  x [M, K], lora_a [n, rank, K], lora_b [n, N,
+    rank], base and out [M, N] (out may be base) of one dtype, scaling [n] fp32.
+    Returns out and, with need_u, the sums x A^T that multi_lora_grads takes."""
+    dev = nat.require_gpu(x, lora_a, lora_b, scaling, plan, base, out)
+    M, K = x.shape
+    code = nat.dtype_code(x.dtype)
+    n, rank, N, a, b = _adapter_operands(x.dtype, K, lora_a, lora_b, scaling)
+    grouped = 0 if plan is None else 1
+    if not grouped and n != 1:
+        raise RuntimeError(f"{n} adapters without the batch's rows by adapter")
+    if base is not None:
+        _check_rows(base, M, N, x.dtype, "base")
+    if out is not None:
+        _check_rows(out, M, N, x.dtype, "out")
+    with on(dev):
+        if grouped and plan.numel() != _bytes("rq_adapter_rows_size", dev.index, M, n):
+            raise RuntimeError(f"the rows by adapter are not those of {M} rows and {n} adapters")
+        if out is None:
+            out = torch.empty((M, N), dtype=x.dtype, device=dev)
+        u = None
+        if need_u:
+            slots = _bytes("rq_multi_lora_slots", dev.index, M, n, grouped)
+            u = torch.empty((slots, -(-rank // 16) * 16), dtype=torch.float32, device=dev)
+        if M > 0:
+            x, ldx = _rows(x, K)
+            scratch = _scratch("rq_multi_lora_scratch_size", dev, code, M, K, N, n, rank, grouped, 0)
+            nat.call("rq_multi_lora", x.data_ptr(), code, M, K, ldx, nat.ptr(plan), plan.numel() if grouped else 0,
+                     a.data_ptr(), b.data_ptr(), scaling.data_ptr(), n, rank, N,
+                     nat.ptr(base), _ld(base) if base is not None else 0, out.data_ptr(), _ld(out), nat.ptr(u),
+                     scratch.data_ptr(), scratch.numel(), nat.stream_handle(dev))
+    return (out, u) if need_u else out
+
+
+def multi_lora_grads(x, dy: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: torch.Tensor,
+                     plan: Optional[torch.Tensor] = None, u: Optional[torch.Tensor] = None, *, need_x: bool = True,
+                     need_a: bool = True, need_b: bool = True, dx: Optional[torch.Tensor] = None):
+    """Gradients of multi_lora: (dx, dA, dB), None where not asked for.  x: the rows
+    [M, K] or act8_quantize's (codes, exponents) of them, read for dA alone; u:
+    multi_lora's, read for dB alone.  dx: [M, K], to which the adapters' input
+    gradient is added (None: a new tensor of that term)."""
+    dev = nat.require_gpu(dy, lora_a, lora_b, scaling, plan, u, dx)
+    M, N = dy.shape
+    K = lora_a.shape[-1]
+    code = nat.dtype_code(dy.dtype)
+    n, rank, n_out, a, b = _adapter_operands(dy.dtype, K, lora_a, lora_b, scaling)
+    grouped = 0 if plan is None else 1
+    if n_out != N:
+        raise RuntimeError(f"dY has {N} columns, the factors {n_out}")
+    if not grouped and n != 1:
+        raise RuntimeError(f"{n} adapters without the batch's rows by adapter")
+    need_x = need_x or dx is not None
+    codes = exps = None
+    xr, ldx = None, 0
+    pitch = -(-K // ACT8_BLOCK) * ACT8_BLOCK
+    if need_a:
+        if isinstance(x, tuple):
+            codes, exps = x
+            nat.require_gpu(dy, codes, exps)
+            if codes.shape != (M, pitch) or exps.shape != (M, pitch // ACT8_BLOCK) or codes.dtype != torch.uint8 or \
+                    exps.dtype != torch.uint8 or not codes.is_contiguous() or not exps.is_contiguous():
+                raise RuntimeError(f"codes {tuple(codes.shape)} / {tuple(exps.shape)} are not act8_quantize's of {M} rows of {K}")
+            xr, ldx = codes, pitch
+        else:
+            nat.require_gpu(dy, x)
+            if x.dtype != dy.dtype or x.shape != (M, K):
+                raise RuntimeError(f"x must be [{M}, {K}] {dy.dtype}, got {tuple(x.shape)} {x.dtype}")
+            xr, ldx = _rows(x, K)
+    if dx is not None:
+        _check_rows(dx, M, K, dy.dtype, "dx")
+    with on(dev):
+        slots = _bytes("rq_multi_lora_slots", dev.index, M, n, grouped)
+        if grouped and plan.numel() != _bytes("rq_adapter_rows_size", dev.index, M, n):
+            raise RuntimeError(f"the rows by adapter are not those of {M} rows and {n} adapters")
+        if need_b and (u is None or u.shape != (slots, -(-rank // 16) * 16) or u.dtype != torch.float32 or
+                       not u.is_contiguous()):
+            raise RuntimeError("u is not multi_lora's of these rows and factors")
+        base = dx
+        da = torch.empty_like(a) if need_a else None
+        db = torch.empty_like(b) if need_b else None
+        if need_x and dx is None:
+            dx = torch.empty((M, K), dtype=dy.dtype, device=dev)
+        if M == 0:
+            for t in (da, db):
+                if t is not None:
+                    t.zero_()
+            return dx, da, db
+        dy2, lddy = _rows(dy, N)
+        scratch = _scratch("rq_multi_lora_scratch_size", dev, code, M, K, N, n, rank, grouped, 1)
+        nat.call("rq_multi_lora_grads", nat.ptr(xr), nat.ptr(exps), code, M, K, ldx, dy2.data_ptr(), N, lddy,
+                 nat.ptr(plan), plan.numel() if grouped else 0, a.data_ptr(), b.data_ptr(), scaling.data_ptr(), n, rank,
+                 nat.ptr(u) if need_b else None, nat.ptr(base), _ld(base) if base is not None else 0,
+                 nat.ptr(dx), _ld(dx) if dx is not None else 0, nat.ptr(da), nat.ptr(db),
+                 scratch.data_ptr(), scratch.numel(), nat.stream_handle(dev))
+    return dx, da, db
+
+
+def act8_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The 8-bit checkpoint of x's rows ([..., K] fp32/bf16/fp16): codes [M, K rounded
+    up to 32] and exponents [M, K / 32 rounded up], both uint8."""
+    dev = nat.require_gpu(x)
+    code = nat.dtype_code(x.dtype)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise RuntimeError(f"rows expected, got shape {tuple(x.shape)}")
+    K = x.shape[-1]
+    with on(dev):
+        x2, ldx = _rows(x, K)
+        M = x2.shape[0]
+        blocks = -(-K // ACT8_BLOCK)
+        codes = torch.empty((M, blocks * ACT8_BLOCK), dtype=torch.uint8, device=dev)
+        exps = torch.empty((M, blocks), dtype=torch.uint8, device=dev)
+        nat.call("rq_act8_quantize", x2.data_ptr(), code, M, K, ldx, codes.data_ptr(), exps.data_ptr(), nat.stream_handle(dev))
+    return codes, exps
+
+
+def act8_dequantize(codes: torch.Tensor, exps: torch.Tensor, cols: int, dtype: torch.dtype) -> torch.Tensor:
+    """The values [M, cols] that act8_quantize's codes stand for."""
+    dev = nat.require_gpu(codes, exps)
+    code = nat.dtype_code(dtype)
+    blocks = -(-cols // ACT8_BLOCK)
+    if cols < 1 or codes.dim() != 2 or codes.shape[1] != blocks * ACT8_BLOCK or exps.shape != (codes.shape[0], blocks) or \
+            codes.dtype != torch.uint8 or exps.dtype != torch.uint8:
+        raise RuntimeError(f"codes {tuple(codes.shape)} / {tuple(exps.shape)} are not act8_quantize's of rows of {cols}")
+    codes, exps = codes.contiguous(), exps.contiguous()
+    with on(dev):
+        out = torch.empty((codes.shape[0], cols), dtype=dtype, device=dev)
+        nat.call("rq_act8_dequantize", codes.data_ptr(), exps.data_ptr(), codes.shape[0], cols, out.data_ptr(), code, cols,
+                 nat.stream_handle(dev))
+    return out
+
+
+def _logit_rows(logits: torch.Tensor) -> Tuple[torch.Tensor, int, int, int, int]:
+    """Logits [T, V] or [B, L, V] without a copy where the vocabulary's stride is 1:
+    (tensor, T, row stride, rows a period, period stride)."""
+    V = logits.shape[-1]
+    if logits.stride(-1) != 1 and V > 1:
+        logits = logits.contiguous()
+    if logits.dim() == 2:
+        if logits.shape[0] > 1 and logits.stride(0) < V:
+            logits = logits.contiguous()
+        return logits, logits.shape[0], logits.stride(0) if logits.shape[0] > 1 else V, 0, 0
+    B, L = logits.shape[:2]
+    if (L > 1 and logits.stride(1) < V) or (B > 1 and logits.stride(0) < V):
+        logits = logits.contiguous()
+    ld = logits.stride(1) if L > 1 else V
+    if B == 1 or logits.stride(0) == L * ld:
+        return logits, B * L, ld, 0, 0
+    return logits, B * L, ld, L, logits.stride(0)
+
+
+def preference_forward(logits: torch.Tensor, labels: torch.Tensor, offsets: Optional[torch.Tensor] = None,
+                       ref_logps: Optional[torch.Tensor] = None, *, beta: float = 0.1, label_smoothing: float = 0.0,
+                       average: bool = False, ignore_index: int = -100, pairs: bool = True):
+    """Log-probabilities of labelled sequences and (with `pairs`) the preference loss of
+    their pairs.  logits [T, V] with offsets [S + 1] (int32/int64), or [B, L, V]: a
+    sequence per batch entry; labels int64 of the logits' leading shape, in the
+    positions of their tokens (row t predicts labels[t + 1]).  Returns (loss or None,
+    logps [S], what preference_backward takes)."""
+    dev = nat.require_gpu(logits, labels, offsets, ref_logps)
+    code = nat.dtype_code(logits.dtype)
+    if logits.dim() not in (2, 3) or logits.numel() == 0:
+        raise RuntimeError(f"logits must be [T, V] or [B, L, V] with a row at least, got {tuple(logits.shape)}")
+    if labels.dtype != torch.int64 or labels.shape != logits.shape[:-1]:
+        raise RuntimeError(f"labels must be int64 {tuple(logits.shape[:-1])}, got {labels.dtype} {tuple(labels.shape)}")
+    if logits.dim() == 2:
+        if offsets is None:
+            raise RuntimeError("packed logits need their sequences' offsets")
+        if offsets.dim() != 1 or offsets.numel() < 2 or offsets.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError(f"offsets must be int32 or int64 [sequences + 1], got {offsets.dtype} {tuple(offsets.shape)}")
+        S = offsets.numel() - 1
+    else:
+        if offsets is not None:
+            raise RuntimeError("offsets go with packed logits [T, V]")
+        S = logits.shape[0]
+    if pairs and S % 2:
+        raise RuntimeError(f"{S} sequences are no pairs")
+    if pairs and not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
+    if ref_logps is not None:
+        if ref_logps.shape != (S,):
+            raise RuntimeError(f"ref_logps must hold {S} values, got {tuple(ref_logps.shape)}")
+        ref_logps = ref_logps.detach().to(torch.float32).contiguous()
+    labels = labels.contiguous()
+    with on(dev):
+        if offsets is not None:
+            offsets = offsets.to(torch.int32).contiguous()
+        z, T, ld, period, outer = _logit_rows(logits)
+        V = z.shape[-1]
+        f32 = functools.partial(torch.empty, dtype=torch.float32, device=dev)
+        logps, coef, info = f32(S), f32(S), f32((T, 4))
+        loss = f32(()) if pairs else None
+        ws = _scratch("rq_preference_workspace_size", dev, code, T, V, S)
+        nat.call("rq_preference_forward", z.data_ptr(), code, T, V, ld, period, outer, labels.data_ptr(), nat.ptr(offsets), S,
+                 int(ignore_index), nat.ptr(ref_logps), float(beta), float(label_smoothing), int(average), logps.data_ptr(),
+                 nat.ptr(loss), coef.data_ptr(), info.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_handle(dev))
+    return loss, logps, (info, coef)
+
+
+def preference_backward(logits: torch.Tensor, state, grad: Optional[torch.Tensor]) -> torch.Tensor:
+    """The logits' gradient, contiguous, from preference_forward's state and the
+    gradient of its loss (a scalar) or of its log-probabilities ([S])."""
+    info, coef = state
+    dev = nat.require_gpu(logits, info, coef, grad)
+    if grad is not None and (grad.dtype != torch.float32 or grad.numel() not in (1, coef.numel())):
+        raise RuntimeError(f"grad must be fp32, one value or {coef.numel()}, got {grad.dtype} {tuple(grad.shape)}")
+    with on(dev):
+        z, T, ld, period, outer = _logit_rows(logits)
+        V = z.shape[-1]
+        dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
+        per_seq = grad is not None and grad.dim() > 0
+        if grad is not None:
+            grad = grad.contiguous()
+        nat.call("rq_preference_backward", z.data_ptr(), nat.dtype_code(z.dtype), T, V, ld, period, outer, info.data_ptr(),
+                 coef.data_ptr(), nat.ptr(grad), int(per_seq), dz.data_ptr(), V, nat.stream_handle(dev))
+    return dz
