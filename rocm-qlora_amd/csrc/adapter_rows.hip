@@ -62,32 +62,36 @@ __global__ __launch_bounds__(kArThreads) void adapter_rows_kernel(const int32_t*
       if (a <= n) first[a] = e;
     }
     if (lane == 0) first[n + 1] = carry;
-    // chunks of the adapters' tiles (none for the rows without one), and the
-    // partial slots of adapters with several
-    const int per_chunk = RowsPlan::chunk_tiles(carry);
-    int chunks = 0, parts = 0;
-    int32_t* tab = plan + P.off_chunks();
-    int32_t* part = plan + P.off_part();
-    for (int a0 = 0; a0 < n; a0 += 64) {
-      const int a = a0 + lane;
-      const int tiles = a < n ? (total[a] + kTileRows - 1) / kTileRows : 0;
-      const int c = (tiles + per_chunk - 1) / per_chunk;
-      const int c0 = wave_excl(c, chunks), p0 = wave_excl(c > 1 ? c : 0, parts);
-      if (a < n) {
-        part[2 * a] = c;
-        part[2 * a + 1] = p0;
+    // chunks of the adapters' tiles (an empty one for an adapter without rows, none for
+    // the rows without one), and the partial slots of adapters with several
+    int used[kChunkTables];
+#pragma unroll
+    for (int k = 0; k < kChunkTables; ++k) {
+      const int per_chunk = RowsPlan::chunk_tiles(carry, k);
+      int chunks = 0, parts = 0;
+      int32_t* tab = plan + P.off_chunks() + 4 * int64_t(P.C) * k;
+      int32_t* part = plan + P.off_part() + 2 * int64_t(n) * k;
+      for (int a0 = 0; a0 < n; a0 += 64) {
+        const int a = a0 + lane;
+        const int tiles = a < n ? (total[a] + kTileRows - 1) / kTileRows : 0;
+        const int c = a < n ? (tiles > per_chunk ? (tiles + per_chunk - 1) / per_chunk : 1) : 0;
+        const int c0 = wave_excl(c, chunks), p0 = wave_excl(c > 1 ? c : 0, parts);
+        const int t0 = a < n ? first[a] : 0;  // this lane's own store above
+        if (a < n) {
+          part[2 * a] = c;
+          part[2 * a + 1] = p0;
+        }
+        for (int i = 0; i < c; ++i) {
+          const int b = t0 + i * per_chunk, e = b + per_chunk < t0 + tiles ? b + per_chunk : t0 + tiles;
+          tab[4 * (c0 + i)] = a;
+          tab[4 * (c0 + i) + 1] = b;
+          tab[4 * (c0 + i) + 2] = e;
+          tab[4 * (c0 + i) + 3] = c > 1 ? p0 + i : -1;
+        }
       }
-      // the tiles' sums are not all in `first` for later adapters, but this one's is:
-      const int t0 = a < n ? first[a] : 0;
-      for (int k = 0; k < c; ++k) {
-        const int b = t0 + k * per_chunk, e = b + per_chunk < t0 + tiles ? b + per_chunk : t0 + tiles;
-        tab[4 * (c0 + k)] = a;
-        tab[4 * (c0 + k) + 1] = b;
-        tab[4 * (c0 + k) + 2] = e;
-        tab[4 * (c0 + k) + 3] = c > 1 ? p0 + k : -1;
-      }
+      used[k] = chunks;
     }
-    if (lane < 16) plan[lane] = lane == 0 ? carry : lane == 1 ? chunks : 0;
+    if (lane < 16) plan[lane] = lane == 0 ? carry : lane == 1 ? used[0] : lane == 2 ? used[1] : 0;
   }
   __syncthreads();
   const int tiles = first[n + 1];

@@ -17,21 +17,49 @@ namespace rq {
 constexpr int kMlThreads = 256;
 constexpr int kMlWaves = kMlThreads / 64;
 
+// The 16-bit halves of fp32 values: hi = RND(v), lo = RND(v - hi) (none for an
+// infinity: inf - inf).
+template <int XT>
+__device__ __forceinline__ void split16(float v, uint32_t& hi, uint32_t& lo) {
+  hi = to_x16<XT>(v);
+  const float h = from_x16<XT>(hi);
+  lo = to_x16<XT>(fabsf(h) == __builtin_inff() ? 0.0f : v - h);
+}
+
 // ---- shrink ---------------------------------------------------------------------
-// A workgroup takes a tile's rows over a split of K; its four waves divide the split
-// and meet in LDS.  A wave holds the tile's 16-row blocks (1 to 4, as many as the
-// tile has) times JB blocks of 16 ranks, so that a factor's piece is loaded once
-// for the tile.
-template <int XT, int NRB, int JB>
-__device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& tile, int t, int split, int j0, float* red) {
+// A workgroup takes a tile's rows over a split of K; its eight waves divide the split
+// and meet in LDS, 16 rows at a time, summed in the waves' order.  A wave holds the
+// tile's 16-row blocks (1 to 4, as many as the tile has) times JB blocks of 16 ranks,
+// so that a factor's piece is loaded once for the tile.
+//
+// The factor is A [r][K], whose rows are operands as they lie, or (TURNED) B [N][r],
+// whose rows run across the contraction: a step's rows are one piece of memory, which
+// a wave copies to LDS as it lies (with 32 bytes between eight-row groups, so that the
+// four lane groups read other banks) and reads back a rank's values at a time.
+constexpr int kShWaves = 8;
+constexpr int kShThreads = 64 * kShWaves;
+
+template <int XT, int JB>
+struct ShrinkLds {
+  static constexpr int kPitch = 16 * JB + 4;
+  static constexpr int kRedFloats = kShWaves * 16 * kPitch;
+  // elements of one wave's turned step, with the gaps
+  static constexpr int kGap = 32 / int(sizeof(typename Elem<XT>::T));
+  static constexpr int kTurn = Elem<XT>::kStep * 16 * JB + 4 * kGap + Elem<XT>::kVec;
+  static constexpr int kTurnFloats = kShWaves * kTurn * int(sizeof(typename Elem<XT>::T)) / 4;
+};
+
+template <int XT, int NRB, int JB, bool TURNED>
+__device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& tile, int t, int split, int j0, float* lds) {
   typedef typename Elem<XT>::T T;
+  typedef ShrinkLds<XT, JB> L;
   constexpr int V = Elem<XT>::kVec, kStep = Elem<XT>::kStep;
+  constexpr int D = NRB == 1 && !TURNED ? 4 : 2;  // steps in flight
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t slot0 = int64_t(kTileRows) * t;
+  const T* s0 = static_cast<const T*>(a.s) + tile.adapter * a.s_adapter;
   const T* xr[NRB];
-  const T* sr[JB];
-  bool jlive[JB];
 #pragma unroll
   for (int b = 0; b < NRB; ++b) {
     const int i = 16 * b + i16;
@@ -39,240 +67,225 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
     const int row = plan_row(a.rows, slot0 + (i < tile.count ? i : 0));
     xr[b] = static_cast<const T*>(a.x) + int64_t(row) * a.ldx + V * g;
   }
+  const T* sr[JB];
+  bool jlive[JB];
 #pragma unroll
   for (int b = 0; b < JB; ++b) {
     const int j = j0 + 16 * b + i16;
     jlive[b] = j < a.r;
-    sr[b] = static_cast<const T*>(a.s) + tile.adapter * a.s_adapter + int64_t(jlive[b] ? j : 0) * a.ld_s + V * g;
+    if constexpr (!TURNED) sr[b] = s0 + int64_t(jlive[b] ? j : 0) * a.K + V * g;
+  }
+  // TURNED: a step's pieces of V values.  Up to 64 ranks lie end to end in LDS as in memory;
+  // of more, this rank block's 64 of each row.  Lanes without a piece repeat the first and
+  // put it past the step.
+  const int pitch = a.r <= 64 ? a.r : 64;
+  T* turn = reinterpret_cast<T*>(lds) + wave * L::kTurn;
+  int put[JB];
+  if constexpr (TURNED) {
+#pragma unroll
+    for (int b = 0; b < JB; ++b) {
+      const int f = V * (64 * b + lane);
+      const bool on = f < kStep * pitch && (a.r <= 64 || j0 + f % 64 < a.r);
+      put[b] = on ? f + f / (V * pitch) * L::kGap : L::kTurn - V;
+      sr[b] = s0 + (!on ? 0 : a.r <= 64 ? f : (f / 64) * a.r + j0 + f % 64);
+    }
   }
   f32x4 acc[NRB][JB];
 #pragma unroll
   for (int b = 0; b < NRB; ++b)
 #pragma unroll
     for (int j = 0; j < JB; ++j) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int64_t per = a.k_per_split / kMlWaves;
+  const int64_t per = a.k_per_split / kShWaves;
   const int64_t kb = split * a.k_per_split + wave * per;
   const int64_t ke = std::min<int64_t>(kb + per, a.K);
-  // whole steps, the next one's loads in flight over this one's products
-  auto load = [&](u32x4 (&x)[NRB], u32x4 (&s)[JB], int64_t k) {
+  u32x4 x[D][NRB], s[D][JB];
+  auto load = [&](u32x4 (&xv)[NRB], u32x4 (&sv)[JB], int64_t k) {
 #pragma unroll
-    for (int b = 0; b < NRB; ++b) x[b] = load16_any(xr[b] + k);
-#pragma unroll
-    for (int j = 0; j < JB; ++j) s[j] = load16_any(sr[j] + k);
-  };
-  auto products = [&](const u32x4 (&x)[NRB], const u32x4 (&s)[JB]) {
+    for (int b = 0; b < NRB; ++b) xv[b] = load16_any(xr[b] + k);
 #pragma unroll
     for (int j = 0; j < JB; ++j) {
-      const u32x4 f = jlive[j] ? s[j] : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int b = 0; b < NRB; ++b) acc[b][j] = mma<XT>(x[b], f, acc[b][j]);
+      sv[j] = load16_any(sr[j] + (TURNED ? k * a.r : k));
     }
   };
-  int64_t k = kb;
-  if (k + kStep <= ke) {
-    u32x4 x0[NRB], s0[JB], x1[NRB], s1[JB];
-    load(x0, s0, k);
-    for (;;) {
-      const int64_t k1 = k + kStep, k2 = k1 + kStep;
-      const bool more1 = k1 + kStep <= ke, more2 = k2 + kStep <= ke;
-      if (more1) load(x1, s1, k1);
-      products(x0, s0);
-      k = k1;
-      if (!more1) break;
-      if (more2) load(x0, s0, k2);
-      products(x1, s1);
-      k = k2;
-      if (!more2) break;
+  auto products = [&](const u32x4 (&xv)[NRB], const u32x4 (&sv)[JB]) {
+    if constexpr (TURNED) {
+#pragma unroll
+      for (int j = 0; j < JB; ++j) store16_any(turn + put[j], sv[j]);
+      __builtin_amdgcn_wave_barrier();
     }
-  }
-  if (k < ke) {  // the end of the rows
-    u32x4 x[NRB], s[JB];
 #pragma unroll
-    for (int b = 0; b < NRB; ++b) x[b] = load16_part<XT>(xr[b] + k, ke - k - V * g);
+    for (int j = 0; j < JB; ++j) {
+      u32x4 f;
+      if constexpr (TURNED) {
+        const T* p = turn + g * (V * pitch + L::kGap) + 16 * j + i16;
 #pragma unroll
-    for (int j = 0; j < JB; ++j) s[j] = load16_part<XT>(sr[j] + k, ke - k - V * g);
-    products(x, s);
-  }
-  // waves summed as (0 + 2) + (1 + 3); register q of lane (i, g) is row 4 g + q, rank i
-  constexpr int kPitch = 16 * JB + 1;
-  auto at = [&](int w, int b, int j, int q) -> float& {
-    return red[(w * 16 * NRB + 16 * b + 4 * g + q) * kPitch + 16 * j + i16];
-  };
-  if (wave >= 2) {
-#pragma unroll
-    for (int b = 0; b < NRB; ++b)
-#pragma unroll
-      for (int j = 0; j < JB; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) at(wave - 2, b, j, q) = acc[b][j][q];
-  }
-  __syncthreads();
-  if (wave < 2) {
-#pragma unroll
-    for (int b = 0; b < NRB; ++b)
-#pragma unroll
-      for (int j = 0; j < JB; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          acc[b][j][q] = __fadd_rn(acc[b][j][q], at(wave, b, j, q));
-          if (wave == 1) at(1, b, j, q) = acc[b][j][q];
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (XT == RQ_DTYPE_F32) f[e] = f2u(p[e * pitch]);
+          else f[e] = uint32_t(p[2 * e * pitch]) | uint32_t(p[(2 * e + 1) * pitch]) << 16;
         }
-  }
-  __syncthreads();
-  if (wave == 0) {
-    float* out = a.part + (int64_t(split) * a.rows.slots() + slot0) * a.r16 + j0;
-#pragma unroll
-    for (int b = 0; b < NRB; ++b)
-#pragma unroll
-      for (int j = 0; j < JB; ++j) {
-        if (j0 + 16 * j >= a.r16) continue;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          out[int64_t(16 * b + 4 * g + q) * a.r16 + 16 * j + i16] = __fadd_rn(acc[b][j][q], at(1, b, j, q));
+      } else {
+        f = sv[j];
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = jlive[j] ? f[e] : 0u;
+#pragma unroll
+      for (int b = 0; b < NRB; ++b) acc[b][j] = mma<XT>(xv[b], f, acc[b][j]);
+      if constexpr (TURNED) __builtin_amdgcn_sched_barrier(0);  // one rank block's reads at a time in registers
+    }
+    __builtin_amdgcn_wave_barrier();  // TURNED: the next step's copy comes after these reads
+  };
+  int64_t steps = ke > kb ? (ke - kb) / kStep : 0;
+  // more than 64 ranks: the factor's last rows are read with their ends in view
+  if (TURNED && a.r > 64 && steps > 0 && kb + steps * kStep == a.K) --steps;
+  int64_t k = kb, left = steps;
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (d < steps) load(x[d], s[d], kb + d * kStep);
+#pragma unroll 1
+  for (; left >= 2 * D; left -= D, k += D * kStep) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      products(x[d], s[d]);
+      load(x[d], s[d], k + (D + d) * kStep);
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < 2 * D - 1; ++d) {
+    if (d >= left) break;
+    products(x[d % D], s[d % D]);
+    if (d + D < left) load(x[d % D], s[d % D], k + (D + d) * kStep);
+  }
+  k = kb + steps * kStep;
+  if (k < ke) {  // the end of the rows
+#pragma unroll
+    for (int b = 0; b < NRB; ++b) x[0][b] = load16_part<XT>(xr[b] + k, ke - k - V * g);
+#pragma unroll
+    for (int j = 0; j < JB; ++j) {
+      if constexpr (TURNED) s[0][j] = load16_part<XT>(sr[j] + k * a.r, (a.K - k) * a.r - (sr[j] - s0));
+      else s[0][j] = load16_part<XT>(sr[j] + k, ke - k - V * g);
+    }
+    products(x[0], s[0]);
+  }
+  // register q of lane (i, g) is row 4 g + q, rank i
+  float* out = a.part + (int64_t(split) * a.rows.slots() + slot0) * a.rp + j0;
+  const int ranks = std::min(16 * JB, a.rp - j0);
+#pragma unroll
+  for (int b = 0; b < NRB; ++b) {
+    __syncthreads();  // the turned steps' and the last block's reads are done
+#pragma unroll
+    for (int j = 0; j < JB; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) lds[(wave * 16 + 4 * g + q) * L::kPitch + 16 * j + i16] = acc[b][j][q];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * ranks; i += kShThreads) {
+      const int row = i / ranks, j = i - row * ranks;
+      float v = lds[row * L::kPitch + j];
+#pragma unroll
+      for (int w = 1; w < kShWaves; ++w) v = __fadd_rn(v, lds[(w * 16 + row) * L::kPitch + j]);
+      out[int64_t(16 * b + row) * a.rp + j] = v;
+    }
   }
 }
 
-template <int XT, int JB>
-__global__ __launch_bounds__(kMlThreads) void shrink_kernel(ShrinkArgs a) {
-  __shared__ float red[2 * 64 * (16 * JB + 1)];
+template <int XT, int JB, bool TURNED>
+__global__ __launch_bounds__(kShThreads) void shrink_kernel(ShrinkArgs a) {
+  typedef ShrinkLds<XT, JB> L;
+  __shared__ float lds[TURNED && L::kTurnFloats > L::kRedFloats ? L::kTurnFloats : L::kRedFloats];
   const int t = int(blockIdx.x % unsigned(a.rows.T)), split = int(blockIdx.x / unsigned(a.rows.T));
   const int j0 = 16 * JB * int(blockIdx.y);
   const Tile tile = plan_tile(a.rows, t);
   if (tile.count == 0 || tile.adapter < 0) return;
-  if (tile.count <= 16) shrink_body<XT, 1, JB>(a, tile, t, split, j0, red);
-  else if (tile.count <= 32) shrink_body<XT, 2, JB>(a, tile, t, split, j0, red);
-  else shrink_body<XT, 4, JB>(a, tile, t, split, j0, red);
+  if (tile.count <= 16) shrink_body<XT, 1, JB, TURNED>(a, tile, t, split, j0, lds);
+  else if (tile.count <= 32) shrink_body<XT, 2, JB, TURNED>(a, tile, t, split, j0, lds);
+  else shrink_body<XT, 4, JB, TURNED>(a, tile, t, split, j0, lds);
 }
 
-// About four workgroups a compute unit, each wave with at least four steps.
+// About two workgroups a compute unit, each wave with at least four steps.
 void plan_shrink(int64_t T, int64_t K, int step, int cus, int* splits, int64_t* per) {
-  const int64_t unit = int64_t(step) * kMlWaves;
-  int64_t s = ceil_div(4 * cus, std::max<int64_t>(T, 1));
+  const int64_t unit = int64_t(step) * kShWaves;
+  int64_t s = ceil_div(2 * cus, std::max<int64_t>(T, 1));
   s = std::min(s, std::max<int64_t>(K / (4 * unit), 1));
-  s = std::min<int64_t>(std::max<int64_t>(s, 1), 16);
+  s = std::min<int64_t>(std::max<int64_t>(s, 1), 8);
   *per = ceil_div(ceil_div(K, s), unit) * unit;
   *splits = int(ceil_div(K, *per));
 }
 
-template <int XT>
+template <int XT, bool TURNED>
 int run_shrink(const ShrinkArgs& a, hipStream_t stream) {
-  const int jb = a.r16 <= 16 ? 1 : (a.r16 <= 32 ? 2 : 4);
-  if (int64_t(a.rows.T) * a.splits > kMaxThreads1D / kMlThreads) return RQ_ERR_UNSUPPORTED;
-  const dim3 grid(unsigned(int64_t(a.rows.T) * a.splits), unsigned(ceil_div(a.r16, 16 * jb)));
-  if (jb == 1) shrink_kernel<XT, 1><<<grid, kMlThreads, 0, stream>>>(a);
-  else if (jb == 2) shrink_kernel<XT, 2><<<grid, kMlThreads, 0, stream>>>(a);
-  else shrink_kernel<XT, 4><<<grid, kMlThreads, 0, stream>>>(a);
+  const int jb = a.rp <= 16 ? 1 : (a.rp <= 32 ? 2 : 4);
+  if (int64_t(a.rows.T) * a.splits > kMaxThreads1D / kShThreads) return RQ_ERR_UNSUPPORTED;
+  const dim3 grid(unsigned(int64_t(a.rows.T) * a.splits), unsigned(ceil_div(a.rp, 16 * jb)));
+  if (jb == 1) shrink_kernel<XT, 1, TURNED><<<grid, kShThreads, 0, stream>>>(a);
+  else if (jb == 2) shrink_kernel<XT, 2, TURNED><<<grid, kShThreads, 0, stream>>>(a);
+  else shrink_kernel<XT, 4, TURNED><<<grid, kShThreads, 0, stream>>>(a);
   return rq_check_launch();
 }
 
-// ---- finish ---------------------------------------------------------------------
-// A thread takes eight slots of one rank.  Slots of a tile past its rows get zeros:
-// the row sums read them.
-template <int XT>
-__global__ __launch_bounds__(kMlThreads) void finish_kernel(FinishArgs a, unsigned per_job) {
-  typedef typename Elem<XT>::T T;
-  const int which = int(blockIdx.x / per_job);
-  const FinishJob& J = a.job[which];
-  const int64_t i = int64_t(blockIdx.x % per_job) * kMlThreads + threadIdx.x;
-  const int64_t s8 = i / a.r16;
-  const int j = int(i - s8 * a.r16);
-  const int64_t slots = a.rows.slots(), s0 = 8 * s8;
-  if (s0 >= slots) return;
-  const int t = int(s0 / kTileRows);
-  const Tile tile = plan_tile(a.rows, t);
-  if (tile.count == 0 || tile.adapter < 0) return;
-  const int live = tile.count - int(s0 - int64_t(kTileRows) * t);  // of these slots
-  float v[8];
+// Sum over the splits, in order, of four adjacent ranks of a slot.
+__device__ __forceinline__ f32x4 split_sum4(const float* p, int splits, int64_t stride) {
+  f32x4 v = *reinterpret_cast<const f32x4*>(p);
+  for (int k = 1; k < splits; k += 4) {
+    f32x4 q[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-  for (int k = 0; k < J.splits; ++k) {
+    for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const f32x4*>(p + (k + i < splits ? k + i : 0) * stride);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < live) v[e] = __fadd_rn(v[e], J.part[(int64_t(k) * slots + s0 + e) * a.r16 + j]);
+    for (int i = 0; i < 4; ++i)
+      if (k + i < splits)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __fadd_rn(v[e], q[i][e]);
   }
-  if (J.sum) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < live) J.sum[(s0 + e) * a.r16 + j] = v[e];
-  }
-  if (J.scaled) {
-    const float s = a.scaling[tile.adapter];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < live ? __fmul_rn(v[e], s) : 0.0f;
-  }
-  if constexpr (XT == RQ_DTYPE_F32) {
-    if (J.op) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) static_cast<float*>(J.op)[(s0 + e) * a.r16 + j] = v[e];
-    }
-    if (J.opt) {
-      f32x4* o = reinterpret_cast<f32x4*>(static_cast<float*>(J.opt) + int64_t(j) * slots + s0);
-      o[0] = f32x4{v[0], v[1], v[2], v[3]};
-      o[1] = f32x4{v[4], v[5], v[6], v[7]};
-    }
-  } else {
-    uint32_t hi[8], lo[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      hi[e] = to_x16<XT>(v[e]);
-      const float h = from_x16<XT>(hi[e]);
-      // an infinity has no second part (inf - inf)
-      lo[e] = to_x16<XT>(fabsf(h) == __builtin_inff() ? 0.0f : v[e] - h);
-    }
-    if (J.op) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        T* o = static_cast<T*>(J.op) + (s0 + e) * (2 * a.r16);
-        o[j] = T(hi[e]);
-        o[a.r16 + j] = T(lo[e]);
-      }
-    }
-    if (J.opt) {
-      T* o = static_cast<T*>(J.opt) + int64_t(j) * slots + s0;
-      *reinterpret_cast<u32x4*>(o) =
-          u32x4{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, hi[4] | hi[5] << 16, hi[6] | hi[7] << 16};
-      *reinterpret_cast<u32x4*>(o + int64_t(a.r16) * slots) =
-          u32x4{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16, lo[4] | lo[5] << 16, lo[6] | lo[7] << 16};
-    }
-  }
-}
-
-template <int XT>
-int run_finish(const FinishArgs& a, hipStream_t stream) {
-  const int64_t per = ceil_div(a.rows.slots() / 8 * a.r16, kMlThreads);
-  if (per * a.jobs > kMaxThreads1D / kMlThreads) return RQ_ERR_UNSUPPORTED;
-  finish_kernel<XT><<<unsigned(per * a.jobs), kMlThreads, 0, stream>>>(a, unsigned(per));
-  return rq_check_launch();
+  return v;
 }
 
 // ---- expand ---------------------------------------------------------------------
-// A wave takes 16 kVec columns of half a tile (two 16-row blocks).  The factor is the
-// A operand and the slots the B operand, so that a result register holds columns; the
-// operand row i of product c is column kVec i + c, so that a lane ends with kVec
-// adjacent columns for each of its four registers: whole 16-byte pieces of a row,
+// A workgroup takes half a tile (two 16-row blocks): it sums the splits of its slots and
+// keeps them in LDS as operands, and its waves walk over columns, 16 kVec of them a step.
+// The factor is the A operand and the slots the B operand, so that a result register holds
+// columns; the operand row i of product c is column kVec i + c, so that a lane ends with
+// kVec adjacent columns for each of its four registers: whole 16-byte pieces of a row,
 // 256 bytes of it by the four lane groups.
-//
-// The contraction runs over the hi ranks, then the lo ranks, 16 at a time in rank
-// order: r16 is a multiple of 16, so a 32-rank step of 16-bit operands is two ranks
-// blocks, hi and lo of the same 16 when r16 = 16.
-// kVec ranks from `v` (of hi | lo) on for each of the kVec columns, lane group g at
-// V g within the step
-template <int XT, bool FACTOR_ROWS>
-__device__ __forceinline__ void load_factor(u32x4 (&f)[Elem<XT>::kVec], const typename Elem<XT>::T* s, int64_t ld,
-                                            int64_t C, int64_t col, int r, int j) {
+constexpr int kExpandBlocks = 2;  // 16-row blocks of a workgroup
+
+// kVec ranks from j on for each of kVec columns from `col` on.  FULL: all columns exist, and
+// reading past a row's last rank stays in the factor.
+template <int XT, bool FACTOR_ROWS, bool FULL>
+__device__ __forceinline__ void load_factor(u32x4 (&f)[Elem<XT>::kVec], const typename Elem<XT>::T* s, int64_t C, int64_t col,
+                                            int r, int j) {
   constexpr int V = Elem<XT>::kVec;
   const u32x4 zero = u32x4{0u, 0u, 0u, 0u};
   if constexpr (FACTOR_ROWS) {
     // column c's ranks j .. j + V - 1 are adjacent
+    if constexpr (FULL) {
 #pragma unroll
-    for (int c = 0; c < V; ++c)
-      f[c] = col + c < C && j < r ? load16_part<XT>(s + (col + c) * ld + j, r - j) : zero;
+      for (int c = 0; c < V; ++c) f[c] = load16_any(s + (col + c) * r + (j < r ? j : 0));
+      if (j + V > r) {
+        u32x4 keep;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (XT == RQ_DTYPE_F32) keep[e] = j + e < r ? ~0u : 0u;
+          else keep[e] = j + 2 * e + 1 < r ? ~0u : (j + 2 * e < r ? 0xFFFFu : 0u);
+        }
+#pragma unroll
+        for (int c = 0; c < V; ++c) f[c] &= keep;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < V; ++c) f[c] = col + c < C && j < r ? load16_part<XT>(s + (col + c) * r + j, r - j) : zero;
+    }
   } else {
     // rank j + e's columns are adjacent: transpose V x V values
     u32x4 row[V];
+    if constexpr (FULL) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) row[e] = j + e < r ? load16_part<XT>(s + (j + e) * ld + col, C - col) : zero;
+      for (int e = 0; e < V; ++e) row[e] = load16_any(s + int64_t(j + e < r ? j + e : 0) * C + col);
+      if (j + V > r) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) row[e] = j + e < r ? row[e] : zero;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) row[e] = j + e < r ? load16_part<XT>(s + int64_t(j + e) * C + col, C - col) : zero;
+    }
     if constexpr (XT == RQ_DTYPE_F32) {
 #pragma unroll
       for (int c = 0; c < V; ++c)
@@ -288,83 +301,226 @@ __device__ __forceinline__ void load_factor(u32x4 (&f)[Elem<XT>::kVec], const ty
   }
 }
 
-constexpr int kExpandBlocks = 2;  // 16-row blocks of a workgroup
+template <int XT>
+struct ExpandWave {
+  const typename Elem<XT>::T* s;     // the adapter's factor, or nullptr: none
+  const typename Elem<XT>::T* op;    // the slots' operands in LDS
+  int pitch;
+  int blocks;                        // 16-row blocks in use
+  float scale;
+  bool based;                        // there is a base
+  int64_t base[kExpandBlocks], out[kExpandBlocks];  // this lane's row (past the tile's last: the first)
+  bool on[kExpandBlocks];            // not past it
+};
 
-template <int XT, bool FACTOR_ROWS>
-__global__ __launch_bounds__(kMlThreads) void expand_kernel(ExpandArgs a) {
-  typedef typename Elem<XT>::T T;
+template <int XT, bool FACTOR_ROWS, bool FULL>
+__device__ __forceinline__ void expand_step(const ExpandArgs& a, const ExpandWave<XT>& w, int64_t c0) {
   constexpr int V = Elem<XT>::kVec, kStep = Elem<XT>::kStep;
-  constexpr int kParts = kTileRows / (16 * kExpandBlocks);
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
+  const int64_t col = c0 + V * i16;
+  // one step of ranks: the factor's piece serves both blocks.  (16 ranks of 16 bits: lane
+  // groups 2 and 3 take the lo parts, of the same ranks as groups 0 and 1.)
+  const bool one = XT == RQ_DTYPE_F32 ? a.rp == kStep : a.rp <= kStep;
+  u32x4 f[V];
+  if (w.s && one) load_factor<XT, FACTOR_ROWS, FULL>(f, w.s, a.C, col, a.r, a.rp < kStep ? V * (g & 1) : V * g);
+#pragma unroll
+  for (int b = 0; b < kExpandBlocks; ++b) {
+    if (b >= w.blocks) break;
+    u32x4 base[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t c = c0 + V * (4 * g + q);
+      const typename Elem<XT>::T* p = static_cast<const typename Elem<XT>::T*>(a.base) + w.base[b] + c;
+      base[q] = u32x4{0u, 0u, 0u, 0u};
+      if (w.based) base[q] = FULL ? load16_any(p) : load16_part<XT>(p, a.C - c);
+    }
+    f32x4 acc[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (w.s) {
+      const typename Elem<XT>::T* op = w.op + (16 * b + i16) * w.pitch + V * g;
+#pragma unroll 1
+      for (int j = 0; j < a.rp; j += kStep) {
+        if (!one) load_factor<XT, FACTOR_ROWS, FULL>(f, w.s, a.C, col, a.r, j + V * g);
+        const u32x4 hi = *reinterpret_cast<const u32x4*>(op + j);
+#pragma unroll
+        for (int c = 0; c < V; ++c) acc[c] = mma<XT>(f[c], hi, acc[c]);
+        if (XT != RQ_DTYPE_F32 && a.rp >= kStep) {
+          const u32x4 lo = *reinterpret_cast<const u32x4*>(op + a.rp + j);
+#pragma unroll
+          for (int c = 0; c < V; ++c) acc[c] = mma<XT>(f[c], lo, acc[c]);
+        }
+      }
+    }
+    if (!w.on[b]) continue;
+    typename Elem<XT>::T* out = static_cast<typename Elem<XT>::T*>(a.out) + w.out[b];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t c = c0 + V * (4 * g + q);
+      float v[V];
+      unpack16<XT>(base[q], v);
+      if (w.s) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = __fadd_rn(v[e], __fmul_rn(w.scale, acc[e][q]));
+      }
+      if constexpr (FULL) store16_any(out + c, pack16<XT>(v));
+      else store16_part<XT>(out + c, v, a.C - c);
+    }
+  }
+}
+
+// Whether the wave's columns from c0 on all exist, and reading V ranks at the last of them
+// stays in the factor.
+template <int XT, bool FACTOR_ROWS>
+__host__ __device__ __forceinline__ bool expand_full(const ExpandArgs& a, int64_t c0) {
+  constexpr int V = Elem<XT>::kVec;
+  const int64_t end = c0 + 16 * V;
+  return end <= a.C && (!FACTOR_ROWS || a.r % V == 0 || end * a.r + V <= a.C * a.r);
+}
+
+// EDGES: there are columns that a whole wave does not fill (their code takes registers
+// that the others would miss: two waves a SIMD instead of three).
+template <int XT, bool FACTOR_ROWS, bool EDGES>
+__global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(EDGES ? 2 : 3))) void expand_kernel(ExpandArgs a) {
+  typedef typename Elem<XT>::T T;
+  constexpr int V = Elem<XT>::kVec;
+  constexpr int kParts = kTileRows / (16 * kExpandBlocks);
+  extern __shared__ uint32_t lds[];
+  const int lane = threadIdx.x & 63, i16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int chunk = int(blockIdx.x % unsigned(a.chunks));
   const unsigned rest = blockIdx.x / unsigned(a.chunks);
   const int t = int(rest / kParts), part = int(rest % kParts);
   const Tile tile = plan_tile(a.rows, t);
-  const int first = 16 * kExpandBlocks * part;
-  if (first >= tile.count) return;
+  const int first = 16 * kExpandBlocks * part, live = tile.count - first;
+  if (live <= 0) return;
   if (tile.adapter < 0 && a.base == a.out && a.ld_base == a.ld_out) return;  // in place, nothing to add
-  const int64_t c0 = (int64_t(chunk) * kMlWaves + wave) * (16 * V);
-  if (c0 >= a.C) return;
   const int64_t slot0 = int64_t(kTileRows) * t + first;
-  const int64_t col = c0 + V * i16;
-  f32x4 acc[kExpandBlocks][V];
+  ExpandWave<XT> w;
+  w.blocks = live > 16 ? 2 : 1;
+  w.s = nullptr;
+  w.scale = 0.0f;
+  w.based = a.base != nullptr;
+  T* op = reinterpret_cast<T*>(lds);
+  w.op = op;
+  w.pitch = (XT == RQ_DTYPE_F32 ? a.rp : 2 * a.rp) + V;
 #pragma unroll
-  for (int b = 0; b < kExpandBlocks; ++b)
-#pragma unroll
-    for (int c = 0; c < V; ++c) acc[b][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int b = 0; b < kExpandBlocks; ++b) {
+    const int i = 16 * b + i16;
+    w.on[b] = i < live;
+    const int64_t row = plan_row(a.rows, slot0 + (w.on[b] ? i : 0));
+    w.base[b] = row * a.ld_base;
+    w.out[b] = row * a.ld_out;
+  }
   if (tile.adapter >= 0) {
-    const T* s = static_cast<const T*>(a.s) + tile.adapter * a.s_adapter;
-    const int width = XT == RQ_DTYPE_F32 ? a.r16 : 2 * a.r16;
-    const T* op = static_cast<const T*>(a.op) + slot0 * width;
-    for (int v = 0; v < width; v += kStep) {
-      const int at = v + V * g;
-      const int j = at >= a.r16 ? at - a.r16 : at;
-      u32x4 f[V];
-      load_factor<XT, FACTOR_ROWS>(f, s, a.ld_s, a.C, col, a.r, j);
+    w.s = static_cast<const T*>(a.s) + tile.adapter * a.s_adapter;
+    w.scale = a.scaling[tile.adapter];
+    const int quads = a.rp / 4, rows = 16 * w.blocks;
+    const int64_t stride = a.rows.slots() * a.rp;
+    for (int i = threadIdx.x; i < rows * quads; i += kMlThreads) {
+      const int row = i / quads, j = 4 * (i - row * quads);
+      const f32x4 v = split_sum4(a.part + (slot0 + row) * a.rp + j, a.splits, stride);
+      if (a.sum && chunk == 0) *reinterpret_cast<f32x4*>(a.sum + (slot0 + row) * a.rp + j) = v;
+      T* o = op + row * w.pitch + j;
+      if constexpr (XT == RQ_DTYPE_F32) {
+        *reinterpret_cast<f32x4*>(o) = v;
+      } else {
+        uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int b = 0; b < kExpandBlocks; ++b) {
-        if (first + 16 * b >= tile.count) break;
-        const u32x4 u = *reinterpret_cast<const u32x4*>(op + int64_t(16 * b + i16) * width + at);
-#pragma unroll
-        for (int c = 0; c < V; ++c) acc[b][c] = mma<XT>(f[c], u, acc[b][c]);
+        for (int e = 0; e < 4; ++e) split16<XT>(v[e], hi[e], lo[e]);
+        *reinterpret_cast<u32x2*>(o) = u32x2{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16};
+        *reinterpret_cast<u32x2*>(o + a.rp) = u32x2{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16};
       }
     }
   }
-  const float scale = a.scaling && tile.adapter >= 0 ? a.scaling[tile.adapter] : 1.0f;
-#pragma unroll
-  for (int b = 0; b < kExpandBlocks; ++b) {
-    const int i = first + 16 * b + i16;
-    if (i >= tile.count) continue;
-    const int64_t row = plan_row(a.rows, int64_t(kTileRows) * t + i);
-    const T* base = static_cast<const T*>(a.base) + (a.base ? row * a.ld_base : 0);
-    T* out = static_cast<T*>(a.out) + row * a.ld_out;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t c = c0 + V * (4 * g + q);
-      if (c >= a.C) continue;
-      float f[V];
-      if (a.base) {
-        unpack16<XT>(load16_part<XT>(base + c, a.C - c), f);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = 0.0f;
+  __syncthreads();
+#pragma unroll 1
+  for (int it = 0; it < a.iters; ++it) {
+    const int64_t c0 = ((int64_t(chunk) * a.iters + it) * kMlWaves + wave) * (16 * V);
+    if (c0 >= a.C) return;
+    if constexpr (EDGES) {
+      if (!expand_full<XT, FACTOR_ROWS>(a, c0)) {
+        expand_step<XT, FACTOR_ROWS, false>(a, w, c0);
+        continue;
       }
-      if (tile.adapter >= 0) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = __fadd_rn(f[e], __fmul_rn(scale, acc[b][e][q]));
-      }
-      store16_part<XT>(out + c, f, a.C - c);
     }
+    expand_step<XT, FACTOR_ROWS, true>(a, w, c0);
   }
 }
 
 template <int XT, bool FACTOR_ROWS>
-int run_expand(ExpandArgs a, hipStream_t stream) {
-  a.chunks = int(ceil_div(a.C, kMlWaves * expand_cols<XT>()));
-  const int64_t blocks = int64_t(a.rows.T) * (kTileRows / (16 * kExpandBlocks)) * a.chunks;
-  if (blocks > kMaxThreads1D / kMlThreads) return RQ_ERR_UNSUPPORTED;
-  expand_kernel<XT, FACTOR_ROWS><<<unsigned(blocks), kMlThreads, 0, stream>>>(a);
+int run_expand(ExpandArgs a, int cus, hipStream_t stream) {
+  const int64_t cols = int64_t(kMlWaves) * 16 * Elem<XT>::kVec, steps = ceil_div(a.C, cols);
+  const int64_t halves = int64_t(a.rows.T) * (kTileRows / (16 * kExpandBlocks));
+  // steps of a workgroup: as many as leave eight workgroups a compute unit
+  a.iters = int(std::max<int64_t>(1, std::min<int64_t>(8, halves * steps / (8 * cus))));
+  a.chunks = int(ceil_div(steps, a.iters));
+  if (halves * a.chunks > kMaxThreads1D / kMlThreads) return RQ_ERR_UNSUPPORTED;
+  const size_t bytes = size_t(16 * kExpandBlocks) * (a.rp * 4 + 16);
+  const bool whole = a.C % (16 * Elem<XT>::kVec) == 0 && expand_full<XT, FACTOR_ROWS>(a, a.C - 16 * Elem<XT>::kVec);
+  const unsigned grid = unsigned(halves * a.chunks);
+  if (whole) expand_kernel<XT, FACTOR_ROWS, false><<<grid, kMlThreads, bytes, stream>>>(a);
+  else expand_kernel<XT, FACTOR_ROWS, true><<<grid, kMlThreads, bytes, stream>>>(a);
+  return rq_check_launch();
+}
+
+// ---- finish ---------------------------------------------------------------------
+// The splits' sum times the adapter's scaling, as rank-major operands of the row sums.  A
+// thread takes eight slots of one rank.  Slots of a tile past its rows get zeros.
+template <int XT>
+__global__ __launch_bounds__(kMlThreads) void finish_kernel(FinishArgs a, unsigned per_job) {
+  typedef typename Elem<XT>::T T;
+  const int which = int(blockIdx.x / per_job);
+  const FinishJob& J = a.job[which];
+  const unsigned i = blockIdx.x % per_job * kMlThreads + threadIdx.x;
+  const int64_t s0 = 8 * int64_t(i / unsigned(a.rp));
+  const int j = int(i % unsigned(a.rp));
+  const int64_t slots = a.rows.slots();
+  if (s0 >= slots) return;
+  const int t = int(s0 / kTileRows);
+  const Tile tile = plan_tile(a.rows, t);
+  if (tile.count == 0 || tile.adapter < 0) return;
+  const int live = tile.count - int(s0 - int64_t(kTileRows) * t);  // of these slots
+  const float scale = a.scaling[tile.adapter];
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+  if (live > 0) {
+    for (int k0 = 0; k0 < J.splits; k0 += 4) {
+      float p[4][8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          p[k][e] = J.part[(int64_t(k0 + k < J.splits ? k0 + k : 0) * slots + s0 + (e < live ? e : 0)) * a.rp + j];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (k0 + k < J.splits) v[e] = __fadd_rn(v[e], p[k][e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = e < live ? __fmul_rn(v[e], scale) : 0.0f;
+  T* o = static_cast<T*>(J.opt) + int64_t(j) * slots + s0;
+  if constexpr (XT == RQ_DTYPE_F32) {
+    reinterpret_cast<f32x4*>(o)[0] = f32x4{v[0], v[1], v[2], v[3]};
+    reinterpret_cast<f32x4*>(o)[1] = f32x4{v[4], v[5], v[6], v[7]};
+  } else {
+    uint32_t hi[8], lo[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) split16<XT>(v[e], hi[e], lo[e]);
+    *reinterpret_cast<u32x4*>(o) = u32x4{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, hi[4] | hi[5] << 16, hi[6] | hi[7] << 16};
+    *reinterpret_cast<u32x4*>(o + int64_t(a.rp) * slots) =
+        u32x4{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16, lo[4] | lo[5] << 16, lo[6] | lo[7] << 16};
+  }
+}
+
+template <int XT>
+int run_finish(const FinishArgs& a, hipStream_t stream) {
+  const int64_t per = ceil_div(a.rows.slots() / 8 * a.rp, kMlThreads);
+  if (per * a.jobs > kMaxThreads1D / kMlThreads) return RQ_ERR_UNSUPPORTED;
+  finish_kernel<XT><<<unsigned(per * a.jobs), kMlThreads, 0, stream>>>(a, unsigned(per));
   return rq_check_launch();
 }
 
@@ -372,257 +528,336 @@ int run_expand(ExpandArgs a, hipStream_t stream) {
 // D[c][j] = sum_m x[row m][c] u[m][j], the contraction over the slow index of x: lane
 // (i, g) loads CW columns of the eight rows of slots 8 g .. 8 g + 7, which byte permutes
 // turn into CW operand rows of eight consecutive slots (16-bit; fp32 values are operands
-// as they are).  A wave's step is 32 slots; the four waves take steps in turn and meet in
-// LDS.  Each column tile of a chunk is a workgroup.
+// as they are).  A wave walks over the rows of a chunk, 32 slots a step, with 16 CW
+// columns of its own; the next step's rows and operands are loaded over this one's
+// products.  A workgroup's four waves are adjacent columns, so that they share the
+// operands in the L1.
 template <int XT, int CW>
 struct ColPiece {
-  uint32_t d[XT == RQ_DTYPE_F32 ? CW : CW / 2];
+  static constexpr int kWords = XT == RQ_DTYPE_F32 ? CW : CW / 2;
+  uint32_t d[kWords];
 };
 
-template <int XT, int CW>
-__device__ __forceinline__ ColPiece<XT, CW> col_piece(const RowSumTask& T_, int64_t row, int64_t col) {
+// columns of a lane, by 16-rank blocks of a wave
+template <int XT>
+constexpr int rowsum_cw(int jb) {
+  return XT == RQ_DTYPE_F32 || jb > 2 ? 4 : 8;
+}
+
+// CODES: the rows are 8-bit codes with exponents.  FULL: all CW columns exist.
+template <int XT, int CW, bool CODES>
+struct RawPiece {
+  uint32_t d[CODES ? CW / 4 : ColPiece<XT, CW>::kWords];
+  uint32_t e;  // of codes
+};
+
+template <int XT, int CW, bool CODES>
+__device__ __forceinline__ RawPiece<XT, CW, CODES> raw_piece(const RowSumTask& K, int64_t row, int64_t col, bool full) {
   typedef typename Elem<XT>::T T;
-  constexpr int kWords = XT == RQ_DTYPE_F32 ? CW : CW / 2;
-  ColPiece<XT, CW> o;
-  if (T_.exps) {
-    const uint8_t* p = static_cast<const uint8_t*>(T_.src) + row * T_.ld + col;
-    const int e = T_.exps[row * (T_.ld / kAct8Block) + col / kAct8Block];
-    uint32_t w[CW / 4];
+  RawPiece<XT, CW, CODES> o;
+  if constexpr (CODES) {
+    const uint8_t* p = static_cast<const uint8_t*>(K.src) + row * K.ld + col;
+    o.e = K.exps[row * (K.ld / kAct8Block) + col / kAct8Block];
     if constexpr (CW == 8) {
       const u32x2 v = *reinterpret_cast<const u32x2*>(p);
-      w[0] = v.x;
-      w[1] = v.y;
-    } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
-#pragma unroll
-    for (int i = 0; i < CW / 4; ++i) {
-      if constexpr (XT == RQ_DTYPE_F32) {
-        o.d[4 * i] = f2u(act8_value<0>(w[i], e));
-        o.d[4 * i + 1] = f2u(act8_value<1>(w[i], e));
-        o.d[4 * i + 2] = f2u(act8_value<2>(w[i], e));
-        o.d[4 * i + 3] = f2u(act8_value<3>(w[i], e));
-      } else {
-        const u32x2 v = act8_pairs<XT>(w[i], e);
-        o.d[2 * i] = v.x;
-        o.d[2 * i + 1] = v.y;
-      }
-    }
-    return o;
-  }
-  const T* p = static_cast<const T*>(T_.src) + row * T_.ld + col;
-  if (col + CW <= T_.C) {
-    if constexpr (kWords == 4) {
-      const u32x4 v = load16_any(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o.d[i] = v[i];
-    } else {
-      const u32x2_any v = *reinterpret_cast<const u32x2_any*>(p);
       o.d[0] = v.x;
       o.d[1] = v.y;
+    } else {
+      o.d[0] = *reinterpret_cast<const uint32_t*>(p);
     }
   } else {
+    constexpr int kWords = ColPiece<XT, CW>::kWords;
+    const T* p = static_cast<const T*>(K.src) + row * K.ld + col;
+    if (full) {
+      if constexpr (kWords == 4) {
+        const u32x4 v = load16_any(p);
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      if constexpr (XT == RQ_DTYPE_F32) {
-        o.d[i] = col + i < T_.C ? f2u(p[i]) : 0u;
+        for (int i = 0; i < 4; ++i) o.d[i] = v[i];
       } else {
-        o.d[i] = (col + 2 * i < T_.C ? uint32_t(p[2 * i]) : 0u) | (col + 2 * i + 1 < T_.C ? uint32_t(p[2 * i + 1]) << 16 : 0u);
+        const u32x2_any v = *reinterpret_cast<const u32x2_any*>(p);
+        o.d[0] = v.x;
+        o.d[1] = v.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        if constexpr (XT == RQ_DTYPE_F32) {
+          o.d[i] = col + i < K.C ? f2u(p[i]) : 0u;
+        } else {
+          o.d[i] = (col + 2 * i < K.C ? uint32_t(p[2 * i]) : 0u) |
+                   (col + 2 * i + 1 < K.C ? uint32_t(p[2 * i + 1]) << 16 : 0u);
+        }
       }
     }
   }
   return o;
 }
 
-template <int XT, int JB>
-__global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(2))) void rowsum_kernel(RowSumArgs a) {
-  typedef typename Elem<XT>::T T;
-  constexpr int CW = rowsum_cw<XT>(JB), kCols = 16 * CW, kPitch = 16 * JB + 1;
-  constexpr int kWords = XT == RQ_DTYPE_F32 ? CW : CW / 2;
-  constexpr int kPlanes = XT == RQ_DTYPE_F32 ? 1 : 2;
-  __shared__ float red[2][kCols][kPitch];
-  const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int adapter = 0, t0, t1, slot = -1;
-  if (a.rows.p) {
-    if (int(blockIdx.y) >= a.rows.p[1]) return;
-    const int32_t* c = a.rows.p + a.rows.off_chunks() + 4 * int64_t(blockIdx.y);
-    adapter = c[0];
-    t0 = c[1];
-    t1 = c[2];
-    slot = c[3];
+template <int XT, int CW, bool CODES>
+__device__ __forceinline__ ColPiece<XT, CW> col_piece(const RawPiece<XT, CW, CODES>& r) {
+  ColPiece<XT, CW> o;
+  if constexpr (!CODES) {
+#pragma unroll
+    for (int i = 0; i < ColPiece<XT, CW>::kWords; ++i) o.d[i] = r.d[i];
   } else {
-    const int per = RowsPlan::chunk_tiles(a.rows.T);
-    t0 = per * int(blockIdx.y);
-    t1 = t0 + per < a.rows.T ? t0 + per : a.rows.T;
-    if (a.rows.C > 1) slot = int(blockIdx.y);
+#pragma unroll
+    for (int i = 0; i < CW / 4; ++i) {
+      if constexpr (XT == RQ_DTYPE_F32) {
+        o.d[4 * i] = f2u(act8_value<0>(r.d[i], int(r.e)));
+        o.d[4 * i + 1] = f2u(act8_value<1>(r.d[i], int(r.e)));
+        o.d[4 * i + 2] = f2u(act8_value<2>(r.d[i], int(r.e)));
+        o.d[4 * i + 3] = f2u(act8_value<3>(r.d[i], int(r.e)));
+      } else {
+        const u32x2 v = act8_pairs<XT>(r.d[i], int(r.e));
+        o.d[2 * i] = v.x;
+        o.d[2 * i + 1] = v.y;
+      }
+    }
   }
-  const int which = int(blockIdx.x) >= a.t[0].tiles ? 1 : 0;
-  const RowSumTask& K = a.t[which];
-  const int64_t c0 = int64_t(int(blockIdx.x) - (which ? a.t[0].tiles : 0)) * kCols;
-  const int j0 = 16 * JB * int(blockIdx.z);
-  const int64_t col = c0 + CW * i16;
-  const bool clive = col < K.C;
-  const int64_t slots = a.rows.slots();
+  return o;
+}
 
+struct RowSumChunk {
+  int adapter, t0, slot;
+  int64_t live;  // slots from the first of tile t0 on
+};
+
+template <int XT, int JB, bool CODES, bool RANK_MAJOR>
+__device__ __forceinline__ void rowsum_body(const RowSumArgs& a, const RowSumTask& K, const RowSumChunk& ch, int64_t c0, int j0) {
+  typedef typename Elem<XT>::T T;
+  constexpr int CW = rowsum_cw<XT>(JB);
+  constexpr int kWords = ColPiece<XT, CW>::kWords;
+  constexpr int kPlanes = XT == RQ_DTYPE_F32 ? 1 : 2;
+  constexpr int kOps = XT == RQ_DTYPE_F32 ? 2 : 1;  // 16-byte operands of eight slots
+  const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
+  const int64_t col = c0 + CW * i16;
+  const bool full = c0 + 16 * CW <= K.C;            // of the wave
+  const int64_t lcol = full || col < K.C ? col : 0;  // lanes past the end repeat column 0: their sums are not stored
+  const int64_t slots = a.rows.slots(), base = int64_t(kTileRows) * ch.t0;
+  const T* opt = static_cast<const T*>(K.opt) + int64_t(j0 + i16) * slots + base + 8 * g;
+
+  // D as columns x ranks (RANK_MAJOR), or as ranks x columns: a register quad is stored as it lies
   f32x4 acc[CW][JB];
 #pragma unroll
   for (int c = 0; c < CW; ++c)
 #pragma unroll
     for (int j = 0; j < JB; ++j) acc[c][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int step = wave; step < 2 * (t1 - t0); step += kMlWaves) {
-    const int t = t0 + (step >> 1);
-    const Tile tile = plan_tile(a.rows, t);
-    const int h = 32 * (step & 1);
-    if (h >= tile.count) continue;
-    const int64_t slot0 = int64_t(kTileRows) * t + h + 8 * g;
+  typedef RawPiece<XT, CW, CODES> Raw;
+  struct Ops {
+    u32x4 u[JB][kPlanes][kOps];
+  };
+  auto rows_of = [&](int (&r)[8], int64_t s) {  // slots base + s + 8 g ..; past the last: -1
+    if (a.rows.p) {
+      const int32_t* p = a.rows.p + a.rows.off_rows() + base + s + 8 * g;
+      const u32x4 lo = *reinterpret_cast<const u32x4*>(p), hi = *reinterpret_cast<const u32x4*>(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        r[e] = int(lo[e]);
+        r[4 + e] = int(hi[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int64_t m = base + s + 8 * g + e;
+        r[e] = m < a.rows.M ? int(m) : -1;
+      }
+    }
+  };
+  auto load = [&](Raw (&raw)[8], const int (&r)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) raw[e] = raw_piece<XT, CW, CODES>(K, r[e] < 0 ? 0 : r[e], lcol, full || lcol + CW <= K.C);
+  };
+  auto operands = [&](Ops& o, int64_t s) {
+#pragma unroll
+    for (int j = 0; j < JB; ++j)
+#pragma unroll
+      for (int p = 0; p < kPlanes; ++p)
+#pragma unroll
+        for (int k = 0; k < kOps; ++k)
+          o.u[j][p][k] = *reinterpret_cast<const u32x4*>(opt + (int64_t(p) * a.rp + 16 * j) * slots + s + 4 * k);
+  };
+  auto products = [&](const Raw (&raw)[8], const Ops& o, const int (&r)[8], bool last) {
     ColPiece<XT, CW> row[8];
-    // the loads first; rows past the tile's last repeat its first and count as zero
-    const int64_t lcol = clive ? col : 0;
-    int r[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = plan_row(a.rows, h + 8 * g + e < tile.count ? slot0 + e : int64_t(kTileRows) * t);
+    for (int e = 0; e < 8; ++e) row[e] = col_piece<XT, CW, CODES>(raw[e]);
+    if (last) {  // rows past the last count as zero
 #pragma unroll
-    for (int e = 0; e < 8; ++e) row[e] = col_piece<XT, CW>(K, r[e], lcol);
+      for (int e = 0; e < 8; ++e)
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+        for (int d = 0; d < kWords; ++d) row[e].d[d] = r[e] < 0 ? 0u : row[e].d[d];
+    }
+    if constexpr (XT == RQ_DTYPE_F32) {
 #pragma unroll
-      for (int d = 0; d < kWords; ++d)
-        if (!clive || h + 8 * g + e >= tile.count) row[e].d[d] = 0u;
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int c = 0; c < CW; ++c)
+#pragma unroll
+          for (int j = 0; j < JB; ++j) {
+            const float x = u2f(row[e].d[c]), u = u2f(o.u[j][0][e >> 2][e & 3]);
+            acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(RANK_MAJOR ? x : u, RANK_MAJOR ? u : x, acc[c][j], 0, 0, 0);
+          }
+    } else {
+#pragma unroll
+      for (int c = 0; c < CW; ++c) {
+        u32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[e] = __builtin_amdgcn_perm(row[2 * e + 1].d[c >> 1], row[2 * e].d[c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int p = 0; p < kPlanes; ++p)
+#pragma unroll
+          for (int j = 0; j < JB; ++j)
+            acc[c][j] = RANK_MAJOR ? mma<XT>(x, o.u[j][p][0], acc[c][j]) : mma<XT>(o.u[j][p][0], x, acc[c][j]);
+      }
+    }
+  };
+  const int64_t live = ch.live;
+  if (live > 0) {
+    // the next step's rows are known before its values are asked for; two to three waves a
+    // SIMD with eight loads each hide the memory's latency
+    int r0[8], r1[8];
+    rows_of(r0, 0);
+    for (int64_t s = 0; s < live; s += 32) {
+      Raw x[8];
+      Ops o;
+      load(x, r0);
+      operands(o, s);
+      if (s + 32 < live) rows_of(r1, s + 32);
+      products(x, o, r0, s + 32 > live);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r0[e] = r1[e];
+    }
+  }
+  const int64_t n = K.C * a.r;
+  float* part = ch.slot >= 0 ? a.part + ch.slot * a.part_size + K.part_off : nullptr;
+  T* out = static_cast<T*>(K.out) + ch.adapter * n;
+  if constexpr (RANK_MAJOR) {
+    // register q of lane (i, g): column CW (4 g + q) + c, rank i
 #pragma unroll
     for (int j = 0; j < JB; ++j) {
-      if (j0 + 16 * j >= a.r16) continue;
-      const T* u = static_cast<const T*>(K.opt) + int64_t(j0 + 16 * j + i16) * slots + slot0;
-      if constexpr (XT == RQ_DTYPE_F32) {
-        const f32x4 u0 = *reinterpret_cast<const f32x4*>(u), u1 = *reinterpret_cast<const f32x4*>(u + 4);
+      const int rank = j0 + 16 * j + i16;
+      if (rank >= a.r) continue;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+      for (int q = 0; q < 4; ++q)
 #pragma unroll
-          for (int c = 0; c < CW; ++c)
-            acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(u2f(row[e].d[c]), e < 4 ? u0[e & 3] : u1[e & 3], acc[c][j], 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int p = 0; p < kPlanes; ++p) {
-          const u32x4 op = *reinterpret_cast<const u32x4*>(u + int64_t(p) * a.r16 * slots);
-#pragma unroll
-          for (int c = 0; c < CW; ++c) {
-            u32x4 x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              x[e] = __builtin_amdgcn_perm(row[2 * e + 1].d[c >> 1], row[2 * e].d[c >> 1],
-                                           c & 1 ? 0x07060302u : 0x05040100u);
-            acc[c][j] = mma<XT>(x, op, acc[c][j]);
-          }
+        for (int c = 0; c < CW; c += 4) {
+          const int64_t at = c0 + CW * (4 * g + q) + c, to = int64_t(rank) * K.C + at;
+          const float v[4] = {acc[c][j][q], acc[c + 1][j][q], acc[c + 2][j][q], acc[c + 3][j][q]};
+          if (part) store4<RQ_DTYPE_F32>(part + to, v, K.C - at);
+          else store4<XT>(out + to, v, K.C - at);
         }
+    }
+  } else {
+    // register q of lane (i, g): rank 4 g + q, column CW i + c
+#pragma unroll
+    for (int c = 0; c < CW; ++c) {
+      if (col + c >= K.C) continue;
+#pragma unroll
+      for (int j = 0; j < JB; ++j) {
+        const int rank = j0 + 16 * j + 4 * g;
+        const float v[4] = {acc[c][j][0], acc[c][j][1], acc[c][j][2], acc[c][j][3]};
+        const int64_t to = (col + c) * a.r + rank;
+        if (part) store4<RQ_DTYPE_F32>(part + to, v, a.r - rank);
+        else store4<XT>(out + to, v, a.r - rank);
       }
     }
   }
-  // waves summed as (0 + 2) + (1 + 3); register q of lane (i, g) is column CW (4 g + q) + c, rank i
-#pragma unroll
-  for (int ph = 0; ph < 2; ++ph) {
-    if ((wave >> 1) == 1 - ph) {
-#pragma unroll
-      for (int c = 0; c < CW; ++c)
-#pragma unroll
-        for (int j = 0; j < JB; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float& o = red[wave & 1][CW * (4 * g + q) + c][16 * j + i16];
-            o = ph == 0 ? acc[c][j][q] : __fadd_rn(acc[c][j][q], o);
-          }
-    }
-    __syncthreads();
-  }
-  const int cols = int(std::min<int64_t>(K.C - c0, kCols)), ranks = std::min(a.r - j0, 16 * JB);
-  for (int i = tid; i < cols * ranks; i += kMlThreads) {
-    const int c = K.rank_major ? i % cols : i / ranks, j = K.rank_major ? i / cols : i % ranks;
-    const float v = __fadd_rn(red[0][c][j], red[1][c][j]);
-    const int64_t at = K.rank_major ? int64_t(j0 + j) * K.C + c0 + c : (c0 + c) * a.r + j0 + j;
-    if (slot >= 0) a.part[slot * a.part_size + K.part_off + at] = v;
-    else static_cast<T*>(K.out)[adapter * K.C * a.r + at] = from_f32<XT>(v);
-  }
 }
 
-// Adapters of several chunks: their partial sums in order.  Adapters without rows:
-// zeros.
+template <int XT, int JB>
+__global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(2))) void rowsum_kernel(RowSumArgs a) {
+  constexpr int kCols = 16 * rowsum_cw<XT>(JB);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  RowSumChunk ch{0, 0, -1, 0};
+  int t1;
+  if (a.rows.p) {
+    if (int(blockIdx.y) >= a.rows.p[1 + a.table]) return;
+    const int32_t* c = a.rows.p + a.rows.off_chunks() + 4 * (int64_t(a.rows.C) * a.table + blockIdx.y);
+    ch.adapter = c[0];
+    ch.t0 = c[1];
+    t1 = c[2];
+    ch.slot = c[3];
+  } else {
+    const int per = RowsPlan::chunk_tiles(a.rows.T, a.table);
+    ch.t0 = per * int(blockIdx.y);
+    if (ch.t0 >= a.rows.T) return;
+    t1 = ch.t0 + per < a.rows.T ? ch.t0 + per : a.rows.T;
+    if (per < a.rows.T) ch.slot = int(blockIdx.y);
+  }
+  // all tiles of an adapter but its last are full
+  if (t1 > ch.t0) ch.live = int64_t(kTileRows) * (t1 - 1 - ch.t0) + plan_tile(a.rows, t1 - 1).count;
+  const int which = int(blockIdx.x) >= a.t[0].tiles ? 1 : 0;
+  const RowSumTask& K = a.t[which];
+  const int64_t c0 = (int64_t(int(blockIdx.x) - (which ? a.t[0].tiles : 0)) * kMlWaves + wave) * kCols;
+  if (c0 >= K.C) return;
+  const int j0 = 16 * JB * int(blockIdx.z);
+  if (!K.rank_major) rowsum_body<XT, JB, false, false>(a, K, ch, c0, j0);
+  else if (K.exps) rowsum_body<XT, JB, true, true>(a, K, ch, c0, j0);
+  else rowsum_body<XT, JB, false, true>(a, K, ch, c0, j0);
+}
+
+// Adapters of several chunks: their partial sums in order.
 template <int XT>
 __global__ __launch_bounds__(kMlThreads) void rowsum_finish_kernel(RowSumArgs a) {
   typedef typename Elem<XT>::T T;
   const int adapter = int(blockIdx.y);
-  int chunks = a.rows.C, first = 0;
+  int chunks, first = 0;
   if (a.rows.p) {
-    chunks = a.rows.p[a.rows.off_part() + 2 * int64_t(adapter)];
-    first = a.rows.p[a.rows.off_part() + 2 * int64_t(adapter) + 1];
+    const int32_t* p = a.rows.p + a.rows.off_part() + 2 * (int64_t(a.rows.n) * a.table + adapter);
+    chunks = p[0];
+    first = p[1];
+  } else {
+    chunks = int(ceil_div(a.rows.T, RowsPlan::chunk_tiles(a.rows.T, a.table)));
   }
   if (chunks == 1) return;
   for (int w = 0; w < a.n; ++w) {
     const RowSumTask& K = a.t[w];
     const int64_t n = K.C * a.r;
     T* out = static_cast<T*>(K.out) + adapter * n;
+    const float* part = a.part + first * a.part_size + K.part_off;
     for (int64_t i = int64_t(blockIdx.x) * kMlThreads + threadIdx.x; i < n; i += int64_t(gridDim.x) * kMlThreads) {
       float v = 0.0f;
-      for (int s = 0; s < chunks; ++s) v = __fadd_rn(v, a.part[(first + s) * a.part_size + K.part_off + i]);
+#pragma unroll 4
+      for (int s = 0; s < chunks; ++s) v = __fadd_rn(v, part[s * a.part_size + i]);
       out[i] = from_f32<XT>(v);
     }
   }
 }
 
+// The table of chunks: the coarser one, whose sums seldom meet in a second launch, where
+// its workgroups fill the GPU.
+int rowsum_table(const RowsPlan& rows, int64_t cols, int wave_cols, int cus) {
+  const int64_t tiles = ceil_div(cols, int64_t(kMlWaves) * wave_cols);
+  return tiles * ceil_div(ceil_div(rows.M, kTileRows), chunk_least(1)) >= cus ? 1 : 0;
+}
+
+// Partial slots that `table` may take.
+int64_t rowsum_parts(const RowsPlan& rows, int table) {
+  if (rows.p) return rows.T > chunk_least(table) ? std::min<int64_t>(kMaxParts, 2 * ceil_div(rows.T, chunk_least(table))) : 0;
+  const int64_t c = ceil_div(rows.T, RowsPlan::chunk_tiles(rows.T, table));
+  return c > 1 ? c : 0;
+}
+
 template <int XT>
 int run_rowsum(RowSumArgs a, hipStream_t stream) {
-  const int jb = a.r16 <= 16 ? 1 : (a.r16 <= 32 ? 2 : 4);
+  const int jb = a.rp <= 16 ? 1 : (a.rp <= 32 ? 2 : 4);
   int tiles = 0;
   int64_t most = 0;
   for (int i = 0; i < a.n; ++i) {
-    a.t[i].tiles = int(ceil_div(a.t[i].C, 16 * rowsum_cw<XT>(jb)));
+    a.t[i].tiles = int(ceil_div(a.t[i].C, int64_t(kMlWaves) * 16 * rowsum_cw<XT>(jb)));
     tiles += a.t[i].tiles;
     most = std::max(most, a.t[i].C * a.r);
   }
   if (a.rows.C > 65535) return RQ_ERR_UNSUPPORTED;
-  int st = RQ_OK;
-  if (a.rows.C > 0) {
-    const dim3 grid(unsigned(tiles), unsigned(a.rows.C), unsigned(ceil_div(a.r16, 16 * jb)));
-    if (jb == 1) rowsum_kernel<XT, 1><<<grid, kMlThreads, 0, stream>>>(a);
-    else if (jb == 2) rowsum_kernel<XT, 2><<<grid, kMlThreads, 0, stream>>>(a);
-    else rowsum_kernel<XT, 4><<<grid, kMlThreads, 0, stream>>>(a);
-    if ((st = rq_check_launch()) != RQ_OK) return st;
-  }
-  if (!a.rows.p && a.rows.C == 1) return RQ_OK;
-  const dim3 grid(unsigned(std::min<int64_t>(ceil_div(most, kMlThreads), 1024)), unsigned(a.rows.p ? a.rows.n : 1));
-  rowsum_finish_kernel<XT><<<grid, kMlThreads, 0, stream>>>(a);
-  return rq_check_launch();
-}
-
-// ---- B [N, r] as rows of ranks [r16][ldt], for the backward's shrink --------------------
-// A workgroup turns 256 rows of B of one adapter through LDS, if the adapter has rows.
-constexpr int kTurnRows = 256, kTurnRanks = 16;
-
-template <int XT>
-__global__ __launch_bounds__(kMlThreads) void turn_kernel(RowsPlan rows, const void* b, int64_t N, int64_t ldb, int64_t b_adapter,
-                                                          int r, int r16, void* bt, int64_t ldt) {
-  typedef typename Elem<XT>::T T;
-  __shared__ T tile[kTurnRanks][kTurnRows + 2];
-  const int adapter = int(blockIdx.z), j0 = kTurnRanks * int(blockIdx.y);
-  if (rows.p && rows.p[rows.off_part() + 2 * int64_t(adapter)] == 0) return;
-  const int64_t n0 = int64_t(blockIdx.x) * kTurnRows;
-  const T* src = static_cast<const T*>(b) + adapter * b_adapter;
-  for (int i = threadIdx.x; i < kTurnRanks * kTurnRows; i += kMlThreads) {
-    const int j = i % kTurnRanks, k = i / kTurnRanks;
-    tile[j][k] = j0 + j < r && n0 + k < N ? src[(n0 + k) * ldb + j0 + j] : T(0);
-  }
-  __syncthreads();
-  T* dst = static_cast<T*>(bt) + (int64_t(adapter) * r16 + j0) * ldt + n0;
-  for (int i = threadIdx.x; i < kTurnRanks * kTurnRows; i += kMlThreads) {
-    const int j = i / kTurnRows, k = i % kTurnRows;
-    if (n0 + k < ldt) dst[j * ldt + k] = tile[j][k];
-  }
-}
-
-template <int XT>
-int run_turn(const RowsPlan& rows, const void* b, int64_t N, int64_t ldb, int64_t b_adapter, int r, int r16, void* bt,
-             int64_t ldt, hipStream_t stream) {
-  const dim3 grid(unsigned(ceil_div(ldt, kTurnRows)), unsigned(r16 / kTurnRanks), unsigned(rows.p ? rows.n : 1));
-  turn_kernel<XT><<<grid, kMlThreads, 0, stream>>>(rows, b, N, ldb, b_adapter, r, r16, bt, ldt);
+  const dim3 grid(unsigned(tiles), unsigned(a.rows.C), unsigned(ceil_div(a.rp, 16 * jb)));
+  if (jb == 1) rowsum_kernel<XT, 1><<<grid, kMlThreads, 0, stream>>>(a);
+  else if (jb == 2) rowsum_kernel<XT, 2><<<grid, kMlThreads, 0, stream>>>(a);
+  else rowsum_kernel<XT, 4><<<grid, kMlThreads, 0, stream>>>(a);
+  const int st = rq_check_launch();
+  if (st != RQ_OK || rowsum_parts(a.rows, a.table) == 0) return st;
+  const dim3 fgrid(unsigned(std::min<int64_t>(ceil_div(most, kMlThreads), 1024)), unsigned(a.rows.p ? a.rows.n : 1));
+  rowsum_finish_kernel<XT><<<fgrid, kMlThreads, 0, stream>>>(a);
   return rq_check_launch();
 }
 
@@ -646,50 +881,46 @@ int check_sizes(int dtype, int64_t M, int64_t K, int64_t N, int64_t n, int64_t r
   return RQ_OK;
 }
 
-// widths of the finished operands of a slot: fp32, or hi | lo
-size_t op_bytes(const Sizes& s, int64_t slots) { return size_t(slots) * rank16(s.r) * 4; }
+// the row sums' operands: fp32, or hi and lo
+size_t op_bytes(const Sizes& s, int64_t slots) { return size_t(slots) * rank_pad(s.r) * 4; }
 
 struct ForwardPlan {
   int splits;
   int64_t per;
-  size_t part, op, bytes;
+  size_t bytes;  // the splits' sums
 };
 
 ForwardPlan plan_forward(const Sizes& s, const RowsPlan& rows) {
   ForwardPlan p{};
   plan_shrink(rows.T, s.K, s.step, device_cus(), &p.splits, &p.per);
-  p.part = 0;
-  p.op = up256(size_t(p.splits) * rows.slots() * rank16(s.r) * 4);
-  p.bytes = p.op + up256(op_bytes(s, rows.slots()));
+  p.bytes = up256(size_t(p.splits) * rows.slots() * rank_pad(s.r) * 4);
   return p;
 }
 
 struct BackwardPlan {
-  int splits;
-  int64_t per, ldt;
-  size_t bt, part, op, gt, ut, sums, bytes;
+  int splits, table;
+  int64_t per;
+  size_t part, gt, ut, sums, bytes;
   int64_t part_size;
 };
 
 BackwardPlan plan_backward(const Sizes& s, const RowsPlan& rows) {
   BackwardPlan p{};
-  const int64_t r16 = rank16(s.r), slots = rows.slots();
-  plan_shrink(rows.T, s.N, s.step, device_cus(), &p.splits, &p.per);
-  p.ldt = ceil_div(s.N, 8) * 8;
-  p.part_size = (s.K + s.N) * s.r;
+  const int64_t rp = rank_pad(s.r), slots = rows.slots();
+  const int cus = device_cus(), jb = rp <= 16 ? 1 : (rp <= 32 ? 2 : 4);
+  plan_shrink(rows.T, s.N, s.step, cus, &p.splits, &p.per);
+  p.table = rowsum_table(rows, s.K + s.N, 16 * (s.es == 4 ? rowsum_cw<RQ_DTYPE_F32>(jb) : rowsum_cw<RQ_DTYPE_BF16>(jb)), cus);
+  p.part_size = ceil_div((s.K + s.N) * s.r, 8) * 8;
   size_t off = 0;
   auto take = [&](size_t b) {
     const size_t o = off;
     off += up256(b);
     return o;
   };
-  p.bt = take(size_t(s.n) * r16 * p.ldt * s.es);
-  p.part = take(size_t(p.splits) * slots * r16 * 4);
-  p.op = take(op_bytes(s, slots));
+  p.part = take(size_t(p.splits) * slots * rp * 4);
   p.gt = take(op_bytes(s, slots));
   p.ut = take(op_bytes(s, slots));
-  const int64_t parts = rows.p ? std::min<int64_t>(kMaxParts, 2 * ceil_div(rows.T, kChunkTiles)) : (rows.C > 1 ? rows.C : 0);
-  p.sums = take(size_t(parts) * p.part_size * 4);
+  p.sums = take(size_t(rowsum_parts(rows, p.table)) * p.part_size * 4);
   p.bytes = off;
   return p;
 }
@@ -712,44 +943,14 @@ struct ForwardCall {
 template <int XT>
 int forward(const ForwardCall& c, char* ws, hipStream_t stream) {
   const ForwardPlan p = plan_forward(c.s, c.rows);
-  const int r16 = int(rank16(c.s.r));
-  ShrinkArgs sh{};
-  sh.rows = c.rows;
-  sh.x = c.x;
-  sh.ldx = c.ldx;
-  sh.K = c.s.K;
-  sh.s = c.a;
-  sh.ld_s = c.s.K;
-  sh.s_adapter = c.s.r * c.s.K;
-  sh.r = int(c.s.r);
-  sh.r16 = r16;
-  sh.splits = p.splits;
-  sh.k_per_split = p.per;
-  sh.part = reinterpret_cast<float*>(ws + p.part);
-  int st = run_shrink<XT>(sh, stream);
+  const int r = int(c.s.r), rp = int(rank_pad(c.s.r));
+  float* part = reinterpret_cast<float*>(ws);
+  const ShrinkArgs sh{c.rows, c.x, c.ldx, c.s.K, c.a, c.s.r * c.s.K, r, rp, p.splits, p.per, part};
+  const int st = run_shrink<XT, false>(sh, stream);
   if (st != RQ_OK) return st;
-  FinishArgs f{};
-  f.rows = c.rows;
-  f.r16 = r16;
-  f.scaling = c.scaling;
-  f.jobs = 1;
-  f.job[0] = FinishJob{sh.part, p.splits, false, c.u, ws + p.op, nullptr};
-  if ((st = run_finish<XT>(f, stream)) != RQ_OK) return st;
-  ExpandArgs e{};
-  e.rows = c.rows;
-  e.op = ws + p.op;
-  e.r = int(c.s.r);
-  e.r16 = r16;
-  e.s = c.b;
-  e.s_adapter = c.s.N * c.s.r;
-  e.ld_s = c.s.r;
-  e.C = c.s.N;
-  e.scaling = c.scaling;
-  e.base = c.base;
-  e.ld_base = c.ld_base;
-  e.out = c.out;
-  e.ld_out = c.ld_out;
-  return run_expand<XT, true>(e, stream);
+  const ExpandArgs e{c.rows, part, p.splits, r, rp, c.b, c.s.N * c.s.r, c.s.N, c.scaling, c.base, c.ld_base, c.out, c.ld_out,
+                     c.u, 0, 0};
+  return run_expand<XT, true>(e, device_cus(), stream);
 }
 
 struct BackwardCall {
@@ -775,58 +976,35 @@ struct BackwardCall {
 template <int XT>
 int backward(const BackwardCall& c, char* ws, hipStream_t stream) {
   const BackwardPlan p = plan_backward(c.s, c.rows);
-  const int r16 = int(rank16(c.s.r));
+  const int r = int(c.s.r), rp = int(rank_pad(c.s.r));
+  float* part = reinterpret_cast<float*>(ws + p.part);
   int st = RQ_OK;
   FinishArgs f{};
   f.rows = c.rows;
-  f.r16 = r16;
+  f.rp = rp;
   f.scaling = c.scaling;
   if (c.dx || c.da) {
-    if ((st = run_turn<XT>(c.rows, c.b, c.s.N, c.s.r, c.s.N * c.s.r, int(c.s.r), r16, ws + p.bt, p.ldt, stream)) != RQ_OK) return st;
-    ShrinkArgs sh{};
-    sh.rows = c.rows;
-    sh.x = c.dy;
-    sh.ldx = c.lddy;
-    sh.K = c.s.N;
-    sh.s = ws + p.bt;
-    sh.ld_s = p.ldt;
-    sh.s_adapter = r16 * p.ldt;
-    sh.r = int(c.s.r);
-    sh.r16 = r16;
-    sh.splits = p.splits;
-    sh.k_per_split = p.per;
-    sh.part = reinterpret_cast<float*>(ws + p.part);
-    if ((st = run_shrink<XT>(sh, stream)) != RQ_OK) return st;
-    f.job[f.jobs++] = FinishJob{sh.part, p.splits, true, nullptr, c.dx ? ws + p.op : nullptr, c.da ? ws + p.gt : nullptr};
+    const ShrinkArgs sh{c.rows, c.dy, c.lddy, c.s.N, c.b, c.s.N * c.s.r, r, rp, p.splits, p.per, part};
+    if ((st = run_shrink<XT, true>(sh, stream)) != RQ_OK) return st;
+    if (c.da) f.job[f.jobs++] = FinishJob{part, p.splits, ws + p.gt};
   }
-  if (c.db) f.job[f.jobs++] = FinishJob{c.u, 1, true, nullptr, nullptr, ws + p.ut};
-  if (f.jobs == 0) return RQ_OK;
-  if ((st = run_finish<XT>(f, stream)) != RQ_OK) return st;
+  if (c.db) f.job[f.jobs++] = FinishJob{c.u, 1, ws + p.ut};
+  if (f.jobs > 0 && (st = run_finish<XT>(f, stream)) != RQ_OK) return st;
   if (c.dx) {
-    ExpandArgs e{};
-    e.rows = c.rows;
-    e.op = ws + p.op;
-    e.r = int(c.s.r);
-    e.r16 = r16;
-    e.s = c.a;
-    e.s_adapter = c.s.r * c.s.K;
-    e.ld_s = c.s.K;
-    e.C = c.s.K;
-    e.base = c.dx_base;
-    e.ld_base = c.ld_dx_base;
-    e.out = c.dx;
-    e.ld_out = c.lddx;
-    if ((st = run_expand<XT, false>(e, stream)) != RQ_OK) return st;
+    const ExpandArgs e{c.rows, part, p.splits, r, rp, c.a, c.s.r * c.s.K, c.s.K, c.scaling, c.dx_base, c.ld_dx_base, c.dx, c.lddx,
+                       nullptr, 0, 0};
+    if ((st = run_expand<XT, false>(e, device_cus(), stream)) != RQ_OK) return st;
   }
-  RowSumArgs r{};
-  r.rows = c.rows;
-  r.r = int(c.s.r);
-  r.r16 = r16;
-  r.part = reinterpret_cast<float*>(ws + p.sums);
-  r.part_size = p.part_size;
-  if (c.db) r.t[r.n++] = RowSumTask{c.dy, nullptr, c.lddy, c.s.N, ws + p.ut, c.db, false, 0, 0};
-  if (c.da) r.t[r.n++] = RowSumTask{c.x, c.exps, c.ldx, c.s.K, ws + p.gt, c.da, true, c.s.N * c.s.r, 0};
-  return r.n > 0 ? run_rowsum<XT>(r, stream) : RQ_OK;
+  RowSumArgs q{};
+  q.rows = c.rows;
+  q.table = p.table;
+  q.r = r;
+  q.rp = rp;
+  q.part = reinterpret_cast<float*>(ws + p.sums);
+  q.part_size = p.part_size;
+  if (c.db) q.t[q.n++] = RowSumTask{c.dy, nullptr, c.lddy, c.s.N, ws + p.ut, c.db, false, 0, 0};
+  if (c.da) q.t[q.n++] = RowSumTask{c.x, c.exps, c.ldx, c.s.K, ws + p.gt, c.da, true, c.s.N * c.s.r, 0};
+  return q.n > 0 ? run_rowsum<XT>(q, stream) : RQ_OK;
 }
 
 // Rows of the plan given, or of one adapter.

@@ -43,19 +43,34 @@ __device__ __forceinline__ void store16_any(void* p, u32x4 v) {
   *static_cast<u32x4_any*>(p) = u32x4_any{v.x, v.y, v.z, v.w};
 }
 
-// The first `n` elements at p (n <= 0: none) as 16 bytes, zeros after them.
+// Less than 16 bytes, element by element: the ends of rows.  Not inlined: the addresses of
+// the elements would take registers from the loops around.
 template <int XT>
-__device__ __forceinline__ u32x4 load16_part(const typename Elem<XT>::T* p, int64_t n) {
-  constexpr int V = Elem<XT>::kVec;
-  if (n >= V) return load16_any(p);
+__attribute__((noinline)) __device__ u32x4 load_edge(const typename Elem<XT>::T* p, int n) {
   u32x4 v = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+  for (int i = 0; i < Elem<XT>::kVec; ++i) {
     if (i >= n) break;
     if constexpr (XT == RQ_DTYPE_F32) v[i] = f2u(p[i]);
     else v[i >> 1] |= uint32_t(p[i]) << (16 * (i & 1));
   }
   return v;
+}
+template <int XT>
+__attribute__((noinline)) __device__ void store_edge(typename Elem<XT>::T* p, u32x4 v, int n) {
+#pragma unroll
+  for (int i = 0; i < Elem<XT>::kVec; ++i) {
+    if (i >= n) break;
+    if constexpr (XT == RQ_DTYPE_F32) p[i] = u2f(v[i]);
+    else p[i] = uint16_t(v[i >> 1] >> (16 * (i & 1)));
+  }
+}
+
+// The first `n` elements at p (n <= 0: none) as 16 bytes, zeros after them.
+template <int XT>
+__device__ __forceinline__ u32x4 load16_part(const typename Elem<XT>::T* p, int64_t n) {
+  if (n >= Elem<XT>::kVec) return load16_any(p);
+  return load_edge<XT>(p, int(n));
 }
 
 // 16 bytes as fp32 values, and back (rounded to nearest even).
@@ -84,13 +99,20 @@ __device__ __forceinline__ u32x4 pack16(const float (&f)[Elem<XT>::kVec]) {
 
 template <int XT>
 __device__ __forceinline__ void store16_part(typename Elem<XT>::T* p, const float (&f)[Elem<XT>::kVec], int64_t n) {
-  constexpr int V = Elem<XT>::kVec;
-  if (n >= V) {
-    store16_any(p, pack16<XT>(f));
+  if (n >= Elem<XT>::kVec) store16_any(p, pack16<XT>(f));
+  else store_edge<XT>(p, pack16<XT>(f), int(n));
+}
+
+// The first `n` of four values.
+template <int XT>
+__device__ __forceinline__ void store4(typename Elem<XT>::T* p, const float (&f)[4], int64_t n) {
+  if (n >= 4) {
+    if constexpr (XT == RQ_DTYPE_F32) store16_any(p, u32x4{f2u(f[0]), f2u(f[1]), f2u(f[2]), f2u(f[3])});
+    else *reinterpret_cast<u32x2_any*>(p) = u32x2_any{cvt_pk<XT>(f[0], f[1]), cvt_pk<XT>(f[2], f[3])};
     return;
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i)
+  for (int i = 0; i < 4; ++i)
     if (i < n) p[i] = from_f32<XT>(f[i]);
 }
 

@@ -5,15 +5,16 @@
 // rows without an adapter.  What is computed per row between two launches (the
 // rank-wide operands) is stored by slot, so that a tile's rows are adjacent
 // whatever their order in the batch.  Sums over an adapter's rows run over chunks
-// of its tiles; an adapter of one chunk writes its result at once, the others'
-// partial sums are added in order.
+// of its tiles; an adapter of one chunk (or of no row) writes its result at once, the
+// others' partial sums are added in order.  There are two tables of chunks, of 4 and of
+// 16 tiles at least: few columns take the finer one.
 //
 // The plan is int32 device memory:
-//   [0] tiles in use, [1] chunks in use, [2..15] zero
+//   [0] tiles in use, [1], [2] chunks in use of the two tables, [3..15] zero
 //   tile_adapter[T], tile_count[T]    (adapter -1: rows without one)
 //   slot_row[64 T]                    (-1: padding)
-//   chunk[C][4]                       (adapter, first tile, end tile, partial slot or -1)
-//   part[n][2]                        (chunks of the adapter, its first partial slot)
+//   chunk[2][C][4]                    (adapter, first tile, end tile, partial slot or -1)
+//   part[2][n][2]                     (chunks of the adapter, its first partial slot)
 // A null plan stands for M rows of adapter 0 in their own order.
 #pragma once
 
@@ -23,11 +24,12 @@ namespace rq {
 
 constexpr int kTileRows = 64;
 constexpr int kMaxAdapters = 1024;
-// An adapter whose tiles are more than 1 / kRowChunks of all is summed in chunks of
-// that many tiles (at least kChunkTiles), so that partial sums are bounded:
-// adapters of several chunks have at most 2 kRowChunks of them in all.
+// Tiles of a chunk: at least these, and at least 1 / kRowChunks of all, so that
+// partial sums are bounded: adapters of several chunks have at most 2 kRowChunks of
+// them in all.
 constexpr int kRowChunks = 16;
-constexpr int kChunkTiles = 8;
+constexpr int kChunkTables = 2;
+__host__ __device__ constexpr int chunk_least(int table) { return table == 0 ? 4 : 16; }
 constexpr int kMaxParts = 2 * kRowChunks;
 
 struct RowsPlan {
@@ -35,19 +37,19 @@ struct RowsPlan {
   int64_t M;
   int32_t n;         // adapters
   int32_t T;         // tiles, at most
-  int32_t C;         // chunks, at most
+  int32_t C;         // chunks of a table, at most
 
   __host__ __device__ int64_t off_count() const { return 16 + ((int64_t(T) + 3) & ~int64_t(3)); }
   __host__ __device__ int64_t off_rows() const { return 16 + 2 * ((int64_t(T) + 3) & ~int64_t(3)); }
   __host__ __device__ int64_t off_chunks() const { return off_rows() + int64_t(kTileRows) * T; }
-  __host__ __device__ int64_t off_part() const { return off_chunks() + 4 * int64_t(C); }
-  __host__ __device__ int64_t words() const { return off_part() + 2 * int64_t(n); }
+  __host__ __device__ int64_t off_part() const { return off_chunks() + kChunkTables * 4 * int64_t(C); }
+  __host__ __device__ int64_t words() const { return off_part() + kChunkTables * 2 * int64_t(n); }
   __host__ __device__ int64_t slots() const { return int64_t(kTileRows) * T; }
 
   // tiles per chunk when `tiles` are in use
-  __host__ __device__ static int chunk_tiles(int tiles) {
+  __host__ __device__ static int chunk_tiles(int tiles, int table) {
     const int c = (tiles + kRowChunks - 1) / kRowChunks;
-    return c > kChunkTiles ? c : kChunkTiles;
+    return c > chunk_least(table) ? c : chunk_least(table);
   }
 };
 
@@ -75,13 +77,8 @@ __device__ __forceinline__ int plan_row(const RowsPlan& P, int64_t slot) {
 inline RowsPlan rows_plan(const int32_t* p, int64_t M, int64_t n) {
   const int64_t some = n + 1 < M ? n + 1 : M;
   RowsPlan P{p, M, int32_t(n), 0, 0};
-  if (!p) {
-    P.T = int32_t(ceil_div(M, kTileRows));
-    P.C = P.T > 0 ? int32_t(ceil_div(P.T, RowsPlan::chunk_tiles(P.T))) : 0;
-  } else {
-    P.T = int32_t(M / kTileRows + some);
-    P.C = int32_t((n < M ? n : M) + kMaxParts);
-  }
+  P.T = int32_t(p ? M / kTileRows + some : ceil_div(M, kTileRows));
+  P.C = int32_t(p ? n + kMaxParts : ceil_div(P.T, RowsPlan::chunk_tiles(P.T, 0)));
   return P;
 }
 
