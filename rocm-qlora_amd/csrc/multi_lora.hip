@@ -2,8 +2,11 @@
 //
 // All of them are bound by memory: a row meets r <= 64 ranks, some 4 r operations a
 // byte at most, a tenth of what the matrix cores do in the time the byte takes.
-// So rows are loaded straight into operand registers, 16 bytes a lane, and the
-// adapters' factors, which the tiles of an adapter share, come from the L2.
+// What bounds them beside HBM is the L1: it serves 64 bytes a cycle when four adjacent
+// lanes ask for one piece of 64, but a sixteenth lane's row at a time when every lane asks
+// for a row of its own, as operand registers hold a matrix.  So rows are loaded straight
+// into operand registers where they pass once, and the factors, which serve many rows, go
+// through LDS or are read along their rows.
 #include "rq_multi_lora.h"
 
 #include "rq_act8.h"
@@ -27,25 +30,26 @@ __device__ __forceinline__ void split16(float v, uint32_t& hi, uint32_t& lo) {
 }
 
 // ---- shrink ---------------------------------------------------------------------
-// A workgroup takes a tile's rows over a split of K; its eight waves divide the split
+// A workgroup takes a tile's rows over a split of K; its four waves divide the split
 // and meet in LDS, 16 rows at a time, summed in the waves' order.  A wave holds the
 // tile's 16-row blocks (1 to 4, as many as the tile has) times JB blocks of 16 ranks,
 // so that a factor's piece is loaded once for the tile.
 //
-// The factor is A [r][K], whose rows are operands as they lie, or (TURNED) B [N][r],
-// whose rows run across the contraction: a step's rows are one piece of memory, which
-// a wave copies to LDS as it lies (with 32 bytes between eight-row groups, so that the
-// four lane groups read other banks) and reads back a rank's values at a time.
-constexpr int kShWaves = 8;
+// The factor goes through a wave's own piece of LDS.  A [r][K]: a step's 64 bytes of each
+// rank, whose four pieces are exchanged by the rank so that the lanes of a read meet other
+// banks.  B [N][r] (TURNED), whose rows run across the contraction: a step's rows are one
+// piece of memory, copied as it lies (with 32 bytes between eight-row groups, so that the
+// four lane groups read other banks) and read back a rank's values at a time.
+constexpr int kShWaves = 4;
 constexpr int kShThreads = 64 * kShWaves;
 
 template <int XT, int JB>
 struct ShrinkLds {
   static constexpr int kPitch = 16 * JB + 4;
   static constexpr int kRedFloats = kShWaves * 16 * kPitch;
-  // elements of one wave's turned step, with the gaps
+  // elements of one wave's step, with the gaps
   static constexpr int kGap = 32 / int(sizeof(typename Elem<XT>::T));
-  static constexpr int kTurn = Elem<XT>::kStep * 16 * JB + 4 * kGap + Elem<XT>::kVec;
+  static constexpr int kTurn = Elem<XT>::kStep * 16 * JB + 4 * kGap + 2 * Elem<XT>::kVec;  // whole 16 bytes; the last kVec: no one's
   static constexpr int kTurnFloats = kShWaves * kTurn * int(sizeof(typename Elem<XT>::T)) / 4;
 };
 
@@ -73,7 +77,6 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
   for (int b = 0; b < JB; ++b) {
     const int j = j0 + 16 * b + i16;
     jlive[b] = j < a.r;
-    if constexpr (!TURNED) sr[b] = s0 + int64_t(jlive[b] ? j : 0) * a.K + V * g;
   }
   // TURNED: a step's pieces of V values.  Up to 64 ranks lie end to end in LDS as in memory;
   // of more, this rank block's 64 of each row.  Lanes without a piece repeat the first and
@@ -88,6 +91,13 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
       const bool on = f < kStep * pitch && (a.r <= 64 || j0 + f % 64 < a.r);
       put[b] = on ? f + f / (V * pitch) * L::kGap : L::kTurn - V;
       sr[b] = s0 + (!on ? 0 : a.r <= 64 ? f : (f / 64) * a.r + j0 + f % 64);
+    }
+  } else {
+#pragma unroll
+    for (int b = 0; b < JB; ++b) {
+      const int row = 16 * b + (lane >> 2);
+      put[b] = V * (4 * row + ((lane ^ row >> 1) & 3));
+      sr[b] = s0 + int64_t(j0 + row < a.r ? j0 + row : 0) * a.K + V * (lane & 3);
     }
   }
   f32x4 acc[NRB][JB];
@@ -108,11 +118,9 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
     }
   };
   auto products = [&](const u32x4 (&xv)[NRB], const u32x4 (&sv)[JB]) {
-    if constexpr (TURNED) {
 #pragma unroll
-      for (int j = 0; j < JB; ++j) store16_any(turn + put[j], sv[j]);
-      __builtin_amdgcn_wave_barrier();
-    }
+    for (int j = 0; j < JB; ++j) *reinterpret_cast<u32x4*>(turn + put[j]) = sv[j];
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int j = 0; j < JB; ++j) {
       u32x4 f;
@@ -124,15 +132,16 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
           else f[e] = uint32_t(p[2 * e * pitch]) | uint32_t(p[(2 * e + 1) * pitch]) << 16;
         }
       } else {
-        f = sv[j];
+        const int row = 16 * j + i16;
+        f = *reinterpret_cast<const u32x4*>(turn + V * (4 * row + ((g ^ row >> 1) & 3)));
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] = jlive[j] ? f[e] : 0u;
 #pragma unroll
       for (int b = 0; b < NRB; ++b) acc[b][j] = mma<XT>(xv[b], f, acc[b][j]);
-      if constexpr (TURNED) __builtin_amdgcn_sched_barrier(0);  // one rank block's reads at a time in registers
+      __builtin_amdgcn_sched_barrier(0);  // one rank block's reads at a time in registers
     }
-    __builtin_amdgcn_wave_barrier();  // TURNED: the next step's copy comes after these reads
+    __builtin_amdgcn_wave_barrier();  // the next step's copy comes after these reads
   };
   int64_t steps = ke > kb ? (ke - kb) / kStep : 0;
   // more than 64 ranks: the factor's last rows are read with their ends in view
@@ -162,7 +171,7 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
 #pragma unroll
     for (int j = 0; j < JB; ++j) {
       if constexpr (TURNED) s[0][j] = load16_part<XT>(sr[j] + k * a.r, (a.K - k) * a.r - (sr[j] - s0));
-      else s[0][j] = load16_part<XT>(sr[j] + k, ke - k - V * g);
+      else s[0][j] = load16_part<XT>(sr[j] + k, ke - k - V * (lane & 3));
     }
     products(x[0], s[0]);
   }
@@ -188,9 +197,9 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
 }
 
 template <int XT, int JB, bool TURNED>
-__global__ __launch_bounds__(kShThreads) void shrink_kernel(ShrinkArgs a) {
+__global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(JB == 4 ? 2 : 3))) void shrink_kernel(ShrinkArgs a) {
   typedef ShrinkLds<XT, JB> L;
-  __shared__ float lds[TURNED && L::kTurnFloats > L::kRedFloats ? L::kTurnFloats : L::kRedFloats];
+  __shared__ __attribute__((aligned(16))) float lds[L::kTurnFloats > L::kRedFloats ? L::kTurnFloats : L::kRedFloats];
   const int t = int(blockIdx.x % unsigned(a.rows.T)), split = int(blockIdx.x / unsigned(a.rows.T));
   const int j0 = 16 * JB * int(blockIdx.y);
   const Tile tile = plan_tile(a.rows, t);
@@ -200,12 +209,18 @@ __global__ __launch_bounds__(kShThreads) void shrink_kernel(ShrinkArgs a) {
   else shrink_body<XT, 4, JB, TURNED>(a, tile, t, split, j0, lds);
 }
 
-// About two workgroups a compute unit, each wave with at least four steps.
+// About RQ_SH_WGS workgroups a compute unit, each wave with at least four steps.
+#ifndef RQ_SH_WGS
+#define RQ_SH_WGS 2
+#endif
+#ifndef RQ_SH_MIN
+#define RQ_SH_MIN 4
+#endif
 void plan_shrink(int64_t T, int64_t K, int step, int cus, int* splits, int64_t* per) {
   const int64_t unit = int64_t(step) * kShWaves;
-  int64_t s = ceil_div(2 * cus, std::max<int64_t>(T, 1));
-  s = std::min(s, std::max<int64_t>(K / (4 * unit), 1));
-  s = std::min<int64_t>(std::max<int64_t>(s, 1), 8);
+  int64_t s = ceil_div(RQ_SH_WGS * cus, std::max<int64_t>(T, 1));
+  s = std::min(s, std::max<int64_t>(K / (RQ_SH_MIN * unit), 1));
+  s = std::min<int64_t>(std::max<int64_t>(s, 1), 16);
   *per = ceil_div(ceil_div(K, s), unit) * unit;
   *splits = int(ceil_div(K, *per));
 }
@@ -238,190 +253,123 @@ __device__ __forceinline__ f32x4 split_sum4(const float* p, int splits, int64_t 
 }
 
 // ---- expand ---------------------------------------------------------------------
-// A workgroup takes half a tile (two 16-row blocks): it sums the splits of its slots and
-// keeps them in LDS as operands, and its waves walk over columns, 16 kVec of them a step.
-// The factor is the A operand and the slots the B operand, so that a result register holds
-// columns; the operand row i of product c is column kVec i + c, so that a lane ends with
-// kVec adjacent columns for each of its four registers: whole 16-byte pieces of a row,
-// 256 bytes of it by the four lane groups.
-constexpr int kExpandBlocks = 2;  // 16-row blocks of a workgroup
-
-// kVec ranks from j on for each of kVec columns from `col` on.  FULL: all columns exist, and
-// reading past a row's last rank stays in the factor.
-template <int XT, bool FACTOR_ROWS, bool FULL>
-__device__ __forceinline__ void load_factor(u32x4 (&f)[Elem<XT>::kVec], const typename Elem<XT>::T* s, int64_t C, int64_t col,
-                                            int r, int j) {
-  constexpr int V = Elem<XT>::kVec;
-  const u32x4 zero = u32x4{0u, 0u, 0u, 0u};
-  if constexpr (FACTOR_ROWS) {
-    // column c's ranks j .. j + V - 1 are adjacent
-    if constexpr (FULL) {
-#pragma unroll
-      for (int c = 0; c < V; ++c) f[c] = load16_any(s + (col + c) * r + (j < r ? j : 0));
-      if (j + V > r) {
-        u32x4 keep;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (XT == RQ_DTYPE_F32) keep[e] = j + e < r ? ~0u : 0u;
-          else keep[e] = j + 2 * e + 1 < r ? ~0u : (j + 2 * e < r ? 0xFFFFu : 0u);
-        }
-#pragma unroll
-        for (int c = 0; c < V; ++c) f[c] &= keep;
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < V; ++c) f[c] = col + c < C && j < r ? load16_part<XT>(s + (col + c) * r + j, r - j) : zero;
-    }
-  } else {
-    // rank j + e's columns are adjacent: transpose V x V values
-    u32x4 row[V];
-    if constexpr (FULL) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) row[e] = load16_any(s + int64_t(j + e < r ? j + e : 0) * C + col);
-      if (j + V > r) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) row[e] = j + e < r ? row[e] : zero;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) row[e] = j + e < r ? load16_part<XT>(s + int64_t(j + e) * C + col, C - col) : zero;
-    }
-    if constexpr (XT == RQ_DTYPE_F32) {
-#pragma unroll
-      for (int c = 0; c < V; ++c)
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[c][e] = row[e][c];
-    } else {
-#pragma unroll
-      for (int c = 0; c < V; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          f[c][e] = __builtin_amdgcn_perm(row[2 * e + 1][c >> 1], row[2 * e][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
-    }
-  }
-}
-
+// A workgroup takes a tile: it sums the splits of its slots and keeps them in LDS as operands.
+// Its four waves divide the tile's 16-row blocks (1, 2 or 4) and, where there are fewer than
+// four, adjacent columns; a wave's step is 16 kVec columns.  The slots are the A operand and
+// column kVec i + c of the factor is row i of the B operand of product c, so that a lane ends
+// with kVec adjacent columns of rows 4 g + q: 256 bytes of a row by 16 adjacent lanes.
+//
+// B's rows [N][r] go through LDS, one rank step (32 ranks of 16 bits, 16 of fp32) of all the
+// waves' columns at a time, copied as they lie (up to a step of ranks; of more, a step's ranks
+// of each row) with 16 bytes between groups of kVec rows, so that the lanes of a read meet
+// other banks.  A's rows [r][K] are read along the row and transposed in registers.
 template <int XT>
-struct ExpandWave {
-  const typename Elem<XT>::T* s;     // the adapter's factor, or nullptr: none
-  const typename Elem<XT>::T* op;    // the slots' operands in LDS
-  int pitch;
-  int blocks;                        // 16-row blocks in use
-  float scale;
-  bool based;                        // there is a base
-  int64_t base[kExpandBlocks], out[kExpandBlocks];  // this lane's row (past the tile's last: the first)
-  bool on[kExpandBlocks];            // not past it
+struct ExpandLds {
+  static constexpr int kCols = 16 * Elem<XT>::kVec;   // of a wave
+  // elements of one wave's columns of a rank step, with the gaps
+  static constexpr int kStage = kCols * Elem<XT>::kStep + 16 * Elem<XT>::kVec;
 };
 
-template <int XT, bool FACTOR_ROWS, bool FULL>
-__device__ __forceinline__ void expand_step(const ExpandArgs& a, const ExpandWave<XT>& w, int64_t c0) {
-  constexpr int V = Elem<XT>::kVec, kStep = Elem<XT>::kStep;
-  const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
-  const int64_t col = c0 + V * i16;
-  // one step of ranks: the factor's piece serves both blocks.  (16 ranks of 16 bits: lane
-  // groups 2 and 3 take the lo parts, of the same ranks as groups 0 and 1.)
-  const bool one = XT == RQ_DTYPE_F32 ? a.rp == kStep : a.rp <= kStep;
-  u32x4 f[V];
-  if (w.s && one) load_factor<XT, FACTOR_ROWS, FULL>(f, w.s, a.C, col, a.r, a.rp < kStep ? V * (g & 1) : V * g);
+// kVec ranks from j on for each of kVec columns from `col` on of A's rows.
+template <int XT, bool EDGE>
+__device__ __forceinline__ void factor_of_rows(u32x4 (&f)[Elem<XT>::kVec], const typename Elem<XT>::T* s, int64_t C, int64_t col,
+                                               int r, int j) {
+  constexpr int V = Elem<XT>::kVec;
+  u32x4 row[V];
 #pragma unroll
-  for (int b = 0; b < kExpandBlocks; ++b) {
-    if (b >= w.blocks) break;
-    u32x4 base[4];
+  for (int e = 0; e < V; ++e) {
+    const typename Elem<XT>::T* p = s + int64_t(j + e < r ? j + e : 0) * C + col;
+    row[e] = EDGE ? load16_part<XT>(p, C - col) : load16_any(p);
+  }
+  if (j + V > r) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t c = c0 + V * (4 * g + q);
-      const typename Elem<XT>::T* p = static_cast<const typename Elem<XT>::T*>(a.base) + w.base[b] + c;
-      base[q] = u32x4{0u, 0u, 0u, 0u};
-      if (w.based) base[q] = FULL ? load16_any(p) : load16_part<XT>(p, a.C - c);
-    }
-    f32x4 acc[V];
+    for (int e = 0; e < V; ++e)
 #pragma unroll
-    for (int c = 0; c < V; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (w.s) {
-      const typename Elem<XT>::T* op = w.op + (16 * b + i16) * w.pitch + V * g;
-#pragma unroll 1
-      for (int j = 0; j < a.rp; j += kStep) {
-        if (!one) load_factor<XT, FACTOR_ROWS, FULL>(f, w.s, a.C, col, a.r, j + V * g);
-        const u32x4 hi = *reinterpret_cast<const u32x4*>(op + j);
+      for (int d = 0; d < 4; ++d) row[e][d] = j + e < r ? row[e][d] : 0u;
+  }
 #pragma unroll
-        for (int c = 0; c < V; ++c) acc[c] = mma<XT>(f[c], hi, acc[c]);
-        if (XT != RQ_DTYPE_F32 && a.rp >= kStep) {
-          const u32x4 lo = *reinterpret_cast<const u32x4*>(op + a.rp + j);
+  for (int c = 0; c < V; ++c) {
+    if constexpr (XT == RQ_DTYPE_F32) {
 #pragma unroll
-          for (int c = 0; c < V; ++c) acc[c] = mma<XT>(f[c], lo, acc[c]);
-        }
-      }
-    }
-    if (!w.on[b]) continue;
-    typename Elem<XT>::T* out = static_cast<typename Elem<XT>::T*>(a.out) + w.out[b];
+      for (int e = 0; e < V; ++e) f[c][e] = row[e][c];
+    } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t c = c0 + V * (4 * g + q);
-      float v[V];
-      unpack16<XT>(base[q], v);
-      if (w.s) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = __fadd_rn(v[e], __fmul_rn(w.scale, acc[e][q]));
-      }
-      if constexpr (FULL) store16_any(out + c, pack16<XT>(v));
-      else store16_part<XT>(out + c, v, a.C - c);
+      for (int e = 0; e < 4; ++e)
+        f[c][e] = __builtin_amdgcn_perm(row[2 * e + 1][c >> 1], row[2 * e][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
     }
   }
 }
 
-// Whether the wave's columns from c0 on all exist, and reading V ranks at the last of them
-// stays in the factor.
-template <int XT, bool FACTOR_ROWS>
-__host__ __device__ __forceinline__ bool expand_full(const ExpandArgs& a, int64_t c0) {
-  constexpr int V = Elem<XT>::kVec;
-  const int64_t end = c0 + 16 * V;
-  return end <= a.C && (!FACTOR_ROWS || a.r % V == 0 || end * a.r + V <= a.C * a.r);
-}
-
-// EDGES: there are columns that a whole wave does not fill (their code takes registers
-// that the others would miss: two waves a SIMD instead of three).
-template <int XT, bool FACTOR_ROWS, bool EDGES>
-__global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(EDGES ? 2 : 3))) void expand_kernel(ExpandArgs a) {
+// BLOCKS: 16-row blocks that the waves divide (1, 2, 4).  EDGES: there are columns that a
+// whole wave does not fill, or ranks of B's rows that 16 bytes run past.
+template <int XT, bool FACTOR_ROWS, bool EDGES, int BLOCKS>
+__device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& tile, int t, int chunk, typename Elem<XT>::T* lds) {
   typedef typename Elem<XT>::T T;
-  constexpr int V = Elem<XT>::kVec;
-  constexpr int kParts = kTileRows / (16 * kExpandBlocks);
-  extern __shared__ uint32_t lds[];
-  const int lane = threadIdx.x & 63, i16 = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int chunk = int(blockIdx.x % unsigned(a.chunks));
-  const unsigned rest = blockIdx.x / unsigned(a.chunks);
-  const int t = int(rest / kParts), part = int(rest % kParts);
-  const Tile tile = plan_tile(a.rows, t);
-  const int first = 16 * kExpandBlocks * part, live = tile.count - first;
-  if (live <= 0) return;
-  if (tile.adapter < 0 && a.base == a.out && a.ld_base == a.ld_out) return;  // in place, nothing to add
-  const int64_t slot0 = int64_t(kTileRows) * t + first;
-  ExpandWave<XT> w;
-  w.blocks = live > 16 ? 2 : 1;
-  w.s = nullptr;
-  w.scale = 0.0f;
-  w.based = a.base != nullptr;
-  T* op = reinterpret_cast<T*>(lds);
-  w.op = op;
-  w.pitch = (XT == RQ_DTYPE_F32 ? a.rp : 2 * a.rp) + V;
+  typedef ExpandLds<XT> L;
+  constexpr int V = Elem<XT>::kVec, kStep = Elem<XT>::kStep;
+  constexpr int GROUPS = kMlWaves / BLOCKS;                      // of columns
+  constexpr int PIECES = GROUPS * L::kCols * kStep / V / kMlThreads;
+  const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int block = wave % BLOCKS, group = wave / BLOCKS;
+  const int64_t slot0 = int64_t(kTileRows) * t;
+  const bool adapted = tile.adapter >= 0;
+  const int pitch = (XT == RQ_DTYPE_F32 ? a.rp : 2 * a.rp) + V;  // of the slots' operands
+  T* op = lds + (FACTOR_ROWS ? GROUPS * L::kStage : 0);
+  // 16 ranks of 16 bits: lane groups 2 and 3 take the lo parts, of the same ranks as 0 and 1
+  const bool half = XT != RQ_DTYPE_F32 && a.rp < kStep;
+  const T* s = static_cast<const T*>(a.s) + (adapted ? tile.adapter : 0) * a.s_adapter;
+  const float scale = adapted ? a.scaling[tile.adapter] : 0.0f;
+  const int64_t c_first = int64_t(chunk) * a.iters * (kMlWaves * L::kCols);
+  const int steps = adapted ? int(ceil_div(a.rp, kStep)) : 1;    // of ranks
+  const int sp = a.r < kStep ? a.r : kStep;                      // ranks of a column in LDS
+
+  // this lane's rows (past the tile's last: the first)
+  int row[4];
+  bool on[4];
 #pragma unroll
-  for (int b = 0; b < kExpandBlocks; ++b) {
-    const int i = 16 * b + i16;
-    w.on[b] = i < live;
-    const int64_t row = plan_row(a.rows, slot0 + (w.on[b] ? i : 0));
-    w.base[b] = row * a.ld_base;
-    w.out[b] = row * a.ld_out;
+  for (int q = 0; q < 4; ++q) {
+    const int i = 16 * block + 4 * g + q;
+    on[q] = i < tile.count;
+    row[q] = plan_row(a.rows, slot0 + (on[q] ? i : 0));
   }
-  if (tile.adapter >= 0) {
-    w.s = static_cast<const T*>(a.s) + tile.adapter * a.s_adapter;
-    w.scale = a.scaling[tile.adapter];
-    const int quads = a.rp / 4, rows = 16 * w.blocks;
+  // a step's pieces of B, as this thread copies them: piece p of the waves' columns
+  u32x4 piece[PIECES];
+  auto fetch = [&](int64_t c0, int j0) {
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+      const int f = V * (tid + kMlThreads * k);
+      int64_t at;
+      bool there;
+      if (a.r <= kStep) {
+        at = c0 * a.r + f;
+        there = f < GROUPS * L::kCols * sp;
+      } else {
+        const int n = f / kStep, j = j0 + f % kStep;
+        at = (c0 + n) * a.r + j;
+        there = j < a.r;
+      }
+      const int64_t left = a.C * a.r - at;
+      if constexpr (EDGES) piece[k] = load16_part<XT>(s + at, there ? left : 0);
+      else piece[k] = load16_any(s + (there && left > 0 ? at : 0));
+    }
+  };
+  auto stage = [&]() {
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+      const int f = V * (tid + kMlThreads * k);
+      if (f < GROUPS * L::kCols * sp) *reinterpret_cast<u32x4*>(lds + f + f / (V * sp) * V) = piece[k];
+    }
+  };
+  if (FACTOR_ROWS && adapted) fetch(c_first, 0);
+  if (adapted) {
+    const int quads = a.rp / 4, rows = (tile.count + 15) & ~15;
     const int64_t stride = a.rows.slots() * a.rp;
-    for (int i = threadIdx.x; i < rows * quads; i += kMlThreads) {
-      const int row = i / quads, j = 4 * (i - row * quads);
-      const f32x4 v = split_sum4(a.part + (slot0 + row) * a.rp + j, a.splits, stride);
-      if (a.sum && chunk == 0) *reinterpret_cast<f32x4*>(a.sum + (slot0 + row) * a.rp + j) = v;
-      T* o = op + row * w.pitch + j;
+    for (int i = tid; i < rows * quads; i += kMlThreads) {
+      const int m = i / quads, j = 4 * (i - m * quads);
+      const f32x4 v = split_sum4(a.part + (slot0 + m) * a.rp + j, a.splits, stride);
+      if (a.sum && chunk == 0) *reinterpret_cast<f32x4*>(a.sum + (slot0 + m) * a.rp + j) = v;
+      T* o = op + m * pitch + j;
       if constexpr (XT == RQ_DTYPE_F32) {
         *reinterpret_cast<f32x4*>(o) = v;
       } else {
@@ -433,40 +381,131 @@ __global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(EDGE
       }
     }
   }
-  __syncthreads();
+  if (!FACTOR_ROWS) __syncthreads();
+  const bool rows_here = 16 * block < tile.count;
 #pragma unroll 1
-  for (int it = 0; it < a.iters; ++it) {
-    const int64_t c0 = ((int64_t(chunk) * a.iters + it) * kMlWaves + wave) * (16 * V);
-    if (c0 >= a.C) return;
-    if constexpr (EDGES) {
-      if (!expand_full<XT, FACTOR_ROWS>(a, c0)) {
-        expand_step<XT, FACTOR_ROWS, false>(a, w, c0);
-        continue;
+  for (int it = 0; it < a.iters * BLOCKS; ++it) {
+    const int64_t w0 = c_first + int64_t(it) * (GROUPS * L::kCols);  // of the workgroup
+    if (w0 >= a.C) return;
+    const int64_t c0 = w0 + group * L::kCols, col = c0 + V * i16;
+    const bool here = rows_here && c0 < a.C;
+    u32x4 base[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      base[q] = u32x4{0u, 0u, 0u, 0u};
+      const T* p = static_cast<const T*>(a.base) + row[q] * a.ld_base + col;
+      if (a.base && here) base[q] = EDGES ? load16_part<XT>(p, a.C - col) : load16_any(p);
+    }
+    f32x4 acc[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (adapted) {
+#pragma unroll 1
+      for (int k = 0; k < steps; ++k) {
+        u32x4 f[V];
+        const int j = k * kStep + (half ? V * (g & 1) : V * g);
+        if constexpr (FACTOR_ROWS) {
+          stage();
+          __syncthreads();
+          if (k + 1 < steps) fetch(w0, (k + 1) * kStep);
+          else if (it + 1 < a.iters * BLOCKS && w0 + GROUPS * L::kCols < a.C) fetch(w0 + GROUPS * L::kCols, 0);
+          const T* p = lds + (group * L::kCols + V * i16) * sp + (group * 16 + i16) * V + (j - k * kStep);
+#pragma unroll
+          for (int c = 0; c < V; ++c) f[c] = load16_any(p + c * sp);
+          if (j + V > a.r) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t keep;
+              if constexpr (XT == RQ_DTYPE_F32) keep = j + e < a.r ? ~0u : 0u;
+              else keep = j + 2 * e + 1 < a.r ? ~0u : (j + 2 * e < a.r ? 0xFFFFu : 0u);
+#pragma unroll
+              for (int c = 0; c < V; ++c) f[c][e] &= keep;
+            }
+          }
+        } else if (here) {
+          factor_of_rows<XT, EDGES>(f, s, a.C, EDGES && col >= a.C ? 0 : col, a.r, j);
+        }
+        if (here) {
+          const T* u = op + (16 * block + i16) * pitch + k * kStep + V * g;
+          const u32x4 hi = *reinterpret_cast<const u32x4*>(u);
+#pragma unroll
+          for (int c = 0; c < V; ++c) acc[c] = mma<XT>(hi, f[c], acc[c]);
+          if (XT != RQ_DTYPE_F32 && !half) {
+            const u32x4 lo = *reinterpret_cast<const u32x4*>(u + a.rp);
+#pragma unroll
+            for (int c = 0; c < V; ++c) acc[c] = mma<XT>(lo, f[c], acc[c]);
+          }
+        }
+        if (FACTOR_ROWS) __syncthreads();
       }
     }
-    expand_step<XT, FACTOR_ROWS, true>(a, w, c0);
+    if (!here) continue;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float v[V];
+      unpack16<XT>(base[q], v);
+      if (adapted) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = __fadd_rn(v[e], __fmul_rn(scale, acc[e][q]));
+      }
+      T* o = static_cast<T*>(a.out) + row[q] * a.ld_out + col;
+      if (!on[q]) continue;
+      if constexpr (EDGES) store16_part<XT>(o, v, a.C - col);
+      else store16_any(o, pack16<XT>(v));
+    }
   }
+}
+
+template <int XT, bool FACTOR_ROWS, bool EDGES>
+__global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(EDGES ? 2 : 3))) void expand_kernel(ExpandArgs a) {
+  typedef typename Elem<XT>::T T;
+  extern __shared__ uint32_t expand_lds[];
+  T* lds = reinterpret_cast<T*>(expand_lds);
+  const int chunk = int(blockIdx.x % unsigned(a.chunks)), t = int(blockIdx.x / unsigned(a.chunks));
+  const Tile tile = plan_tile(a.rows, t);
+  if (tile.count == 0) return;
+  if (tile.adapter < 0 && a.base == a.out && a.ld_base == a.ld_out) return;  // in place, nothing to add
+  if (tile.count <= 16) expand_body<XT, FACTOR_ROWS, EDGES, 1>(a, tile, t, chunk, lds);
+  else if (tile.count <= 32) expand_body<XT, FACTOR_ROWS, EDGES, 2>(a, tile, t, chunk, lds);
+  else expand_body<XT, FACTOR_ROWS, EDGES, 4>(a, tile, t, chunk, lds);
 }
 
 template <int XT, bool FACTOR_ROWS>
 int run_expand(ExpandArgs a, int cus, hipStream_t stream) {
-  const int64_t cols = int64_t(kMlWaves) * 16 * Elem<XT>::kVec, steps = ceil_div(a.C, cols);
-  const int64_t halves = int64_t(a.rows.T) * (kTileRows / (16 * kExpandBlocks));
-  // steps of a workgroup: as many as leave eight workgroups a compute unit
-  a.iters = int(std::max<int64_t>(1, std::min<int64_t>(8, halves * steps / (8 * cus))));
+  typedef ExpandLds<XT> L;
+  constexpr int V = Elem<XT>::kVec, es = int(sizeof(typename Elem<XT>::T));
+  const int64_t steps = ceil_div(a.C, int64_t(kMlWaves) * L::kCols);
+#ifndef RQ_EX_WGS
+#define RQ_EX_WGS 4
+#endif
+  // steps of a workgroup: as many as leave four workgroups a compute unit
+  a.iters = int(std::max<int64_t>(1, std::min<int64_t>(8, a.rows.T * steps / (RQ_EX_WGS * cus))));
   a.chunks = int(ceil_div(steps, a.iters));
-  if (halves * a.chunks > kMaxThreads1D / kMlThreads) return RQ_ERR_UNSUPPORTED;
-  const size_t bytes = size_t(16 * kExpandBlocks) * (a.rp * 4 + 16);
-  const bool whole = a.C % (16 * Elem<XT>::kVec) == 0 && expand_full<XT, FACTOR_ROWS>(a, a.C - 16 * Elem<XT>::kVec);
-  const unsigned grid = unsigned(halves * a.chunks);
-  if (whole) expand_kernel<XT, FACTOR_ROWS, false><<<grid, kMlThreads, bytes, stream>>>(a);
-  else expand_kernel<XT, FACTOR_ROWS, true><<<grid, kMlThreads, bytes, stream>>>(a);
+  if (int64_t(a.rows.T) * a.chunks > kMaxThreads1D / kMlThreads) return RQ_ERR_UNSUPPORTED;
+  // LDS: the staged columns and the operands of 1, 2 or 4 row blocks, whichever is largest
+  const int pitch = (es == 4 ? a.rp : 2 * a.rp) + V;
+  size_t bytes = 0;
+  for (int blocks = 1; blocks <= kMlWaves; blocks *= 2)
+    bytes = std::max(bytes, size_t((FACTOR_ROWS ? kMlWaves / blocks * L::kStage : 0) + 16 * blocks * pitch) * es);
+  const bool edges = a.C % L::kCols != 0 || (FACTOR_ROWS && a.r > Elem<XT>::kStep && a.r % V != 0);
+  const unsigned grid = unsigned(int64_t(a.rows.T) * a.chunks);
+  if (edges) expand_kernel<XT, FACTOR_ROWS, true><<<grid, kMlThreads, bytes, stream>>>(a);
+  else expand_kernel<XT, FACTOR_ROWS, false><<<grid, kMlThreads, bytes, stream>>>(a);
   return rq_check_launch();
 }
 
 // ---- finish ---------------------------------------------------------------------
-// The splits' sum times the adapter's scaling, as rank-major operands of the row sums.  A
-// thread takes eight slots of one rank.  Slots of a tile past its rows get zeros.
+// The splits' sum times the adapter's scaling, as the operands of the row sums, in the order
+// in which their lanes load them: for 32 slots and 16 ranks, 1 KiB of hi parts and 1 KiB of
+// lo parts (fp32: of slots 8 g .. 8 g + 3 and the four after them), 16 bytes of lane (i, g)
+// = rank i, slots 8 g .. 8 g + 7.  A thread takes eight slots of one rank.  Slots of a tile
+// past its rows get zeros.
+template <int XT>
+__device__ __forceinline__ int64_t opt_at(int64_t slot, int rank, int rp) {  // slot: a multiple of 8
+  constexpr int kBlock = XT == RQ_DTYPE_F32 ? 512 : 1024, kLane = Elem<XT>::kVec;
+  return ((slot >> 5) * (rp >> 4) + (rank >> 4)) * kBlock + ((rank & 15) + 2 * (slot & 24)) * kLane;
+}
+
 template <int XT>
 __global__ __launch_bounds__(kMlThreads) void finish_kernel(FinishArgs a, unsigned per_job) {
   typedef typename Elem<XT>::T T;
@@ -502,17 +541,16 @@ __global__ __launch_bounds__(kMlThreads) void finish_kernel(FinishArgs a, unsign
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = e < live ? __fmul_rn(v[e], scale) : 0.0f;
-  T* o = static_cast<T*>(J.opt) + int64_t(j) * slots + s0;
+  T* o = static_cast<T*>(J.opt) + opt_at<XT>(s0, j, a.rp);
   if constexpr (XT == RQ_DTYPE_F32) {
-    reinterpret_cast<f32x4*>(o)[0] = f32x4{v[0], v[1], v[2], v[3]};
-    reinterpret_cast<f32x4*>(o)[1] = f32x4{v[4], v[5], v[6], v[7]};
+    *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4*>(o + 256) = f32x4{v[4], v[5], v[6], v[7]};
   } else {
     uint32_t hi[8], lo[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) split16<XT>(v[e], hi[e], lo[e]);
     *reinterpret_cast<u32x4*>(o) = u32x4{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, hi[4] | hi[5] << 16, hi[6] | hi[7] << 16};
-    *reinterpret_cast<u32x4*>(o + int64_t(a.rp) * slots) =
-        u32x4{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16, lo[4] | lo[5] << 16, lo[6] | lo[7] << 16};
+    *reinterpret_cast<u32x4*>(o + 512) = u32x4{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16, lo[4] | lo[5] << 16, lo[6] | lo[7] << 16};
   }
 }
 
@@ -528,10 +566,8 @@ int run_finish(const FinishArgs& a, hipStream_t stream) {
 // D[c][j] = sum_m x[row m][c] u[m][j], the contraction over the slow index of x: lane
 // (i, g) loads CW columns of the eight rows of slots 8 g .. 8 g + 7, which byte permutes
 // turn into CW operand rows of eight consecutive slots (16-bit; fp32 values are operands
-// as they are).  A wave walks over the rows of a chunk, 32 slots a step, with 16 CW
-// columns of its own; the next step's rows and operands are loaded over this one's
-// products.  A workgroup's four waves are adjacent columns, so that they share the
-// operands in the L1.
+// as they are).  A workgroup takes 16 CW columns over the rows of a chunk, 32 slots a
+// step; its four waves take steps in turn and meet in LDS, summed as (0 + 2) + (1 + 3).
 template <int XT, int CW>
 struct ColPiece {
   static constexpr int kWords = XT == RQ_DTYPE_F32 ? CW : CW / 2;
@@ -622,21 +658,22 @@ struct RowSumChunk {
   int64_t live;  // slots from the first of tile t0 on
 };
 
-template <int XT, int JB, bool CODES, bool RANK_MAJOR>
-__device__ __forceinline__ void rowsum_body(const RowSumArgs& a, const RowSumTask& K, const RowSumChunk& ch, int64_t c0, int j0) {
+template <int XT, int JB, bool CODES>
+__device__ __forceinline__ void rowsum_body(const RowSumArgs& a, const RowSumTask& K, const RowSumChunk& ch, int64_t c0, int j0,
+                                            float (*red)[16 * rowsum_cw<XT>(JB)][16 * JB + 1]) {
   typedef typename Elem<XT>::T T;
   constexpr int CW = rowsum_cw<XT>(JB);
   constexpr int kWords = ColPiece<XT, CW>::kWords;
   constexpr int kPlanes = XT == RQ_DTYPE_F32 ? 1 : 2;
   constexpr int kOps = XT == RQ_DTYPE_F32 ? 2 : 1;  // 16-byte operands of eight slots
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t col = c0 + CW * i16;
-  const bool full = c0 + 16 * CW <= K.C;            // of the wave
+  const bool full = c0 + 16 * CW <= K.C;            // all columns
   const int64_t lcol = full || col < K.C ? col : 0;  // lanes past the end repeat column 0: their sums are not stored
-  const int64_t slots = a.rows.slots(), base = int64_t(kTileRows) * ch.t0;
-  const T* opt = static_cast<const T*>(K.opt) + int64_t(j0 + i16) * slots + base + 8 * g;
+  const int64_t base = int64_t(kTileRows) * ch.t0;
+  const T* opt = static_cast<const T*>(K.opt) + opt_at<XT>(base + 8 * g, j0 + i16, a.rp);
 
-  // D as columns x ranks (RANK_MAJOR), or as ranks x columns: a register quad is stored as it lies
   f32x4 acc[CW][JB];
 #pragma unroll
   for (int c = 0; c < CW; ++c)
@@ -675,7 +712,7 @@ __device__ __forceinline__ void rowsum_body(const RowSumArgs& a, const RowSumTas
       for (int p = 0; p < kPlanes; ++p)
 #pragma unroll
         for (int k = 0; k < kOps; ++k)
-          o.u[j][p][k] = *reinterpret_cast<const u32x4*>(opt + (int64_t(p) * a.rp + 16 * j) * slots + s + 4 * k);
+          o.u[j][p][k] = *reinterpret_cast<const u32x4*>(opt + opt_at<XT>(s, 16 * j, a.rp) + 512 * p + 256 * k);
   };
   auto products = [&](const Raw (&raw)[8], const Ops& o, const int (&r)[8], bool last) {
     ColPiece<XT, CW> row[8];
@@ -695,7 +732,7 @@ __device__ __forceinline__ void rowsum_body(const RowSumArgs& a, const RowSumTas
 #pragma unroll
           for (int j = 0; j < JB; ++j) {
             const float x = u2f(row[e].d[c]), u = u2f(o.u[j][0][e >> 2][e & 3]);
-            acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(RANK_MAJOR ? x : u, RANK_MAJOR ? u : x, acc[c][j], 0, 0, 0);
+            acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, u, acc[c][j], 0, 0, 0);
           }
     } else {
 #pragma unroll
@@ -708,67 +745,67 @@ __device__ __forceinline__ void rowsum_body(const RowSumArgs& a, const RowSumTas
         for (int p = 0; p < kPlanes; ++p)
 #pragma unroll
           for (int j = 0; j < JB; ++j)
-            acc[c][j] = RANK_MAJOR ? mma<XT>(x, o.u[j][p][0], acc[c][j]) : mma<XT>(o.u[j][p][0], x, acc[c][j]);
+            acc[c][j] = mma<XT>(x, o.u[j][p][0], acc[c][j]);
       }
     }
   };
+  // this step's operands, which the L2 has, are asked for behind its rows and before the
+  // next step's rows, so that the wait for them leaves those in flight
   const int64_t live = ch.live;
-  if (live > 0) {
-    // the next step's rows are known before its values are asked for; two to three waves a
-    // SIMD with eight loads each hide the memory's latency
+  constexpr int64_t kAhead = 32 * kMlWaves;
+  int64_t s = 32 * wave;
+  if (s < live) {
     int r0[8], r1[8];
-    rows_of(r0, 0);
-    for (int64_t s = 0; s < live; s += 32) {
-      Raw x[8];
-      Ops o;
-      load(x, r0);
+    Raw x0[8], x1[8];
+    Ops o;
+    rows_of(r0, s);
+    load(x0, r0);
+    if (s + kAhead < live) rows_of(r1, s + kAhead);
+    for (;;) {
       operands(o, s);
-      if (s + 32 < live) rows_of(r1, s + 32);
-      products(x, o, r0, s + 32 > live);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) r0[e] = r1[e];
+      if (s + kAhead < live) load(x1, r1);
+      products(x0, o, r0, s + 32 > live);
+      if ((s += kAhead) >= live) break;
+      if (s + kAhead < live) rows_of(r0, s + kAhead);
+      operands(o, s);
+      if (s + kAhead < live) load(x0, r0);
+      products(x1, o, r1, s + 32 > live);
+      if ((s += kAhead) >= live) break;
+      if (s + kAhead < live) rows_of(r1, s + kAhead);
     }
   }
-  const int64_t n = K.C * a.r;
+  // register q of lane (i, g): column CW (4 g + q) + c, rank i
+#pragma unroll
+  for (int ph = 0; ph < 2; ++ph) {
+    if ((wave >> 1) == 1 - ph) {
+#pragma unroll
+      for (int c = 0; c < CW; ++c)
+#pragma unroll
+        for (int j = 0; j < JB; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float& v = red[wave & 1][CW * (4 * g + q) + c][16 * j + i16];
+            v = ph == 0 ? acc[c][j][q] : __fadd_rn(acc[c][j][q], v);
+          }
+    }
+    __syncthreads();
+  }
+  const int cols = int(std::min<int64_t>(K.C - c0, 16 * CW)), ranks = std::min(a.r - j0, 16 * JB);
   float* part = ch.slot >= 0 ? a.part + ch.slot * a.part_size + K.part_off : nullptr;
-  T* out = static_cast<T*>(K.out) + ch.adapter * n;
-  if constexpr (RANK_MAJOR) {
-    // register q of lane (i, g): column CW (4 g + q) + c, rank i
-#pragma unroll
-    for (int j = 0; j < JB; ++j) {
-      const int rank = j0 + 16 * j + i16;
-      if (rank >= a.r) continue;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int c = 0; c < CW; c += 4) {
-          const int64_t at = c0 + CW * (4 * g + q) + c, to = int64_t(rank) * K.C + at;
-          const float v[4] = {acc[c][j][q], acc[c + 1][j][q], acc[c + 2][j][q], acc[c + 3][j][q]};
-          if (part) store4<RQ_DTYPE_F32>(part + to, v, K.C - at);
-          else store4<XT>(out + to, v, K.C - at);
-        }
-    }
-  } else {
-    // register q of lane (i, g): rank 4 g + q, column CW i + c
-#pragma unroll
-    for (int c = 0; c < CW; ++c) {
-      if (col + c >= K.C) continue;
-#pragma unroll
-      for (int j = 0; j < JB; ++j) {
-        const int rank = j0 + 16 * j + 4 * g;
-        const float v[4] = {acc[c][j][0], acc[c][j][1], acc[c][j][2], acc[c][j][3]};
-        const int64_t to = (col + c) * a.r + rank;
-        if (part) store4<RQ_DTYPE_F32>(part + to, v, a.r - rank);
-        else store4<XT>(out + to, v, a.r - rank);
-      }
-    }
+  T* out = static_cast<T*>(K.out) + ch.adapter * K.C * a.r;
+  for (int i = threadIdx.x; i < cols * ranks; i += kMlThreads) {
+    const int c = K.rank_major ? i % cols : i / ranks, j = K.rank_major ? i / cols : i % ranks;
+    const float v = __fadd_rn(red[0][c][j], red[1][c][j]);
+    const int64_t to = K.rank_major ? int64_t(j0 + j) * K.C + c0 + c : (c0 + c) * a.r + j0 + j;
+    if (part) part[to] = v;
+    else out[to] = from_f32<XT>(v);
   }
 }
 
 template <int XT, int JB>
 __global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(2))) void rowsum_kernel(RowSumArgs a) {
   constexpr int kCols = 16 * rowsum_cw<XT>(JB);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ float red[2][kCols][16 * JB + 1];
   RowSumChunk ch{0, 0, -1, 0};
   int t1;
   if (a.rows.p) {
@@ -789,12 +826,10 @@ __global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(2)))
   if (t1 > ch.t0) ch.live = int64_t(kTileRows) * (t1 - 1 - ch.t0) + plan_tile(a.rows, t1 - 1).count;
   const int which = int(blockIdx.x) >= a.t[0].tiles ? 1 : 0;
   const RowSumTask& K = a.t[which];
-  const int64_t c0 = (int64_t(int(blockIdx.x) - (which ? a.t[0].tiles : 0)) * kMlWaves + wave) * kCols;
-  if (c0 >= K.C) return;
+  const int64_t c0 = int64_t(int(blockIdx.x) - (which ? a.t[0].tiles : 0)) * kCols;
   const int j0 = 16 * JB * int(blockIdx.z);
-  if (!K.rank_major) rowsum_body<XT, JB, false, false>(a, K, ch, c0, j0);
-  else if (K.exps) rowsum_body<XT, JB, true, true>(a, K, ch, c0, j0);
-  else rowsum_body<XT, JB, false, true>(a, K, ch, c0, j0);
+  if (K.exps) rowsum_body<XT, JB, true>(a, K, ch, c0, j0, red);
+  else rowsum_body<XT, JB, false>(a, K, ch, c0, j0, red);
 }
 
 // Adapters of several chunks: their partial sums in order.
@@ -827,8 +862,8 @@ __global__ __launch_bounds__(kMlThreads) void rowsum_finish_kernel(RowSumArgs a)
 
 // The table of chunks: the coarser one, whose sums seldom meet in a second launch, where
 // its workgroups fill the GPU.
-int rowsum_table(const RowsPlan& rows, int64_t cols, int wave_cols, int cus) {
-  const int64_t tiles = ceil_div(cols, int64_t(kMlWaves) * wave_cols);
+int rowsum_table(const RowsPlan& rows, int64_t cols, int wg_cols, int cus) {
+  const int64_t tiles = ceil_div(cols, wg_cols);
   return tiles * ceil_div(ceil_div(rows.M, kTileRows), chunk_least(1)) >= cus ? 1 : 0;
 }
 
@@ -845,7 +880,7 @@ int run_rowsum(RowSumArgs a, hipStream_t stream) {
   int tiles = 0;
   int64_t most = 0;
   for (int i = 0; i < a.n; ++i) {
-    a.t[i].tiles = int(ceil_div(a.t[i].C, int64_t(kMlWaves) * 16 * rowsum_cw<XT>(jb)));
+    a.t[i].tiles = int(ceil_div(a.t[i].C, 16 * rowsum_cw<XT>(jb)));
     tiles += a.t[i].tiles;
     most = std::max(most, a.t[i].C * a.r);
   }
@@ -856,7 +891,7 @@ int run_rowsum(RowSumArgs a, hipStream_t stream) {
   else rowsum_kernel<XT, 4><<<grid, kMlThreads, 0, stream>>>(a);
   const int st = rq_check_launch();
   if (st != RQ_OK || rowsum_parts(a.rows, a.table) == 0) return st;
-  const dim3 fgrid(unsigned(std::min<int64_t>(ceil_div(most, kMlThreads), 1024)), unsigned(a.rows.p ? a.rows.n : 1));
+  const dim3 fgrid(unsigned(std::min<int64_t>(ceil_div(most, kMlThreads), std::max<int64_t>(1024 / a.rows.n, 64))), unsigned(a.rows.p ? a.rows.n : 1));
   rowsum_finish_kernel<XT><<<fgrid, kMlThreads, 0, stream>>>(a);
   return rq_check_launch();
 }
