@@ -323,6 +323,7 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
   const int64_t c_first = int64_t(chunk) * a.iters * (kMlWaves * L::kCols);
   const int steps = adapted ? int(ceil_div(a.rp, kStep)) : 1;    // of ranks
   const int sp = a.r < kStep ? a.r : kStep;                      // ranks of a column in LDS
+  const float per_sp = 1.0f / float(sp);
 
   // this lane's rows (past the tile's last: the first)
   int row[4];
@@ -333,32 +334,35 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
     on[q] = i < tile.count;
     row[q] = plan_row(a.rows, slot0 + (on[q] ? i : 0));
   }
-  // a step's pieces of B, as this thread copies them: piece p of the waves' columns
+  // a step's pieces of B, as this thread copies them: 32-bit offsets from a uniform address
   u32x4 piece[PIECES];
-  auto fetch = [&](int64_t c0, int j0) {
+  uint32_t off[PIECES], put[PIECES];
+  if constexpr (FACTOR_ROWS) {
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
       const int f = V * (tid + kMlThreads * k);
-      int64_t at;
-      bool there;
-      if (a.r <= kStep) {
-        at = c0 * a.r + f;
-        there = f < GROUPS * L::kCols * sp;
-      } else {
-        const int n = f / kStep, j = j0 + f % kStep;
-        at = (c0 + n) * a.r + j;
-        there = j < a.r;
-      }
-      const int64_t left = a.C * a.r - at;
-      if constexpr (EDGES) piece[k] = load16_part<XT>(s + at, there ? left : 0);
-      else piece[k] = load16_any(s + (there && left > 0 ? at : 0));
+      off[k] = uint32_t(a.r <= kStep ? f : f / kStep * a.r + f % kStep);
+      // f / (V sp), exact: the quotient is 1 / (2 sp) or more from an integer
+      put[k] = uint32_t(f + int((float(f / V) + 0.5f) * per_sp) * V);
+    }
+  }
+  auto fetch = [&](int64_t c0, int j0) {
+    const T* from = s + c0 * a.r + j0;
+    const int64_t left = (a.C - c0) * a.r - j0;
+    const uint32_t end = uint32_t(left < INT32_MAX ? left : INT32_MAX);
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+      const int f = V * (tid + kMlThreads * k);
+      const bool there = a.r <= kStep ? f < GROUPS * L::kCols * sp : j0 + f % kStep < a.r;
+      if constexpr (EDGES) piece[k] = load16_part<XT>(from + off[k], there && off[k] < end ? int64_t(end - off[k]) : 0);
+      else piece[k] = load16_any(from + (there && off[k] < end ? off[k] : 0u));
     }
   };
   auto stage = [&]() {
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
       const int f = V * (tid + kMlThreads * k);
-      if (f < GROUPS * L::kCols * sp) *reinterpret_cast<u32x4*>(lds + f + f / (V * sp) * V) = piece[k];
+      if (f < GROUPS * L::kCols * sp) *reinterpret_cast<u32x4*>(lds + put[k]) = piece[k];
     }
   };
   if (FACTOR_ROWS && adapted) fetch(c_first, 0);
@@ -389,6 +393,10 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
     if (w0 >= a.C) return;
     const int64_t c0 = w0 + group * L::kCols, col = c0 + V * i16;
     const bool here = rows_here && c0 < a.C;
+    auto ahead = [&](int k) {  // the next step's pieces
+      if (k + 1 < steps) fetch(w0, (k + 1) * kStep);
+      else if (it + 1 < a.iters * BLOCKS && w0 + GROUPS * L::kCols < a.C) fetch(w0 + GROUPS * L::kCols, 0);
+    };
     u32x4 base[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -407,8 +415,7 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
         if constexpr (FACTOR_ROWS) {
           stage();
           __syncthreads();
-          if (k + 1 < steps) fetch(w0, (k + 1) * kStep);
-          else if (it + 1 < a.iters * BLOCKS && w0 + GROUPS * L::kCols < a.C) fetch(w0 + GROUPS * L::kCols, 0);
+          if (BLOCKS > 1) ahead(k);
           const T* p = lds + (group * L::kCols + V * i16) * sp + (group * 16 + i16) * V + (j - k * kStep);
 #pragma unroll
           for (int c = 0; c < V; ++c) f[c] = load16_any(p + c * sp);
@@ -436,7 +443,10 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
             for (int c = 0; c < V; ++c) acc[c] = mma<XT>(lo, f[c], acc[c]);
           }
         }
-        if (FACTOR_ROWS) __syncthreads();
+        if constexpr (FACTOR_ROWS) {
+          __syncthreads();
+          if (BLOCKS == 1) ahead(k);  // eight pieces: not over the products, for the registers
+        }
       }
     }
     if (!here) continue;
