@@ -2,7 +2,7 @@
 // workgroup, stable and without an atomic whose order shows.  Each of eight waves
 // counts its own stretch of the rows, the counts are summed over waves and
 // adapters, and each wave then places its stretch 64 rows at a time, rows of the
-// same adapter ranked by a ballot.  Bound by latency: it runs once for a batch,
+// same adapter found by a ballot for each bit of its number.  Bound by latency: it runs once for a batch,
 // for all the projections of all its layers.
 #include "rq_launch.h"
 #include "rq_rows.h"
@@ -37,7 +37,8 @@ __global__ __launch_bounds__(kArThreads) void adapter_rows_kernel(const int32_t*
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = P.n;
   const int64_t M = P.M;
-  for (int i = tid; i < kArWaves * (kMaxAdapters + 1); i += kArThreads) (&hist[0][0])[i] = 0;
+  for (int w = 0; w < kArWaves; ++w)
+    for (int a = tid; a <= n; a += kArThreads) hist[w][a] = 0;
   __syncthreads();
   const int64_t per = ceil_div(ceil_div(M, kArWaves), 64) * 64;
   const int64_t r0 = per * wave < M ? per * wave : M, r1 = r0 + per < M ? r0 + per : M;
@@ -67,14 +68,14 @@ __global__ __launch_bounds__(kArThreads) void adapter_rows_kernel(const int32_t*
     int used[kChunkTables];
 #pragma unroll
     for (int k = 0; k < kChunkTables; ++k) {
-      const int per_chunk = RowsPlan::chunk_tiles(carry, k);
       int chunks = 0, parts = 0;
       int32_t* tab = plan + P.off_chunks() + 4 * int64_t(P.C) * k;
       int32_t* part = plan + P.off_part() + 2 * int64_t(n) * k;
       for (int a0 = 0; a0 < n; a0 += 64) {
         const int a = a0 + lane;
         const int tiles = a < n ? (total[a] + kTileRows - 1) / kTileRows : 0;
-        const int c = a < n ? (tiles > per_chunk ? (tiles + per_chunk - 1) / per_chunk : 1) : 0;
+        const Chunks ch = adapter_chunks(tiles, carry, k);
+        const int c = a < n ? ch.n : 0;
         const int c0 = wave_excl(c, chunks), p0 = wave_excl(c > 1 ? c : 0, parts);
         const int t0 = a < n ? first[a] : 0;  // this lane's own store above
         if (a < n) {
@@ -82,7 +83,7 @@ __global__ __launch_bounds__(kArThreads) void adapter_rows_kernel(const int32_t*
           part[2 * a + 1] = p0;
         }
         for (int i = 0; i < c; ++i) {
-          const int b = t0 + i * per_chunk, e = b + per_chunk < t0 + tiles ? b + per_chunk : t0 + tiles;
+          const int b = t0 + i * ch.tiles, e = b + ch.tiles < t0 + tiles ? b + ch.tiles : t0 + tiles;
           tab[4 * (c0 + i)] = a;
           tab[4 * (c0 + i) + 1] = b;
           tab[4 * (c0 + i) + 2] = e;
@@ -103,27 +104,33 @@ __global__ __launch_bounds__(kArThreads) void adapter_rows_kernel(const int32_t*
       else hi = mid - 1;
     }
     const int left = total[lo] - kTileRows * (t - first[lo]);
-    plan[16 + t] = lo < n ? lo : -1;
-    plan[P.off_count() + t] = left < kTileRows ? left : kTileRows;
+    plan[16 + 2 * t] = lo < n ? lo : -1;
+    plan[16 + 2 * t + 1] = left < kTileRows ? left : kTileRows;
     // the slots after the last row of an adapter
     for (int s = left; s < kTileRows; ++s) plan[P.off_rows() + int64_t(kTileRows) * t + s] = -1;
   }
+  for (int t = tiles + tid; t < P.T; t += kArThreads) {
+    plan[16 + 2 * t] = -1;
+    plan[16 + 2 * t + 1] = 0;
+  }
+  const int bits = 32 - __clz(n);
   for (int64_t b = r0; b < r1; b += 64) {
     const int64_t r = b + lane;
-    const int a = r < r1 ? adapter_of(ids, r, n) : -1;
-    unsigned long long left = __ballot(r < r1);
-    while (left) {
-      const int la = __shfl(a, int(__ffsll(left)) - 1);
-      const unsigned long long same = __ballot(a == la);
-      const int base = hist[wave][la];
-      if (a == la) {
-        const int place = base + __popcll(same & ((1ull << lane) - 1));
-        plan[P.off_rows() + int64_t(kTileRows) * first[la] + place] = int32_t(r);
-      }
-      if (lane == 0) hist[wave][la] = base + __popcll(same);
-      __builtin_amdgcn_wave_barrier();
-      left &= ~same;
+    const bool on = r < r1;
+    const int a = on ? adapter_of(ids, r, n) : 0;
+    unsigned long long same = __ballot(on);  // the lanes with this one's adapter: alike in every bit
+    for (int k = 0; k < bits; ++k) {
+      const unsigned long long set = __ballot(a >> k & 1);
+      same &= a >> k & 1 ? set : ~set;
     }
+    const unsigned long long before = same & ((1ull << lane) - 1);
+    if (on) {
+      const int base = hist[wave][a];
+      plan[P.off_rows() + int64_t(kTileRows) * first[a] + base + __popcll(before)] = int32_t(r);
+      __builtin_amdgcn_wave_barrier();  // all lanes have read before the first of each adapter writes
+      if (!before) hist[wave][a] = base + __popcll(same);
+    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 

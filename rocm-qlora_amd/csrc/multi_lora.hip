@@ -35,9 +35,9 @@ __device__ __forceinline__ void split16(float v, uint32_t& hi, uint32_t& lo) {
 // tile's 16-row blocks (1 to 4, as many as the tile has) times JB blocks of 16 ranks,
 // so that a factor's piece is loaded once for the tile.
 //
-// The factor goes through a wave's own piece of LDS.  A [r][K]: a step's 64 bytes of each
-// rank, whose four pieces are exchanged by the rank so that the lanes of a read meet other
-// banks.  B [N][r] (TURNED), whose rows run across the contraction: a step's rows are one
+// Rows and factor go through a wave's own piece of LDS.  Rows and A [r][K]: a step's 64
+// bytes of each, loaded by four adjacent lanes, the four pieces exchanged by the row so that
+// the lanes of a read meet other banks.  B [N][r] (TURNED), whose rows run across the contraction: a step's rows are one
 // piece of memory, copied as it lies (with 32 bytes between eight-row groups, so that the
 // four lane groups read other banks) and read back a rank's values at a time.
 constexpr int kShWaves = 4;
@@ -50,11 +50,13 @@ struct ShrinkLds {
   // elements of one wave's step, with the gaps
   static constexpr int kGap = 32 / int(sizeof(typename Elem<XT>::T));
   static constexpr int kTurn = Elem<XT>::kStep * 16 * JB + 4 * kGap + 2 * Elem<XT>::kVec;  // whole 16 bytes; the last kVec: no one's
-  static constexpr int kTurnFloats = kShWaves * kTurn * int(sizeof(typename Elem<XT>::T)) / 4;
+  static constexpr int kRows = 64 * 4 * Elem<XT>::kVec;  // of the tile's rows, a step
+  static constexpr int kTurnFloats = kShWaves * (kTurn + kRows) * int(sizeof(typename Elem<XT>::T)) / 4;
 };
 
 template <int XT, int NRB, int JB, bool TURNED>
-__device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& tile, int t, int split, int j0, float* lds) {
+__device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& tile, const int (&row)[4], int t, int split, int j0,
+                                            float* lds) {
   typedef typename Elem<XT>::T T;
   typedef ShrinkLds<XT, JB> L;
   constexpr int V = Elem<XT>::kVec, kStep = Elem<XT>::kStep;
@@ -66,10 +68,8 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
   const T* xr[NRB];
 #pragma unroll
   for (int b = 0; b < NRB; ++b) {
-    const int i = 16 * b + i16;
-    // rows past the tile's last repeat its first: their sums are not read
-    const int row = plan_row(a.rows, slot0 + (i < tile.count ? i : 0));
-    xr[b] = static_cast<const T*>(a.x) + int64_t(row) * a.ldx + V * g;
+    // the row is asked for along with the tile; past the tile's last, row 0: its sums are not read
+    xr[b] = static_cast<const T*>(a.x) + int64_t(row[b] < 0 ? 0 : row[b]) * a.ldx + V * (lane & 3);
   }
   const T* sr[JB];
   bool jlive[JB];
@@ -78,11 +78,14 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
     const int j = j0 + 16 * b + i16;
     jlive[b] = j < a.r;
   }
+  // 16 rows of four pieces: piece p of row m lies at 4 m + (p ^ m / 2)
+  const int xput = V * (4 * (lane >> 2) + ((lane ^ lane >> 3) & 3)), xget = V * (4 * i16 + ((g ^ i16 >> 1) & 3));
   // TURNED: a step's pieces of V values.  Up to 64 ranks lie end to end in LDS as in memory;
   // of more, this rank block's 64 of each row.  Lanes without a piece repeat the first and
   // put it past the step.
   const int pitch = a.r <= 64 ? a.r : 64;
-  T* turn = reinterpret_cast<T*>(lds) + wave * L::kTurn;
+  T* turn = reinterpret_cast<T*>(lds) + wave * (L::kTurn + L::kRows);
+  T* xl = turn + L::kTurn;
   int put[JB];
   if constexpr (TURNED) {
 #pragma unroll
@@ -95,9 +98,9 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
   } else {
 #pragma unroll
     for (int b = 0; b < JB; ++b) {
-      const int row = 16 * b + (lane >> 2);
-      put[b] = V * (4 * row + ((lane ^ row >> 1) & 3));
-      sr[b] = s0 + int64_t(j0 + row < a.r ? j0 + row : 0) * a.K + V * (lane & 3);
+      const int j = j0 + 16 * b + (lane >> 2);
+      put[b] = V * 64 * b + xput;
+      sr[b] = s0 + int64_t(j < a.r ? j : 0) * a.K + V * (lane & 3);
     }
   }
   f32x4 acc[NRB][JB];
@@ -120,7 +123,12 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
   auto products = [&](const u32x4 (&xv)[NRB], const u32x4 (&sv)[JB]) {
 #pragma unroll
     for (int j = 0; j < JB; ++j) *reinterpret_cast<u32x4*>(turn + put[j]) = sv[j];
+#pragma unroll
+    for (int b = 0; b < NRB; ++b) *reinterpret_cast<u32x4*>(xl + V * 64 * b + xput) = xv[b];
     __builtin_amdgcn_wave_barrier();
+    u32x4 xo[NRB];
+#pragma unroll
+    for (int b = 0; b < NRB; ++b) xo[b] = *reinterpret_cast<const u32x4*>(xl + V * 64 * b + xget);
 #pragma unroll
     for (int j = 0; j < JB; ++j) {
       u32x4 f;
@@ -132,13 +140,12 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
           else f[e] = uint32_t(p[2 * e * pitch]) | uint32_t(p[(2 * e + 1) * pitch]) << 16;
         }
       } else {
-        const int row = 16 * j + i16;
-        f = *reinterpret_cast<const u32x4*>(turn + V * (4 * row + ((g ^ row >> 1) & 3)));
+        f = *reinterpret_cast<const u32x4*>(turn + V * 64 * j + xget);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] = jlive[j] ? f[e] : 0u;
 #pragma unroll
-      for (int b = 0; b < NRB; ++b) acc[b][j] = mma<XT>(xv[b], f, acc[b][j]);
+      for (int b = 0; b < NRB; ++b) acc[b][j] = mma<XT>(xo[b], f, acc[b][j]);
       __builtin_amdgcn_sched_barrier(0);  // one rank block's reads at a time in registers
     }
     __builtin_amdgcn_wave_barrier();  // the next step's copy comes after these reads
@@ -167,7 +174,7 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
   k = kb + steps * kStep;
   if (k < ke) {  // the end of the rows
 #pragma unroll
-    for (int b = 0; b < NRB; ++b) x[0][b] = load16_part<XT>(xr[b] + k, ke - k - V * g);
+    for (int b = 0; b < NRB; ++b) x[0][b] = load16_part<XT>(xr[b] + k, ke - k - V * (lane & 3));
 #pragma unroll
     for (int j = 0; j < JB; ++j) {
       if constexpr (TURNED) s[0][j] = load16_part<XT>(sr[j] + k * a.r, (a.K - k) * a.r - (sr[j] - s0));
@@ -203,10 +210,13 @@ __global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(JB =
   const int t = int(blockIdx.x % unsigned(a.rows.T)), split = int(blockIdx.x / unsigned(a.rows.T));
   const int j0 = 16 * JB * int(blockIdx.y);
   const Tile tile = plan_tile(a.rows, t);
+  int row[4];  // of the lane's loads: lane / 4 in each 16-row block
+#pragma unroll
+  for (int b = 0; b < 4; ++b) row[b] = plan_row(a.rows, int64_t(kTileRows) * t + 16 * b + ((threadIdx.x & 63) >> 2));
   if (tile.count == 0 || tile.adapter < 0) return;
-  if (tile.count <= 16) shrink_body<XT, 1, JB, TURNED>(a, tile, t, split, j0, lds);
-  else if (tile.count <= 32) shrink_body<XT, 2, JB, TURNED>(a, tile, t, split, j0, lds);
-  else shrink_body<XT, 4, JB, TURNED>(a, tile, t, split, j0, lds);
+  if (tile.count <= 16) shrink_body<XT, 1, JB, TURNED>(a, tile, row, t, split, j0, lds);
+  else if (tile.count <= 32) shrink_body<XT, 2, JB, TURNED>(a, tile, row, t, split, j0, lds);
+  else shrink_body<XT, 4, JB, TURNED>(a, tile, row, t, split, j0, lds);
 }
 
 // About RQ_SH_WGS workgroups a compute unit, each wave with at least four steps.
@@ -325,15 +335,10 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
   const int sp = a.r < kStep ? a.r : kStep;                      // ranks of a column in LDS
   const float per_sp = 1.0f / float(sp);
 
-  // this lane's rows (past the tile's last: the first)
+  // this lane's rows (past the tile's last: -1)
   int row[4];
-  bool on[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int i = 16 * block + 4 * g + q;
-    on[q] = i < tile.count;
-    row[q] = plan_row(a.rows, slot0 + (on[q] ? i : 0));
-  }
+  for (int q = 0; q < 4; ++q) row[q] = plan_row(a.rows, slot0 + 16 * block + 4 * g + q);
   // a step's pieces of B, as this thread copies them: 32-bit offsets from a uniform address
   u32x4 piece[PIECES];
   uint32_t off[PIECES], put[PIECES];
@@ -366,6 +371,16 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
     }
   };
   if (FACTOR_ROWS && adapted) fetch(c_first, 0);
+  u32x4 base[4];
+  auto fetch_base = [&](int64_t at) {  // from column `at` on
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      base[q] = u32x4{0u, 0u, 0u, 0u};
+      const T* p = static_cast<const T*>(a.base) + (row[q] < 0 ? 0 : row[q]) * a.ld_base + at;
+      if (a.base && at - V * i16 < a.C) base[q] = EDGES ? load16_part<XT>(p, a.C - at) : load16_any(p);
+    }
+  };
+  fetch_base(c_first + group * L::kCols + V * i16);
   if (adapted) {
     const int quads = a.rp / 4, rows = (tile.count + 15) & ~15;
     const int64_t stride = a.rows.slots() * a.rp;
@@ -397,13 +412,6 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
       if (k + 1 < steps) fetch(w0, (k + 1) * kStep);
       else if (it + 1 < a.iters * BLOCKS && w0 + GROUPS * L::kCols < a.C) fetch(w0 + GROUPS * L::kCols, 0);
     };
-    u32x4 base[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      base[q] = u32x4{0u, 0u, 0u, 0u};
-      const T* p = static_cast<const T*>(a.base) + row[q] * a.ld_base + col;
-      if (a.base && here) base[q] = EDGES ? load16_part<XT>(p, a.C - col) : load16_any(p);
-    }
     f32x4 acc[V];
 #pragma unroll
     for (int c = 0; c < V; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -449,19 +457,21 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
         }
       }
     }
+    float v[4][V];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) unpack16<XT>(base[q], v[q]);
+    if (it + 1 < a.iters * BLOCKS) fetch_base(col + GROUPS * L::kCols);
     if (!here) continue;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      float v[V];
-      unpack16<XT>(base[q], v);
       if (adapted) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = __fadd_rn(v[e], __fmul_rn(scale, acc[e][q]));
+        for (int e = 0; e < V; ++e) v[q][e] = __fadd_rn(v[q][e], __fmul_rn(scale, acc[e][q]));
       }
+      if (row[q] < 0) continue;
       T* o = static_cast<T*>(a.out) + row[q] * a.ld_out + col;
-      if (!on[q]) continue;
-      if constexpr (EDGES) store16_part<XT>(o, v, a.C - col);
-      else store16_any(o, pack16<XT>(v));
+      if constexpr (EDGES) store16_part<XT>(o, v[q], a.C - col);
+      else store16_any(o, pack16<XT>(v[q]));
     }
   }
 }
@@ -548,6 +558,11 @@ __global__ __launch_bounds__(kMlThreads) void finish_kernel(FinishArgs a, unsign
         for (int e = 0; e < 8; ++e)
           if (k0 + k < J.splits) v[e] = __fadd_rn(v[e], p[k][e]);
     }
+  }
+  if (J.sum) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < live) J.sum[(s0 + e) * a.rp + j] = v[e];
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = e < live ? __fmul_rn(v[e], scale) : 0.0f;
@@ -826,11 +841,11 @@ __global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(2)))
     t1 = c[2];
     ch.slot = c[3];
   } else {
-    const int per = RowsPlan::chunk_tiles(a.rows.T, a.table);
-    ch.t0 = per * int(blockIdx.y);
-    if (ch.t0 >= a.rows.T) return;
-    t1 = ch.t0 + per < a.rows.T ? ch.t0 + per : a.rows.T;
-    if (per < a.rows.T) ch.slot = int(blockIdx.y);
+    const Chunks c = adapter_chunks(a.rows.T, a.rows.T, a.table);
+    if (int(blockIdx.y) >= c.n) return;
+    ch.t0 = c.tiles * int(blockIdx.y);
+    t1 = ch.t0 + c.tiles < a.rows.T ? ch.t0 + c.tiles : a.rows.T;
+    if (c.n > 1) ch.slot = int(blockIdx.y);
   }
   // all tiles of an adapter but its last are full
   if (t1 > ch.t0) ch.live = int64_t(kTileRows) * (t1 - 1 - ch.t0) + plan_tile(a.rows, t1 - 1).count;
@@ -853,7 +868,7 @@ __global__ __launch_bounds__(kMlThreads) void rowsum_finish_kernel(RowSumArgs a)
     chunks = p[0];
     first = p[1];
   } else {
-    chunks = int(ceil_div(a.rows.T, RowsPlan::chunk_tiles(a.rows.T, a.table)));
+    chunks = adapter_chunks(a.rows.T, a.rows.T, a.table).n;
   }
   if (chunks == 1) return;
   for (int w = 0; w < a.n; ++w) {
@@ -880,7 +895,7 @@ int rowsum_table(const RowsPlan& rows, int64_t cols, int wg_cols, int cus) {
 // Partial slots that `table` may take.
 int64_t rowsum_parts(const RowsPlan& rows, int table) {
   if (rows.p) return rows.T > chunk_least(table) ? std::min<int64_t>(kMaxParts, 2 * ceil_div(rows.T, chunk_least(table))) : 0;
-  const int64_t c = ceil_div(rows.T, RowsPlan::chunk_tiles(rows.T, table));
+  const int64_t c = adapter_chunks(rows.T, rows.T, table).n;
   return c > 1 ? c : 0;
 }
 
@@ -901,7 +916,7 @@ int run_rowsum(RowSumArgs a, hipStream_t stream) {
   else rowsum_kernel<XT, 4><<<grid, kMlThreads, 0, stream>>>(a);
   const int st = rq_check_launch();
   if (st != RQ_OK || rowsum_parts(a.rows, a.table) == 0) return st;
-  const dim3 fgrid(unsigned(std::min<int64_t>(ceil_div(most, kMlThreads), std::max<int64_t>(1024 / a.rows.n, 64))), unsigned(a.rows.p ? a.rows.n : 1));
+  const dim3 fgrid(unsigned(std::min<int64_t>(ceil_div(most, kMlThreads), std::max<int64_t>(4096 / a.rows.n, 64))), unsigned(a.rows.p ? a.rows.n : 1));
   rowsum_finish_kernel<XT><<<fgrid, kMlThreads, 0, stream>>>(a);
   return rq_check_launch();
 }
@@ -945,7 +960,7 @@ ForwardPlan plan_forward(const Sizes& s, const RowsPlan& rows) {
 struct BackwardPlan {
   int splits, table;
   int64_t per;
-  size_t part, gt, ut, sums, bytes;
+  size_t part, g, gt, ut, sums, bytes;
   int64_t part_size;
 };
 
@@ -963,6 +978,7 @@ BackwardPlan plan_backward(const Sizes& s, const RowsPlan& rows) {
     return o;
   };
   p.part = take(size_t(p.splits) * slots * rp * 4);
+  p.g = take(size_t(slots) * rp * 4);
   p.gt = take(op_bytes(s, slots));
   p.ut = take(op_bytes(s, slots));
   p.sums = take(size_t(rowsum_parts(rows, p.table)) * p.part_size * 4);
@@ -1031,12 +1047,12 @@ int backward(const BackwardCall& c, char* ws, hipStream_t stream) {
   if (c.dx || c.da) {
     const ShrinkArgs sh{c.rows, c.dy, c.lddy, c.s.N, c.b, c.s.N * c.s.r, r, rp, p.splits, p.per, part};
     if ((st = run_shrink<XT, true>(sh, stream)) != RQ_OK) return st;
-    if (c.da) f.job[f.jobs++] = FinishJob{part, p.splits, ws + p.gt};
+    if (c.da) f.job[f.jobs++] = FinishJob{part, p.splits, c.dx ? reinterpret_cast<float*>(ws + p.g) : nullptr, ws + p.gt};
   }
-  if (c.db) f.job[f.jobs++] = FinishJob{c.u, 1, ws + p.ut};
+  if (c.db) f.job[f.jobs++] = FinishJob{c.u, 1, nullptr, ws + p.ut};
   if (f.jobs > 0 && (st = run_finish<XT>(f, stream)) != RQ_OK) return st;
   if (c.dx) {
-    const ExpandArgs e{c.rows, part, p.splits, r, rp, c.a, c.s.r * c.s.K, c.s.K, c.scaling, c.dx_base, c.ld_dx_base, c.dx, c.lddx,
+    const ExpandArgs e{c.rows, c.da ? reinterpret_cast<float*>(ws + p.g) : part, c.da ? 1 : p.splits, r, rp, c.a, c.s.r * c.s.K, c.s.K, c.scaling, c.dx_base, c.ld_dx_base, c.dx, c.lddx,
                        nullptr, 0, 0};
     if ((st = run_expand<XT, false>(e, device_cus(), stream)) != RQ_OK) return st;
   }

@@ -54,7 +54,8 @@ struct ExpandArgs {
 struct FinishJob {
   const float* part;    // [splits][slots][rp]
   int splits;
-  void* opt;            // 16-bit: [2][rp][slots], hi and lo; fp32: [rp][slots]; times the scaling
+  float* sum;           // [slots][rp], or nullptr
+  void* opt;            // [slots][rp] values, in the order of rowsum's lanes, times the scaling
 };
 
 struct FinishArgs {

@@ -11,8 +11,8 @@
 //
 // The plan is int32 device memory:
 //   [0] tiles in use, [1], [2] chunks in use of the two tables, [3..15] zero
-//   tile_adapter[T], tile_count[T]    (adapter -1: rows without one)
-//   slot_row[64 T]                    (-1: padding)
+//   tile[T][2]                        (adapter, -1: rows without one; rows, 0: not in use)
+//   slot_row[64 T]                    (-1: padding; of tiles in use)
 //   chunk[2][C][4]                    (adapter, first tile, end tile, partial slot or -1)
 //   part[2][n][2]                     (chunks of the adapter, its first partial slot)
 // A null plan stands for M rows of adapter 0 in their own order.
@@ -24,7 +24,7 @@ namespace rq {
 
 constexpr int kTileRows = 64;
 constexpr int kMaxAdapters = 1024;
-// Tiles of a chunk: at least these, and at least 1 / kRowChunks of all, so that
+// Tiles of a chunk, before an adapter's chunks are made alike: at least these, and at least 1 / kRowChunks of all, so that
 // partial sums are bounded: adapters of several chunks have at most 2 kRowChunks of
 // them in all.
 constexpr int kRowChunks = 16;
@@ -39,8 +39,7 @@ struct RowsPlan {
   int32_t T;         // tiles, at most
   int32_t C;         // chunks of a table, at most
 
-  __host__ __device__ int64_t off_count() const { return 16 + ((int64_t(T) + 3) & ~int64_t(3)); }
-  __host__ __device__ int64_t off_rows() const { return 16 + 2 * ((int64_t(T) + 3) & ~int64_t(3)); }
+  __host__ __device__ int64_t off_rows() const { return 16 + ((2 * int64_t(T) + 3) & ~int64_t(3)); }
   __host__ __device__ int64_t off_chunks() const { return off_rows() + int64_t(kTileRows) * T; }
   __host__ __device__ int64_t off_part() const { return off_chunks() + kChunkTables * 4 * int64_t(C); }
   __host__ __device__ int64_t words() const { return off_part() + kChunkTables * 2 * int64_t(n); }
@@ -53,6 +52,15 @@ struct RowsPlan {
   }
 };
 
+// An adapter's chunks: as few as chunk_tiles allows, of the same size but for the last.
+struct Chunks {
+  int n, tiles;
+};
+__host__ __device__ inline Chunks adapter_chunks(int tiles, int all, int table) {
+  const int most = RowsPlan::chunk_tiles(all, table), n = tiles > most ? (tiles + most - 1) / most : 1;
+  return Chunks{n, (tiles + n - 1) / n};
+}
+
 // A tile's adapter and rows in use, as every workgroup of the tile reads them.
 struct Tile {
   int adapter;
@@ -64,10 +72,11 @@ __device__ __forceinline__ Tile plan_tile(const RowsPlan& P, int t) {
     const int64_t left = P.M - int64_t(kTileRows) * t;
     return Tile{0, left < kTileRows ? int(left > 0 ? left : 0) : kTileRows};
   }
-  if (t >= P.p[0]) return Tile{-1, 0};
-  return Tile{P.p[16 + t], P.p[P.off_count() + t]};
+  const u32x2 v = *reinterpret_cast<const u32x2*>(P.p + 16 + 2 * int64_t(t));
+  return Tile{int(v.x), int(v.y)};
 }
 
+// The slot's row, -1 for padding (slots of tiles not in use: anything).
 __device__ __forceinline__ int plan_row(const RowsPlan& P, int64_t slot) {
   if (!P.p) return slot < P.M ? int(slot) : -1;
   return P.p[P.off_rows() + slot];
