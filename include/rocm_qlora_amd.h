@@ -542,10 +542,9 @@ int rq_adamw_step(const rq_adamw_tensor* tensors, int64_t n_tensors, void* devic
 int rq_adapter_rows_size(int64_t M, int64_t n, int64_t* bytes);
 int rq_adapter_rows(const int32_t* ids, int64_t M, int64_t n, void* plan, int64_t plan_bytes, hipStream_t stream);
 
-/* Row slots of a grouped batch (grouped = 0: of rows that all belong to adapter 0,
- * whose plan is NULL): the rank-wide sums u below are [slots][rank rounded up to
- * 16] fp32. */
-int rq_multi_lora_slots(int64_t M, int64_t n, int grouped, int64_t* slots);
+/* Bytes of u below, x A^T as the gradients read it (grouped = 0: for rows that all
+ * belong to adapter 0, whose plan is NULL). */
+int rq_multi_lora_u_size(int64_t M, int64_t n, int64_t rank, int grouped, int64_t* bytes);
 
 /* Scratch memory of one call (256-byte aligned, contents ignored). */
 int rq_multi_lora_scratch_size(int dtype, int64_t M, int64_t K, int64_t N, int64_t n, int64_t rank, int grouped,
@@ -556,12 +555,12 @@ int rq_multi_lora_scratch_size(int dtype, int64_t M, int64_t K, int64_t N, int64
  *   x [M, K] stride ldx, lora_a [n, rank, K], lora_b [n, N, rank], base [M, N]
  *   stride ld_base or NULL (zeros), out [M, N] stride ld_out (may be base), all of
  *   `dtype`; scaling [n] fp32; plan: rq_adapter_rows' of the same M and n, or NULL
- *   with n = 1: every row adapter 0's.  u: NULL, or the sums x A^T for the backward
- *   pass.  Sums are fp32, x A^T is passed on in 16 bits or more, the result is
+ *   with n = 1: every row adapter 0's.  u: NULL, or 16-byte aligned memory of
+ *   rq_multi_lora_u_size bytes, filled for the gradients.  Sums are fp32, x A^T is passed on in 16 bits or more, the result is
  *   rounded once.  rank <= 512, any sizes, strides and element alignment. */
 int rq_multi_lora(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* plan, int64_t plan_bytes,
                   const void* lora_a, const void* lora_b, const float* scaling, int64_t n, int64_t rank, int64_t N,
-                  const void* base, int64_t ld_base, void* out, int64_t ld_out, float* u, void* scratch,
+                  const void* base, int64_t ld_base, void* out, int64_t ld_out, void* u, void* scratch,
                   int64_t scratch_bytes, hipStream_t stream);
 
 /* Its gradients, with g[m] = scaling[a] dY[m] B[a]:
@@ -574,7 +573,7 @@ int rq_multi_lora(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, c
 int rq_multi_lora_grads(const void* x, const uint8_t* x_exponents, int dtype, int64_t M, int64_t K, int64_t ldx,
                         const void* dy, int64_t N, int64_t lddy, const void* plan, int64_t plan_bytes,
                         const void* lora_a, const void* lora_b, const float* scaling, int64_t n, int64_t rank,
-                        const float* u, const void* dx_base, int64_t ld_dx_base, void* dx, int64_t lddx, void* da,
+                        const void* u, const void* dx_base, int64_t ld_dx_base, void* dx, int64_t lddx, void* da,
                         void* db, void* scratch, int64_t scratch_bytes, hipStream_t stream);
 
 /* ------------------------------------------------------------------------

@@ -262,6 +262,102 @@ __device__ __forceinline__ f32x4 split_sum4(const float* p, int splits, int64_t 
   return v;
 }
 
+// ---- the row sums' operands -------------------------------------------------------
+// In the order in which rowsum's lanes load them: for 32 slots and 16 ranks, 1 KiB of hi
+// parts and 1 KiB of lo parts (fp32: of slots 8 g .. 8 g + 3 and of the four after them), 16
+// bytes of lane (i, g) = rank i, slots 8 g .. 8 g + 7.
+template <int XT>
+__device__ __forceinline__ int64_t opt_at(int64_t slot, int rank, int rp) {  // slot: a multiple of 8
+  constexpr int kBlock = XT == RQ_DTYPE_F32 ? 512 : 1024, kLane = Elem<XT>::kVec;
+  return ((slot >> 5) * (rp >> 4) + (rank >> 4)) * kBlock + ((rank & 15) + 2 * (slot & 24)) * kLane;
+}
+
+// A tile's operands from LDS, rows of `pitch` (16-bit: hi | lo); zeros past its `count` rows.
+template <int XT>
+__device__ __forceinline__ void store_operands(typename Elem<XT>::T* opt, const typename Elem<XT>::T* op, int pitch, int rp,
+                                               int64_t slot0, int count) {
+  typedef typename Elem<XT>::T T;
+  const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4, blocks = rp >> 4;
+  for (int k = threadIdx.x >> 6; k < (count > 32 ? 2 : 1) * blocks; k += kMlWaves) {
+    const int first = 32 * (k / blocks) + 8 * g, j = 16 * (k % blocks) + i16;
+    T* o = opt + opt_at<XT>(slot0 + first, j, rp);
+    const T* p = op + first * pitch + j;
+    if constexpr (XT == RQ_DTYPE_F32) {
+      f32x4 v[2];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e >> 2][e & 3] = first + e < count ? p[e * pitch] : 0.0f;
+      *reinterpret_cast<f32x4*>(o) = v[0];
+      *reinterpret_cast<f32x4*>(o + 256) = v[1];
+    } else {
+      u32x4 hi = u32x4{0u, 0u, 0u, 0u}, lo = hi;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (first + e >= count) break;
+        hi[e >> 1] |= uint32_t(p[e * pitch]) << (16 * (e & 1));
+        lo[e >> 1] |= uint32_t(p[e * pitch + rp]) << (16 * (e & 1));
+      }
+      *reinterpret_cast<u32x4*>(o) = hi;
+      *reinterpret_cast<u32x4*>(o + 512) = lo;
+    }
+  }
+}
+
+// The splits' sum of a tile's slots, in order, as operands in LDS rows of `pitch`.
+template <int XT>
+__device__ __forceinline__ void sum_operands(typename Elem<XT>::T* op, int pitch, const float* part, int splits, int64_t slots,
+                                             int rp, int64_t slot0, int count) {
+  const int quads = rp / 4, rows = (count + 15) & ~15;
+  const int64_t stride = slots * rp;
+  for (int i = threadIdx.x; i < rows * quads; i += kMlThreads) {
+    const int m = i / quads, j = 4 * (i - m * quads);
+    const f32x4 v = split_sum4(part + (slot0 + m) * rp + j, splits, stride);
+    typename Elem<XT>::T* o = op + m * pitch + j;
+    if constexpr (XT == RQ_DTYPE_F32) {
+      *reinterpret_cast<f32x4*>(o) = v;
+    } else {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split16<XT>(v[e], hi[e], lo[e]);
+      *reinterpret_cast<u32x2*>(o) = u32x2{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16};
+      *reinterpret_cast<u32x2*>(o + rp) = u32x2{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16};
+    }
+  }
+}
+
+// The operands alone, for gradients without one of the rows: a workgroup a tile.
+template <int XT>
+__global__ __launch_bounds__(kMlThreads) void operands_kernel(OperandsArgs a) {
+  typedef typename Elem<XT>::T T;
+  extern __shared__ uint32_t operands_lds[];
+  T* op = reinterpret_cast<T*>(operands_lds);
+  const Tile tile = plan_tile(a.rows, int(blockIdx.x));
+  if (tile.count == 0 || tile.adapter < 0) return;
+  const int pitch = (XT == RQ_DTYPE_F32 ? a.rp : 2 * a.rp) + Elem<XT>::kVec;
+  const int64_t slot0 = int64_t(kTileRows) * blockIdx.x;
+  sum_operands<XT>(op, pitch, a.part, a.splits, a.rows.slots(), a.rp, slot0, tile.count);
+  __syncthreads();
+  store_operands<XT>(static_cast<T*>(a.opt), op, pitch, a.rp, slot0, tile.count);
+}
+
+// Dynamic LDS of a launch: past 64 KiB (ranks above 200) the kernel has to be told.
+template <typename K>
+int allow_lds(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  constexpr int kMost = 160 << 10;
+  if (bytes <= (64u << 10)) return RQ_OK;
+  return bytes > size_t(kMost) ? RQ_ERR_UNSUPPORTED : allow_dynamic_lds(reinterpret_cast<const void*>(kernel), kMost, done);
+}
+
+template <int XT>
+int run_operands(const OperandsArgs& a, hipStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  const int pitch = (XT == RQ_DTYPE_F32 ? a.rp : 2 * a.rp) + Elem<XT>::kVec;
+  const size_t bytes = size_t(kTileRows) * pitch * sizeof(typename Elem<XT>::T);
+  const int st = allow_lds(operands_kernel<XT>, bytes, done);
+  if (st != RQ_OK) return st;
+  operands_kernel<XT><<<unsigned(a.rows.T), kMlThreads, bytes, stream>>>(a);
+  return rq_check_launch();
+}
+
 // ---- expand ---------------------------------------------------------------------
 // A workgroup takes a tile: it sums the splits of its slots and keeps them in LDS as operands.
 // Its four waves divide the tile's 16-row blocks (1, 2 or 4) and, where there are fewer than
@@ -381,26 +477,9 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
     }
   };
   fetch_base(c_first + group * L::kCols + V * i16);
-  if (adapted) {
-    const int quads = a.rp / 4, rows = (tile.count + 15) & ~15;
-    const int64_t stride = a.rows.slots() * a.rp;
-    for (int i = tid; i < rows * quads; i += kMlThreads) {
-      const int m = i / quads, j = 4 * (i - m * quads);
-      const f32x4 v = split_sum4(a.part + (slot0 + m) * a.rp + j, a.splits, stride);
-      if (a.sum && chunk == 0) *reinterpret_cast<f32x4*>(a.sum + (slot0 + m) * a.rp + j) = v;
-      T* o = op + m * pitch + j;
-      if constexpr (XT == RQ_DTYPE_F32) {
-        *reinterpret_cast<f32x4*>(o) = v;
-      } else {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) split16<XT>(v[e], hi[e], lo[e]);
-        *reinterpret_cast<u32x2*>(o) = u32x2{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16};
-        *reinterpret_cast<u32x2*>(o + a.rp) = u32x2{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16};
-      }
-    }
-  }
-  if (!FACTOR_ROWS) __syncthreads();
+  if (adapted) sum_operands<XT>(op, pitch, a.part, a.splits, a.rows.slots(), a.rp, slot0, tile.count);
+  __syncthreads();
+  if (a.opt && adapted && chunk == 0) store_operands<XT>(static_cast<T*>(a.opt), op, pitch, a.rp, slot0, tile.count);
   const bool rows_here = 16 * block < tile.count;
 #pragma unroll 1
   for (int it = 0; it < a.iters * BLOCKS; ++it) {
@@ -509,81 +588,12 @@ int run_expand(ExpandArgs a, int cus, hipStream_t stream) {
     bytes = std::max(bytes, size_t((FACTOR_ROWS ? kMlWaves / blocks * L::kStage : 0) + 16 * blocks * pitch) * es);
   const bool edges = a.C % L::kCols != 0 || (FACTOR_ROWS && a.r > Elem<XT>::kStep && a.r % V != 0);
   const unsigned grid = unsigned(int64_t(a.rows.T) * a.chunks);
+  static std::atomic<uint64_t> done[2];
+  const int st = edges ? allow_lds(expand_kernel<XT, FACTOR_ROWS, true>, bytes, done[0])
+                       : allow_lds(expand_kernel<XT, FACTOR_ROWS, false>, bytes, done[1]);
+  if (st != RQ_OK) return st;
   if (edges) expand_kernel<XT, FACTOR_ROWS, true><<<grid, kMlThreads, bytes, stream>>>(a);
   else expand_kernel<XT, FACTOR_ROWS, false><<<grid, kMlThreads, bytes, stream>>>(a);
-  return rq_check_launch();
-}
-
-// ---- finish ---------------------------------------------------------------------
-// The splits' sum times the adapter's scaling, as the operands of the row sums, in the order
-// in which their lanes load them: for 32 slots and 16 ranks, 1 KiB of hi parts and 1 KiB of
-// lo parts (fp32: of slots 8 g .. 8 g + 3 and the four after them), 16 bytes of lane (i, g)
-// = rank i, slots 8 g .. 8 g + 7.  A thread takes eight slots of one rank.  Slots of a tile
-// past its rows get zeros.
-template <int XT>
-__device__ __forceinline__ int64_t opt_at(int64_t slot, int rank, int rp) {  // slot: a multiple of 8
-  constexpr int kBlock = XT == RQ_DTYPE_F32 ? 512 : 1024, kLane = Elem<XT>::kVec;
-  return ((slot >> 5) * (rp >> 4) + (rank >> 4)) * kBlock + ((rank & 15) + 2 * (slot & 24)) * kLane;
-}
-
-template <int XT>
-__global__ __launch_bounds__(kMlThreads) void finish_kernel(FinishArgs a, unsigned per_job) {
-  typedef typename Elem<XT>::T T;
-  const int which = int(blockIdx.x / per_job);
-  const FinishJob& J = a.job[which];
-  const unsigned i = blockIdx.x % per_job * kMlThreads + threadIdx.x;
-  const int64_t s0 = 8 * int64_t(i / unsigned(a.rp));
-  const int j = int(i % unsigned(a.rp));
-  const int64_t slots = a.rows.slots();
-  if (s0 >= slots) return;
-  const int t = int(s0 / kTileRows);
-  const Tile tile = plan_tile(a.rows, t);
-  if (tile.count == 0 || tile.adapter < 0) return;
-  const int live = tile.count - int(s0 - int64_t(kTileRows) * t);  // of these slots
-  const float scale = a.scaling[tile.adapter];
-  float v[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-  if (live > 0) {
-    for (int k0 = 0; k0 < J.splits; k0 += 4) {
-      float p[4][8];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          p[k][e] = J.part[(int64_t(k0 + k < J.splits ? k0 + k : 0) * slots + s0 + (e < live ? e : 0)) * a.rp + j];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (k0 + k < J.splits) v[e] = __fadd_rn(v[e], p[k][e]);
-    }
-  }
-  if (J.sum) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < live) J.sum[(s0 + e) * a.rp + j] = v[e];
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = e < live ? __fmul_rn(v[e], scale) : 0.0f;
-  T* o = static_cast<T*>(J.opt) + opt_at<XT>(s0, j, a.rp);
-  if constexpr (XT == RQ_DTYPE_F32) {
-    *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<f32x4*>(o + 256) = f32x4{v[4], v[5], v[6], v[7]};
-  } else {
-    uint32_t hi[8], lo[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) split16<XT>(v[e], hi[e], lo[e]);
-    *reinterpret_cast<u32x4*>(o) = u32x4{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, hi[4] | hi[5] << 16, hi[6] | hi[7] << 16};
-    *reinterpret_cast<u32x4*>(o + 512) = u32x4{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16, lo[4] | lo[5] << 16, lo[6] | lo[7] << 16};
-  }
-}
-
-template <int XT>
-int run_finish(const FinishArgs& a, hipStream_t stream) {
-  const int64_t per = ceil_div(a.rows.slots() / 8 * a.rp, kMlThreads);
-  if (per * a.jobs > kMaxThreads1D / kMlThreads) return RQ_ERR_UNSUPPORTED;
-  finish_kernel<XT><<<unsigned(per * a.jobs), kMlThreads, 0, stream>>>(a, unsigned(per));
   return rq_check_launch();
 }
 
@@ -818,9 +828,10 @@ __device__ __forceinline__ void rowsum_body(const RowSumArgs& a, const RowSumTas
   const int cols = int(std::min<int64_t>(K.C - c0, 16 * CW)), ranks = std::min(a.r - j0, 16 * JB);
   float* part = ch.slot >= 0 ? a.part + ch.slot * a.part_size + K.part_off : nullptr;
   T* out = static_cast<T*>(K.out) + ch.adapter * K.C * a.r;
+  const float scale = live > 0 ? a.scaling[ch.adapter] : 0.0f;  // an adapter without rows: zeros, whatever its scaling
   for (int i = threadIdx.x; i < cols * ranks; i += kMlThreads) {
     const int c = K.rank_major ? i % cols : i / ranks, j = K.rank_major ? i / cols : i % ranks;
-    const float v = __fadd_rn(red[0][c][j], red[1][c][j]);
+    const float v = live > 0 ? __fmul_rn(scale, __fadd_rn(red[0][c][j], red[1][c][j])) : 0.0f;
     const int64_t to = K.rank_major ? int64_t(j0 + j) * K.C + c0 + c : (c0 + c) * a.r + j0 + j;
     if (part) part[to] = v;
     else out[to] = from_f32<XT>(v);
@@ -885,11 +896,11 @@ __global__ __launch_bounds__(kMlThreads) void rowsum_finish_kernel(RowSumArgs a)
   }
 }
 
-// The table of chunks: the coarser one, whose sums seldom meet in a second launch, where
-// its workgroups fill the GPU.
+// The table of chunks: the coarser one where its sums cannot meet in a second launch, or
+// where its workgroups fill the GPU.
 int rowsum_table(const RowsPlan& rows, int64_t cols, int wg_cols, int cus) {
   const int64_t tiles = ceil_div(cols, wg_cols);
-  return tiles * ceil_div(ceil_div(rows.M, kTileRows), chunk_least(1)) >= cus ? 1 : 0;
+  return rows.T <= chunk_least(1) || tiles * ceil_div(ceil_div(rows.M, kTileRows), chunk_least(1)) >= cus ? 1 : 0;
 }
 
 // Partial slots that `table` may take.
@@ -941,9 +952,6 @@ int check_sizes(int dtype, int64_t M, int64_t K, int64_t N, int64_t n, int64_t r
   return RQ_OK;
 }
 
-// the row sums' operands: fp32, or hi and lo
-size_t op_bytes(const Sizes& s, int64_t slots) { return size_t(slots) * rank_pad(s.r) * 4; }
-
 struct ForwardPlan {
   int splits;
   int64_t per;
@@ -960,7 +968,7 @@ ForwardPlan plan_forward(const Sizes& s, const RowsPlan& rows) {
 struct BackwardPlan {
   int splits, table;
   int64_t per;
-  size_t part, g, gt, ut, sums, bytes;
+  size_t part, gt, sums, bytes;
   int64_t part_size;
 };
 
@@ -978,9 +986,7 @@ BackwardPlan plan_backward(const Sizes& s, const RowsPlan& rows) {
     return o;
   };
   p.part = take(size_t(p.splits) * slots * rp * 4);
-  p.g = take(size_t(slots) * rp * 4);
-  p.gt = take(op_bytes(s, slots));
-  p.ut = take(op_bytes(s, slots));
+  p.gt = take(size_t(slots) * rp * 4);
   p.sums = take(size_t(rowsum_parts(rows, p.table)) * p.part_size * 4);
   p.bytes = off;
   return p;
@@ -998,7 +1004,7 @@ struct ForwardCall {
   int64_t ld_base;
   void* out;
   int64_t ld_out;
-  float* u;
+  void* u;
 };
 
 template <int XT>
@@ -1025,7 +1031,7 @@ struct BackwardCall {
   const void* a;
   const void* b;
   const float* scaling;
-  const float* u;
+  const void* u;
   const void* dx_base;
   int64_t ld_dx_base;
   void* dx;
@@ -1040,31 +1046,29 @@ int backward(const BackwardCall& c, char* ws, hipStream_t stream) {
   const int r = int(c.s.r), rp = int(rank_pad(c.s.r));
   float* part = reinterpret_cast<float*>(ws + p.part);
   int st = RQ_OK;
-  FinishArgs f{};
-  f.rows = c.rows;
-  f.rp = rp;
-  f.scaling = c.scaling;
   if (c.dx || c.da) {
     const ShrinkArgs sh{c.rows, c.dy, c.lddy, c.s.N, c.b, c.s.N * c.s.r, r, rp, p.splits, p.per, part};
     if ((st = run_shrink<XT, true>(sh, stream)) != RQ_OK) return st;
-    if (c.da) f.job[f.jobs++] = FinishJob{part, p.splits, c.dx ? reinterpret_cast<float*>(ws + p.g) : nullptr, ws + p.gt};
   }
-  if (c.db) f.job[f.jobs++] = FinishJob{c.u, 1, nullptr, ws + p.ut};
-  if (f.jobs > 0 && (st = run_finish<XT>(f, stream)) != RQ_OK) return st;
+  void* gt = c.da ? ws + p.gt : nullptr;
   if (c.dx) {
-    const ExpandArgs e{c.rows, c.da ? reinterpret_cast<float*>(ws + p.g) : part, c.da ? 1 : p.splits, r, rp, c.a, c.s.r * c.s.K, c.s.K, c.scaling, c.dx_base, c.ld_dx_base, c.dx, c.lddx,
-                       nullptr, 0, 0};
-    if ((st = run_expand<XT, false>(e, device_cus(), stream)) != RQ_OK) return st;
+    const ExpandArgs e{c.rows, part, p.splits, r, rp, c.a, c.s.r * c.s.K, c.s.K, c.scaling, c.dx_base, c.ld_dx_base, c.dx, c.lddx,
+                       gt, 0, 0};
+    st = run_expand<XT, false>(e, device_cus(), stream);
+  } else if (c.da) {
+    st = run_operands<XT>(OperandsArgs{c.rows, rp, part, p.splits, gt}, stream);
   }
+  if (st != RQ_OK) return st;
   RowSumArgs q{};
   q.rows = c.rows;
   q.table = p.table;
   q.r = r;
   q.rp = rp;
+  q.scaling = c.scaling;
   q.part = reinterpret_cast<float*>(ws + p.sums);
   q.part_size = p.part_size;
-  if (c.db) q.t[q.n++] = RowSumTask{c.dy, nullptr, c.lddy, c.s.N, ws + p.ut, c.db, false, 0, 0};
-  if (c.da) q.t[q.n++] = RowSumTask{c.x, c.exps, c.ldx, c.s.K, ws + p.gt, c.da, true, c.s.N * c.s.r, 0};
+  if (c.db) q.t[q.n++] = RowSumTask{c.dy, nullptr, c.lddy, c.s.N, c.u, c.db, false, 0, 0};
+  if (c.da) q.t[q.n++] = RowSumTask{c.x, c.exps, c.ldx, c.s.K, gt, c.da, true, c.s.N * c.s.r, 0};
   return q.n > 0 ? run_rowsum<XT>(q, stream) : RQ_OK;
 }
 
@@ -1079,12 +1083,13 @@ int check_rows(const void* plan, int64_t plan_bytes, const Sizes& s, RowsPlan* r
 }  // namespace
 }  // namespace rq
 
-extern "C" int rq_multi_lora_slots(int64_t M, int64_t n, int grouped, int64_t* slots) {
-  if (!slots) return RQ_ERR_NULL_POINTER;
-  if (M < 0 || n < 1 || M > (int64_t(1) << 30)) return RQ_ERR_BAD_SHAPE;
-  if (n > rq::kMaxAdapters) return RQ_ERR_UNSUPPORTED;
+extern "C" int rq_multi_lora_u_size(int64_t M, int64_t n, int64_t rank, int grouped, int64_t* bytes) {
+  using namespace rq;
+  if (!bytes) return RQ_ERR_NULL_POINTER;
+  if (M < 0 || n < 1 || rank < 1 || M > (int64_t(1) << 30)) return RQ_ERR_BAD_SHAPE;
+  if (n > kMaxAdapters || rank > kMaxRank) return RQ_ERR_UNSUPPORTED;
   static const int32_t some = 0;
-  *slots = rq::rows_plan(grouped ? &some : nullptr, M, n).slots();
+  *bytes = rows_plan(grouped ? &some : nullptr, M, n).slots() * rank_pad(rank) * 4;
   return RQ_OK;
 }
 
@@ -1104,7 +1109,7 @@ extern "C" int rq_multi_lora_scratch_size(int dtype, int64_t M, int64_t K, int64
 extern "C" int rq_multi_lora(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* plan,
                              int64_t plan_bytes, const void* lora_a, const void* lora_b, const float* scaling, int64_t n,
                              int64_t rank, int64_t N, const void* base, int64_t ld_base, void* out, int64_t ld_out,
-                             float* u, void* scratch, int64_t scratch_bytes, hipStream_t stream) {
+                             void* u, void* scratch, int64_t scratch_bytes, hipStream_t stream) {
   using namespace rq;
   ForwardCall c{};
   int st = check_sizes(dtype, M, K, N, n, rank, &c.s);
@@ -1134,7 +1139,7 @@ extern "C" int rq_multi_lora(const void* x, int dtype, int64_t M, int64_t K, int
 extern "C" int rq_multi_lora_grads(const void* x, const uint8_t* x_exponents, int dtype, int64_t M, int64_t K, int64_t ldx,
                                    const void* dy, int64_t N, int64_t lddy, const void* plan, int64_t plan_bytes,
                                    const void* lora_a, const void* lora_b, const float* scaling, int64_t n, int64_t rank,
-                                   const float* u, const void* dx_base, int64_t ld_dx_base, void* dx, int64_t lddx, void* da,
+                                   const void* u, const void* dx_base, int64_t ld_dx_base, void* dx, int64_t lddx, void* da,
                                    void* db, void* scratch, int64_t scratch_bytes, hipStream_t stream) {
   using namespace rq;
   BackwardCall c{};

@@ -3,8 +3,9 @@
 //
 //   shrink   part[split][slot][j] = sum over a split's k of x[row][k] S[j][k]
 //   expand   out[row][c] = base[row][c] + scale * sum_j u[slot][j] S[c, j], u the splits' sum
-//   finish   u as the operands that rowsum reads
-//   rowsum   D[c][j] = sum over an adapter's rows of x[row][c] u[slot][j]
+//            (and u as the operands that rowsum reads)
+//   operands those operands alone
+//   rowsum   D[c][j] = scale * sum over an adapter's rows of x[row][c] u[slot][j]
 //
 // 16-bit rows: u is an fp32 sum, and the matrix instructions take 16-bit operands.
 // It is passed as two of them, hi = RND(u) and lo = RND(u - hi), whose products
@@ -47,23 +48,16 @@ struct ExpandArgs {
   int64_t ld_base;
   void* out;
   int64_t ld_out;
-  float* sum;           // [slots][rp]: the splits' sum, or nullptr
+  void* opt;            // rowsum's operands of the splits' sum, or nullptr
   int chunks, iters;    // column chunks of a tile, steps of a wave in each
 };
 
-struct FinishJob {
-  const float* part;    // [splits][slots][rp]
-  int splits;
-  float* sum;           // [slots][rp], or nullptr
-  void* opt;            // [slots][rp] values, in the order of rowsum's lanes, times the scaling
-};
-
-struct FinishArgs {
+struct OperandsArgs {
   RowsPlan rows;
   int rp;
-  const float* scaling;
-  FinishJob job[2];
-  int jobs;
+  const float* part;    // [splits][slots][rp]
+  int splits;
+  void* opt;            // slots * rp values of 32 bits
 };
 
 struct RowSumTask {
@@ -71,7 +65,7 @@ struct RowSumTask {
   const uint8_t* exps;  // of the codes, or nullptr: src holds values
   int64_t ld;           // elements (codes) per row
   int64_t C;            // columns
-  const void* opt;      // finish's
+  const void* opt;      // operands of u
   void* out;            // [n][C][r], or [n][r][C] when rank_major
   bool rank_major;
   int64_t part_off;     // of this task's values in a partial slot
@@ -82,6 +76,7 @@ struct RowSumArgs {
   RowsPlan rows;
   int table;            // chunk table of the plan
   int r, rp;
+  const float* scaling; // [n]
   RowSumTask t[2];
   int n;
   float* part;          // [parts][part_size]

@@ -112,7 +112,7 @@ SIGNATURES = {
                                                                   # chunks [b, e), m, v, stream
     "rq_adapter_rows_size": [_I64, _I64, _P],
     "rq_adapter_rows": [_P, _I64, _I64, _P, _I64, _P],       # ids, M, n, plan, bytes, stream
-    "rq_multi_lora_slots": [_I64, _I64, _I32, _P],
+    "rq_multi_lora_u_size": [_I64, _I64, _I64, _I32, _P],
     "rq_multi_lora_scratch_size": [_I32, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _P],
     "rq_multi_lora": [_P, _I32, _I64, _I64, _I64, _P, _I64,  # x, dtype, M, K, ldx, plan, bytes
                       _P, _P, _P, _I64, _I64, _I64,          # A, B, scaling, n, rank, N

@@ -17,6 +17,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from rocm_qlora import ops
+from rocm_qlora._device import on
 from rocm_qlora.lora.lora_layer import LoRALinear
 from rocm_qlora.quantization.quant_linear import QuantLinear
 
@@ -55,42 +56,43 @@ class _MultiLoRA(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, lora_a, lora_b, base, scaling, rows, bits, linear):
-        a, b = lora_a.to(x.dtype), lora_b.to(x.dtype)
-        N = b.shape[1]
-        need_x, need_a, need_b = ctx.needs_input_grad[:3]
-        x2 = x.reshape(-1, x.shape[-1])
+        need = ctx.needs_input_grad
+        dtype = x.dtype
+        a = lora_a if lora_a.dtype == dtype else lora_a.to(dtype)
+        b = lora_b if lora_b.dtype == dtype else lora_b.to(dtype)
+        flat = x.dim() == 2
+        x2 = x if flat else x.reshape(-1, x.shape[-1])
+        out = None
         if linear is not None:
-            y = linear[0](x2)
-            out = y
-        else:
-            y, out = (base.reshape(-1, N) if base is not None else None), None
-        res = ops.multi_lora(x2, a, b, scaling, rows.plan, y, out, need_u=need_b)
-        y, u = res if need_b else (res, None)
-        ctx.plan, ctx.linear, ctx.bits, ctx.shape = rows.plan, linear, bits, x.shape
-        ctx.dtypes = (lora_a.dtype, lora_b.dtype)
-        held = (None, None)
-        if need_a:
-            held = ops.act8_quantize(x2) if bits == 8 else (x2, None)
-        ctx.save_for_backward(*held, a, b, scaling, u)
-        return y.view(*x.shape[:-1], N)
+            base = out = linear[0](x2)
+        elif base is not None and not flat:
+            base = base.reshape(-1, b.shape[1])
+        y = ops.multi_lora(x2, a, b, scaling, rows.plan, base, out, need_u=need[2])
+        u = None
+        if need[2]:
+            y, u = y
+        ctx.args = (rows.plan, linear, None if flat else x.shape, lora_a.dtype, lora_b.dtype)
+        held, exps = (None, None) if not need[1] else ops.act8_quantize(x2) if bits == 8 else (x2, None)
+        ctx.save_for_backward(held, exps, a if a.is_contiguous() else a.contiguous(), b if b.is_contiguous() else b.contiguous(),
+                              scaling, u)
+        return y if flat else y.view(*x.shape[:-1], y.shape[-1])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, exps, a, b, scaling, u = ctx.saved_tensors
-        need_x, need_a, need_b, need_base = ctx.needs_input_grad[:4]
-        dy2 = dy.reshape(-1, dy.shape[-1])
-        dx = ctx.linear[1](dy2) if need_x and ctx.linear is not None else None
-        dx, da, db = ops.multi_lora_grads((x, exps) if exps is not None else x, dy2, a, b, scaling, ctx.plan, u,
-                                          need_x=need_x, need_a=need_a, need_b=need_b, dx=dx)
-        return (dx.view(ctx.shape) if need_x else None, da.to(ctx.dtypes[0]) if need_a else None,
-                db.to(ctx.dtypes[1]) if need_b else None, dy if need_base else None, None, None, None, None)
-
-
-def _scalings(scaling: Union[float, torch.Tensor], n: int, dev: torch.device) -> torch.Tensor:
-    if isinstance(scaling, torch.Tensor):
-        return scaling
-    return torch.full((n,), float(scaling), dtype=torch.float32, device=dev)
+        plan, linear, shape, a_dtype, b_dtype = ctx.args
+        need = ctx.needs_input_grad
+        dy2 = dy if shape is None else dy.reshape(-1, dy.shape[-1])
+        dx = linear[1](dy2) if linear is not None and need[0] else None
+        with on(dy.device):
+            dx, da, db = ops._multi_lora_grads((x, exps) if exps is not None else x, dy2, a, b, scaling, plan, u, need[0],
+                                               need[1], need[2], dx, dy.device)
+        if da is not None and a_dtype != da.dtype:
+            da = da.to(a_dtype)
+        if db is not None and b_dtype != db.dtype:
+            db = db.to(b_dtype)
+        return dx if shape is None or dx is None else dx.view(shape), da, db, dy if need[3] else None, None, None, None, None
 
 
 def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: Union[float, torch.Tensor],
@@ -107,13 +109,18 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
     if base is not None and (base.dtype != x.dtype or base.shape[:-1] != x.shape[:-1] or base.shape[-1] != lora_b.shape[1]):
         raise RuntimeError(f"base {tuple(base.shape)} {base.dtype} does not fit x {tuple(x.shape)} {x.dtype} and "
                            f"{lora_b.shape[1]} columns")
-    scaling = _scalings(scaling, rows.n, x.device)
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (x, lora_a, lora_b, base)):
-        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if not isinstance(scaling, torch.Tensor):
+        scaling = torch.full((rows.n,), float(scaling), dtype=torch.float32, device=x.device)
+    if not (torch.is_grad_enabled() and (x.requires_grad or lora_a.requires_grad or lora_b.requires_grad or
+                                         (base is not None and base.requires_grad))):
+        dtype = x.dtype
+        a = lora_a if lora_a.dtype == dtype else lora_a.to(dtype)
+        b = lora_b if lora_b.dtype == dtype else lora_b.to(dtype)
+        if x.dim() == 2:
+            return ops.multi_lora(x, a, b, scaling, rows.plan, base)
         N = lora_b.shape[1]
-        y = ops.multi_lora(x2, lora_a.to(x.dtype), lora_b.to(x.dtype), scaling, rows.plan,
-                           base if base is None or base.dim() == 2 else base.reshape(-1, N))
-        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+        y = ops.multi_lora(x.reshape(-1, x.shape[-1]), a, b, scaling, rows.plan, None if base is None else base.reshape(-1, N))
+        return y.view(*x.shape[:-1], N)
     return _MultiLoRA.apply(x, lora_a, lora_b, base, scaling, rows, activation_bits, None)
 
 

@@ -23,14 +23,14 @@ class _PreferenceLoss(torch.autograd.Function):
         loss, logps, state = ops.preference_forward(logits, labels, offsets, ref_logps, beta=beta,
                                                     label_smoothing=label_smoothing, average=average,
                                                     ignore_index=ignore_index)
-        ctx.save_for_backward(logits, *state)
+        ctx.save_for_backward(logits, state)
         ctx.mark_non_differentiable(logps)
         return loss, logps
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss, _):
-        logits, *state = ctx.saved_tensors
+        logits, state = ctx.saved_tensors
         return (ops.preference_backward(logits, state, dloss),) + (None,) * 7
 
 
@@ -39,13 +39,13 @@ class _SequenceLogps(torch.autograd.Function):
     def forward(ctx, logits, labels, offsets, average, ignore_index):
         _, logps, state = ops.preference_forward(logits, labels, offsets, average=average, ignore_index=ignore_index,
                                                  pairs=False)
-        ctx.save_for_backward(logits, *state)
+        ctx.save_for_backward(logits, state)
         return logps
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dlogps):
-        logits, *state = ctx.saved_tensors
+        logits, state = ctx.saved_tensors
         return (ops.preference_backward(logits, state, dlogps),) + (None,) * 4
 
 

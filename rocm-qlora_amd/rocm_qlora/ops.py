@@ -774,33 +774,37 @@ def _ld(t: torch.Tensor) -> int:
     return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
 
 
+def _check_plan(plan: Optional[torch.Tensor], dev, M: int, n: int) -> None:
+    if plan is None:
+        if n != 1:
+            raise RuntimeError(f"{n} adapters without the batch's rows by adapter")
+    elif plan.numel() != _bytes("rq_adapter_rows_size", dev.index, M, n):
+        raise RuntimeError(f"the rows by adapter are not those of {M} rows and {n} adapters")
+
+
 def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: torch.Tensor,
                plan: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None,
                out: Optional[torch.Tensor] = None, need_u: bool = False):
     """out[m] = base[m] + scaling[a] (x[m] A[a]^T) B[a]^T, a the adapter of row m in
     `plan` (None: adapter 0 of one).  x [M, K], lora_a [n, rank, K], lora_b [n, N,
     rank], base and out [M, N] (out may be base) of one dtype, scaling [n] fp32.
-    Returns out and, with need_u, the sums x A^T that multi_lora_grads takes."""
+    Returns out and, with need_u, what multi_lora_grads takes as u."""
     dev = nat.require_gpu(x, lora_a, lora_b, scaling, plan, base, out)
     M, K = x.shape
     code = nat.dtype_code(x.dtype)
     n, rank, N, a, b = _adapter_operands(x.dtype, K, lora_a, lora_b, scaling)
-    grouped = 0 if plan is None else 1
-    if not grouped and n != 1:
-        raise RuntimeError(f"{n} adapters without the batch's rows by adapter")
     if base is not None:
         _check_rows(base, M, N, x.dtype, "base")
-    if out is not None:
+    if out is not None and out is not base:
         _check_rows(out, M, N, x.dtype, "out")
     with on(dev):
-        if grouped and plan.numel() != _bytes("rq_adapter_rows_size", dev.index, M, n):
-            raise RuntimeError(f"the rows by adapter are not those of {M} rows and {n} adapters")
+        _check_plan(plan, dev, M, n)
+        grouped = 0 if plan is None else 1
         if out is None:
             out = torch.empty((M, N), dtype=x.dtype, device=dev)
         u = None
         if need_u:
-            slots = _bytes("rq_multi_lora_slots", dev.index, M, n, grouped)
-            u = torch.empty((slots, -(-rank // 16) * 16), dtype=torch.float32, device=dev)
+            u = torch.empty(_bytes("rq_multi_lora_u_size", dev.index, M, n, rank, grouped), dtype=torch.uint8, device=dev)
         if M > 0:
             x, ldx = _rows(x, K)
             scratch = _scratch("rq_multi_lora_scratch_size", dev, code, M, K, N, n, rank, grouped, 0)
@@ -821,56 +825,64 @@ def multi_lora_grads(x, dy: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Te
     dev = nat.require_gpu(dy, lora_a, lora_b, scaling, plan, u, dx)
     M, N = dy.shape
     K = lora_a.shape[-1]
-    code = nat.dtype_code(dy.dtype)
+    nat.dtype_code(dy.dtype)
     n, rank, n_out, a, b = _adapter_operands(dy.dtype, K, lora_a, lora_b, scaling)
-    grouped = 0 if plan is None else 1
     if n_out != N:
         raise RuntimeError(f"dY has {N} columns, the factors {n_out}")
-    if not grouped and n != 1:
-        raise RuntimeError(f"{n} adapters without the batch's rows by adapter")
-    need_x = need_x or dx is not None
-    codes = exps = None
-    xr, ldx = None, 0
-    pitch = -(-K // ACT8_BLOCK) * ACT8_BLOCK
     if need_a:
         if isinstance(x, tuple):
             codes, exps = x
             nat.require_gpu(dy, codes, exps)
+            pitch = -(-K // ACT8_BLOCK) * ACT8_BLOCK
             if codes.shape != (M, pitch) or exps.shape != (M, pitch // ACT8_BLOCK) or codes.dtype != torch.uint8 or \
                     exps.dtype != torch.uint8 or not codes.is_contiguous() or not exps.is_contiguous():
                 raise RuntimeError(f"codes {tuple(codes.shape)} / {tuple(exps.shape)} are not act8_quantize's of {M} rows of {K}")
-            xr, ldx = codes, pitch
         else:
             nat.require_gpu(dy, x)
             if x.dtype != dy.dtype or x.shape != (M, K):
                 raise RuntimeError(f"x must be [{M}, {K}] {dy.dtype}, got {tuple(x.shape)} {x.dtype}")
-            xr, ldx = _rows(x, K)
     if dx is not None:
         _check_rows(dx, M, K, dy.dtype, "dx")
     with on(dev):
-        slots = _bytes("rq_multi_lora_slots", dev.index, M, n, grouped)
-        if grouped and plan.numel() != _bytes("rq_adapter_rows_size", dev.index, M, n):
-            raise RuntimeError(f"the rows by adapter are not those of {M} rows and {n} adapters")
-        if need_b and (u is None or u.shape != (slots, -(-rank // 16) * 16) or u.dtype != torch.float32 or
-                       not u.is_contiguous()):
+        _check_plan(plan, dev, M, n)
+        if need_b and (u is None or u.dtype != torch.uint8 or not u.is_contiguous() or
+                       u.numel() != _bytes("rq_multi_lora_u_size", dev.index, M, n, rank, 0 if plan is None else 1)):
             raise RuntimeError("u is not multi_lora's of these rows and factors")
-        base = dx
-        da = torch.empty_like(a) if need_a else None
-        db = torch.empty_like(b) if need_b else None
-        if need_x and dx is None:
-            dx = torch.empty((M, K), dtype=dy.dtype, device=dev)
-        if M == 0:
-            for t in (da, db):
-                if t is not None:
-                    t.zero_()
-            return dx, da, db
-        dy2, lddy = _rows(dy, N)
-        scratch = _scratch("rq_multi_lora_scratch_size", dev, code, M, K, N, n, rank, grouped, 1)
-        nat.call("rq_multi_lora_grads", nat.ptr(xr), nat.ptr(exps), code, M, K, ldx, dy2.data_ptr(), N, lddy,
-                 nat.ptr(plan), plan.numel() if grouped else 0, a.data_ptr(), b.data_ptr(), scaling.data_ptr(), n, rank,
-                 nat.ptr(u) if need_b else None, nat.ptr(base), _ld(base) if base is not None else 0,
-                 nat.ptr(dx), _ld(dx) if dx is not None else 0, nat.ptr(da), nat.ptr(db),
-                 scratch.data_ptr(), scratch.numel(), nat.stream_handle(dev))
+        return _multi_lora_grads(x, dy, a, b, scaling, plan, u, need_x or dx is not None, need_a, need_b, dx, dev)
+
+
+def _multi_lora_grads(x, dy, a, b, scaling, plan, u, need_x, need_a, need_b, dx, dev):
+    """multi_lora_grads of operands that are known to fit, on the current device."""
+    M, N = dy.shape
+    n, rank, K = a.shape
+    base = dx
+    da = torch.empty_like(a) if need_a else None
+    db = torch.empty_like(b) if need_b else None
+    if need_x and dx is None:
+        dx = torch.empty((M, K), dtype=dy.dtype, device=dev)
+    if M == 0:
+        for t in (da, db):
+            if t is not None:
+                t.zero_()
+        return dx, da, db
+    xp = exps = None
+    ldx = 0
+    if need_a:
+        if isinstance(x, tuple):
+            x, exps = x
+            ldx = x.shape[1]
+        else:
+            x, ldx = _rows(x, K)
+        xp = x.data_ptr()
+    dy, lddy = _rows(dy, N)
+    code = nat.dtype_code(dy.dtype)
+    grouped = 0 if plan is None else 1
+    scratch = _scratch("rq_multi_lora_scratch_size", dev, code, M, K, N, n, rank, grouped, 1)
+    nat.call("rq_multi_lora_grads", xp, nat.ptr(exps), code, M, K, ldx, dy.data_ptr(), N, lddy,
+             nat.ptr(plan), plan.numel() if grouped else 0, a.data_ptr(), b.data_ptr(), scaling.data_ptr(), n, rank,
+             nat.ptr(u) if need_b else None, nat.ptr(base), _ld(base) if base is not None else 0,
+             nat.ptr(dx), _ld(dx) if dx is not None else 0, nat.ptr(da), nat.ptr(db),
+             scratch.data_ptr(), scratch.numel(), nat.stream_handle(dev))
     return dx, da, db
 
 
@@ -958,37 +970,42 @@ def preference_forward(logits: torch.Tensor, labels: torch.Tensor, offsets: Opti
     if ref_logps is not None:
         if ref_logps.shape != (S,):
             raise RuntimeError(f"ref_logps must hold {S} values, got {tuple(ref_logps.shape)}")
-        ref_logps = ref_logps.detach().to(torch.float32).contiguous()
+        if ref_logps.dtype != torch.float32 or not ref_logps.is_contiguous():
+            ref_logps = ref_logps.detach().to(torch.float32).contiguous()
     labels = labels.contiguous()
     with on(dev):
-        if offsets is not None:
+        if offsets is not None and (offsets.dtype != torch.int32 or not offsets.is_contiguous()):
             offsets = offsets.to(torch.int32).contiguous()
         z, T, ld, period, outer = _logit_rows(logits)
         V = z.shape[-1]
-        f32 = functools.partial(torch.empty, dtype=torch.float32, device=dev)
-        logps, coef, info = f32(S), f32(S), f32((T, 4))
-        loss = f32(()) if pairs else None
+        # one allocation for what the backward pass keeps: 16 bytes a row, one value a sequence
+        state = torch.empty(4 * T + S, dtype=torch.float32, device=dev)
+        logps = torch.empty(S, dtype=torch.float32, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev) if pairs else None
         ws = _scratch("rq_preference_workspace_size", dev, code, T, V, S)
+        info = state.data_ptr()
         nat.call("rq_preference_forward", z.data_ptr(), code, T, V, ld, period, outer, labels.data_ptr(), nat.ptr(offsets), S,
                  int(ignore_index), nat.ptr(ref_logps), float(beta), float(label_smoothing), int(average), logps.data_ptr(),
-                 nat.ptr(loss), coef.data_ptr(), info.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_handle(dev))
-    return loss, logps, (info, coef)
+                 nat.ptr(loss), info + 16 * T, info, ws.data_ptr(), ws.numel(), nat.stream_handle(dev))
+    return loss, logps, state
 
 
 def preference_backward(logits: torch.Tensor, state, grad: Optional[torch.Tensor]) -> torch.Tensor:
     """The logits' gradient, contiguous, from preference_forward's state and the
     gradient of its loss (a scalar) or of its log-probabilities ([S])."""
-    info, coef = state
-    dev = nat.require_gpu(logits, info, coef, grad)
-    if grad is not None and (grad.dtype != torch.float32 or grad.numel() not in (1, coef.numel())):
-        raise RuntimeError(f"grad must be fp32, one value or {coef.numel()}, got {grad.dtype} {tuple(grad.shape)}")
+    dev = nat.require_gpu(logits, state, grad)
     with on(dev):
         z, T, ld, period, outer = _logit_rows(logits)
         V = z.shape[-1]
-        dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
-        per_seq = grad is not None and grad.dim() > 0
+        S = state.numel() - 4 * T
+        if S < 1 or state.dtype != torch.float32 or not state.is_contiguous():
+            raise RuntimeError(f"state is not preference_forward's of {T} rows")
         if grad is not None:
+            if grad.dtype != torch.float32 or grad.shape not in ((), (S,)):
+                raise RuntimeError(f"grad must be fp32, one value or {S}, got {grad.dtype} {tuple(grad.shape)}")
             grad = grad.contiguous()
-        nat.call("rq_preference_backward", z.data_ptr(), nat.dtype_code(z.dtype), T, V, ld, period, outer, info.data_ptr(),
-                 coef.data_ptr(), nat.ptr(grad), int(per_seq), dz.data_ptr(), V, nat.stream_handle(dev))
+        dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
+        info = state.data_ptr()
+        nat.call("rq_preference_backward", z.data_ptr(), nat.dtype_code(z.dtype), T, V, ld, period, outer, info, info + 16 * T,
+                 nat.ptr(grad), int(grad is not None and grad.dim() > 0), dz.data_ptr(), V, nat.stream_handle(dev))
     return dz
