@@ -784,30 +784,22 @@ __device__ __forceinline__ void rowsum_body(const RowSumArgs& a, const RowSumTas
       }
     }
   };
-  // this step's operands, which the L2 has, are asked for behind its rows and before the
-  // next step's rows, so that the wait for them leaves those in flight
+  // the next step's rows are known before its values are asked for; two or three waves a SIMD
+  // with eight loads each cover more latency than fewer waves with two steps in flight
   const int64_t live = ch.live;
   constexpr int64_t kAhead = 32 * kMlWaves;
   int64_t s = 32 * wave;
-  if (s < live) {
-    int r0[8], r1[8];
-    Raw x0[8], x1[8];
+  int r0[8], r1[8];
+  if (s < live) rows_of(r0, s);
+  for (; s < live; s += kAhead) {
+    Raw x[8];
     Ops o;
-    rows_of(r0, s);
-    load(x0, r0);
+    load(x, r0);
+    operands(o, s);
     if (s + kAhead < live) rows_of(r1, s + kAhead);
-    for (;;) {
-      operands(o, s);
-      if (s + kAhead < live) load(x1, r1);
-      products(x0, o, r0, s + 32 > live);
-      if ((s += kAhead) >= live) break;
-      if (s + kAhead < live) rows_of(r0, s + kAhead);
-      operands(o, s);
-      if (s + kAhead < live) load(x0, r0);
-      products(x1, o, r1, s + 32 > live);
-      if ((s += kAhead) >= live) break;
-      if (s + kAhead < live) rows_of(r1, s + kAhead);
-    }
+    products(x, o, r0, s + 32 > live);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r0[e] = r1[e];
   }
   // register q of lane (i, g): column CW (4 g + q) + c, rank i
 #pragma unroll

@@ -8,8 +8,10 @@
 //   dz[t, v] = c_i ([v = y_t] - exp(z[t, v] - max z[t]) / sum),  c_i = d loss / d L_i
 //
 // Three launches.  The rows' maxima and sums are one pass over the labelled
-// rows: every thread keeps its own running maximum and rescales its sum when a
-// piece of the row raises it; a row is split over workgroups when there are few.
+// rows: every thread keeps its own running maximum m and the sum of 2^(x log2 e - n),
+// n = ceil(m log2 e), which it rescales, by a power of two, when a piece of the row
+// raises n; a row is split over workgroups when there are few.  With an integer n the
+// argument is one fused multiply-add, rounded once and by 2^-24 of itself.
 // The second launch joins the splits and sums each sequence, in fp64 and in a
 // fixed order; the workgroup that ends last takes the pairs.  The gradient is a
 // second pass: a pair's coefficient depends on every row of the pair.
@@ -25,9 +27,12 @@ namespace rq {
 namespace {
 
 constexpr int kPfThreads = 256;
-constexpr int kPfUnroll = 4;       // 16-byte loads of a thread in flight
+#ifndef RQ_PF_U
+#define RQ_PF_U 4
+#endif
+constexpr int kPfUnroll = RQ_PF_U;       // 16-byte loads of a thread in flight
 constexpr int kPfSeqThreads = 1024;
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f;  // rounded to fp32
 
 // Rows of logits: T of them, row t at z + (t / period) * outer + (t % period) * ld.
 struct Rows {
@@ -76,24 +81,34 @@ __device__ __forceinline__ RowTarget row_target(const Labels& L, const Rows& r, 
 }
 
 // What the forward leaves for every row: its target (as above), sequence, maximum
-// and 1 / sum.
+// and sum (NaN for a row without a finite logit).
 struct RowInfo {
   int32_t target;
   int32_t seq;
   float top;
-  float inv;
+  float sum;
 };
 
-__device__ __forceinline__ float exp_diff(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * kLog2e); }
+// A maximum too large for its multiple of log2 e and the differences from it to mean
+// anything but "equal" or "nothing beside it".
+constexpr float kHuge = 0x1p100f;
+__device__ __forceinline__ bool huge(float m) { return !(fabsf(m) < kHuge); }
 
-// (m, s) joined with (m2, s2); an empty side has m = -inf, s = 0.
+// n of a maximum m, and a term of the sum relative to it.
+__device__ __forceinline__ float base_of(float m) {
+  return huge(m) ? (m > 0.0f ? 0x1p102f : -0x1p102f) : __builtin_ceilf(m * kLog2e);
+}
+__device__ __forceinline__ float term(float x, float n) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, -n)); }
+
+// (m, s) joined with (m2, s2); an empty side has m = -inf, s = 0, and an infinite maximum
+// makes the sum NaN, as exp(inf - inf) does.
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   const float top = fmaxf(m, m2);
-  if (top == -__builtin_inff()) {
-    s += s2;  // 0, or the NaN of a side that holds one
-    return;
-  }
-  s = s * exp_diff(m, top) + s2 * exp_diff(m2, top);
+  const float n = base_of(top);
+  // sides of a huge maximum count for nothing beside another one
+  const float f = m == top ? 1.0f : (huge(m) || huge(top)) ? 0.0f : __builtin_amdgcn_exp2f(base_of(m) - n);
+  const float f2 = m2 == top ? 1.0f : (huge(m2) || huge(top)) ? 0.0f : __builtin_amdgcn_exp2f(base_of(m2) - n);
+  s = s * f + s2 * f2;  // a NaN on either side stays one
   m = top;
 }
 
@@ -129,19 +144,28 @@ __global__ __launch_bounds__(kPfThreads) void row_sums_kernel(Rows r, Labels L, 
   const T* row = static_cast<const T*>(z) + r.at(t);
   const Piece<XT> p = piece_of<XT>(r.V, split, splits);
   float m = -__builtin_inff(), s = 0.0f;
-  auto take = [&](const float* f, int n) {
+  float base = base_of(m);
+  auto take = [&](const float* f, int count) {
     float top = m;
 #pragma unroll
-    for (int i = 0; i < n; ++i) top = fmaxf(top, f[i]);
-    if (top == -__builtin_inff()) {  // nothing above -inf yet; a NaN still has to show
+    for (int i = 0; i < count; ++i) top = fmaxf(top, f[i]);
+    if (huge(top)) {  // -inf so far, or one that only its equals stand beside; a NaN still has to show
+      if (top != m && !(s != s)) s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < n; ++i) s += f[i] != f[i] ? f[i] : 0.0f;
+      for (int i = 0; i < count; ++i) s += f[i] != f[i] ? f[i] : (f[i] == top && top > -__builtin_inff() ? 1.0f : 0.0f);
+      m = top;
+      base = base_of(top);
       return;
     }
-    s *= exp_diff(m, top);
+    if (top > m) {
+      const float n = base_of(top);
+      // what a huge negative maximum or none left behind counts for nothing (but a NaN)
+      s = huge(m) ? (s != s ? s : 0.0f) : s * __builtin_amdgcn_exp2f(base - n);
+      base = n;
+      m = top;
+    }
 #pragma unroll
-    for (int i = 0; i < n; ++i) s += exp_diff(f[i], top);
-    m = top;
+    for (int i = 0; i < count; ++i) s += term(f[i], base);
   };
   constexpr int64_t kSpan = int64_t(kPfThreads) * VW;
   int64_t v = p.v0 + threadIdx.x * VW;
@@ -178,6 +202,7 @@ __global__ __launch_bounds__(kPfThreads) void row_sums_kernel(Rows r, Labels L, 
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int w = 1; w < kPfThreads / 64; ++w) join(m, s, wm[w], wsum[w]);
+    if (m == __builtin_inff()) s = __builtin_nanf("");
     part[2 * (t * splits + split)] = m;
     part[2 * (t * splits + split) + 1] = s;
   }
@@ -219,13 +244,15 @@ __global__ __launch_bounds__(kPfSeqThreads) void sequences_kernel(Rows r, Labels
     if (y >= 0) {
       for (int k = 0; k < splits; ++k) join(m, s, part[2 * (t * splits + k)], part[2 * (t * splits + k) + 1]);
       const float x = to_f32<XT>(static_cast<const T*>(z)[r.at(t) + y]);
-      sum += double(x) - double(m) - log(double(s));
+      // log2 e as the sum's terms have it, so that its rounding is no error of x - m
+      sum += huge(m) ? double(x) - double(m) - log(double(s))
+                     : (double(x) * double(kLog2e) - double(base_of(m)) - log2(double(s))) / double(kLog2e);
     } else {
       s = __builtin_nanf("");
       sum = __builtin_nan("");
     }
     info[t].top = m;
-    info[t].inv = 1.0f / s;
+    info[t].sum = s > 0.0f ? s : __builtin_nanf("");
   }
   __shared__ double wsum[kPfSeqThreads / 64];
   __shared__ int64_t wcount[kPfSeqThreads / 64];
@@ -292,7 +319,11 @@ __global__ __launch_bounds__(kPfThreads) void logits_grad_kernel(Rows r, const v
                                                                  void* dz, int64_t lddz) {
   typedef typename Elem<XT>::T T;
   constexpr int VW = Elem<XT>::kVec;
+#ifdef RQ_REV
+  const int64_t t = r.T - 1 - blockIdx.x / unsigned(splits);
+#else
   const int64_t t = blockIdx.x / unsigned(splits);
+#endif
   const int split = int(blockIdx.x % unsigned(splits));
   const RowInfo I = info[t];
   const T* row = static_cast<const T*>(z) + r.at(t);
@@ -307,14 +338,21 @@ __global__ __launch_bounds__(kPfThreads) void logits_grad_kernel(Rows r, const v
   }
   float c = coef[I.seq];
   if (grad) c *= per_seq ? grad[I.seq] : grad[0];
-  const float k = -c * I.inv;
+  const float k = -c / I.sum, base = base_of(I.top);
+  const bool equal = huge(I.top);  // of the row
   auto put = [&](float (&f)[VW], int64_t at, int64_t n) {
+    float e[VW];
 #pragma unroll
-    for (int i = 0; i < VW; ++i) f[i] = k * exp_diff(f[i], I.top);
+    for (int i = 0; i < VW; ++i) {
+      e[i] = equal ? (f[i] == I.top ? 1.0f : 0.0f) : term(f[i], base);
+      f[i] = k * e[i];
+    }
     const int64_t y = I.target - at;
     if (y >= 0 && y < VW) {
+      // the label's 1 - p cancels: p by a division, 1 where nothing stands beside it
 #pragma unroll
-      for (int i = 0; i < VW; ++i) f[i] += i == y ? c : 0.0f;
+      for (int i = 0; i < VW; ++i)
+        if (i == y) f[i] = c * (1.0f - e[i] / I.sum);
     }
     store16_part<XT>(out + at, f, n);
   };
