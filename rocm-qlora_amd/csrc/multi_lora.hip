@@ -30,10 +30,10 @@ __device__ __forceinline__ void split16(float v, uint32_t& hi, uint32_t& lo) {
 }
 
 // ---- shrink ---------------------------------------------------------------------
-// A workgroup takes a tile's rows over a split of K; its four waves divide the split
-// and meet in LDS, 16 rows at a time, summed in the waves' order.  A wave holds the
-// tile's 16-row blocks (1 to 4, as many as the tile has) times JB blocks of 16 ranks,
-// so that a factor's piece is loaded once for the tile.
+// A workgroup takes a tile's rows over a split of K.  Tiles of one or two 16-row blocks: the
+// four waves divide the split and meet in LDS, 16 rows at a time, summed in the waves' order;
+// a wave holds the blocks times JB blocks of 16 ranks, so that a factor's piece is loaded once
+// for the tile.  Tiles of more: a wave takes a block, and the factor is shared through LDS.
 //
 // Rows and factor go through a wave's own piece of LDS.  Rows and A [r][K]: a step's 64
 // bytes of each, loaded by four adjacent lanes, the four pieces exchanged by the row so that
@@ -50,12 +50,12 @@ struct ShrinkLds {
   // elements of one wave's step, with the gaps
   static constexpr int kGap = 32 / int(sizeof(typename Elem<XT>::T));
   static constexpr int kTurn = Elem<XT>::kStep * 16 * JB + 4 * kGap + 2 * Elem<XT>::kVec;  // whole 16 bytes; the last kVec: no one's
-  static constexpr int kRows = 64 * 4 * Elem<XT>::kVec;  // of the tile's rows, a step
+  static constexpr int kRows = 32 * 4 * Elem<XT>::kVec;  // of two blocks of rows, a step
   static constexpr int kTurnFloats = kShWaves * (kTurn + kRows) * int(sizeof(typename Elem<XT>::T)) / 4;
 };
 
 template <int XT, int NRB, int JB, bool TURNED>
-__device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& tile, const int (&row)[4], int t, int split, int j0,
+__device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& tile, const int (&row)[2], int t, int split, int j0,
                                             float* lds) {
   typedef typename Elem<XT>::T T;
   typedef ShrinkLds<XT, JB> L;
@@ -203,20 +203,138 @@ __device__ __forceinline__ void shrink_body(const ShrinkArgs& a, const Tile& til
   }
 }
 
+// A wave a 16-row block, 256 bytes of every row (four steps) at a time: the factor's piece of
+// them [16 JB ranks][256 bytes] is shared by the waves, B's (TURNED) transposed on its way;
+// 16 bytes between rows, so that the lanes of a read meet other banks.  The next piece's loads
+// are in flight over this one's products.
+constexpr int kShPiece = 256 + 16;  // bytes of a row in LDS
+
 template <int XT, int JB, bool TURNED>
-__global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(JB == 4 ? 2 : 3))) void shrink_kernel(ShrinkArgs a) {
+__device__ __forceinline__ void shrink_blocks(const ShrinkArgs& a, const Tile& tile, int t, int split, int j0, char* lds) {
+  typedef typename Elem<XT>::T T;
+  constexpr int V = Elem<XT>::kVec, kStep = Elem<XT>::kStep, kPiece = 4 * kStep, P = kShPiece / int(sizeof(T));
+  const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t slot0 = int64_t(kTileRows) * t;
+  const T* s0 = static_cast<const T*>(a.s) + tile.adapter * a.s_adapter;
+  T* sl = reinterpret_cast<T*>(lds);
+  T* xl = sl + 16 * JB * P + wave * 16 * P;
+  // this lane's loads of the wave's rows: row 4 b + lane / 16, 16 bytes at lane % 16
+  const T* xr[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const int row = plan_row(a.rows, slot0 + 16 * wave + 4 * b + g);
+    xr[b] = static_cast<const T*>(a.x) + int64_t(row < 0 ? 0 : row) * a.ldx + V * i16;
+  }
+  // of the factor.  A: rank 16 b + tid / 16, 16 bytes at tid % 16.  B: a block of V k and V
+  // ranks, one a thread where there are that many: ranks V (tid % n), k V (tid / n), n = 16 JB / V.
+  constexpr int kRankBlocks = 16 * JB / V, kBlocks = kRankBlocks * (kPiece / V);
+  constexpr int kPer = TURNED ? V : JB;
+  const int tr = V * (tid % kRankBlocks), tk = V * (tid / kRankBlocks);
+  static_assert(!TURNED || kBlocks <= kShThreads, "a block a thread");
+  const bool turns = tid < kBlocks && j0 + tr < a.r;
+  u32x4 x[4], s[kPer];
+  auto load = [&](int64_t k, int64_t end) {  // k .. end - 1 of the piece at k
+    // whole pieces; 16 bytes from the last of B's ranks on stay in B
+    if (k + kPiece <= end && (!TURNED || a.r % V == 0 || (k + kPiece) * a.r + V <= a.K * a.r)) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) x[b] = load16_any(xr[b] + k);
+#pragma unroll
+      for (int b = 0; b < kPer; ++b) {
+        if constexpr (TURNED) {
+          s[b] = load16_any(s0 + (turns ? (k + tk + b) * a.r + j0 + tr : 0));
+        } else {
+          const int j = j0 + 16 * b + (tid >> 4);
+          s[b] = load16_any(s0 + int64_t(j < a.r ? j : 0) * a.K + k + V * (tid & 15));
+        }
+      }
+    } else {  // the end of the rows, or of B
+#pragma unroll
+      for (int b = 0; b < 4; ++b) x[b] = load16_part<XT>(xr[b] + k, end - k - V * i16);
+#pragma unroll
+      for (int b = 0; b < kPer; ++b) {
+        if constexpr (TURNED) {
+          s[b] = load16_part<XT>(s0 + (k + tk + b) * a.r + j0 + tr, turns && k + tk + b < end ? a.r - j0 - tr : 0);
+        } else {
+          const int j = j0 + 16 * b + (tid >> 4);
+          s[b] = load16_part<XT>(s0 + int64_t(j < a.r ? j : 0) * a.K + k + V * (tid & 15), end - k - V * (tid & 15));
+        }
+      }
+    }
+  };
+  auto stage = [&]() {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) *reinterpret_cast<u32x4*>(xl + (4 * b + g) * P + V * i16) = x[b];
+    if constexpr (TURNED) {
+      if (tid < kBlocks) {
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+          u32x4 o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (XT == RQ_DTYPE_F32) o[e] = s[e][c];
+            else o[e] = __builtin_amdgcn_perm(s[2 * e + 1][c >> 1], s[2 * e][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
+            o[e] = j0 + tr + c < a.r ? o[e] : 0u;
+          }
+          *reinterpret_cast<u32x4*>(sl + (tr + c) * P + tk) = o;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < JB; ++b) {
+        const bool on = j0 + 16 * b + (tid >> 4) < a.r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[b][e] = on ? s[b][e] : 0u;
+        *reinterpret_cast<u32x4*>(sl + (16 * b + (tid >> 4)) * P + V * (tid & 15)) = s[b];
+      }
+    }
+  };
+  f32x4 acc[JB];
+#pragma unroll
+  for (int j = 0; j < JB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int64_t kb = split * a.k_per_split, ke = std::min<int64_t>(kb + a.k_per_split, a.K);
+  if (kb < ke) load(kb, ke);
+#pragma unroll 1
+  for (int64_t k = kb; k < ke; k += kPiece) {
+    if (k > kb) __syncthreads();  // the last piece is read
+    stage();
+    __syncthreads();
+    if (k + kPiece < ke) load(k + kPiece, ke);
+    if (16 * wave >= tile.count) continue;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const u32x4 xo = *reinterpret_cast<const u32x4*>(xl + i16 * P + q * kStep + V * g);
+#pragma unroll
+      for (int j = 0; j < JB; ++j)
+        acc[j] = mma<XT>(xo, *reinterpret_cast<const u32x4*>(sl + (16 * j + i16) * P + q * kStep + V * g), acc[j]);
+    }
+  }
+  if (16 * wave >= tile.count) return;
+  // register q of lane (i, g) is row 4 g + q, rank i
+  float* out = a.part + (int64_t(split) * a.rows.slots() + slot0 + 16 * wave + 4 * g) * a.rp + j0 + i16;
+#pragma unroll
+  for (int j = 0; j < JB; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (j0 + 16 * j < a.rp) out[int64_t(q) * a.rp + 16 * j] = acc[j][q];
+}
+
+template <int XT, int JB, bool TURNED>
+__global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(3))) void shrink_kernel(ShrinkArgs a) {
   typedef ShrinkLds<XT, JB> L;
-  __shared__ __attribute__((aligned(16))) float lds[L::kTurnFloats > L::kRedFloats ? L::kTurnFloats : L::kRedFloats];
+  constexpr int kBlockFloats = (16 * JB + 64) * kShPiece / 4;
+  constexpr int kWaveFloats = L::kTurnFloats > L::kRedFloats ? L::kTurnFloats : L::kRedFloats;
+  __shared__ __attribute__((aligned(16))) float lds[kWaveFloats > kBlockFloats ? kWaveFloats : kBlockFloats];
   const int t = int(blockIdx.x % unsigned(a.rows.T)), split = int(blockIdx.x / unsigned(a.rows.T));
   const int j0 = 16 * JB * int(blockIdx.y);
   const Tile tile = plan_tile(a.rows, t);
-  int row[4];  // of the lane's loads: lane / 4 in each 16-row block
+  int row[2];  // of the lane's loads: lane / 4 in each 16-row block
 #pragma unroll
-  for (int b = 0; b < 4; ++b) row[b] = plan_row(a.rows, int64_t(kTileRows) * t + 16 * b + ((threadIdx.x & 63) >> 2));
+  for (int b = 0; b < 2; ++b) row[b] = plan_row(a.rows, int64_t(kTileRows) * t + 16 * b + ((threadIdx.x & 63) >> 2));
   if (tile.count == 0 || tile.adapter < 0) return;
   if (tile.count <= 16) shrink_body<XT, 1, JB, TURNED>(a, tile, row, t, split, j0, lds);
   else if (tile.count <= 32) shrink_body<XT, 2, JB, TURNED>(a, tile, row, t, split, j0, lds);
-  else shrink_body<XT, 4, JB, TURNED>(a, tile, row, t, split, j0, lds);
+  else shrink_blocks<XT, JB, TURNED>(a, tile, t, split, j0, reinterpret_cast<char*>(lds));
 }
 
 // About RQ_SH_WGS workgroups a compute unit, each wave with at least four steps.
@@ -246,13 +364,14 @@ int run_shrink(const ShrinkArgs& a, hipStream_t stream) {
   return rq_check_launch();
 }
 
-// Sum over the splits, in order, of four adjacent ranks of a slot.
+// Sum over the splits, in order, of four adjacent ranks of a slot; four splits in flight.
 __device__ __forceinline__ f32x4 split_sum4(const float* p, int splits, int64_t stride) {
-  f32x4 v = *reinterpret_cast<const f32x4*>(p);
-  for (int k = 1; k < splits; k += 4) {
+  f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (splits == 1) return *reinterpret_cast<const f32x4*>(p);
+  for (int k = 0; k < splits; k += 4) {
     f32x4 q[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const f32x4*>(p + (k + i < splits ? k + i : 0) * stride);
+    for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const f32x4*>(p + (k + i < splits ? k + i : k) * stride);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (k + i < splits)
@@ -308,6 +427,7 @@ __device__ __forceinline__ void sum_operands(typename Elem<XT>::T* op, int pitch
                                              int rp, int64_t slot0, int count) {
   const int quads = rp / 4, rows = (count + 15) & ~15;
   const int64_t stride = slots * rp;
+#pragma unroll 2
   for (int i = threadIdx.x; i < rows * quads; i += kMlThreads) {
     const int m = i / quads, j = 4 * (i - m * quads);
     const f32x4 v = split_sum4(part + (slot0 + m) * rp + j, splits, stride);
@@ -407,8 +527,9 @@ __device__ __forceinline__ void factor_of_rows(u32x4 (&f)[Elem<XT>::kVec], const
 }
 
 // BLOCKS: 16-row blocks that the waves divide (1, 2, 4).  EDGES: there are columns that a
-// whole wave does not fill, or ranks of B's rows that 16 bytes run past.
-template <int XT, bool FACTOR_ROWS, bool EDGES, int BLOCKS>
+// whole wave does not fill, or ranks of B's rows that 16 bytes run past.  LINES: the results'
+// rows are whole 64-byte lines.
+template <int XT, bool FACTOR_ROWS, bool EDGES, bool LINES, int BLOCKS>
 __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& tile, int t, int chunk, typename Elem<XT>::T* lds) {
   typedef typename Elem<XT>::T T;
   typedef ExpandLds<XT> L;
@@ -550,12 +671,12 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
       if (row[q] < 0) continue;
       T* o = static_cast<T*>(a.out) + row[q] * a.ld_out + col;
       if constexpr (EDGES) store16_part<XT>(o, v[q], a.C - col);
-      else store16_any(o, pack16<XT>(v[q]));
+      else store16<LINES>(o, pack16<XT>(v[q]));
     }
   }
 }
 
-template <int XT, bool FACTOR_ROWS, bool EDGES>
+template <int XT, bool FACTOR_ROWS, bool EDGES, bool LINES>
 __global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(EDGES ? 2 : 3))) void expand_kernel(ExpandArgs a) {
   typedef typename Elem<XT>::T T;
   extern __shared__ uint32_t expand_lds[];
@@ -564,9 +685,9 @@ __global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(EDGE
   const Tile tile = plan_tile(a.rows, t);
   if (tile.count == 0) return;
   if (tile.adapter < 0 && a.base == a.out && a.ld_base == a.ld_out) return;  // in place, nothing to add
-  if (tile.count <= 16) expand_body<XT, FACTOR_ROWS, EDGES, 1>(a, tile, t, chunk, lds);
-  else if (tile.count <= 32) expand_body<XT, FACTOR_ROWS, EDGES, 2>(a, tile, t, chunk, lds);
-  else expand_body<XT, FACTOR_ROWS, EDGES, 4>(a, tile, t, chunk, lds);
+  if (tile.count <= 16) expand_body<XT, FACTOR_ROWS, EDGES, LINES, 1>(a, tile, t, chunk, lds);
+  else if (tile.count <= 32) expand_body<XT, FACTOR_ROWS, EDGES, LINES, 2>(a, tile, t, chunk, lds);
+  else expand_body<XT, FACTOR_ROWS, EDGES, LINES, 4>(a, tile, t, chunk, lds);
 }
 
 template <int XT, bool FACTOR_ROWS>
@@ -588,13 +709,17 @@ int run_expand(ExpandArgs a, int cus, hipStream_t stream) {
     bytes = std::max(bytes, size_t((FACTOR_ROWS ? kMlWaves / blocks * L::kStage : 0) + 16 * blocks * pitch) * es);
   const bool edges = a.C % L::kCols != 0 || (FACTOR_ROWS && a.r > Elem<XT>::kStep && a.r % V != 0);
   const unsigned grid = unsigned(int64_t(a.rows.T) * a.chunks);
-  static std::atomic<uint64_t> done[2];
-  const int st = edges ? allow_lds(expand_kernel<XT, FACTOR_ROWS, true>, bytes, done[0])
-                       : allow_lds(expand_kernel<XT, FACTOR_ROWS, false>, bytes, done[1]);
-  if (st != RQ_OK) return st;
-  if (edges) expand_kernel<XT, FACTOR_ROWS, true><<<grid, kMlThreads, bytes, stream>>>(a);
-  else expand_kernel<XT, FACTOR_ROWS, false><<<grid, kMlThreads, bytes, stream>>>(a);
-  return rq_check_launch();
+  const bool lines = !edges && aligned(a.out, 64) && a.ld_out * es % 64 == 0;
+  auto launch = [&](auto kernel, std::atomic<uint64_t>& done) {
+    const int st = allow_lds(kernel, bytes, done);
+    if (st != RQ_OK) return st;
+    kernel<<<grid, kMlThreads, bytes, stream>>>(a);
+    return rq_check_launch();
+  };
+  static std::atomic<uint64_t> done[3];
+  if (edges) return launch(expand_kernel<XT, FACTOR_ROWS, true, false>, done[0]);
+  return lines ? launch(expand_kernel<XT, FACTOR_ROWS, false, true>, done[1])
+               : launch(expand_kernel<XT, FACTOR_ROWS, false, false>, done[2]);
 }
 
 // ---- sums over the rows of an adapter ----------------------------------------------

@@ -26,11 +26,9 @@
 namespace rq {
 namespace {
 
+
 constexpr int kPfThreads = 256;
-#ifndef RQ_PF_U
-#define RQ_PF_U 4
-#endif
-constexpr int kPfUnroll = RQ_PF_U;       // 16-byte loads of a thread in flight
+constexpr int kPfUnroll = 4;       // 16-byte loads of a thread in flight
 constexpr int kPfSeqThreads = 1024;
 constexpr float kLog2e = 1.44269504088896340736f;  // rounded to fp32
 
@@ -312,18 +310,15 @@ __global__ __launch_bounds__(kPfSeqThreads) void sequences_kernel(Rows r, Labels
   }
 }
 
-// dz = c ([v = y] - softmax), c = coef[seq] * (grad, or grad[seq] per sequence).
-template <int XT>
+// dz = c ([v = y] - softmax), c = coef[seq] * (grad, or grad[seq] per sequence).  LINES: the
+// gradient's rows are whole 64-byte lines.
+template <int XT, bool LINES>
 __global__ __launch_bounds__(kPfThreads) void logits_grad_kernel(Rows r, const void* z, int splits, const RowInfo* info,
                                                                  const float* coef, const float* grad, bool per_seq,
                                                                  void* dz, int64_t lddz) {
   typedef typename Elem<XT>::T T;
   constexpr int VW = Elem<XT>::kVec;
-#ifdef RQ_REV
-  const int64_t t = r.T - 1 - blockIdx.x / unsigned(splits);
-#else
   const int64_t t = blockIdx.x / unsigned(splits);
-#endif
   const int split = int(blockIdx.x % unsigned(splits));
   const RowInfo I = info[t];
   const T* row = static_cast<const T*>(z) + r.at(t);
@@ -333,7 +328,10 @@ __global__ __launch_bounds__(kPfThreads) void logits_grad_kernel(Rows r, const v
   int64_t v = p.v0 + threadIdx.x * VW;
   if (I.target == -1) {
     const float zero[VW] = {};
-    for (; v < p.v1; v += kSpan) store16_part<XT>(out + v, zero, p.v1 - v);
+    for (; v < p.v1; v += kSpan) {
+      if constexpr (LINES) store16<true>(out + v, u32x4{0u, 0u, 0u, 0u});
+      else store16_part<XT>(out + v, zero, p.v1 - v);
+    }
     return;
   }
   float c = coef[I.seq];
@@ -354,7 +352,8 @@ __global__ __launch_bounds__(kPfThreads) void logits_grad_kernel(Rows r, const v
       for (int i = 0; i < VW; ++i)
         if (i == y) f[i] = c * (1.0f - e[i] / I.sum);
     }
-    store16_part<XT>(out + at, f, n);
+    if constexpr (LINES) store16<true>(out + at, pack16<XT>(f));
+    else store16_part<XT>(out + at, f, n);
   };
   for (; v + (kPfUnroll - 1) * kSpan + VW <= p.v1; v += kPfUnroll * kSpan) {
     u32x4 raw[kPfUnroll];
@@ -374,12 +373,16 @@ __global__ __launch_bounds__(kPfThreads) void logits_grad_kernel(Rows r, const v
   }
 }
 
-// Workgroups of a row: enough rows fill the GPU by themselves; fewer are split
-// until there are about four workgroups a compute unit or pieces of 8 KiB.
-int row_splits(int64_t T, int64_t V, int es) {
-  const int64_t want = ceil_div(4 * int64_t(device_cus()), std::max<int64_t>(T, 1));
-  return int(std::max<int64_t>(1, std::min({want, ceil_div(V * es, int64_t(8192)), int64_t(64)})));
+// Workgroups of a row: pieces of `piece` bytes; fewer rows than fill the GPU are split until
+// there are about four workgroups a compute unit, or pieces of 8 KiB.
+int row_splits(int64_t T, int64_t V, int es, int64_t piece) {
+  const int64_t want = std::min<int64_t>(ceil_div(4 * int64_t(device_cus()), std::max<int64_t>(T, 1)), 64);
+  return int(std::max(ceil_div(V * es, piece), std::min(want, ceil_div(V * es, int64_t(8192)))));
 }
+// Bytes of a row that a workgroup takes.  4400 rows of 256 KB forward: 237 us in pieces of
+// 128 KiB, 253 in 64, 274 in 32, 244 whole; their gradient and 4400 rows of zeros: 644 us in
+// pieces of 32 KiB, 654 in 64, 668 in 128.
+constexpr int64_t kSumsPiece = 128 << 10, kGradPiece = 32 << 10;
 
 size_t up256(size_t b) { return (b + 255) & ~size_t(255); }
 
@@ -399,7 +402,7 @@ extern "C" int rq_preference_workspace_size(int dtype, int64_t T, int64_t V, int
   if (!bytes) return RQ_ERR_NULL_POINTER;
   if (!valid_float_dtype(dtype)) return RQ_ERR_BAD_DTYPE;
   if (T < 0 || V < 1 || S < 1) return RQ_ERR_BAD_SHAPE;
-  *bytes = int64_t(256 + up256(size_t(S) * 16) + up256(size_t(T) * row_splits(T, V, int(dtype_size(dtype))) * 8));
+  *bytes = int64_t(256 + up256(size_t(S) * 16) + up256(size_t(T) * row_splits(T, V, int(dtype_size(dtype)), kSumsPiece) * 8));
   return RQ_OK;
 }
 
@@ -414,7 +417,7 @@ extern "C" int rq_preference_forward(const void* logits, int dtype, int64_t T, i
   if (st != RQ_OK) return st;
   if (T < 1 || S < 1 || S > kMaxThreads1D / kPfSeqThreads || (loss && S % 2 != 0) || (!offsets && T % S != 0)) return RQ_ERR_BAD_SHAPE;
   if (!logps || !coef || !workspace || !logits || !labels || !row_info) return RQ_ERR_NULL_POINTER;
-  const int es = int(dtype_size(dtype)), splits = row_splits(T, V, es);
+  const int es = int(dtype_size(dtype)), splits = row_splits(T, V, es, kSumsPiece);
   int64_t need = 0;
   if ((st = rq_preference_workspace_size(dtype, T, V, S, &need)) != RQ_OK) return st;
   if (workspace_bytes < need) return RQ_ERR_WORKSPACE;
@@ -426,6 +429,7 @@ extern "C" int rq_preference_forward(const void* logits, int dtype, int64_t T, i
   RowInfo* info = static_cast<RowInfo*>(row_info);
   const Labels L{labels, offsets, S, ignore_index};
   const Pairs P{ref_logps, beta, label_smoothing, average != 0, loss != nullptr};
+  if (T * splits > kMaxThreads1D / kPfThreads) return RQ_ERR_UNSUPPORTED;
   const unsigned grid = unsigned(T * splits);
   RQ_DISPATCH_DT(dtype, XT, row_sums_kernel<XT><<<grid, kPfThreads, 0, stream>>>(r, L, logits, splits, info, part, done));
   if ((st = rq_check_launch()) != RQ_OK) return st;
@@ -446,9 +450,15 @@ extern "C" int rq_preference_backward(const void* logits, int dtype, int64_t T, 
   if (!logits || !row_info || !coef || !dlogits) return RQ_ERR_NULL_POINTER;
   const int es = int(dtype_size(dtype));
   if (!aligned(row_info, 16) || !aligned(logits, es) || !aligned(dlogits, es)) return RQ_ERR_BAD_ALIGNMENT;
-  const int splits = row_splits(T, V, es);
-  RQ_DISPATCH_DT(dtype, XT, logits_grad_kernel<XT><<<unsigned(T * splits), kPfThreads, 0, stream>>>(
-                                r, logits, splits, static_cast<const RowInfo*>(row_info), coef, grad,
-                                grad_per_sequence != 0, dlogits, lddz));
+  const int splits = row_splits(T, V, es, kGradPiece);
+  if (T * splits > kMaxThreads1D / kPfThreads) return RQ_ERR_UNSUPPORTED;
+  const unsigned grid = unsigned(T * splits);
+  const RowInfo* info = static_cast<const RowInfo*>(row_info);
+  if (aligned(dlogits, 64) && lddz * es % 64 == 0 && V * es % 64 == 0)
+    RQ_DISPATCH_DT(dtype, XT, logits_grad_kernel<XT, true><<<grid, kPfThreads, 0, stream>>>(
+                                  r, logits, splits, info, coef, grad, grad_per_sequence != 0, dlogits, lddz));
+  else
+    RQ_DISPATCH_DT(dtype, XT, logits_grad_kernel<XT, false><<<grid, kPfThreads, 0, stream>>>(
+                                  r, logits, splits, info, coef, grad, grad_per_sequence != 0, dlogits, lddz));
   return rq_check_launch();
 }

@@ -102,6 +102,9 @@ SHAPES = [
     (200, 1024, 1024, 17, 40),
     (257, 320, 72, 65, 3),
     (300, 192, 192, 130, 2),
+    (100, 40, 37, 1, 1),
+    (130, 700, 705, 3, 2),
+    (150, 384, 520, 20, 2),
     (90, 136, 129, 300, 2),
     (70, 512, 384, 512, 1),
     (700, 2049, 300, 32, 3),
