@@ -29,6 +29,14 @@ __device__ __forceinline__ void split16(float v, uint32_t& hi, uint32_t& lo) {
   lo = to_x16<XT>(fabsf(h) == __builtin_inff() ? 0.0f : v - h);
 }
 
+// Workgroup id -> unit of work, 0 .. n - 1 (n or more: none).  Workgroup ids go round the
+// eight XCDs; each gets adjacent units, so that what they share stays in its L2.
+constexpr int kXcds = 8;
+__device__ __forceinline__ unsigned xcd_unit(unsigned id, unsigned n) {
+  return id % kXcds * ((n + kXcds - 1) / kXcds) + id / kXcds;
+}
+inline unsigned xcd_grid(int64_t n) { return unsigned(ceil_div(n, kXcds) * kXcds); }
+
 // ---- shrink ---------------------------------------------------------------------
 // A workgroup takes a tile's rows over a split of K.  Tiles of one or two 16-row blocks: the
 // four waves divide the split and meet in LDS, 16 rows at a time, summed in the waves' order;
@@ -233,6 +241,7 @@ __device__ __forceinline__ void shrink_blocks(const ShrinkArgs& a, const Tile& t
   const int tr = V * (tid % kRankBlocks), tk = V * (tid / kRankBlocks);
   static_assert(!TURNED || kBlocks <= kShThreads, "a block a thread");
   const bool turns = tid < kBlocks && j0 + tr < a.r;
+  auto at = [](int row, int piece) { return V * (piece ^ ((row >> 3) & 7)); };  // of a factor's row
   u32x4 x[4], s[kPer];
   auto load = [&](int64_t k, int64_t end) {  // k .. end - 1 of the piece at k
     // whole pieces; 16 bytes from the last of B's ranks on stay in B
@@ -276,7 +285,7 @@ __device__ __forceinline__ void shrink_blocks(const ShrinkArgs& a, const Tile& t
             else o[e] = __builtin_amdgcn_perm(s[2 * e + 1][c >> 1], s[2 * e][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
             o[e] = j0 + tr + c < a.r ? o[e] : 0u;
           }
-          *reinterpret_cast<u32x4*>(sl + (tr + c) * P + tk) = o;
+          *reinterpret_cast<u32x4*>(sl + (tr + c) * P + at(tr + c, tk / V)) = o;
         }
       }
     } else {
@@ -285,7 +294,7 @@ __device__ __forceinline__ void shrink_blocks(const ShrinkArgs& a, const Tile& t
         const bool on = j0 + 16 * b + (tid >> 4) < a.r;
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[b][e] = on ? s[b][e] : 0u;
-        *reinterpret_cast<u32x4*>(sl + (16 * b + (tid >> 4)) * P + V * (tid & 15)) = s[b];
+        *reinterpret_cast<u32x4*>(sl + (16 * b + (tid >> 4)) * P + at(16 * b + (tid >> 4), tid & 15)) = s[b];
       }
     }
   };
@@ -306,7 +315,7 @@ __device__ __forceinline__ void shrink_blocks(const ShrinkArgs& a, const Tile& t
       const u32x4 xo = *reinterpret_cast<const u32x4*>(xl + i16 * P + q * kStep + V * g);
 #pragma unroll
       for (int j = 0; j < JB; ++j)
-        acc[j] = mma<XT>(xo, *reinterpret_cast<const u32x4*>(sl + (16 * j + i16) * P + q * kStep + V * g), acc[j]);
+        acc[j] = mma<XT>(xo, *reinterpret_cast<const u32x4*>(sl + (16 * j + i16) * P + at(16 * j + i16, 4 * q + g)), acc[j]);
     }
   }
   if (16 * wave >= tile.count) return;
@@ -325,7 +334,10 @@ __global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(3)))
   constexpr int kBlockFloats = (16 * JB + 64) * kShPiece / 4;
   constexpr int kWaveFloats = L::kTurnFloats > L::kRedFloats ? L::kTurnFloats : L::kRedFloats;
   __shared__ __attribute__((aligned(16))) float lds[kWaveFloats > kBlockFloats ? kWaveFloats : kBlockFloats];
-  const int t = int(blockIdx.x % unsigned(a.rows.T)), split = int(blockIdx.x / unsigned(a.rows.T));
+  // an XCD's workgroups take one split's piece of the factors, or two
+  const unsigned unit = xcd_unit(blockIdx.x, unsigned(a.rows.T) * unsigned(a.splits));
+  const int t = int(unit % unsigned(a.rows.T)), split = int(unit / unsigned(a.rows.T));
+  if (split >= a.splits) return;
   const int j0 = 16 * JB * int(blockIdx.y);
   const Tile tile = plan_tile(a.rows, t);
   int row[2];  // of the lane's loads: lane / 4 in each 16-row block
@@ -337,17 +349,12 @@ __global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(3)))
   else shrink_blocks<XT, JB, TURNED>(a, tile, t, split, j0, reinterpret_cast<char*>(lds));
 }
 
-// About RQ_SH_WGS workgroups a compute unit, each wave with at least four steps.
-#ifndef RQ_SH_WGS
-#define RQ_SH_WGS 2
-#endif
-#ifndef RQ_SH_MIN
-#define RQ_SH_MIN 4
-#endif
+// About two workgroups a compute unit, each with four steps a wave (many tiles: eight, since
+// every later workgroup of a tile sums the splits).
 void plan_shrink(int64_t T, int64_t K, int step, int cus, int* splits, int64_t* per) {
   const int64_t unit = int64_t(step) * kShWaves;
-  int64_t s = ceil_div(RQ_SH_WGS * cus, std::max<int64_t>(T, 1));
-  s = std::min(s, std::max<int64_t>(K / (RQ_SH_MIN * unit), 1));
+  int64_t s = ceil_div(2 * cus, std::max<int64_t>(T, 1));
+  s = std::min(s, std::max<int64_t>(K / ((T >= 48 ? 8 : 4) * unit), 1));
   s = std::min<int64_t>(std::max<int64_t>(s, 1), 16);
   *per = ceil_div(ceil_div(K, s), unit) * unit;
   *splits = int(ceil_div(K, *per));
@@ -356,8 +363,8 @@ void plan_shrink(int64_t T, int64_t K, int step, int cus, int* splits, int64_t* 
 template <int XT, bool TURNED>
 int run_shrink(const ShrinkArgs& a, hipStream_t stream) {
   const int jb = a.rp <= 16 ? 1 : (a.rp <= 32 ? 2 : 4);
-  if (int64_t(a.rows.T) * a.splits > kMaxThreads1D / kShThreads) return RQ_ERR_UNSUPPORTED;
-  const dim3 grid(unsigned(int64_t(a.rows.T) * a.splits), unsigned(ceil_div(a.rp, 16 * jb)));
+  if (int64_t(a.rows.T) * a.splits > kMaxThreads1D / kShThreads - kXcds) return RQ_ERR_UNSUPPORTED;
+  const dim3 grid(xcd_grid(int64_t(a.rows.T) * a.splits), unsigned(ceil_div(a.rp, 16 * jb)));
   if (jb == 1) shrink_kernel<XT, 1, TURNED><<<grid, kShThreads, 0, stream>>>(a);
   else if (jb == 2) shrink_kernel<XT, 2, TURNED><<<grid, kShThreads, 0, stream>>>(a);
   else shrink_kernel<XT, 4, TURNED><<<grid, kShThreads, 0, stream>>>(a);
@@ -681,7 +688,13 @@ __global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(EDGE
   typedef typename Elem<XT>::T T;
   extern __shared__ uint32_t expand_lds[];
   T* lds = reinterpret_cast<T*>(expand_lds);
+#ifdef RQ_EX_XCD
+  const unsigned unit = xcd_unit(blockIdx.x, unsigned(a.chunks) * unsigned(a.rows.T));
+  const int chunk = int(unit / unsigned(a.rows.T)), t = int(unit % unsigned(a.rows.T));
+  if (chunk >= a.chunks) return;
+#else
   const int chunk = int(blockIdx.x % unsigned(a.chunks)), t = int(blockIdx.x / unsigned(a.chunks));
+#endif
   const Tile tile = plan_tile(a.rows, t);
   if (tile.count == 0) return;
   if (tile.adapter < 0 && a.base == a.out && a.ld_base == a.ld_out) return;  // in place, nothing to add
@@ -708,7 +721,11 @@ int run_expand(ExpandArgs a, int cus, hipStream_t stream) {
   for (int blocks = 1; blocks <= kMlWaves; blocks *= 2)
     bytes = std::max(bytes, size_t((FACTOR_ROWS ? kMlWaves / blocks * L::kStage : 0) + 16 * blocks * pitch) * es);
   const bool edges = a.C % L::kCols != 0 || (FACTOR_ROWS && a.r > Elem<XT>::kStep && a.r % V != 0);
+#ifdef RQ_EX_XCD
+  const unsigned grid = xcd_grid(int64_t(a.rows.T) * a.chunks);
+#else
   const unsigned grid = unsigned(int64_t(a.rows.T) * a.chunks);
+#endif
   const bool lines = !edges && aligned(a.out, 64) && a.ld_out * es % 64 == 0;
   auto launch = [&](auto kernel, std::atomic<uint64_t>& done) {
     const int st = allow_lds(kernel, bytes, done);
