@@ -503,23 +503,20 @@ struct ExpandLds {
   static constexpr int kStage = kCols * Elem<XT>::kStep + 16 * Elem<XT>::kVec;
 };
 
-// kVec ranks from j on for each of kVec columns from `col` on of A's rows.
+// kVec columns from `col` on of A's rows j .. j + kVec - 1, and their transpose (zeros for
+// ranks from r on).
 template <int XT, bool EDGE>
-__device__ __forceinline__ void factor_of_rows(u32x4 (&f)[Elem<XT>::kVec], const typename Elem<XT>::T* s, int64_t C, int64_t col,
-                                               int r, int j) {
-  constexpr int V = Elem<XT>::kVec;
-  u32x4 row[V];
+__device__ __forceinline__ void load_ranks(u32x4 (&row)[Elem<XT>::kVec], const typename Elem<XT>::T* s, int64_t C, int64_t col,
+                                           int r, int j) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
+  for (int e = 0; e < Elem<XT>::kVec; ++e) {
     const typename Elem<XT>::T* p = s + int64_t(j + e < r ? j + e : 0) * C + col;
     row[e] = EDGE ? load16_part<XT>(p, C - col) : load16_any(p);
   }
-  if (j + V > r) {
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) row[e][d] = j + e < r ? row[e][d] : 0u;
-  }
+}
+template <int XT>
+__device__ __forceinline__ void turn_ranks(u32x4 (&f)[Elem<XT>::kVec], const u32x4 (&row)[Elem<XT>::kVec], int r, int j) {
+  constexpr int V = Elem<XT>::kVec;
 #pragma unroll
   for (int c = 0; c < V; ++c) {
     if constexpr (XT == RQ_DTYPE_F32) {
@@ -529,6 +526,16 @@ __device__ __forceinline__ void factor_of_rows(u32x4 (&f)[Elem<XT>::kVec], const
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         f[c][e] = __builtin_amdgcn_perm(row[2 * e + 1][c >> 1], row[2 * e][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
+    }
+  }
+  if (j + V > r) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t keep;
+      if constexpr (XT == RQ_DTYPE_F32) keep = j + e < r ? ~0u : 0u;
+      else keep = j + 2 * e + 1 < r ? ~0u : (j + 2 * e < r ? 0xFFFFu : 0u);
+#pragma unroll
+      for (int c = 0; c < V; ++c) f[c][e] &= keep;
     }
   }
 }
@@ -542,7 +549,7 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
   typedef ExpandLds<XT> L;
   constexpr int V = Elem<XT>::kVec, kStep = Elem<XT>::kStep;
   constexpr int GROUPS = kMlWaves / BLOCKS;                      // of columns
-  constexpr int PIECES = GROUPS * L::kCols * kStep / V / kMlThreads;
+  constexpr int PIECES = FACTOR_ROWS ? GROUPS * L::kCols * kStep / V / kMlThreads : V;
   const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int block = wave % BLOCKS, group = wave / BLOCKS;
@@ -563,9 +570,10 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
   int row[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) row[q] = plan_row(a.rows, slot0 + 16 * block + 4 * g + q);
-  // a step's pieces of B, as this thread copies them: 32-bit offsets from a uniform address
+  // a step's pieces of B, as this thread copies them (32-bit offsets from a uniform address),
+  // or of A, as its lane uses them
   u32x4 piece[PIECES];
-  uint32_t off[PIECES], put[PIECES];
+  uint32_t off[FACTOR_ROWS ? PIECES : 1], put[FACTOR_ROWS ? PIECES : 1];
   if constexpr (FACTOR_ROWS) {
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
@@ -576,25 +584,32 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
     }
   }
   auto fetch = [&](int64_t c0, int j0) {
-    const T* from = s + c0 * a.r + j0;
-    const int64_t left = (a.C - c0) * a.r - j0;
-    const uint32_t end = uint32_t(left < INT32_MAX ? left : INT32_MAX);
+    if constexpr (!FACTOR_ROWS) {
+      const int64_t col = c0 + group * L::kCols + V * i16;
+      load_ranks<XT, EDGES>(piece, s, a.C, col < a.C ? col : 0, a.r, j0 + (half ? V * (g & 1) : V * g));
+    } else {
+      const T* from = s + c0 * a.r + j0;
+      const int64_t left = (a.C - c0) * a.r - j0;
+      const uint32_t end = uint32_t(left < INT32_MAX ? left : INT32_MAX);
 #pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
-      const int f = V * (tid + kMlThreads * k);
-      const bool there = a.r <= kStep ? f < GROUPS * L::kCols * sp : j0 + f % kStep < a.r;
-      if constexpr (EDGES) piece[k] = load16_part<XT>(from + off[k], there && off[k] < end ? int64_t(end - off[k]) : 0);
-      else piece[k] = load16_any(from + (there && off[k] < end ? off[k] : 0u));
+      for (int k = 0; k < PIECES; ++k) {
+        const int f = V * (tid + kMlThreads * k);
+        const bool there = a.r <= kStep ? f < GROUPS * L::kCols * sp : j0 + f % kStep < a.r;
+        if constexpr (EDGES) piece[k] = load16_part<XT>(from + off[k], there && off[k] < end ? int64_t(end - off[k]) : 0);
+        else piece[k] = load16_any(from + (there && off[k] < end ? off[k] : 0u));
+      }
     }
   };
   auto stage = [&]() {
+    if constexpr (FACTOR_ROWS) {
 #pragma unroll
-    for (int k = 0; k < PIECES; ++k) {
-      const int f = V * (tid + kMlThreads * k);
-      if (f < GROUPS * L::kCols * sp) *reinterpret_cast<u32x4*>(lds + put[k]) = piece[k];
+      for (int k = 0; k < PIECES; ++k) {
+        const int f = V * (tid + kMlThreads * k);
+        if (f < GROUPS * L::kCols * sp) *reinterpret_cast<u32x4*>(lds + put[k]) = piece[k];
+      }
     }
   };
-  if (FACTOR_ROWS && adapted) fetch(c_first, 0);
+  if (adapted) fetch(c_first, 0);
   u32x4 base[4];
   auto fetch_base = [&](int64_t at) {  // from column `at` on
 #pragma unroll
@@ -616,8 +631,10 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
     const int64_t c0 = w0 + group * L::kCols, col = c0 + V * i16;
     const bool here = rows_here && c0 < a.C;
     auto ahead = [&](int k) {  // the next step's pieces
-      if (k + 1 < steps) fetch(w0, (k + 1) * kStep);
-      else if (it + 1 < a.iters * BLOCKS && w0 + GROUPS * L::kCols < a.C) fetch(w0 + GROUPS * L::kCols, 0);
+      const bool next = k + 1 == steps;
+      const int64_t from = next ? w0 + GROUPS * L::kCols : w0;
+      if (next && (it + 1 == a.iters * BLOCKS || from >= a.C)) return;
+      fetch(from, next ? 0 : (k + 1) * kStep);
     };
     f32x4 acc[V];
 #pragma unroll
@@ -644,8 +661,9 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
               for (int c = 0; c < V; ++c) f[c][e] &= keep;
             }
           }
-        } else if (here) {
-          factor_of_rows<XT, EDGES>(f, s, a.C, EDGES && col >= a.C ? 0 : col, a.r, j);
+        } else {
+          turn_ranks<XT>(f, piece, a.r, j);
+          ahead(k);
         }
         if (here) {
           const T* u = op + (16 * block + i16) * pitch + k * kStep + V * g;
@@ -688,13 +706,7 @@ __global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(EDGE
   typedef typename Elem<XT>::T T;
   extern __shared__ uint32_t expand_lds[];
   T* lds = reinterpret_cast<T*>(expand_lds);
-#ifdef RQ_EX_XCD
-  const unsigned unit = xcd_unit(blockIdx.x, unsigned(a.chunks) * unsigned(a.rows.T));
-  const int chunk = int(unit / unsigned(a.rows.T)), t = int(unit % unsigned(a.rows.T));
-  if (chunk >= a.chunks) return;
-#else
   const int chunk = int(blockIdx.x % unsigned(a.chunks)), t = int(blockIdx.x / unsigned(a.chunks));
-#endif
   const Tile tile = plan_tile(a.rows, t);
   if (tile.count == 0) return;
   if (tile.adapter < 0 && a.base == a.out && a.ld_base == a.ld_out) return;  // in place, nothing to add
@@ -708,11 +720,8 @@ int run_expand(ExpandArgs a, int cus, hipStream_t stream) {
   typedef ExpandLds<XT> L;
   constexpr int V = Elem<XT>::kVec, es = int(sizeof(typename Elem<XT>::T));
   const int64_t steps = ceil_div(a.C, int64_t(kMlWaves) * L::kCols);
-#ifndef RQ_EX_WGS
-#define RQ_EX_WGS 4
-#endif
-  // steps of a workgroup: as many as leave four workgroups a compute unit
-  a.iters = int(std::max<int64_t>(1, std::min<int64_t>(8, a.rows.T * steps / (RQ_EX_WGS * cus))));
+  // steps of a workgroup: as many as leave eight workgroups a compute unit
+  a.iters = int(std::max<int64_t>(1, std::min<int64_t>(8, a.rows.T * steps / (8 * cus))));
   a.chunks = int(ceil_div(steps, a.iters));
   if (int64_t(a.rows.T) * a.chunks > kMaxThreads1D / kMlThreads) return RQ_ERR_UNSUPPORTED;
   // LDS: the staged columns and the operands of 1, 2 or 4 row blocks, whichever is largest
@@ -721,11 +730,7 @@ int run_expand(ExpandArgs a, int cus, hipStream_t stream) {
   for (int blocks = 1; blocks <= kMlWaves; blocks *= 2)
     bytes = std::max(bytes, size_t((FACTOR_ROWS ? kMlWaves / blocks * L::kStage : 0) + 16 * blocks * pitch) * es);
   const bool edges = a.C % L::kCols != 0 || (FACTOR_ROWS && a.r > Elem<XT>::kStep && a.r % V != 0);
-#ifdef RQ_EX_XCD
-  const unsigned grid = xcd_grid(int64_t(a.rows.T) * a.chunks);
-#else
   const unsigned grid = unsigned(int64_t(a.rows.T) * a.chunks);
-#endif
   const bool lines = !edges && aligned(a.out, 64) && a.ld_out * es % 64 == 0;
   auto launch = [&](auto kernel, std::atomic<uint64_t>& done) {
     const int st = allow_lds(kernel, bytes, done);
