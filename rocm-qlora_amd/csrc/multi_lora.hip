@@ -353,7 +353,10 @@ __global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(3)))
 // every later workgroup of a tile sums the splits).
 void plan_shrink(int64_t T, int64_t K, int step, int cus, int* splits, int64_t* per) {
   const int64_t unit = int64_t(step) * kShWaves;
-  int64_t s = ceil_div(2 * cus, std::max<int64_t>(T, 1));
+  #ifndef RQ_SH_WGS
+#define RQ_SH_WGS 4
+#endif
+  int64_t s = ceil_div(RQ_SH_WGS * cus / 2, std::max<int64_t>(T, 1));
   s = std::min(s, std::max<int64_t>(K / ((T >= 48 ? 8 : 4) * unit), 1));
   s = std::min<int64_t>(std::max<int64_t>(s, 1), 16);
   *per = ceil_div(ceil_div(K, s), unit) * unit;
@@ -369,23 +372,6 @@ int run_shrink(const ShrinkArgs& a, hipStream_t stream) {
   else if (jb == 2) shrink_kernel<XT, 2, TURNED><<<grid, kShThreads, 0, stream>>>(a);
   else shrink_kernel<XT, 4, TURNED><<<grid, kShThreads, 0, stream>>>(a);
   return rq_check_launch();
-}
-
-// Sum over the splits, in order, of four adjacent ranks of a slot; four splits in flight.
-__device__ __forceinline__ f32x4 split_sum4(const float* p, int splits, int64_t stride) {
-  f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (splits == 1) return *reinterpret_cast<const f32x4*>(p);
-  for (int k = 0; k < splits; k += 4) {
-    f32x4 q[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const f32x4*>(p + (k + i < splits ? k + i : k) * stride);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (k + i < splits)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __fadd_rn(v[e], q[i][e]);
-  }
-  return v;
 }
 
 // ---- the row sums' operands -------------------------------------------------------
@@ -428,25 +414,49 @@ __device__ __forceinline__ void store_operands(typename Elem<XT>::T* opt, const 
   }
 }
 
-// The splits' sum of a tile's slots, in order, as operands in LDS rows of `pitch`.
+// The splits' sum of a tile's slots, in order, as operands in LDS rows of `pitch`.  A thread
+// takes four adjacent ranks of two slots at a time, four splits of each in flight.
 template <int XT>
 __device__ __forceinline__ void sum_operands(typename Elem<XT>::T* op, int pitch, const float* part, int splits, int64_t slots,
                                              int rp, int64_t slot0, int count) {
-  const int quads = rp / 4, rows = (count + 15) & ~15;
+  const int quads = rp / 4, items = ((count + 15) & ~15) * quads;
   const int64_t stride = slots * rp;
-#pragma unroll 2
-  for (int i = threadIdx.x; i < rows * quads; i += kMlThreads) {
-    const int m = i / quads, j = 4 * (i - m * quads);
-    const f32x4 v = split_sum4(part + (slot0 + m) * rp + j, splits, stride);
-    typename Elem<XT>::T* o = op + m * pitch + j;
-    if constexpr (XT == RQ_DTYPE_F32) {
-      *reinterpret_cast<f32x4*>(o) = v;
-    } else {
-      uint32_t hi[4], lo[4];
+  const float* p0 = part + slot0 * rp;
+  for (int i0 = threadIdx.x; i0 < items; i0 += 2 * kMlThreads) {
+    f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    const float* p[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) split16<XT>(v[e], hi[e], lo[e]);
-      *reinterpret_cast<u32x2*>(o) = u32x2{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16};
-      *reinterpret_cast<u32x2*>(o + rp) = u32x2{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16};
+    for (int h = 0; h < 2; ++h) p[h] = p0 + 4 * (i0 + h * kMlThreads < items ? i0 + h * kMlThreads : i0);  // rows are end to end
+    for (int k = 0; k < splits; k += 4) {
+      f32x4 q[2][4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (n == 0 || k + n < splits) q[h][n] = *reinterpret_cast<const f32x4*>(p[h] + (k + n) * stride);
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (n == 0 || k + n < splits)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[h][e] = __fadd_rn(v[h][e], q[h][n][e]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = i0 + h * kMlThreads;
+      if (i >= items) break;
+      const int m = i / quads;
+      typename Elem<XT>::T* o = op + m * pitch + 4 * (i - m * quads);
+      if constexpr (XT == RQ_DTYPE_F32) {
+        *reinterpret_cast<f32x4*>(o) = v[h];
+      } else {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split16<XT>(v[h][e], hi[e], lo[e]);
+        *reinterpret_cast<u32x2*>(o) = u32x2{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16};
+        *reinterpret_cast<u32x2*>(o + rp) = u32x2{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16};
+      }
     }
   }
 }
