@@ -552,8 +552,8 @@ __device__ __forceinline__ void turn_ranks(u32x4 (&f)[Elem<XT>::kVec], const u32
 
 // BLOCKS: 16-row blocks that the waves divide (1, 2, 4).  EDGES: there are columns that a
 // whole wave does not fill, or ranks of B's rows that 16 bytes run past.  LINES: the results'
-// rows are whole 64-byte lines.
-template <int XT, bool FACTOR_ROWS, bool EDGES, bool LINES, int BLOCKS>
+// rows are whole 64-byte lines.  BASED: there is a base.
+template <int XT, bool FACTOR_ROWS, bool EDGES, bool LINES, bool BASED, int BLOCKS>
 __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& tile, int t, int chunk, typename Elem<XT>::T* lds) {
   typedef typename Elem<XT>::T T;
   typedef ExpandLds<XT> L;
@@ -622,11 +622,13 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
   if (adapted) fetch(c_first, 0);
   u32x4 base[4];
   auto fetch_base = [&](int64_t at) {  // from column `at` on
+    if constexpr (BASED) {
+      if (!EDGES && at - V * i16 >= a.C) at = V * i16;  // not used
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      base[q] = u32x4{0u, 0u, 0u, 0u};
-      const T* p = static_cast<const T*>(a.base) + (row[q] < 0 ? 0 : row[q]) * a.ld_base + at;
-      if (a.base && at - V * i16 < a.C) base[q] = EDGES ? load16_part<XT>(p, a.C - at) : load16_any(p);
+      for (int q = 0; q < 4; ++q) {
+        const T* p = static_cast<const T*>(a.base) + (row[q] < 0 ? 0 : row[q]) * a.ld_base + at;
+        base[q] = EDGES ? load16_part<XT>(p, a.C - at) : load16_any(p);
+      }
     }
   };
   fetch_base(c_first + group * L::kCols + V * i16);
@@ -640,12 +642,10 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
     if (w0 >= a.C) return;
     const int64_t c0 = w0 + group * L::kCols, col = c0 + V * i16;
     const bool here = rows_here && c0 < a.C;
-    auto ahead = [&](int k) {  // the next step's pieces
-      const bool next = k + 1 == steps;
-      const int64_t from = next ? w0 + GROUPS * L::kCols : w0;
-      if (next && (it + 1 == a.iters * BLOCKS || from >= a.C)) return;
-      fetch(from, next ? 0 : (k + 1) * kStep);
-    };
+    // the next step's pieces (after the last step: these again, so that no branch makes the
+    // loads' results wait)
+    const int64_t w1 = it + 1 < a.iters * BLOCKS && w0 + GROUPS * L::kCols < a.C ? w0 + GROUPS * L::kCols : w0;
+    auto ahead = [&](int k) { fetch(k + 1 < steps ? w0 : w1, k + 1 < steps ? (k + 1) * kStep : 0); };
     f32x4 acc[V];
 #pragma unroll
     for (int c = 0; c < V; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -694,8 +694,8 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
     }
     float v[4][V];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) unpack16<XT>(base[q], v[q]);
-    if (it + 1 < a.iters * BLOCKS) fetch_base(col + GROUPS * L::kCols);
+    for (int q = 0; q < 4; ++q) unpack16<XT>(BASED ? base[q] : u32x4{0u, 0u, 0u, 0u}, v[q]);
+    fetch_base(w1 + group * L::kCols + V * i16);
     if (!here) continue;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -711,7 +711,7 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
   }
 }
 
-template <int XT, bool FACTOR_ROWS, bool EDGES, bool LINES>
+template <int XT, bool FACTOR_ROWS, bool EDGES, bool LINES, bool BASED>
 __global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(EDGES ? 2 : 3))) void expand_kernel(ExpandArgs a) {
   typedef typename Elem<XT>::T T;
   extern __shared__ uint32_t expand_lds[];
@@ -720,9 +720,9 @@ __global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(EDGE
   const Tile tile = plan_tile(a.rows, t);
   if (tile.count == 0) return;
   if (tile.adapter < 0 && a.base == a.out && a.ld_base == a.ld_out) return;  // in place, nothing to add
-  if (tile.count <= 16) expand_body<XT, FACTOR_ROWS, EDGES, LINES, 1>(a, tile, t, chunk, lds);
-  else if (tile.count <= 32) expand_body<XT, FACTOR_ROWS, EDGES, LINES, 2>(a, tile, t, chunk, lds);
-  else expand_body<XT, FACTOR_ROWS, EDGES, LINES, 4>(a, tile, t, chunk, lds);
+  if (tile.count <= 16) expand_body<XT, FACTOR_ROWS, EDGES, LINES, BASED, 1>(a, tile, t, chunk, lds);
+  else if (tile.count <= 32) expand_body<XT, FACTOR_ROWS, EDGES, LINES, BASED, 2>(a, tile, t, chunk, lds);
+  else expand_body<XT, FACTOR_ROWS, EDGES, LINES, BASED, 4>(a, tile, t, chunk, lds);
 }
 
 template <int XT, bool FACTOR_ROWS>
@@ -748,10 +748,15 @@ int run_expand(ExpandArgs a, int cus, hipStream_t stream) {
     kernel<<<grid, kMlThreads, bytes, stream>>>(a);
     return rq_check_launch();
   };
-  static std::atomic<uint64_t> done[3];
-  if (edges) return launch(expand_kernel<XT, FACTOR_ROWS, true, false>, done[0]);
-  return lines ? launch(expand_kernel<XT, FACTOR_ROWS, false, true>, done[1])
-               : launch(expand_kernel<XT, FACTOR_ROWS, false, false>, done[2]);
+  static std::atomic<uint64_t> done[6];
+  if (!a.base) {
+    if (edges) return launch(expand_kernel<XT, FACTOR_ROWS, true, false, false>, done[0]);
+    return lines ? launch(expand_kernel<XT, FACTOR_ROWS, false, true, false>, done[1])
+                 : launch(expand_kernel<XT, FACTOR_ROWS, false, false, false>, done[2]);
+  }
+  if (edges) return launch(expand_kernel<XT, FACTOR_ROWS, true, false, true>, done[3]);
+  return lines ? launch(expand_kernel<XT, FACTOR_ROWS, false, true, true>, done[4])
+               : launch(expand_kernel<XT, FACTOR_ROWS, false, false, true>, done[5]);
 }
 
 // ---- sums over the rows of an adapter ----------------------------------------------
