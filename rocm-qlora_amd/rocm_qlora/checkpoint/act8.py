@@ -15,6 +15,7 @@ from dataclasses import dataclass
 import torch
 
 from rocm_qlora import ops
+from rocm_qlora.torch_ops import eager_only
 
 
 @dataclass(frozen=True)
@@ -29,12 +30,14 @@ class Act8:
         return self.codes.numel() + self.exponents.numel()
 
 
+@eager_only
 def compress(x: torch.Tensor) -> Act8:
     """x ([..., K], fp32/bf16/fp16, on the GPU) as its 8-bit checkpoint."""
     codes, exps = ops.act8_quantize(x.detach())
     return Act8(codes, exps, x.shape, x.dtype)
 
 
+@eager_only
 def decompress(c: Act8) -> torch.Tensor:
     """The values that a checkpoint stands for, in the shape and dtype it was made from."""
     return ops.act8_dequantize(c.codes, c.exponents, c.shape[-1], c.dtype).view(c.shape)

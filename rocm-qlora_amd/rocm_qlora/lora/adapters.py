@@ -18,8 +18,10 @@ from torch.autograd.function import once_differentiable
 
 from rocm_qlora import ops
 from rocm_qlora._device import on
+from rocm_qlora.kernels import dequant_matmul as dm
 from rocm_qlora.lora.lora_layer import LoRALinear
 from rocm_qlora.quantization.quant_linear import QuantLinear
+from rocm_qlora.torch_ops import eager_only
 
 
 class AdapterRows:
@@ -95,6 +97,7 @@ class _MultiLoRA(torch.autograd.Function):
         return dx if shape is None or dx is None else dx.view(shape), da, db, dy if need[3] else None, None, None, None, None
 
 
+@eager_only
 def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: Union[float, torch.Tensor],
                rows: AdapterRows, base: Optional[torch.Tensor] = None, activation_bits: int = 16) -> torch.Tensor:
     """base[m] + scaling[a] (x[m] A[a]^T) B[a]^T for the adapter a of every row m.
@@ -111,8 +114,7 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
                            f"{lora_b.shape[1]} columns")
     if not isinstance(scaling, torch.Tensor):
         scaling = torch.full((rows.n,), float(scaling), dtype=torch.float32, device=x.device)
-    if not (torch.is_grad_enabled() and (x.requires_grad or lora_a.requires_grad or lora_b.requires_grad or
-                                         (base is not None and base.requires_grad))):
+    if dm._nothing_recorded(x, lora_a, lora_b, base):
         dtype = x.dtype
         a = lora_a if lora_a.dtype == dtype else lora_a.to(dtype)
         b = lora_b if lora_b.dtype == dtype else lora_b.to(dtype)
@@ -159,23 +161,22 @@ class MultiLoRALinear(nn.Module):
 
     def _linear(self):
         """The quantized linear and its input gradient as functions of 2-D rows."""
-        from rocm_qlora import torch_ops
-        from rocm_qlora.kernels import dequant_matmul as dm
         base = self.base_layer
         if base.bits == 4:
             w = base.nf4_weight()
             return (lambda x: ops.nf4_linear(x, w.packed, w.scales, w.N, w.block_size, base.bias, **w.dq_kwargs()),
-                    lambda dy: torch_ops.call_nf4_linear_dx(dy, w.packed, w.scales, w.K, w.block_size, **w.dq_kwargs()))
+                    lambda dy: ops.nf4_linear_dx(dy, w.packed, w.scales, w.K, w.block_size, **w.dq_kwargs()))
         w = base.int8_weight()
-        return (lambda x: ops.int8_linear(x, w.q, w.scales, w.N, w.block_size, base.bias), lambda dy: dm.int8_dx(dy, w))
+        return (lambda x: ops.int8_linear(x, w.q, w.scales, w.N, w.block_size, base.bias), lambda dy: ops.int8_linear_dx(dy, w.q, w.scales, w.K, w.block_size))
 
+    @eager_only
     def forward(self, x: torch.Tensor, rows: Optional[AdapterRows] = None) -> torch.Tensor:
         rows = rows if rows is not None else self.rows
         if rows is None:
             raise RuntimeError("no adapter rows: pass them, or set them with set_adapter_rows(model, rows)")
         _check(x, self.lora_A, rows, self.activation_bits)
         linear = self._linear()
-        if torch.is_grad_enabled() and (x.requires_grad or self.lora_A.requires_grad or self.lora_B.requires_grad):
+        if not dm._nothing_recorded(x, self.lora_A, self.lora_B):
             return _MultiLoRA.apply(x, self.lora_A, self.lora_B, None, self.scaling, rows, self.activation_bits, linear)
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         y = linear[0](x2)
@@ -198,7 +199,8 @@ def set_adapter_rows(model: nn.Module, rows: Optional[AdapterRows]) -> int:
 
 def attach_adapters(model: nn.Module, n: int, activation_bits: int = 16) -> nn.Module:
     """Replace every LoRALinear (quantize_model's) by a MultiLoRALinear of n adapters of
-    its rank over the same quantized weight; adapter 0 is the layer's own."""
+    its rank over the same quantized weight; adapter 0 is the layer's own (without its
+    dropout)."""
     for name, m in list(model.named_modules()):
         if isinstance(m, LoRALinear):
             if m.merged:

@@ -15,6 +15,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from rocm_qlora import ops
+from rocm_qlora.kernels.dequant_matmul import _nothing_recorded
+from rocm_qlora.torch_ops import eager_only
 
 
 class _PreferenceLoss(torch.autograd.Function):
@@ -49,6 +51,7 @@ class _SequenceLogps(torch.autograd.Function):
         return (ops.preference_backward(logits, state, dlogps),) + (None,) * 4
 
 
+@eager_only
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, offsets: Optional[torch.Tensor] = None,
                     ref_logps: Optional[torch.Tensor] = None, *, beta: float = 0.1, label_smoothing: float = 0.0,
                     average: bool = False, ignore_index: int = -100) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -62,18 +65,19 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, offsets: Optiona
     ref_logps: the reference model's sequence_logps, [2 P] (None: zeros).
     average: log-probabilities per labelled token instead of their sum.
     loss is differentiable by the logits; logps [2 P] (fp32) is not."""
-    if not (torch.is_grad_enabled() and logits.requires_grad):
+    if _nothing_recorded(logits):
         return ops.preference_forward(logits, labels, offsets, ref_logps, beta=beta, label_smoothing=label_smoothing,
                                       average=average, ignore_index=ignore_index)[:2]
     return _PreferenceLoss.apply(logits, labels, offsets, ref_logps, float(beta), float(label_smoothing), bool(average),
                                  int(ignore_index))
 
 
+@eager_only
 def sequence_logps(logits: torch.Tensor, labels: torch.Tensor, offsets: Optional[torch.Tensor] = None, *,
                    average: bool = False, ignore_index: int = -100) -> torch.Tensor:
     """Log-probabilities [S] (fp32) of the labelled tokens of S sequences, laid out as
     preference_loss takes them; differentiable by the logits.  Under torch.no_grad
     these are preference_loss's ref_logps when the reference model gives the logits."""
-    if not (torch.is_grad_enabled() and logits.requires_grad):
+    if _nothing_recorded(logits):
         return ops.preference_forward(logits, labels, offsets, average=average, ignore_index=ignore_index, pairs=False)[1]
     return _SequenceLogps.apply(logits, labels, offsets, bool(average), int(ignore_index))

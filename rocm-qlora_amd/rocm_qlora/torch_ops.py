@@ -19,6 +19,7 @@ goes through these operators (`call`).
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -122,6 +123,21 @@ def compiling() -> bool:
         return torch.compiler.is_compiling()
     except AttributeError:  # older torch
         return False
+
+
+def eager_only(fn):
+    """fn, which calls kernels on its tensors' memory: torch.compile runs it as it is,
+    between the traced parts, and torch.jit.trace, which would record a result that
+    nothing fills, is refused."""
+    uncompiled = torch.compiler.disable(fn)
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        if torch._C._is_tracing():
+            raise RuntimeError(f"{fn.__qualname__} cannot be traced by torch.jit.trace")
+        return uncompiled(*args, **kwargs) if compiling() else fn(*args, **kwargs)
+
+    return call
 
 
 def call_nf4_linear(x, weight_quant, weight_scales, out_features, block_size=64, bias=None, *, c2=None,

@@ -368,6 +368,23 @@ def test_attach_adapters(dev):
     assert bool((err <= 2 * U[BF16] * (one[:10].double().abs() + 2 * term[:10])).all())
 
 
+def test_traced_calls_are_refused_or_run_eagerly(dev):
+    """torch.jit.trace raises rather than record a result that nothing fills; torch.compile
+    runs the call as it is, between the traced parts."""
+    d = make(12, 64, 32, 4, 2, BF16, dev)
+    rows = AdapterRows(d["ids"], 2)
+    f = lambda x: multi_lora(x, d["a"], d["b"], d["s"], rows, d["base"])
+    with torch.no_grad():
+        want = f(d["x"])
+        with pytest.raises(RuntimeError):
+            torch.jit.trace(f, (d["x"],), check_trace=False)
+        torch._dynamo.reset()
+        g = torch.compile(lambda x: f(x * 1.0) + 1.0, backend="eager")
+        assert torch.equal(g(d["x"]), want + 1.0)
+    x = d["x"].clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(g(x), x, d["dy"])[0], run_all(d, rows)[1])
+
+
 # ---- refusals ---------------------------------------------------------------------
 def test_refusals(dev):
     d = make(8, 32, 16, 4, 2, BF16, dev)
