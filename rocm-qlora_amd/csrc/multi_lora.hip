@@ -353,10 +353,7 @@ __global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(3)))
 // every later workgroup of a tile sums the splits).
 void plan_shrink(int64_t T, int64_t K, int step, int cus, int* splits, int64_t* per) {
   const int64_t unit = int64_t(step) * kShWaves;
-  #ifndef RQ_SH_WGS
-#define RQ_SH_WGS 4
-#endif
-  int64_t s = ceil_div(RQ_SH_WGS * cus / 2, std::max<int64_t>(T, 1));
+  int64_t s = ceil_div(2 * cus, std::max<int64_t>(T, 1));
   s = std::min(s, std::max<int64_t>(K / ((T >= 48 ? 8 : 4) * unit), 1));
   s = std::min<int64_t>(std::max<int64_t>(s, 1), 16);
   *per = ceil_div(ceil_div(K, s), unit) * unit;
@@ -415,10 +412,11 @@ __device__ __forceinline__ void store_operands(typename Elem<XT>::T* opt, const 
 }
 
 // The splits' sum of a tile's slots, in order, as operands in LDS rows of `pitch`.  A thread
-// takes four adjacent ranks of two slots at a time, four splits of each in flight.
+// takes four adjacent ranks of two slots at a time, four splits of each in flight.  Ranks from
+// r on are zeros whatever the row held: an infinity times their zero factors is no zero.
 template <int XT>
 __device__ __forceinline__ void sum_operands(typename Elem<XT>::T* op, int pitch, const float* part, int splits, int64_t slots,
-                                             int rp, int64_t slot0, int count) {
+                                             int r, int rp, int64_t slot0, int count) {
   const int quads = rp / 4, items = ((count + 15) & ~15) * quads;
   const int64_t stride = slots * rp;
   const float* p0 = part + slot0 * rp;
@@ -446,8 +444,10 @@ __device__ __forceinline__ void sum_operands(typename Elem<XT>::T* op, int pitch
     for (int h = 0; h < 2; ++h) {
       const int i = i0 + h * kMlThreads;
       if (i >= items) break;
-      const int m = i / quads;
-      typename Elem<XT>::T* o = op + m * pitch + 4 * (i - m * quads);
+      const int m = i / quads, j = 4 * (i - m * quads);
+      typename Elem<XT>::T* o = op + m * pitch + j;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[h][e] = j + e < r ? v[h][e] : 0.0f;
       if constexpr (XT == RQ_DTYPE_F32) {
         *reinterpret_cast<f32x4*>(o) = v[h];
       } else {
@@ -471,7 +471,7 @@ __global__ __launch_bounds__(kMlThreads) void operands_kernel(OperandsArgs a) {
   if (tile.count == 0 || tile.adapter < 0) return;
   const int pitch = (XT == RQ_DTYPE_F32 ? a.rp : 2 * a.rp) + Elem<XT>::kVec;
   const int64_t slot0 = int64_t(kTileRows) * blockIdx.x;
-  sum_operands<XT>(op, pitch, a.part, a.splits, a.rows.slots(), a.rp, slot0, tile.count);
+  sum_operands<XT>(op, pitch, a.part, a.splits, a.rows.slots(), a.r, a.rp, slot0, tile.count);
   __syncthreads();
   store_operands<XT>(static_cast<T*>(a.opt), op, pitch, a.rp, slot0, tile.count);
 }
@@ -632,7 +632,7 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
     }
   };
   fetch_base(c_first + group * L::kCols + V * i16);
-  if (adapted) sum_operands<XT>(op, pitch, a.part, a.splits, a.rows.slots(), a.rp, slot0, tile.count);
+  if (adapted) sum_operands<XT>(op, pitch, a.part, a.splits, a.rows.slots(), a.r, a.rp, slot0, tile.count);
   __syncthreads();
   if (a.opt && adapted && chunk == 0) store_operands<XT>(static_cast<T*>(a.opt), op, pitch, a.rp, slot0, tile.count);
   const bool rows_here = 16 * block < tile.count;
@@ -1210,7 +1210,7 @@ int backward(const BackwardCall& c, char* ws, hipStream_t stream) {
                        gt, 0, 0};
     st = run_expand<XT, false>(e, device_cus(), stream);
   } else if (c.da) {
-    st = run_operands<XT>(OperandsArgs{c.rows, rp, part, p.splits, gt}, stream);
+    st = run_operands<XT>(OperandsArgs{c.rows, r, rp, part, p.splits, gt}, stream);
   }
   if (st != RQ_OK) return st;
   RowSumArgs q{};

@@ -112,19 +112,6 @@ __device__ __forceinline__ void store16_part(typename Elem<XT>::T* p, const floa
   else store_edge<XT>(p, pack16<XT>(f), int(n));
 }
 
-// The first `n` of four values.
-template <int XT>
-__device__ __forceinline__ void store4(typename Elem<XT>::T* p, const float (&f)[4], int64_t n) {
-  if (n >= 4) {
-    if constexpr (XT == RQ_DTYPE_F32) store16_any(p, u32x4{f2u(f[0]), f2u(f[1]), f2u(f[2]), f2u(f[3])});
-    else *reinterpret_cast<u32x2_any*>(p) = u32x2_any{cvt_pk<XT>(f[0], f[1]), cvt_pk<XT>(f[2], f[3])};
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < n) p[i] = from_f32<XT>(f[i]);
-}
-
 // acc += A B over kStep contraction steps, both operands as 16 bytes a lane: lane
 // (i, g) = (l % 16, l / 16) holds A[i][V g + e] and B[V g + e][i], e < V = kVec;
 // register r of the result is D[4 g + r][i].

@@ -11,7 +11,9 @@
 // It is passed as two of them, hi = RND(u) and lo = RND(u - hi), whose products
 // are both added: 16 bits of u (bf16; 22 fp16) instead of 8 (11), at twice the
 // products over the rank alone, which memory hides.  fp32 rows run on the fp32
-// matrix instructions.
+// matrix instructions.  So fp16 rows take u up to 65504, as a first product rounded
+// to fp16 would, and an infinity in B, or in a gradient's x or dY, may come out as NaN
+// (infinity times a lo part of zero); what is not finite never comes out finite.
 #pragma once
 
 #include "rq_io.h"
@@ -54,7 +56,7 @@ struct ExpandArgs {
 
 struct OperandsArgs {
   RowsPlan rows;
-  int rp;
+  int r, rp;
   const float* part;    // [splits][slots][rp]
   int splits;
   void* opt;            // slots * rp values of 32 bits

@@ -196,6 +196,16 @@ def test_not_a_number_stays_in_its_rows(dev):
     assert not bool(da[1].isnan().any(0).all())  # adapter 1's rows hold no NaN; its infinity shows in one column of dA
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_infinity_of_a_row_stays_one(dev, dtype):
+    # one sign throughout, so that the formula's results are infinities, whatever the padded ranks
+    for M, r in ((1, 1), (20, 3), (70, 1)):
+        d = make(M, 40, 36, r, 1, dtype, dev, ids=[0] * M)
+        d["a"], d["b"], d["x"][0, 7] = d["a"].abs() + 0.01, d["b"].abs() + 0.01, float("inf")
+        y = multi_lora(d["x"], d["a"], d["b"], d["s"], AdapterRows(d["ids"], 1), d["base"])
+        assert bool((y[0] == float("inf")).all()) and bool(torch.isfinite(y[1:]).all())
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_strides_and_alignment(dev, dtype):
     M, K, N, r, n = 37, 72, 90, 6, 2
