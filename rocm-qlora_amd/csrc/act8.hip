@@ -2,7 +2,9 @@
 //
 // Bound by memory: a value is read once and 33/32 of a byte written (and back).
 // A thread takes 16 values, two threads a block, so that codes leave as whole
-// 16-byte stores and the block's maximum is one lane swap.
+// 16-byte stores and the block's maximum is one lane swap.  4096 x 14336 bf16 (178 MB a way):
+// 29 us to codes and 28 back, 6.1 and 6.4 TB/s (a copy reaches 5.2; part of the codes stays in
+// the cache between the two); 333 x 1001 3 us each, a launch.
 #include "rq_act8.h"
 #include "rq_io.h"
 #include "rq_launch.h"

@@ -6,7 +6,9 @@
 // lanes ask for one piece of 64, but a sixteenth lane's row at a time when every lane asks
 // for a row of its own, as operand registers hold a matrix.  So rows are loaded straight
 // into operand registers where they pass once, and the factors, which serve many rows, go
-// through LDS or are read along their rows.
+// through LDS or are read along their rows.  (Rows and factors read as operand registers hold
+// them: 296 us for a training step of 4096 rows, K 4096, N 14336, r 64 on four adapters; in
+// whole pieces 212; 167 now, of 411 MB that it cannot do without.)
 #include "rq_multi_lora.h"
 
 #include "rq_act8.h"
@@ -41,13 +43,21 @@ inline unsigned xcd_grid(int64_t n) { return unsigned(ceil_div(n, kXcds) * kXcds
 // A workgroup takes a tile's rows over a split of K.  Tiles of one or two 16-row blocks: the
 // four waves divide the split and meet in LDS, 16 rows at a time, summed in the waves' order;
 // a wave holds the blocks times JB blocks of 16 ranks, so that a factor's piece is loaded once
-// for the tile.  Tiles of more: a wave takes a block, and the factor is shared through LDS.
+// for the tile.  Tiles of more: a wave takes a block, and the factor is shared through LDS
+// (four blocks in a wave's registers left it two steps in flight: 44 us for the 27 below).
 //
 // Rows and factor go through a wave's own piece of LDS.  Rows and A [r][K]: a step's 64
 // bytes of each, loaded by four adjacent lanes, the four pieces exchanged by the row so that
-// the lanes of a read meet other banks.  B [N][r] (TURNED), whose rows run across the contraction: a step's rows are one
-// piece of memory, copied as it lies (with 32 bytes between eight-row groups, so that the
-// four lane groups read other banks) and read back a rank's values at a time.
+// the lanes of a read meet other banks.  B [N][r] (TURNED), whose rows run across the
+// contraction: a step's rows are one piece of memory, copied as it lies (with 32 bytes between
+// eight-row groups, so that the four lane groups read other banks) and read back a rank's
+// values at a time.
+//
+// Bound by a workgroup's chain of loads (tile, rows, values, the exchange in LDS) and then by
+// HBM: dY B of 3342 rows, N 14336, r 64 27 us (96 MB, 3.5 TB/s; a copy reaches 5.2), x A^T of
+// 2610 rows, K 11008, r 12 15 us (57 MB, 3.9 TB/s), of 3342 rows, K 4096, r 64 14 us; 224 rows
+// on 64 adapters, K 4096, r 32 8 us (19 MB), 8 rows 4.4.  Two pieces in flight instead of one
+// in shrink_blocks changed none of it.
 constexpr int kShWaves = 4;
 constexpr int kShThreads = 64 * kShWaves;
 
@@ -350,7 +360,8 @@ __global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(3)))
 }
 
 // About two workgroups a compute unit, each with four steps a wave (many tiles: eight, since
-// every later workgroup of a tile sums the splits).
+// every later workgroup of a tile sums the splits; a training step of 4096 rows, K 4096,
+// N 14336, r 64 160 - 165 us, with sixteen 167, with twenty-eight 188).
 void plan_shrink(int64_t T, int64_t K, int step, int cus, int* splits, int64_t* per) {
   const int64_t unit = int64_t(step) * kShWaves;
   int64_t s = ceil_div(2 * cus, std::max<int64_t>(T, 1));
@@ -506,6 +517,12 @@ int run_operands(const OperandsArgs& a, hipStream_t stream) {
 // waves' columns at a time, copied as they lie (up to a step of ranks; of more, a step's ranks
 // of each row) with 16 bytes between groups of kVec rows, so that the lanes of a read meet
 // other banks.  A's rows [r][K] are read along the row and transposed in registers.
+//
+// Bound by HBM with a base: 4096 rows, N 14336, r 64 56 us (base and result 235 MB, 4.2 TB/s),
+// 3001 rows, N 4096, r 12 15.6 us (3.2 TB/s).  Without one (dX of 4096 rows, K 4096: 22 us,
+// 34 MB written) by a workgroup's chain: rows, splits, factor pieces, each waiting for the
+// last; there are two workgroups a compute unit, and more of them sum the splits more often.
+// Four slots' splits in flight instead of two: no faster.
 template <int XT>
 struct ExpandLds {
   static constexpr int kCols = 16 * Elem<XT>::kVec;   // of a wave
@@ -730,7 +747,8 @@ int run_expand(ExpandArgs a, int cus, hipStream_t stream) {
   typedef ExpandLds<XT> L;
   constexpr int V = Elem<XT>::kVec, es = int(sizeof(typename Elem<XT>::T));
   const int64_t steps = ceil_div(a.C, int64_t(kMlWaves) * L::kCols);
-  // steps of a workgroup: as many as leave eight workgroups a compute unit
+  // steps of a workgroup: as many as leave eight workgroups a compute unit (both products of
+  // 4096 rows, N 14336: 63 - 68 us with four or eight, 71 with two)
   a.iters = int(std::max<int64_t>(1, std::min<int64_t>(8, a.rows.T * steps / (8 * cus))));
   a.chunks = int(ceil_div(steps, a.iters));
   if (int64_t(a.rows.T) * a.chunks > kMaxThreads1D / kMlThreads) return RQ_ERR_UNSUPPORTED;
@@ -765,6 +783,12 @@ int run_expand(ExpandArgs a, int cus, hipStream_t stream) {
 // turn into CW operand rows of eight consecutive slots (16-bit; fp32 values are operands
 // as they are).  A workgroup takes 16 CW columns over the rows of a chunk, 32 slots a
 // step; its four waves take steps in turn and meet in LDS, summed as (0 + 2) + (1 + 3).
+// Where a wave holds 64 ranks CW is 4: with 8 the accumulators leave two waves a SIMD (a
+// backward pass of 4096 rows, r 64: 97 -> 109 us), and two steps in flight do not fit the
+// registers.  dA and dB of 3342 rows, K 4096, N 14336, r 64: 41 us (123 MB of rows, 3.0 TB/s),
+// bound by what passes through the L1 (its return path is busy 84 % of the time, its address
+// unit 67): at 64 columns by 64 ranks a wave's operands are twice its rows' bytes.  From an
+// 8-bit checkpoint of 2048 rows, K = N = 4096, r 16: 11 us.
 template <int XT, int CW>
 struct ColPiece {
   static constexpr int kWords = XT == RQ_DTYPE_F32 ? CW : CW / 2;
@@ -1051,7 +1075,8 @@ __global__ __launch_bounds__(kMlThreads) void rowsum_finish_kernel(RowSumArgs a)
 }
 
 // The table of chunks: the coarser one where its sums cannot meet in a second launch, or
-// where its workgroups fill the GPU.
+// where its workgroups fill the GPU (4096 rows, K + N 18432, r 64: backward 97 us coarse,
+// 123 fine, whose partial sums are four times as many).
 int rowsum_table(const RowsPlan& rows, int64_t cols, int wg_cols, int cus) {
   const int64_t tiles = ceil_div(cols, wg_cols);
   return rows.T <= chunk_least(1) || tiles * ceil_div(ceil_div(rows.M, kTileRows), chunk_least(1)) >= cus ? 1 : 0;

@@ -105,7 +105,8 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
     x: [..., K] fp32, bf16 or fp16; lora_a [n, r, K] and lora_b [n, N, r] (rounded to
     x's dtype when they have another); scaling: fp32 [n], or one number; base: [...,
     N] in x's dtype (None: zeros).  Sums are fp32; x A^T is passed to the second
-    product in 16 bits or more and the result rounded once.  Differentiable by x,
+    product in 16 bits or more and the result rounded once (fp16: x A^T up to 65504; an
+    infinity in lora_b, or in a gradient's x, may come out as NaN).  Differentiable by x,
     lora_a, lora_b and base; activation_bits=8 holds x for dA as an 8-bit checkpoint
     (rocm_qlora.checkpoint), which the gradient kernel reads as it is."""
     _check(x, lora_a, rows, activation_bits)
