@@ -30,13 +30,17 @@ def to_gpu(t: torch.Tensor) -> Tuple[torch.Tensor, torch.device]:
     return (t if t.device == dev else t.to(dev)), t.device
 
 
+# the current device without torch.cuda's check that it is initialised
+_current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 class on:
     """`with on(device)`: that GPU current inside the block (nothing is changed
     when it already is, which costs one query)."""
     __slots__ = ("_guard",)
 
     def __init__(self, device: torch.device):
-        same = device.index is not None and device.index == torch.cuda.current_device()
+        same = device.index is not None and device.index == _current()
         self._guard = None if same else torch.cuda.device(device)
 
     def __enter__(self):

@@ -141,6 +141,7 @@ _RESTYPE = {"rq_status_string": ctypes.c_char_p, "rq_build_arch": ctypes.c_char_
             "rq_set_gemv_wait_us": ctypes.c_uint32}
 
 _lib: Optional[ctypes.CDLL] = None
+_fns: dict = {}  # the library's functions by name
 _lock = threading.Lock()
 
 
@@ -164,6 +165,7 @@ def load() -> ctypes.CDLL:
                 fn = getattr(lib, name)
                 fn.argtypes = argtypes
                 fn.restype = _RESTYPE.get(name, ctypes.c_int)
+                _fns[name] = fn
             _lib = lib
     return _lib
 
@@ -182,7 +184,10 @@ def status_string(status: int) -> str:
 
 def call(name: str, *args) -> None:
     """Call an rq_* entry point and raise RuntimeError on a non-zero status."""
-    status = getattr(load(), name)(*args)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = getattr(load(), name)
+    status = fn(*args)
     if status != 0:
         raise RuntimeError(f"{name} failed: {status_string(status)} (status {status})")
 
@@ -232,18 +237,18 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def require_gpu(*tensors: Optional[torch.Tensor]) -> torch.device:
     """All tensors must live on one GPU; returns that device."""
-    dev = None
+    dev = index = None
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
             raise RuntimeError(
                 f"rocm_qlora_amd kernels run on the GPU; got a tensor on {t.device}")
-        d = t.device
         if dev is None:
-            dev = d
-        elif d != dev:
-            raise RuntimeError(f"tensors on different devices: {dev} and {d}")
+            dev = t.device
+            index = dev.index
+        elif t.get_device() != index:
+            raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
     if dev is None:
         raise RuntimeError("no tensor given")
     return dev

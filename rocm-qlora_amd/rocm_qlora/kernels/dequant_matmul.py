@@ -285,8 +285,10 @@ def _nothing_recorded(*inputs) -> bool:
     forward can run without its autograd function: no gradient asked for, and
     neither tracing, a functorch transform nor forward-mode AD active (those go
     through the function, which accepts or refuses them)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
-        return False
+    if torch.is_grad_enabled():
+        for t in inputs:
+            if t is not None and t.requires_grad:
+                return False
     return _plain_eager()
 
 

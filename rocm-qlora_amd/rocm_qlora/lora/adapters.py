@@ -14,14 +14,13 @@ from typing import Optional, Union
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from rocm_qlora import ops
 from rocm_qlora._device import on
 from rocm_qlora.kernels import dequant_matmul as dm
 from rocm_qlora.lora.lora_layer import LoRALinear
 from rocm_qlora.quantization.quant_linear import QuantLinear
-from rocm_qlora.torch_ops import eager_only
+from rocm_qlora.torch_ops import eager_only, first_order
 
 
 class AdapterRows:
@@ -80,7 +79,7 @@ class _MultiLoRA(torch.autograd.Function):
         return y if flat else y.view(*x.shape[:-1], y.shape[-1])
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, dy):
         x, exps, a, b, scaling, u = ctx.saved_tensors
         plan, linear, shape, a_dtype, b_dtype = ctx.args
@@ -110,7 +109,9 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
     lora_a, lora_b and base; activation_bits=8 holds x for dA as an 8-bit checkpoint
     (rocm_qlora.checkpoint), which the gradient kernel reads as it is."""
     _check(x, lora_a, rows, activation_bits)
-    if base is not None and (base.dtype != x.dtype or base.shape[:-1] != x.shape[:-1] or base.shape[-1] != lora_b.shape[1]):
+    # (2-D rows' base is checked with the other operands)
+    if base is not None and x.dim() != 2 and (base.dtype != x.dtype or base.shape[:-1] != x.shape[:-1] or
+                                              base.shape[-1] != lora_b.shape[1]):
         raise RuntimeError(f"base {tuple(base.shape)} {base.dtype} does not fit x {tuple(x.shape)} {x.dtype} and "
                            f"{lora_b.shape[1]} columns")
     if not isinstance(scaling, torch.Tensor):

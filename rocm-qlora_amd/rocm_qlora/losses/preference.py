@@ -12,11 +12,10 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from rocm_qlora import ops
 from rocm_qlora.kernels.dequant_matmul import _nothing_recorded
-from rocm_qlora.torch_ops import eager_only
+from rocm_qlora.torch_ops import eager_only, first_order
 
 
 class _PreferenceLoss(torch.autograd.Function):
@@ -30,7 +29,7 @@ class _PreferenceLoss(torch.autograd.Function):
         return loss, logps
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, dloss, _):
         logits, state = ctx.saved_tensors
         return (ops.preference_backward(logits, state, dloss),) + (None,) * 7
@@ -45,7 +44,7 @@ class _SequenceLogps(torch.autograd.Function):
         return logps
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, dlogps):
         logits, state = ctx.saved_tensors
         return (ops.preference_backward(logits, state, dlogps),) + (None,) * 4

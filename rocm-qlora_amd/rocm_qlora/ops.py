@@ -739,13 +739,13 @@ def adapter_rows(ids: torch.Tensor, n: int) -> torch.Tensor:
         raise TypeError(f"adapter ids must be int32 or int64, got {ids.dtype}")
     if not 1 <= n <= MAX_ADAPTERS:
         raise RuntimeError(f"{n} adapters: 1 to {MAX_ADAPTERS} are taken at once")
-    ids = ids.reshape(-1)
-    if ids.dtype == torch.int64:
-        ids = ids.clamp(-1, n)  # whatever int32 cannot hold has no adapter either
-    ids = ids.to(torch.int32).contiguous()
+    M = ids.numel()
     with on(dev):
-        plan = _scratch("rq_adapter_rows_size", dev, ids.numel(), n)
-        nat.call("rq_adapter_rows", ids.data_ptr(), ids.numel(), n, plan.data_ptr(), plan.numel(), nat.stream_handle(dev))
+        if ids.dtype == torch.int64:
+            ids = ids.clamp(-1, n).to(torch.int32)  # whatever int32 cannot hold has no adapter either
+        ids = ids.contiguous()
+        plan = _scratch("rq_adapter_rows_size", dev, M, n)
+        nat.call("rq_adapter_rows", ids.data_ptr(), M, n, plan.data_ptr(), plan.numel(), nat.stream_handle(dev))
     return plan
 
 
@@ -764,14 +764,16 @@ def _adapter_operands(dtype, K: int, lora_a, lora_b, scaling) -> Tuple[int, int,
     return n, rank, N, lora_a.contiguous(), lora_b.contiguous()
 
 
-def _check_rows(t: torch.Tensor, M: int, cols: int, dtype: torch.dtype, name: str) -> None:
-    if t.dtype != dtype or t.shape != (M, cols) or (t.stride(1) != 1 and cols > 1) or (M > 1 and t.stride(0) < cols):
-        raise RuntimeError(f"{name} must be [{M}, {cols}] {dtype} with adjacent columns, got {tuple(t.shape)} {t.dtype} "
-                           f"of strides {t.stride()}")
-
-
-def _ld(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+def _check_rows(t: torch.Tensor, M: int, cols: int, dtype: torch.dtype, name: str) -> int:
+    """The row stride of t, which has to be [M, cols] of dtype with adjacent columns."""
+    if t.dtype == dtype and t.shape == (M, cols):
+        ld, inner = t.stride()
+        if M <= 1:
+            ld = cols
+        if ld >= cols and (inner == 1 or cols == 1):
+            return ld
+    raise RuntimeError(f"{name} must be [{M}, {cols}] {dtype} with adjacent columns, got {tuple(t.shape)} {t.dtype} "
+                       f"of strides {t.stride()}")
 
 
 def _check_plan(plan: Optional[torch.Tensor], dev, M: int, n: int) -> None:
@@ -791,17 +793,16 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
     Returns out and, with need_u, what multi_lora_grads takes as u."""
     dev = nat.require_gpu(x, lora_a, lora_b, scaling, plan, base, out)
     M, K = x.shape
-    code = nat.dtype_code(x.dtype)
-    n, rank, N, a, b = _adapter_operands(x.dtype, K, lora_a, lora_b, scaling)
-    if base is not None:
-        _check_rows(base, M, N, x.dtype, "base")
-    if out is not None and out is not base:
-        _check_rows(out, M, N, x.dtype, "out")
+    dtype = x.dtype
+    code = nat.dtype_code(dtype)
+    n, rank, N, a, b = _adapter_operands(dtype, K, lora_a, lora_b, scaling)
+    ld_base = _check_rows(base, M, N, dtype, "base") if base is not None else 0
+    ld_out = N if out is None else ld_base if out is base else _check_rows(out, M, N, dtype, "out")
     with on(dev):
         _check_plan(plan, dev, M, n)
         grouped = 0 if plan is None else 1
         if out is None:
-            out = torch.empty((M, N), dtype=x.dtype, device=dev)
+            out = x.new_empty((M, N))
         u = None
         if need_u:
             u = torch.empty(_bytes("rq_multi_lora_u_size", dev.index, M, n, rank, grouped), dtype=torch.uint8, device=dev)
@@ -810,7 +811,7 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
             scratch = _scratch("rq_multi_lora_scratch_size", dev, code, M, K, N, n, rank, grouped, 0)
             nat.call("rq_multi_lora", x.data_ptr(), code, M, K, ldx, nat.ptr(plan), plan.numel() if grouped else 0,
                      a.data_ptr(), b.data_ptr(), scaling.data_ptr(), n, rank, N,
-                     nat.ptr(base), _ld(base) if base is not None else 0, out.data_ptr(), _ld(out), nat.ptr(u),
+                     nat.ptr(base), ld_base, out.data_ptr(), ld_out, nat.ptr(u),
                      scratch.data_ptr(), scratch.numel(), nat.stream_handle(dev))
     return (out, u) if need_u else out
 
@@ -855,11 +856,11 @@ def _multi_lora_grads(x, dy, a, b, scaling, plan, u, need_x, need_a, need_b, dx,
     """multi_lora_grads of operands that are known to fit, on the current device."""
     M, N = dy.shape
     n, rank, K = a.shape
-    base = dx
+    base, lddx = dx, K if dx is None or M <= 1 else dx.stride(0)
     da = torch.empty_like(a) if need_a else None
     db = torch.empty_like(b) if need_b else None
     if need_x and dx is None:
-        dx = torch.empty((M, K), dtype=dy.dtype, device=dev)
+        dx = dy.new_empty((M, K))
     if M == 0:
         for t in (da, db):
             if t is not None:
@@ -880,8 +881,7 @@ def _multi_lora_grads(x, dy, a, b, scaling, plan, u, need_x, need_a, need_b, dx,
     scratch = _scratch("rq_multi_lora_scratch_size", dev, code, M, K, N, n, rank, grouped, 1)
     nat.call("rq_multi_lora_grads", xp, nat.ptr(exps), code, M, K, ldx, dy.data_ptr(), N, lddy,
              nat.ptr(plan), plan.numel() if grouped else 0, a.data_ptr(), b.data_ptr(), scaling.data_ptr(), n, rank,
-             nat.ptr(u) if need_b else None, nat.ptr(base), _ld(base) if base is not None else 0,
-             nat.ptr(dx), _ld(dx) if dx is not None else 0, nat.ptr(da), nat.ptr(db),
+             nat.ptr(u) if need_b else None, nat.ptr(base), lddx, nat.ptr(dx), lddx, nat.ptr(da), nat.ptr(db),
              scratch.data_ptr(), scratch.numel(), nat.stream_handle(dev))
     return dx, da, db
 
@@ -927,9 +927,10 @@ def _logit_rows(logits: torch.Tensor) -> Tuple[torch.Tensor, int, int, int, int]
     if logits.stride(-1) != 1 and V > 1:
         logits = logits.contiguous()
     if logits.dim() == 2:
-        if logits.shape[0] > 1 and logits.stride(0) < V:
-            logits = logits.contiguous()
-        return logits, logits.shape[0], logits.stride(0) if logits.shape[0] > 1 else V, 0, 0
+        T, ld = logits.shape[0], logits.stride(0)
+        if T <= 1:
+            return logits, T, V, 0, 0
+        return (logits, T, ld, 0, 0) if ld >= V else (logits.contiguous(), T, V, 0, 0)
     B, L = logits.shape[:2]
     if (L > 1 and logits.stride(1) < V) or (B > 1 and logits.stride(0) < V):
         logits = logits.contiguous()

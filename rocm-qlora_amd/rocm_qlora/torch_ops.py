@@ -24,6 +24,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from rocm_qlora import ops
 
@@ -123,6 +124,18 @@ def compiling() -> bool:
         return torch.compiler.is_compiling()
     except AttributeError:  # older torch
         return False
+
+
+def first_order(backward):
+    """once_differentiable for a backward pass of kernels; where autograd records nothing
+    (no create_graph) there is nothing to guard, and the pass runs as it is."""
+    guarded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call
 
 
 def eager_only(fn):
