@@ -81,7 +81,19 @@ def saved_in_8_bits(min_elements: int = 1 << 16):
     return _saved(lambda t: _floats(t, min_elements) and _activation(t))
 
 
-def inputs_saved_in_8_bits():
-    """The same for one layer's own autograd function, all of whose saved float tensors
-    but its parameters are inputs, whether or not they require a gradient."""
-    return _saved(lambda t: _floats(t, 1))
+def inputs_saved_in_8_bits(x: torch.Tensor):
+    """The same for one layer's input x (and what dropout makes of it), whether or not it
+    requires a gradient: inside the layer's own autograd function saved tensors have no
+    record; where torch's products compose the layer, x shares its memory and dropout its
+    name, and the factors and the first product stay as they are."""
+    shape, place = (x.numel(), x.shape[-1:]), x.untyped_storage().data_ptr()
+
+    def holds(t: torch.Tensor) -> bool:
+        if not _floats(t, 1) or (t.numel(), t.shape[-1:]) != shape:
+            return False
+        node = t.grad_fn
+        while node is not None and node.name() in _VIEWS:
+            node = node.next_functions[0][0]
+        return node is None or node.name() == "NativeDropoutBackward0" or t.untyped_storage().data_ptr() == place
+
+    return _saved(holds)

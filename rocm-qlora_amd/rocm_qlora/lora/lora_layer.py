@@ -21,6 +21,7 @@ import torch.nn as nn
 
 from rocm_qlora.checkpoint.act8 import inputs_saved_in_8_bits
 from rocm_qlora.quantization.quant_linear import QuantLinear
+from rocm_qlora.torch_ops import eager_only
 
 
 class LoRALinear(nn.Module):
@@ -60,8 +61,7 @@ class LoRALinear(nn.Module):
         if isinstance(base, QuantLinear) and not base.merged_mode:
             p = self.lora_dropout.p if self._dropout_active() else 0.0
             if self.activation_bits == 8 and torch.is_grad_enabled():
-                with inputs_saved_in_8_bits():
-                    return base.fused_forward(x, self.lora_A, self.lora_B, self.scaling, p)
+                return self._forward_saved_in_8_bits(x, p)
             return base.fused_forward(x, self.lora_A, self.lora_B, self.scaling, p)
         if hasattr(base, "weight"):
             base_out = base(x.to(base.weight.dtype))
@@ -69,6 +69,11 @@ class LoRALinear(nn.Module):
             base_out = base(x)
         lora_out = self.lora_dropout(x) @ self.lora_A.to(x.dtype).T @ self.lora_B.to(x.dtype).T * self.scaling
         return base_out + lora_out.to(base_out.dtype)
+
+    @eager_only
+    def _forward_saved_in_8_bits(self, x: torch.Tensor, p: float) -> torch.Tensor:
+        with inputs_saved_in_8_bits(x):
+            return self.base_layer.fused_forward(x, self.lora_A, self.lora_B, self.scaling, p)
 
     @torch.no_grad()
     def merge_lora(self) -> None:

@@ -164,6 +164,43 @@ def test_lora_layer_with_8_bit_activations(dev, bits, grad_x, p):
     assert near < 2.0 ** -5  # the held values are within 2^-6 of the block's largest
 
 
+@pytest.mark.parametrize("M,r", [(200, 8), (8, 8), (96, 96)])
+def test_lora_layer_composed_adapter_with_8_bit_activations(dev, M, r):
+    """Where the adapter is composed of torch's products (INT8 with fp32 rows, ranks past
+    64) the factors and the first product stay as they are: y, dX and dB do not change,
+    and dA is the one at the held input."""
+    K, N = 96, 64
+    g = torch.Generator().manual_seed(8)
+    layer = LoRALinear(QuantLinear.from_linear(torch.nn.Linear(K, N).to(dev), bits=8), r=r)
+    with torch.no_grad():
+        layer.lora_B.copy_(torch.randn(N, r, generator=g) * 0.1)
+    x, dy = torch.randn(M, K, generator=g).to(dev), torch.randn(M, N, generator=g).to(dev)
+
+    def run(x, act_bits):
+        layer.activation_bits = act_bits
+        x = x.clone().requires_grad_(True)
+        y = layer(x)
+        return (y, *torch.autograd.grad(y, (x, layer.lora_B, layer.lora_A), dy))
+
+    full, held, at = run(x, 16), run(x, 8), run(decompress(compress(x)), 16)
+    for a, b in zip(full[:-1], held[:-1]):
+        assert torch.equal(a, b)
+    assert torch.equal(held[-1], at[-1]) and not torch.equal(held[-1], full[-1])
+
+
+def test_compiled_layer_runs_its_8_bit_activations_eagerly(dev):
+    layer = LoRALinear(QuantLinear.from_linear(torch.nn.Linear(128, 64).to(dev), bits=4), r=8)
+    layer.activation_bits = 8
+    with torch.no_grad():
+        layer.lora_B.normal_()
+    x, dy = torch.randn(40, 128, device=dev).to(BF16), torch.randn(40, 64, device=dev).to(BF16)
+    torch._dynamo.reset()
+    f = torch.compile(lambda x: layer(x * 1.0) * 1.0, backend="eager")
+    want = torch.autograd.grad(layer(x), (layer.lora_A, layer.lora_B), dy)
+    got = torch.autograd.grad(f(x), (layer.lora_A, layer.lora_B), dy)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_refusals(dev):
     with pytest.raises(RuntimeError, match="GPU"):
         compress(torch.zeros(4, 32))
