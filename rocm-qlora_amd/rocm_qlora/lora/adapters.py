@@ -135,6 +135,8 @@ class MultiLoRALinear(nn.Module):
     model by set_adapter_rows."""
 
     def __init__(self, quant_linear: QuantLinear, n: int, r: int = 8, lora_alpha: float = 16, activation_bits: int = 16):
+        if not isinstance(quant_linear, QuantLinear):
+            raise TypeError(f"adapters go beside a QuantLinear, got {type(quant_linear).__name__}")
         super().__init__()
         self.base_layer = quant_linear
         self.n, self.r = n, r
@@ -203,12 +205,15 @@ def attach_adapters(model: nn.Module, n: int, activation_bits: int = 16) -> nn.M
     """Replace every LoRALinear (quantize_model's) by a MultiLoRALinear of n adapters of
     its rank over the same quantized weight; adapter 0 is the layer's own (without its
     dropout)."""
-    for name, m in list(model.named_modules()):
-        if isinstance(m, LoRALinear):
-            if m.merged:
-                raise RuntimeError(f"{name} is merged: unmerge it first")
-            new = MultiLoRALinear(m.base_layer, n, m.r, m.lora_alpha, activation_bits)
-            new.load_adapter(0, m)
-            parent = model.get_submodule(name.rpartition(".")[0])
-            setattr(parent, name.rpartition(".")[2], new)
+    layers = [(name, m) for name, m in model.named_modules() if isinstance(m, LoRALinear)]
+    for name, m in layers:
+        if m.merged:
+            raise RuntimeError(f"{name} is merged: unmerge it first")
+        if not isinstance(m.base_layer, QuantLinear):
+            raise TypeError(f"{name}: adapters go beside a QuantLinear, got {type(m.base_layer).__name__}")
+    for name, m in layers:
+        new = MultiLoRALinear(m.base_layer, n, m.r, m.lora_alpha, activation_bits).train(m.training)
+        new.load_adapter(0, m)
+        parent = model.get_submodule(name.rpartition(".")[0])
+        setattr(parent, name.rpartition(".")[2], new)
     return model

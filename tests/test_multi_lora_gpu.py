@@ -351,6 +351,22 @@ def test_layer_matches_its_parts(dev, bits, M):
     assert torch.equal(layer.lora_A.grad, da.float()) and torch.equal(layer.lora_B.grad, db.float())
 
 
+def test_attach_adapters_leaves_a_model_that_it_refuses(dev):
+    def layer():
+        return LoRALinear(QuantLinear.from_linear(torch.nn.Linear(64, 64).to(dev), bits=4), r=4)
+
+    merged = torch.nn.Sequential(layer(), layer())
+    merged[1].merge_lora()
+    with pytest.raises(RuntimeError, match="merged"):
+        attach_adapters(merged, 2)
+    other = torch.nn.Sequential(layer(), layer())
+    other[1].base_layer = torch.nn.Linear(64, 64).to(dev)
+    with pytest.raises(TypeError, match="QuantLinear"):
+        attach_adapters(other, 2)
+    assert all(isinstance(m, LoRALinear) for m in (*merged, *other))
+    assert not attach_adapters(torch.nn.Sequential(layer()).eval(), 2)[0].training
+
+
 def test_attach_adapters(dev):
     """A model of LoRALinears becomes one of many adapters: rows of adapter 0 give what the
     single-adapter layer gives (to the roundings of its intermediate, U of the term's
