@@ -171,7 +171,8 @@ class MultiLoRALinear(nn.Module):
             return (lambda x: ops.nf4_linear(x, w.packed, w.scales, w.N, w.block_size, base.bias, **w.dq_kwargs()),
                     lambda dy: ops.nf4_linear_dx(dy, w.packed, w.scales, w.K, w.block_size, **w.dq_kwargs()))
         w = base.int8_weight()
-        return (lambda x: ops.int8_linear(x, w.q, w.scales, w.N, w.block_size, base.bias), lambda dy: ops.int8_linear_dx(dy, w.q, w.scales, w.K, w.block_size))
+        return (lambda x: ops.int8_linear(x, w.q, w.scales, w.N, w.block_size, base.bias),
+                lambda dy: ops.int8_linear_dx(dy, w.q, w.scales, w.K, w.block_size))
 
     @eager_only
     def forward(self, x: torch.Tensor, rows: Optional[AdapterRows] = None) -> torch.Tensor:
@@ -180,11 +181,12 @@ class MultiLoRALinear(nn.Module):
             raise RuntimeError("no adapter rows: pass them, or set them with set_adapter_rows(model, rows)")
         _check(x, self.lora_A, rows, self.activation_bits)
         linear = self._linear()
+        scaling = self.scaling if self.scaling.dtype == torch.float32 else self.scaling.float()  # cast with the model
         if not dm._nothing_recorded(x, self.lora_A, self.lora_B):
-            return _MultiLoRA.apply(x, self.lora_A, self.lora_B, None, self.scaling, rows, self.activation_bits, linear)
+            return _MultiLoRA.apply(x, self.lora_A, self.lora_B, None, scaling, rows, self.activation_bits, linear)
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         y = linear[0](x2)
-        ops.multi_lora(x2, self.lora_A.to(x.dtype), self.lora_B.to(x.dtype), self.scaling, rows.plan, y, y)
+        ops.multi_lora(x2, self.lora_A.to(x.dtype), self.lora_B.to(x.dtype), scaling, rows.plan, y, y)
         return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[-1])
 
     def extra_repr(self) -> str:
@@ -204,16 +206,20 @@ def set_adapter_rows(model: nn.Module, rows: Optional[AdapterRows]) -> int:
 def attach_adapters(model: nn.Module, n: int, activation_bits: int = 16) -> nn.Module:
     """Replace every LoRALinear (quantize_model's) by a MultiLoRALinear of n adapters of
     its rank over the same quantized weight; adapter 0 is the layer's own (without its
-    dropout)."""
-    layers = [(name, m) for name, m in model.named_modules() if isinstance(m, LoRALinear)]
+    dropout).  Returns the model, or what replaces it when it is a LoRALinear itself."""
+    layers = [(name, m) for name, m in model.named_modules(remove_duplicate=False) if isinstance(m, LoRALinear)]
     for name, m in layers:
         if m.merged:
             raise RuntimeError(f"{name} is merged: unmerge it first")
         if not isinstance(m.base_layer, QuantLinear):
             raise TypeError(f"{name}: adapters go beside a QuantLinear, got {type(m.base_layer).__name__}")
+    made = {}  # a layer in several places stays one
     for name, m in layers:
-        new = MultiLoRALinear(m.base_layer, n, m.r, m.lora_alpha, activation_bits).train(m.training)
-        new.load_adapter(0, m)
-        parent = model.get_submodule(name.rpartition(".")[0])
-        setattr(parent, name.rpartition(".")[2], new)
+        if m not in made:
+            made[m] = MultiLoRALinear(m.base_layer, n, m.r, m.lora_alpha, activation_bits).train(m.training)
+            made[m].load_adapter(0, m)
+        if m is model:
+            return made[m]
+        parent, _, child = name.rpartition(".")
+        setattr(model.get_submodule(parent), child, made[m])
     return model

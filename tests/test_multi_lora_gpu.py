@@ -367,6 +367,29 @@ def test_attach_adapters_leaves_a_model_that_it_refuses(dev):
     assert not attach_adapters(torch.nn.Sequential(layer()).eval(), 2)[0].training
 
 
+def test_attached_layers_cast_shared_and_without_rows(dev):
+    torch.manual_seed(3)
+    layer = LoRALinear(QuantLinear.from_linear(torch.nn.Linear(64, 96).to(dev), bits=4), r=4, lora_alpha=8)
+    with torch.no_grad():
+        layer.lora_B.normal_()
+    x = torch.randn(6, 64, device=dev).to(BF16)
+    want = layer(x)
+    model = torch.nn.ModuleDict({"a": layer, "b": layer})  # one layer in two places
+    attach_adapters(model, 2)
+    assert isinstance(model["a"], MultiLoRALinear) and model["b"] is model["a"]
+    alone = attach_adapters(layer, 2)  # the model is the layer
+    assert isinstance(alone, MultiLoRALinear)
+    alone.scaling.data = alone.scaling.data.to(BF16)  # as model.to(torch.bfloat16) leaves it
+    rows = AdapterRows(torch.zeros(6, dtype=torch.int32, device=dev), 2)
+    for m in (model["b"], alone):
+        got = m(x, rows)
+        assert ((got - want).abs() <= 2.0 ** -6 * want.abs() + 2.0 ** -6 * want.abs().max()).all()
+    none = AdapterRows(torch.zeros(0, dtype=torch.int32, device=dev), 2)
+    y = alone(x[:0].requires_grad_(True), none)
+    y.sum().backward()
+    assert y.shape == (0, 96) and not alone.lora_A.grad.any() and not alone.lora_B.grad.any()
+
+
 def test_attach_adapters(dev):
     """A model of LoRALinears becomes one of many adapters: rows of adapter 0 give what the
     single-adapter layer gives (to the roundings of its intermediate, U of the term's
