@@ -233,6 +233,21 @@ def test_strides_and_alignment(dev, dtype):
     assert torch.equal(multi_lora(x3, d["a"], d["b"], d["s"], r3, b3), want[:36].view(4, 9, N))
 
 
+def test_more_than_2_to_the_31_values(dev):
+    """Results and dY of more elements than 32 bits count: the first and the last rows' results,
+    and the gradients of a dY that is zero before the last rows."""
+    M, K, N, r, n, last = 33000, 40, 65568, 8, 2, 50
+    d = make(last + 20, K, N, r, n, BF16, dev, seed=9)
+    held = torch.cat([torch.arange(20, device=dev), torch.arange(M - last, M, device=dev)])
+    big = dict(d, x=torch.randn(M, K, device=dev).to(BF16), ids=torch.randint(-1, n, (M,), dtype=torch.int32, device=dev),
+               base=torch.zeros(M, N, dtype=BF16, device=dev), dy=torch.zeros(M, N, dtype=BF16, device=dev))
+    d["dy"][:20] = 0
+    for k in ("x", "ids", "base", "dy"):
+        big[k][held] = d[k]
+    y, dx, da, db = run_all(big, AdapterRows(big["ids"], n))
+    check_all(d, (y[held], dx[held], da, db))
+
+
 def test_empty_batch(dev):
     d = make(0, 32, 16, 4, 2, BF16, dev)
     y, dx, da, db = run_all(d, AdapterRows(d["ids"], 2))
