@@ -796,8 +796,15 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
     dtype = x.dtype
     code = nat.dtype_code(dtype)
     n, rank, N, a, b = _adapter_operands(dtype, K, lora_a, lora_b, scaling)
-    ld_base = _check_rows(base, M, N, dtype, "base") if base is not None else 0
-    ld_out = N if out is None else ld_base if out is base else _check_rows(out, M, N, dtype, "out")
+    ld_out = N if out is None else _check_rows(out, M, N, dtype, "out")
+    ld_base = 0
+    if base is not None:
+        if base is out:
+            ld_base = ld_out
+        elif base.dtype != dtype or base.shape != (M, N):
+            raise RuntimeError(f"base must be [{M}, {N}] {dtype}, got {tuple(base.shape)} {base.dtype}")
+        else:
+            base, ld_base = _rows(base, N)
     with on(dev):
         _check_plan(plan, dev, M, n)
         grouped = 0 if plan is None else 1

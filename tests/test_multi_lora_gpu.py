@@ -288,6 +288,22 @@ def test_base_gradient_and_partial_needs(dev):
         assert torch.equal(torch.autograd.grad(y, t, d["dy"])[0], full[i])
 
 
+def test_broadcast_and_transposed_base(dev):
+    d = make(20, 64, 48, 8, 2, BF16, dev)
+    rows = AdapterRows(d["ids"], 2)
+    bias = d["base"][0].clone().requires_grad_(True)
+    y = multi_lora(d["x"], d["a"], d["b"], d["s"], rows, bias.expand(20, 48))
+    assert torch.equal(y, multi_lora(d["x"], d["a"], d["b"], d["s"], rows, bias.detach().repeat(20, 1)))
+    (db,) = torch.autograd.grad(y, bias, d["dy"])
+    want = d["dy"].double().sum(0)  # torch's own sum over the broadcast rows
+    assert bool(((db.double() - want).abs() <= U[BF16] * want.abs() + 20 * E32 * d["dy"].double().abs().sum(0)).all())
+    turned = d["base"].t().contiguous().t()
+    want = multi_lora(d["x"], d["a"], d["b"], d["s"], rows, d["base"])
+    assert torch.equal(multi_lora(d["x"], d["a"], d["b"], d["s"], rows, turned), want)
+    with pytest.raises(RuntimeError, match="adjacent columns"):  # in place there is no copy
+        ops.multi_lora(d["x"], d["a"], d["b"], d["s"], rows.plan, turned, turned)
+
+
 def test_fp32_factors_beside_16_bit_rows(dev):
     d = make(20, 64, 48, 8, 2, BF16, dev)
     rows = AdapterRows(d["ids"], 2)
