@@ -99,16 +99,58 @@ __device__ __forceinline__ float base_of(float m) {
 }
 __device__ __forceinline__ float term(float x, float n) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, -n)); }
 
-// (m, s) joined with (m2, s2); an empty side has m = -inf, s = 0, and an infinite maximum
-// makes the sum NaN, as exp(inf - inf) does.
+// What a sum relative to m counts for relative to `top`, the largest of several: sides of a huge
+// maximum count for nothing beside another one.
+__device__ __forceinline__ float weight(float m, float top) {
+  return m == top ? 1.0f : (huge(m) || huge(top)) ? 0.0f : __builtin_amdgcn_exp2f(base_of(m) - base_of(top));
+}
+
+// (m, s) joined with (m2, s2); an empty side has m = -inf, s = 0.
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
-  const float top = fmaxf(m, m2);
-  const float n = base_of(top);
-  // sides of a huge maximum count for nothing beside another one
-  const float f = m == top ? 1.0f : (huge(m) || huge(top)) ? 0.0f : __builtin_amdgcn_exp2f(base_of(m) - n);
-  const float f2 = m2 == top ? 1.0f : (huge(m2) || huge(top)) ? 0.0f : __builtin_amdgcn_exp2f(base_of(m2) - n);
+  const float top = fmaxf(m, m2), f = weight(m, top), f2 = weight(m2, top);
   s = s * f + s2 * f2;  // a NaN on either side stays one
   m = top;
+}
+
+// The value of the lane that CTRL names, in the rows of 16 lanes that ROWS names (others: none).
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T from_lane(T v, T none) {
+  constexpr int kWords = sizeof(T) / 4;
+  struct Words {
+    int w[kWords];
+  };
+  Words a = __builtin_bit_cast(Words, v), o = __builtin_bit_cast(Words, none);
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) a.w[i] = __builtin_amdgcn_update_dpp(o.w[i], a.w[i], CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(T, a);
+}
+
+// op over the values of a wave's 64 lanes, for all of them: shifts by 1, 2, 4 and 8 within rows
+// of 16 lanes, then the rows' last lanes.  Registers alone: with lane shuffles, which pass the
+// LDS unit, and the sums joined in pairs the forward of 2084 rows of 32000 took 41.4 us for 39.0.
+template <typename T, typename Op>
+__device__ __forceinline__ T over_wave(T v, T none, Op op) {
+  v = op(v, from_lane<0x111, 0xF>(v, none));
+  v = op(v, from_lane<0x112, 0xF>(v, none));
+  v = op(v, from_lane<0x114, 0xF>(v, none));
+  v = op(v, from_lane<0x118, 0xF>(v, none));
+  v = op(v, from_lane<0x142, 0xA>(v, none));
+  v = op(v, from_lane<0x143, 0xC>(v, none));
+  constexpr int kWords = sizeof(T) / 4;
+  struct Words {
+    int w[kWords];
+  };
+  Words a = __builtin_bit_cast(Words, v);
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) a.w[i] = __builtin_amdgcn_readlane(a.w[i], 63);
+  return __builtin_bit_cast(T, a);
+}
+__device__ __forceinline__ float wave_max(float v) {
+  return over_wave(v, -__builtin_inff(), [](float a, float b) { return fmaxf(a, b); });
+}
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v) {
+  return over_wave(v, T(0), [](T a, T b) { return a + b; });
 }
 
 // Piece [v0, v1) of a row that a workgroup takes: whole KiB but for the row's last.
@@ -190,7 +232,9 @@ __global__ __launch_bounds__(kPfThreads) void row_sums_kernel(Rows r, Labels L, 
       }
     }
   }
-  for (int o = 1; o < 64; o <<= 1) join(m, s, __shfl_xor(m, o), __shfl_xor(s, o));
+  const float top = wave_max(m);
+  s = wave_sum(s * weight(m, top));  // a NaN stays one
+  m = top;
   __shared__ float wm[kPfThreads / 64], wsum[kPfThreads / 64];
   if ((threadIdx.x & 63) == 0) {
     wm[threadIdx.x >> 6] = m;
@@ -233,7 +277,7 @@ __global__ __launch_bounds__(kPfSeqThreads) void sequences_kernel(Rows r, Labels
     e = b + r.T / L.S;
   }
   double sum = 0.0;
-  int64_t count = 0;
+  int count = 0;
   for (int64_t t = b + threadIdx.x; t < e; t += kPfSeqThreads) {
     const int y = info[t].target;
     if (y == -1 || info[t].seq != i) continue;
@@ -253,12 +297,10 @@ __global__ __launch_bounds__(kPfSeqThreads) void sequences_kernel(Rows r, Labels
     info[t].sum = s > 0.0f ? s : __builtin_nanf("");
   }
   __shared__ double wsum[kPfSeqThreads / 64];
-  __shared__ int64_t wcount[kPfSeqThreads / 64];
+  __shared__ int wcount[kPfSeqThreads / 64];
   __shared__ bool last;
-  for (int o = 1; o < 64; o <<= 1) {
-    sum += __shfl_xor(sum, o);
-    count += __shfl_xor(count, o);
-  }
+  sum = wave_sum(sum);
+  count = wave_sum(count);
   if ((threadIdx.x & 63) == 0) {
     wsum[threadIdx.x >> 6] = sum;
     wcount[threadIdx.x >> 6] = count;
@@ -300,7 +342,7 @@ __global__ __launch_bounds__(kPfSeqThreads) void sequences_kernel(Rows r, Labels
     coef[p] = float(c / n[0]);
     coef[p + pairs] = float(-c / n[1]);
   }
-  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+  total = wave_sum(total);
   __syncthreads();  // wsum's sequence sums are read
   if ((threadIdx.x & 63) == 0) wsum[threadIdx.x >> 6] = total;
   __syncthreads();
