@@ -285,11 +285,20 @@ def _nothing_recorded(*inputs) -> bool:
     forward can run without its autograd function: no gradient asked for, and
     neither tracing, a functorch transform nor forward-mode AD active (those go
     through the function, which accepts or refuses them)."""
+    return not _gradient_asked(inputs) and _plain_eager()
+
+
+def _nothing_recorded_eagerly(*inputs) -> bool:
+    """_nothing_recorded for a call that is known not to be traced (eager_only)."""
+    return not _gradient_asked(inputs) and forward_ad._current_level < 0 and not _functorch_active()
+
+
+def _gradient_asked(inputs) -> bool:
     if torch.is_grad_enabled():
         for t in inputs:
             if t is not None and t.requires_grad:
-                return False
-    return _plain_eager()
+                return True
+    return False
 
 
 def nf4_linear(x: torch.Tensor, w: NF4Weight, bias: Optional[torch.Tensor] = None,

@@ -116,7 +116,7 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
                            f"{lora_b.shape[1]} columns")
     if not isinstance(scaling, torch.Tensor):
         scaling = torch.full((rows.n,), float(scaling), dtype=torch.float32, device=x.device)
-    if dm._nothing_recorded(x, lora_a, lora_b, base):
+    if dm._nothing_recorded_eagerly(x, lora_a, lora_b, base):
         dtype = x.dtype
         a = lora_a if lora_a.dtype == dtype else lora_a.to(dtype)
         b = lora_b if lora_b.dtype == dtype else lora_b.to(dtype)
@@ -182,7 +182,7 @@ class MultiLoRALinear(nn.Module):
         _check(x, self.lora_A, rows, self.activation_bits)
         linear = self._linear()
         scaling = self.scaling if self.scaling.dtype == torch.float32 else self.scaling.float()  # cast with the model
-        if not dm._nothing_recorded(x, self.lora_A, self.lora_B):
+        if not dm._nothing_recorded_eagerly(x, self.lora_A, self.lora_B):
             return _MultiLoRA.apply(x, self.lora_A, self.lora_B, None, scaling, rows, self.activation_bits, linear)
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         y = linear[0](x2)

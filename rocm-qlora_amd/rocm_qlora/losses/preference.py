@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from rocm_qlora import ops
-from rocm_qlora.kernels.dequant_matmul import _nothing_recorded
+from rocm_qlora.kernels.dequant_matmul import _nothing_recorded_eagerly
 from rocm_qlora.torch_ops import eager_only, first_order
 
 
@@ -64,7 +64,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, offsets: Optiona
     ref_logps: the reference model's sequence_logps, [2 P] (None: zeros).
     average: log-probabilities per labelled token instead of their sum.
     loss is differentiable by the logits; logps [2 P] (fp32) is not."""
-    if _nothing_recorded(logits):
+    if _nothing_recorded_eagerly(logits):
         return ops.preference_forward(logits, labels, offsets, ref_logps, beta=beta, label_smoothing=label_smoothing,
                                       average=average, ignore_index=ignore_index)[:2]
     return _PreferenceLoss.apply(logits, labels, offsets, ref_logps, float(beta), float(label_smoothing), bool(average),
@@ -77,6 +77,6 @@ def sequence_logps(logits: torch.Tensor, labels: torch.Tensor, offsets: Optional
     """Log-probabilities [S] (fp32) of the labelled tokens of S sequences, laid out as
     preference_loss takes them; differentiable by the logits.  Under torch.no_grad
     these are preference_loss's ref_logps when the reference model gives the logits."""
-    if _nothing_recorded(logits):
+    if _nothing_recorded_eagerly(logits):
         return ops.preference_forward(logits, labels, offsets, average=average, ignore_index=ignore_index, pairs=False)[1]
     return _SequenceLogps.apply(logits, labels, offsets, bool(average), int(ignore_index))

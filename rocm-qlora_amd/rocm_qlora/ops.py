@@ -751,12 +751,13 @@ def adapter_rows(ids: torch.Tensor, n: int) -> torch.Tensor:
 
 def _adapter_operands(dtype, K: int, lora_a, lora_b, scaling) -> Tuple[int, int, int, torch.Tensor, torch.Tensor]:
     """n, rank and N of stacked factors, and the factors as the kernels take them."""
-    if lora_a.dim() != 3 or lora_b.dim() != 3:
-        raise RuntimeError(f"stacked factors are [n, rank, K] and [n, N, rank], got {tuple(lora_a.shape)} and "
-                           f"{tuple(lora_b.shape)}")
-    n, rank, N = lora_a.shape[0], lora_a.shape[1], lora_b.shape[1]
-    if lora_a.shape[2] != K or lora_b.shape[0] != n or lora_b.shape[2] != rank or rank < 1 or N < 1:
-        raise RuntimeError(f"LoRA shapes {tuple(lora_a.shape)} / {tuple(lora_b.shape)} do not fit rows of {K}")
+    of_a, of_b = lora_a.shape, lora_b.shape
+    if len(of_a) != 3 or len(of_b) != 3:
+        raise RuntimeError(f"stacked factors are [n, rank, K] and [n, N, rank], got {tuple(of_a)} and {tuple(of_b)}")
+    n, rank, cols = of_a
+    n_b, N, rank_b = of_b
+    if cols != K or n_b != n or rank_b != rank or rank < 1 or N < 1:
+        raise RuntimeError(f"LoRA shapes {tuple(of_a)} / {tuple(of_b)} do not fit rows of {K}")
     if lora_a.dtype != dtype or lora_b.dtype != dtype:
         raise TypeError(f"stacked factors must have the rows' dtype {dtype}, got {lora_a.dtype} and {lora_b.dtype}")
     if scaling.dtype != torch.float32 or scaling.shape != (n,) or not scaling.is_contiguous():
@@ -957,11 +958,13 @@ def preference_forward(logits: torch.Tensor, labels: torch.Tensor, offsets: Opti
     logps [S], what preference_backward takes)."""
     dev = nat.require_gpu(logits, labels, offsets, ref_logps)
     code = nat.dtype_code(logits.dtype)
-    if logits.dim() not in (2, 3) or logits.numel() == 0:
-        raise RuntimeError(f"logits must be [T, V] or [B, L, V] with a row at least, got {tuple(logits.shape)}")
-    if labels.dtype != torch.int64 or labels.shape != logits.shape[:-1]:
-        raise RuntimeError(f"labels must be int64 {tuple(logits.shape[:-1])}, got {labels.dtype} {tuple(labels.shape)}")
-    if logits.dim() == 2:
+    shape = logits.shape
+    dims = len(shape)
+    if dims not in (2, 3) or logits.numel() == 0:
+        raise RuntimeError(f"logits must be [T, V] or [B, L, V] with a row at least, got {tuple(shape)}")
+    if labels.dtype != torch.int64 or labels.shape != shape[:-1]:
+        raise RuntimeError(f"labels must be int64 {tuple(shape[:-1])}, got {labels.dtype} {tuple(labels.shape)}")
+    if dims == 2:
         if offsets is None:
             raise RuntimeError("packed logits need their sequences' offsets")
         if offsets.dim() != 1 or offsets.numel() < 2 or offsets.dtype not in (torch.int32, torch.int64):
@@ -970,7 +973,7 @@ def preference_forward(logits: torch.Tensor, labels: torch.Tensor, offsets: Opti
     else:
         if offsets is not None:
             raise RuntimeError("offsets go with packed logits [T, V]")
-        S = logits.shape[0]
+        S = shape[0]
     if pairs and S % 2:
         raise RuntimeError(f"{S} sequences are no pairs")
     if pairs and not 0.0 <= label_smoothing <= 1.0:
