@@ -5,7 +5,7 @@
 // same adapter found by a ballot for each bit of its number.  Bound by latency, the chain of
 // loads, counts and sums: 3.6 us for 8 rows, 4.9 for 256 rows of 64 adapters, 7.4 for 4096 of
 // 4, 35 for 4096 of 1024 (one of two tables after the other, sums by lane shuffles, padding a
-// tile a thread: 6.6, 7.5, 10 and 63).
+// tile a thread: 6.6, 7.5, 10 and 63; a graph's replays).
 // It runs once for a batch, for all the projections of all its layers.
 #include "rq_launch.h"
 #include "rq_rows.h"

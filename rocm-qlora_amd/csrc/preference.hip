@@ -16,9 +16,9 @@
 // fixed order; the workgroup that ends last takes the pairs.  The gradient is a
 // second pass: a pair's coefficient depends on every row of the pair.
 // Bound by memory: the labelled rows read twice, every row of the gradient
-// written once.  8336 rows of 128256 bf16 logits, 4862 of them labelled: sums 220 us
-// (5.7 TB/s), gradient 633 (1.2 GB read, 2.1 written, 5.3 TB/s).  The sequences' launch is
-// latency, 7 to 10 us.
+// written once.  8336 rows of 128256 bf16 logits, 4862 of them labelled: sums 218 us
+// (5.7 TB/s), gradient 635 (1.2 GB read, 2.1 written, 5.3 TB/s).  The sequences' launch is
+// latency, 6.5 to 10 us.
 #include "rq_io.h"
 #include "rq_launch.h"
 #include "rq_linear_dev.h"
