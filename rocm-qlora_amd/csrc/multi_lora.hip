@@ -382,16 +382,7 @@ int run_shrink(const ShrinkArgs& a, hipStream_t stream) {
   return rq_check_launch();
 }
 
-// ---- the row sums' operands -------------------------------------------------------
-// In the order in which rowsum's lanes load them: for 32 slots and 16 ranks, 1 KiB of hi
-// parts and 1 KiB of lo parts (fp32: of slots 8 g .. 8 g + 3 and of the four after them), 16
-// bytes of lane (i, g) = rank i, slots 8 g .. 8 g + 7.
-template <int XT>
-__device__ __forceinline__ int64_t opt_at(int64_t slot, int rank, int rp) {  // slot: a multiple of 8
-  constexpr int kBlock = XT == RQ_DTYPE_F32 ? 512 : 1024, kLane = Elem<XT>::kVec;
-  return ((slot >> 5) * (rp >> 4) + (rank >> 4)) * kBlock + ((rank & 15) + 2 * (slot & 24)) * kLane;
-}
-
+// ---- the row sums' operands (their layout: opt_at, rq_multi_lora.h) -----------------
 // A tile's operands from LDS, rows of `pitch` (16-bit: hi | lo); zeros past its `count` rows.
 template <int XT>
 __device__ __forceinline__ void store_operands(typename Elem<XT>::T* opt, const typename Elem<XT>::T* op, int pitch, int rp,
@@ -893,7 +884,7 @@ __device__ __forceinline__ void rowsum_body(const RowSumArgs& a, const RowSumTas
   const bool full = c0 + 16 * CW <= K.C;            // all columns
   const int64_t lcol = full || col < K.C ? col : 0;  // lanes past the end repeat column 0: their sums are not stored
   const int64_t base = int64_t(kTileRows) * ch.t0;
-  const T* opt = static_cast<const T*>(K.opt) + opt_at<XT>(base + 8 * g, j0 + i16, a.rp);
+  const T* opt = static_cast<const T*>(K.opt) + opt_at<XT>(base + 8 * g, i16, a.rp);
 
   f32x4 acc[CW][JB];
 #pragma unroll
@@ -933,7 +924,7 @@ __device__ __forceinline__ void rowsum_body(const RowSumArgs& a, const RowSumTas
       for (int p = 0; p < kPlanes; ++p)
 #pragma unroll
         for (int k = 0; k < kOps; ++k)
-          o.u[j][p][k] = *reinterpret_cast<const u32x4*>(opt + opt_at<XT>(s, 16 * j, a.rp) + 512 * p + 256 * k);
+          o.u[j][p][k] = *reinterpret_cast<const u32x4*>(opt + opt_at<XT>(s, rowsum_rank(j0, j, a.rp), a.rp) + 512 * p + 256 * k);
   };
   auto products = [&](const Raw (&raw)[8], const Ops& o, const int (&r)[8], bool last) {
     ColPiece<XT, CW> row[8];
@@ -1091,7 +1082,7 @@ int64_t rowsum_parts(const RowsPlan& rows, int table) {
 
 template <int XT>
 int run_rowsum(RowSumArgs a, hipStream_t stream) {
-  const int jb = a.rp <= 16 ? 1 : (a.rp <= 32 ? 2 : 4);
+  const int jb = rowsum_blocks(a.rp);
   int tiles = 0;
   int64_t most = 0;
   for (int i = 0; i < a.n; ++i) {
@@ -1154,7 +1145,7 @@ struct BackwardPlan {
 BackwardPlan plan_backward(const Sizes& s, const RowsPlan& rows) {
   BackwardPlan p{};
   const int64_t rp = rank_pad(s.r), slots = rows.slots();
-  const int cus = device_cus(), jb = rp <= 16 ? 1 : (rp <= 32 ? 2 : 4);
+  const int cus = device_cus(), jb = rowsum_blocks(int(rp));
   plan_shrink(rows.T, s.N, s.step, cus, &p.splits, &p.per);
   p.table = rowsum_table(rows, s.K + s.N, 16 * (s.es == 4 ? rowsum_cw<RQ_DTYPE_F32>(jb) : rowsum_cw<RQ_DTYPE_BF16>(jb)), cus);
   p.part_size = ceil_div((s.K + s.N) * s.r, 8) * 8;

@@ -62,6 +62,23 @@ struct OperandsArgs {
   void* opt;            // slots * rp values of 32 bits
 };
 
+// The row sums' operands in the order in which rowsum's lanes load them: for 32 slots and 16
+// ranks, 1 KiB of hi parts and 1 KiB of lo parts (fp32: of slots 8 g .. 8 g + 3 and of the four
+// after them), 16 bytes of lane (i, g) = rank i, slots 8 g .. 8 g + 7.  slot: a multiple of 8.
+template <int XT>
+__host__ __device__ inline int64_t opt_at(int64_t slot, int rank, int rp) {
+  constexpr int kBlock = XT == RQ_DTYPE_F32 ? 512 : 1024, kLane = Elem<XT>::kVec;
+  return ((slot >> 5) * (rp >> 4) + (rank >> 4)) * kBlock + ((rank & 15) + 2 * (slot & 24)) * kLane;
+}
+
+// 16-rank blocks of a rowsum wave: 1, 2 or 4.
+__host__ __device__ inline int rowsum_blocks(int rp) { return rp <= 16 ? 1 : (rp <= 32 ? 2 : 4); }
+
+// First rank of the operands that block j of the wave from rank j0 on loads: its own, or where
+// the stored ranks end before it (rp 96: blocks 6 and 7) the wave's first again, whose sums are
+// not stored.
+__host__ __device__ inline int rowsum_rank(int j0, int j, int rp) { return j0 + 16 * j < rp ? j0 + 16 * j : j0; }
+
 struct RowSumTask {
   const void* src;      // rows, or 8-bit codes
   const uint8_t* exps;  // of the codes, or nullptr: src holds values
