@@ -88,10 +88,11 @@ struct RowInfo {
   float sum;
 };
 
-// A maximum too large for its multiple of log2 e and the differences from it to mean
-// anything but "equal" or "nothing beside it".
-constexpr float kHuge = 0x1p100f;
-__device__ __forceinline__ bool huge(float m) { return !(fabsf(m) < kHuge); }
+// The largest maximum next to which terms count.  Their argument is off by the rounding of
+// m log2 e, 64 at most: terms and sums stay within fp32, and the log-probability takes the same n.
+// Past it fp32 values are 128 apart or more, and e^-128 is none.
+constexpr float kHuge = 0x1p30f;
+__device__ __forceinline__ bool huge(float m) { return !(fabsf(m) <= kHuge); }
 
 // n of a maximum m, and a term of the sum relative to it.
 __device__ __forceinline__ float base_of(float m) {
