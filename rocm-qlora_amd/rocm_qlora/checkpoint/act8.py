@@ -81,19 +81,28 @@ def saved_in_8_bits(min_elements: int = 1 << 16):
     return _saved(lambda t: _floats(t, min_elements) and _activation(t))
 
 
-def inputs_saved_in_8_bits(x: torch.Tensor):
-    """The same for one layer's input x (and what dropout makes of it), whether or not it
-    requires a gradient: inside the layer's own autograd function saved tensors have no
-    record; where torch's products compose the layer, x shares its memory and dropout its
-    name, and the factors and the first product stay as they are."""
+def inputs_saved_in_8_bits(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor):
+    """The same for the input x of one layer with the factors lora_a [r, K] and lora_b [N,
+    r] (and what dropout makes of x), whether or not it requires a gradient: inside the
+    layer's own autograd function saved tensors have no record; where torch's products
+    compose the layer, x shares its memory and dropout its name, and the factors and the
+    first product stay as they are.  Where one of those has x's shape (a batch of r rows),
+    what has neither a record nor x's memory stays as it is."""
+    (r, K), N = lora_a.shape, lora_b.shape[0]
     shape, place = (x.numel(), x.shape[-1:]), x.untyped_storage().data_ptr()
+    factors = {f.untyped_storage().data_ptr() for f in (lora_a, lora_b)}
+    # A, B, their transposes' and casts', and x A^T
+    alike = r == K or shape in ((r * K, (K,)), (N * r, (r,)), (N * r, (N,)))
 
     def holds(t: torch.Tensor) -> bool:
         if not _floats(t, 1) or (t.numel(), t.shape[-1:]) != shape:
             return False
+        at = t.untyped_storage().data_ptr()
+        if at == place or at in factors:
+            return at == place
         node = t.grad_fn
         while node is not None and node.name() in _VIEWS:
             node = node.next_functions[0][0]
-        return node is None or node.name() == "NativeDropoutBackward0" or t.untyped_storage().data_ptr() == place
+        return not alike if node is None else node.name() == "NativeDropoutBackward0"
 
     return _saved(holds)

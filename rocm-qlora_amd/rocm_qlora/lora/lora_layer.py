@@ -72,7 +72,7 @@ class LoRALinear(nn.Module):
 
     @eager_only
     def _forward_saved_in_8_bits(self, x: torch.Tensor, p: float) -> torch.Tensor:
-        with inputs_saved_in_8_bits(x):
+        with inputs_saved_in_8_bits(x, self.lora_A, self.lora_B):
             return self.base_layer.fused_forward(x, self.lora_A, self.lora_B, self.scaling, p)
 
     @torch.no_grad()
