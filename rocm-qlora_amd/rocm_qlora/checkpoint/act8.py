@@ -43,9 +43,13 @@ def decompress(c: Act8) -> torch.Tensor:
     return ops.act8_dequantize(c.codes, c.exponents, c.shape[-1], c.dtype).view(c.shape)
 
 
-# autograd nodes that leave a parameter a parameter: transposed, viewed or cast
-_VIEWS = {"TBackward0", "TransposeBackward0", "PermuteBackward0", "ViewBackward0", "UnsafeViewBackward0", "AsStridedBackward0",
-          "ToCopyBackward0", "AliasBackward0"}
+# autograd nodes that leave a parameter a parameter: viewed in whatever way, copied into another
+# order or cast
+_VIEWS = {"TBackward0", "TransposeBackward0", "PermuteBackward0", "ViewBackward0", "UnsafeViewBackward0", "ReshapeAliasBackward0",
+          "AsStridedBackward0", "AliasBackward0", "SliceBackward0", "SelectBackward0", "DiagonalBackward0", "UnfoldBackward0",
+          "SplitBackward0", "SplitWithSizesBackward0", "UnsafeSplitBackward0", "UnsafeSplitWithSizesBackward0",
+          "UnbindBackward0", "ExpandBackward0", "UnsqueezeBackward0", "SqueezeBackward0", "SqueezeBackward1",
+          "SqueezeBackward2", "CloneBackward0", "ToCopyBackward0"}
 
 
 def _floats(t: torch.Tensor, min_elements: int) -> bool:
@@ -55,7 +59,7 @@ def _floats(t: torch.Tensor, min_elements: int) -> bool:
 
 def _activation(t: torch.Tensor) -> bool:
     """Whether t was computed from more than a parameter: autograd records how, and the
-    record does not lead through views and casts alone to a parameter.  (What has no
+    record does not lead through views, copies and casts alone to a parameter.  (What has no
     record may be a frozen weight.)"""
     node = t.grad_fn
     while node is not None and node.name() in _VIEWS:
@@ -74,8 +78,8 @@ def _saved(holds):
 def saved_in_8_bits(min_elements: int = 1 << 16):
     """A context in which autograd holds the float activations that it saves for the
     backward pass in 8 bits: GPU tensors of at least min_elements values that were
-    computed from a tensor that requires a gradient.  Parameters, their views and casts,
-    and what requires no gradient stay as they are.  Gradients are then those at the held
+    computed from a tensor that requires a gradient.  Parameters, their views, copies and
+    casts, and what requires no gradient stay as they are.  Gradients are then those at the held
     values; what the forward returns does not change.  For the activations of linears and
     gates; keep ops that differentiate small differences (norms, softmax) outside."""
     return _saved(lambda t: _floats(t, min_elements) and _activation(t))

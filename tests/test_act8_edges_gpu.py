@@ -1,12 +1,53 @@
-"""What 8-bit activations leave as it is: a layer's factors where they have its input's shape."""
+"""What 8-bit activations leave as it is: parameters by whatever view or cast, and a layer's
+factors where they have its input's shape."""
 import pytest
 import torch
 
 from rocm_qlora import LoRALinear, QuantLinear
-from rocm_qlora.checkpoint import compress, decompress
+from rocm_qlora.checkpoint import compress, decompress, saved_in_8_bits
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
+
+VIEWS = {
+    "rows": lambda p: p[8:72],
+    "columns": lambda p: p[:, 16:],
+    "one of several": lambda p: p.view(2, 40, 96)[1],
+    "unbound": lambda p: p.view(2, 40, 96).unbind(0)[0],
+    "split": lambda p: p.split(40)[1],
+    "sized split": lambda p: p.split([30, 50])[1],
+    "chunk": lambda p: p.chunk(2, 1)[0],
+    "unsqueezed": lambda p: p.unsqueeze(0).squeeze(0),
+    "expanded": lambda p: p[:1].expand(40, 96),
+    "transposed copy": lambda p: p.t().contiguous().t(),
+    "cast of a slice": lambda p: p[:40].to(BF16).float(),
+    "slice of a cast": lambda p: p.to(BF16).float()[:40],
+    "movedim": lambda p: p.view(2, 40, 96).movedim(0, 1)[:, 0],
+}
+
+
+@pytest.mark.parametrize("view", list(VIEWS))
+def test_views_of_parameters_stay_as_they_are(dev, view):
+    """The input gradient of a linear is dY W: with W any view, copy or cast of a parameter it
+    does not change, and the weight's gradient is the one at the held input."""
+    g = torch.Generator().manual_seed(4)
+    p = torch.nn.Parameter(torch.randn(80, 96, generator=g).to(dev))
+    w = VIEWS[view](p)
+    x = torch.randn(64, w.shape[1], generator=g).to(dev).requires_grad_(True)
+    dy = torch.randn(64, w.shape[0], generator=g).to(dev)
+
+    def grads(bits):
+        h = x * 1.0
+        if bits == 8:
+            with saved_in_8_bits(min_elements=1):
+                y = torch.nn.functional.linear(h, w)
+        else:
+            y = torch.nn.functional.linear(h, w)
+        return (y, *torch.autograd.grad(y, (x, p), dy, retain_graph=True))
+
+    (y0, dx0, dp0), (y8, dx8, dp8) = grads(16), grads(8)
+    assert torch.equal(y0, y8) and torch.equal(dx0, dx8)
+    assert not torch.equal(dp0, dp8)  # the input itself is held in 8 bits
 
 
 def test_factors_of_the_inputs_shape_stay_as_they_are(dev):
