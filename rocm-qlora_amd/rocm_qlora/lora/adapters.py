@@ -128,6 +128,12 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
     return _MultiLoRA.apply(x, lora_a, lora_b, base, scaling, rows, activation_bits, None)
 
 
+def _refuse_merged(base: QuantLinear, name: str) -> None:
+    """The adapters' term goes beside the quantized weight, not one that an adapter was merged into."""
+    if base.merged_mode:
+        raise RuntimeError(f"{name} is merged: unmerge its adapter first")
+
+
 class MultiLoRALinear(nn.Module):
     """A QuantLinear with n adapters of rank r.  lora_A [n, r, in] and lora_B [n, out,
     r] are parameters (A Kaiming-uniform, B zeros, as LoRALinear's), `scaling` [n] a
@@ -137,6 +143,7 @@ class MultiLoRALinear(nn.Module):
     def __init__(self, quant_linear: QuantLinear, n: int, r: int = 8, lora_alpha: float = 16, activation_bits: int = 16):
         if not isinstance(quant_linear, QuantLinear):
             raise TypeError(f"adapters go beside a QuantLinear, got {type(quant_linear).__name__}")
+        _refuse_merged(quant_linear, "the QuantLinear")
         super().__init__()
         self.base_layer = quant_linear
         self.n, self.r = n, r
@@ -166,6 +173,7 @@ class MultiLoRALinear(nn.Module):
     def _linear(self):
         """The quantized linear and its input gradient as functions of 2-D rows."""
         base = self.base_layer
+        _refuse_merged(base, "the QuantLinear")
         if base.bits == 4:
             w = base.nf4_weight()
             return (lambda x: ops.nf4_linear(x, w.packed, w.scales, w.N, w.block_size, base.bias, **w.dq_kwargs()),
@@ -213,6 +221,7 @@ def attach_adapters(model: nn.Module, n: int, activation_bits: int = 16) -> nn.M
             raise RuntimeError(f"{name} is merged: unmerge it first")
         if not isinstance(m.base_layer, QuantLinear):
             raise TypeError(f"{name}: adapters go beside a QuantLinear, got {type(m.base_layer).__name__}")
+        _refuse_merged(m.base_layer, f"{name}'s QuantLinear")
     made = {}  # a layer in several places stays one
     for name, m in layers:
         if m not in made:

@@ -1,0 +1,33 @@
+"""What the adapters' layers refuse, without a GPU."""
+import pytest
+import torch
+
+from rocm_qlora import LoRALinear, QuantLinear
+from rocm_qlora.lora import AdapterRows, MultiLoRALinear, attach_adapters
+
+
+def merged(q):
+    """As LoRALinear.merge_lora leaves the quantized layer: its forward reads the merged weight."""
+    q.merged_fp16_weight = torch.zeros(q.out_features, q.in_features, dtype=torch.float16)
+    q.merged_mode = True
+    return q
+
+
+def test_merged_quantized_layers_are_refused():
+    with pytest.raises(RuntimeError, match="merged"):
+        MultiLoRALinear(merged(QuantLinear(64, 32, bits=4)), 2)
+    layer = MultiLoRALinear(QuantLinear(64, 32, bits=4), 1)
+    merged(layer.base_layer)
+    with pytest.raises(RuntimeError, match="merged"):
+        layer(torch.zeros(2, 64), AdapterRows.single(2))
+
+
+def test_attach_adapters_refuses_a_merged_weight_before_it_changes_the_model():
+    first = LoRALinear(QuantLinear(64, 64, bits=4), r=4)
+    shared = QuantLinear(64, 64, bits=4)
+    second = LoRALinear(shared, r=4)  # not merged itself; its quantized layer is, by another
+    merged(shared)
+    model = torch.nn.Sequential(first, second)
+    with pytest.raises(RuntimeError, match="merged"):
+        attach_adapters(model, 2)
+    assert model[0] is first and model[1] is second
