@@ -22,13 +22,30 @@ namespace rq {
 constexpr int kMlThreads = 256;
 constexpr int kMlWaves = kMlThreads / 64;
 
-// The 16-bit halves of fp32 values: hi = RND(v), lo = RND(v - hi) (none for an
-// infinity: inf - inf).
+// The 16-bit halves of fp32 values: hi = RND(v), lo = RND((v - hi) 2^kLoBits) (none for an
+// infinity: inf - inf).  fp16's lo part is scaled: |v - hi| is 16 at most (half a step of 65504),
+// so that 2^11 of it is the most that fits, and the smallest step of lo is 2^-35 of v instead of
+// 2^-24, where hi's own ends.  bf16 has fp32's exponents.
+template <int XT>
+constexpr int kLoBits = XT == RQ_DTYPE_F16 ? 11 : 0;
 template <int XT>
 __device__ __forceinline__ void split16(float v, uint32_t& hi, uint32_t& lo) {
   hi = to_x16<XT>(v);
   const float h = from_x16<XT>(hi);
-  lo = to_x16<XT>(fabsf(h) == __builtin_inff() ? 0.0f : v - h);
+  lo = to_x16<XT>(fabsf(h) == __builtin_inff() ? 0.0f : (v - h) * float(1 << kLoBits<XT>));
+}
+
+// acc + the product with lo parts.
+template <int XT>
+__device__ __forceinline__ f32x4 mma_lo(const u32x4& a, const u32x4& b, f32x4 acc) {
+  if constexpr (kLoBits<XT> == 0) {
+    return mma<XT>(a, b, acc);
+  } else {
+    const f32x4 v = mma<XT>(a, b, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[q] = __builtin_fmaf(v[q], 1.0f / float(1 << kLoBits<XT>), acc[q]);
+    return acc;
+  }
 }
 
 // Workgroup id -> unit of work, 0 .. n - 1 (n or more: none).  Workgroup ids go round the
@@ -575,7 +592,8 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
   const bool adapted = tile.adapter >= 0;
   const int pitch = (XT == RQ_DTYPE_F32 ? a.rp : 2 * a.rp) + V;  // of the slots' operands
   T* op = lds + (FACTOR_ROWS ? GROUPS * L::kStage : 0);
-  // 16 ranks of 16 bits: lane groups 2 and 3 take the lo parts, of the same ranks as 0 and 1
+  // 16 ranks of 16 bits: lane groups 2 and 3 take the lo parts, of the same ranks as 0 and 1 (one
+  // matrix instruction where lo is not scaled)
   const bool half = XT != RQ_DTYPE_F32 && a.rp < kStep;
   const T* s = static_cast<const T*>(a.s) + (adapted ? tile.adapter : 0) * a.s_adapter;
   const float scale = adapted ? a.scaling[tile.adapter] : 0.0f;
@@ -685,13 +703,23 @@ __device__ __forceinline__ void expand_body(const ExpandArgs& a, const Tile& til
         }
         if (here) {
           const T* u = op + (16 * block + i16) * pitch + k * kStep + V * g;
-          const u32x4 hi = *reinterpret_cast<const u32x4*>(u);
+          u32x4 hi = *reinterpret_cast<const u32x4*>(u);
+          u32x4 lo = hi;  // `half`: of lane groups 2 and 3
+          const bool apart = XT != RQ_DTYPE_F32 && (!half || kLoBits<XT> > 0);
+          if (XT != RQ_DTYPE_F32 && !half) {
+            lo = *reinterpret_cast<const u32x4*>(u + a.rp);
+          } else if (apart) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              lo[e] = g < 2 ? 0u : lo[e];
+              hi[e] = g < 2 ? hi[e] : 0u;
+            }
+          }
 #pragma unroll
           for (int c = 0; c < V; ++c) acc[c] = mma<XT>(hi, f[c], acc[c]);
-          if (XT != RQ_DTYPE_F32 && !half) {
-            const u32x4 lo = *reinterpret_cast<const u32x4*>(u + a.rp);
+          if (apart) {
 #pragma unroll
-            for (int c = 0; c < V; ++c) acc[c] = mma<XT>(lo, f[c], acc[c]);
+            for (int c = 0; c < V; ++c) acc[c] = mma_lo<XT>(lo, f[c], acc[c]);
           }
         }
         if constexpr (FACTOR_ROWS) {
@@ -957,7 +985,7 @@ __device__ __forceinline__ void rowsum_body(const RowSumArgs& a, const RowSumTas
         for (int p = 0; p < kPlanes; ++p)
 #pragma unroll
           for (int j = 0; j < JB; ++j)
-            acc[c][j] = mma<XT>(x, o.u[j][p][0], acc[c][j]);
+            acc[c][j] = p == 0 ? mma<XT>(x, o.u[j][p][0], acc[c][j]) : mma_lo<XT>(x, o.u[j][p][0], acc[c][j]);
       }
     }
   };
@@ -1007,8 +1035,11 @@ __device__ __forceinline__ void rowsum_body(const RowSumArgs& a, const RowSumTas
   }
 }
 
+// (fp16's lo parts meet in registers of their own: 170 with 64 ranks a wave, two waves a SIMD unless
+// three are asked for; a backward pass of 4096 rows, K 4096, N 14336, r 64: 108 us with two, 98 - 100
+// with three.)
 template <int XT, int JB>
-__global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(2))) void rowsum_kernel(RowSumArgs a) {
+__global__ __launch_bounds__(kMlThreads) __attribute__((amdgpu_waves_per_eu(XT == RQ_DTYPE_F16 && JB == 4 ? 3 : 2))) void rowsum_kernel(RowSumArgs a) {
   constexpr int kCols = 16 * rowsum_cw<XT>(JB);
   __shared__ float red[2][kCols][16 * JB + 1];
   RowSumChunk ch{0, 0, -1, 0};
