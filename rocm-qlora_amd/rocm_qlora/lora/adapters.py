@@ -106,7 +106,7 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
     N] in x's dtype (None: zeros).  Sums are fp32; x A^T is passed to the second
     product in 16 bits or more and the result rounded once (fp16: x A^T up to 65504; an
     infinity in lora_b, or in a gradient's x, may come out as NaN).  Differentiable by x,
-    lora_a, lora_b and base; activation_bits=8 holds x for dA as an 8-bit checkpoint
+    lora_a, lora_b and base (not by scaling); activation_bits=8 holds x for dA as an 8-bit checkpoint
     (rocm_qlora.checkpoint), which the gradient kernel reads as it is."""
     _check(x, lora_a, rows, activation_bits)
     # (2-D rows' base is checked with the other operands)
@@ -116,6 +116,8 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
                            f"{lora_b.shape[1]} columns")
     if not isinstance(scaling, torch.Tensor):
         scaling = torch.full((rows.n,), float(scaling), dtype=torch.float32, device=x.device)
+    elif scaling.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("multi_lora has no gradient by scaling: pass it detached")
     if dm._nothing_recorded_eagerly(x, lora_a, lora_b, base):
         dtype = x.dtype
         a = lora_a if lora_a.dtype == dtype else lora_a.to(dtype)

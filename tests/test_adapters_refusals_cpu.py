@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from rocm_qlora import LoRALinear, QuantLinear
-from rocm_qlora.lora import AdapterRows, MultiLoRALinear, attach_adapters
+from rocm_qlora.lora import AdapterRows, MultiLoRALinear, attach_adapters, multi_lora
 
 
 def merged(q):
@@ -31,3 +31,12 @@ def test_attach_adapters_refuses_a_merged_weight_before_it_changes_the_model():
     with pytest.raises(RuntimeError, match="merged"):
         attach_adapters(model, 2)
     assert model[0] is first and model[1] is second
+
+
+def test_scaling_that_asks_for_a_gradient_is_refused():
+    x, a, b = torch.zeros(4, 32), torch.zeros(1, 4, 32), torch.zeros(1, 8, 4)
+    s = torch.ones(1, requires_grad=True)
+    with pytest.raises(RuntimeError, match="scaling"):
+        multi_lora(x, a, b, s, AdapterRows.single(4))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):  # nothing is recorded: as any other
+        multi_lora(x, a, b, s, AdapterRows.single(4))
