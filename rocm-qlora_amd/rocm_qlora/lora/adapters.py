@@ -10,6 +10,7 @@ that both run as one batch.
 from __future__ import annotations
 
 import math
+import warnings
 from typing import Optional, Union
 
 import torch
@@ -215,8 +216,8 @@ def set_adapter_rows(model: nn.Module, rows: Optional[AdapterRows]) -> int:
 
 def attach_adapters(model: nn.Module, n: int, activation_bits: int = 16) -> nn.Module:
     """Replace every LoRALinear (quantize_model's) by a MultiLoRALinear of n adapters of
-    its rank over the same quantized weight; adapter 0 is the layer's own (without its
-    dropout).  Returns the model, or what replaces it when it is a LoRALinear itself."""
+    its rank over the same quantized weight; adapter 0 is the layer's own, without its
+    dropout (a warning says so).  Returns the model, or what replaces it when it is a LoRALinear itself."""
     layers = [(name, m) for name, m in model.named_modules(remove_duplicate=False) if isinstance(m, LoRALinear)]
     for name, m in layers:
         if m.merged:
@@ -224,6 +225,10 @@ def attach_adapters(model: nn.Module, n: int, activation_bits: int = 16) -> nn.M
         if not isinstance(m.base_layer, QuantLinear):
             raise TypeError(f"{name}: adapters go beside a QuantLinear, got {type(m.base_layer).__name__}")
         _refuse_merged(m.base_layer, f"{name}'s QuantLinear")
+    dropout = [name for name, m in layers if isinstance(m.lora_dropout, nn.Dropout) and m.lora_dropout.p > 0.0]
+    if dropout:
+        warnings.warn(f"the adapters have no dropout: that of {dropout[0] or 'the layer'}"
+                      f"{f' and {len(dropout) - 1} more' if len(dropout) > 1 else ''} is left out", stacklevel=2)
     made = {}  # a layer in several places stays one
     for name, m in layers:
         if m not in made:

@@ -1,4 +1,6 @@
-"""What the adapters' layers refuse, without a GPU."""
+"""What the adapters' layers refuse or warn of, without a GPU."""
+import warnings
+
 import pytest
 import torch
 
@@ -40,3 +42,13 @@ def test_scaling_that_asks_for_a_gradient_is_refused():
         multi_lora(x, a, b, s, AdapterRows.single(4))
     with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):  # nothing is recorded: as any other
         multi_lora(x, a, b, s, AdapterRows.single(4))
+
+
+def test_attach_adapters_warns_of_the_dropout_it_leaves_out():
+    model = torch.nn.Sequential(LoRALinear(QuantLinear(64, 64, bits=4), r=4, lora_dropout=0.1))
+    with pytest.warns(UserWarning, match="dropout"):
+        attach_adapters(model, 2)
+    assert isinstance(model[0], MultiLoRALinear)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        attach_adapters(torch.nn.Sequential(LoRALinear(QuantLinear(64, 64, bits=4), r=4)), 2)
