@@ -337,7 +337,9 @@ __global__ __launch_bounds__(kPfSeqThreads) void sequences_kernel(Rows r, Labels
       n[k] = __hip_atomic_load(sums + 2 * q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     const double beta = P.beta, eps = P.eps, d = beta * (v[0] - v[1]);
-    total += (1.0 - eps) * softplus(-d) + eps * softplus(d);
+    // a side of weight 0 is not there: 0 times the infinity of an answer that the model cannot give is none
+    if (eps < 1.0) total += (1.0 - eps) * softplus(-d);
+    if (eps > 0.0) total += eps * softplus(d);
     const double up = exp(-softplus(-d)), down = exp(-softplus(d));  // sigmoids of d and -d
     const double c = beta / double(pairs) * (eps * up - (1.0 - eps) * down);
     coef[p] = float(c / n[0]);

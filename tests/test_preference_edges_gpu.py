@@ -7,7 +7,7 @@ and e^-128 is no fp32 number: only what equals the maximum counts."""
 import pytest
 import torch
 
-from rocm_qlora.losses import sequence_logps
+from rocm_qlora.losses import preference_loss, sequence_logps
 from test_preference_gpu import BF16, FP32, check_dz, check_logps, oracle
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +53,25 @@ def test_close_logits_below_a_large_maximum(dev):
     # the label a neighbour's step below the maximum
     labels[1::2] = 4
     check_sequences(z, labels, torch.arange(0, 2 * len(at) + 1, 2, device=dev), V, FP32)
+
+
+def test_infinite_ratio_without_smoothing(dev):
+    """A rejected answer that the model cannot give (its token masked to -inf): D is +inf, and
+    without label smoothing its pair's loss is 0, with it +inf; the other pair counts as it does."""
+    z = torch.randn(8, 12, generator=torch.Generator().manual_seed(0)).to(dev)
+    labels = torch.tensor([-100, 3] * 4, device=dev)
+    offsets = torch.tensor([0, 2, 4, 6, 8], device=dev)
+    z[4, 3] = float("-inf")     # sequence 2, the rejected one of pair 0
+    z.requires_grad_(True)
+    loss, logps = preference_loss(z, labels, offsets)
+    other = preference_loss(z[[2, 3, 6, 7]], labels[:4], offsets[:3])[0]
+    assert logps[2].item() == float("-inf")
+    assert abs(loss.item() - other.item() / 2) <= 2.0 ** -23 * other.item()
+    dz = torch.autograd.grad(loss, z)[0]
+    assert not dz[0].any() and not dz[4].any() and bool(dz[2].any()) and bool(torch.isfinite(dz).all())
+    assert preference_loss(z, labels, offsets, label_smoothing=0.1)[0].item() == float("inf")
+    # the chosen one: D is -inf, and all smoothing leaves nothing of it
+    z = z.detach().roll(-4, 0)
+    assert preference_loss(z, labels, offsets)[0].item() == float("inf")
+    all_smooth = preference_loss(z, labels, offsets, label_smoothing=1.0)[0].item()
+    assert abs(all_smooth - preference_loss(z[[2, 3, 6, 7]], labels[:4], offsets[:3], label_smoothing=1.0)[0].item() / 2) <= 2.0 ** -23
