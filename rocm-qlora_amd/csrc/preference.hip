@@ -337,10 +337,11 @@ __global__ __launch_bounds__(kPfSeqThreads) void sequences_kernel(Rows r, Labels
       n[k] = __hip_atomic_load(sums + 2 * q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     const double beta = P.beta, eps = P.eps, d = beta * (v[0] - v[1]);
-    // a side of weight 0 is not there: 0 times the infinity of an answer that the model cannot give is none
-    if (eps < 1.0) total += (1.0 - eps) * softplus(-d);
-    if (eps > 0.0) total += eps * softplus(d);
-    const double up = exp(-softplus(-d)), down = exp(-softplus(d));  // sigmoids of d and -d
+    // a side of weight 0 is not there: 0 times the infinity of an answer that the model cannot give
+    // is none (both sides computed: 1 us less than a branch each, which computes their log twice)
+    const double near = softplus(-d), far = softplus(d);
+    total += (eps < 1.0 ? (1.0 - eps) * near : 0.0) + (eps > 0.0 ? eps * far : 0.0);
+    const double up = exp(-near), down = exp(-far);  // sigmoids of d and -d
     const double c = beta / double(pairs) * (eps * up - (1.0 - eps) * down);
     coef[p] = float(c / n[0]);
     coef[p + pairs] = float(-c / n[1]);
