@@ -73,7 +73,7 @@ inline unsigned xcd_grid(int64_t n) { return unsigned(ceil_div(n, kXcds) * kXcds
 // Bound by a workgroup's chain of loads (tile, rows, values, the exchange in LDS) and then by
 // HBM: dY B of 3342 rows, N 14336, r 64 27 us (96 MB, 3.5 TB/s; a copy reaches 5.2), x A^T of
 // 2610 rows, K 11008, r 12 15 us (57 MB, 3.9 TB/s), of 3342 rows, K 4096, r 64 14 us; 224 rows
-// on 64 adapters, K 4096, r 32 8 us (19 MB), 8 rows 4.4.  Two pieces in flight instead of one
+// on 64 adapters, K 4096, r 32 9 us (19 MB), 8 rows 4.3.  Two pieces in flight instead of one
 // in shrink_blocks changed none of it.
 constexpr int kShWaves = 4;
 constexpr int kShThreads = 64 * kShWaves;
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(3)))
 
 // About two workgroups a compute unit, each with four steps a wave (many tiles: eight, since
 // every later workgroup of a tile sums the splits; a training step of 4096 rows, K 4096,
-// N 14336, r 64 160 - 165 us, with sixteen 167, with twenty-eight 188).
+// N 14336, r 64, replayed from a graph: 162 - 166 us, with sixteen 168, with twenty-eight 187).
 void plan_shrink(int64_t T, int64_t K, int step, int cus, int* splits, int64_t* per) {
   const int64_t unit = int64_t(step) * kShWaves;
   int64_t s = ceil_div(2 * cus, std::max<int64_t>(T, 1));
@@ -527,7 +527,7 @@ int run_operands(const OperandsArgs& a, hipStream_t stream) {
 // other banks.  A's rows [r][K] are read along the row and transposed in registers.
 //
 // Bound by HBM with a base: 4096 rows, N 14336, r 64 56 us (base and result 235 MB, 4.2 TB/s),
-// 3001 rows, N 4096, r 12 15.6 us (3.2 TB/s).  Without one (dX of 4096 rows, K 4096: 22 us,
+// 3001 rows, N 4096, r 12 16 us (3.1 TB/s).  Without one (dX of 4096 rows, K 4096: 22 us,
 // 34 MB written) by a workgroup's chain: rows, splits, factor pieces, each waiting for the
 // last; there are two workgroups a compute unit, and more of them sum the splits more often.
 // Four slots' splits in flight instead of two: no faster.
@@ -820,13 +820,14 @@ constexpr int rowsum_cw(int jb) {
   return XT == RQ_DTYPE_F32 || jb > 2 ? 4 : 8;
 }
 
-// CODES: the rows are 8-bit codes with exponents.  FULL: all CW columns exist.
+// CODES: the rows are 8-bit codes with exponents.
 template <int XT, int CW, bool CODES>
 struct RawPiece {
   uint32_t d[CODES ? CW / 4 : ColPiece<XT, CW>::kWords];
   uint32_t e;  // of codes
 };
 
+// full: all CW columns of this lane exist (of codes they do: rows end in whole blocks).
 template <int XT, int CW, bool CODES>
 __device__ __forceinline__ RawPiece<XT, CW, CODES> raw_piece(const RowSumTask& K, int64_t row, int64_t col, bool full) {
   typedef typename Elem<XT>::T T;

@@ -425,9 +425,9 @@ int row_splits(int64_t T, int64_t V, int es, int64_t piece) {
   const int64_t want = std::min<int64_t>(ceil_div(4 * int64_t(device_cus()), std::max<int64_t>(T, 1)), 64);
   return int(std::max(ceil_div(V * es, piece), std::min(want, ceil_div(V * es, int64_t(8192)))));
 }
-// Bytes of a row that a workgroup takes.  4862 rows of 256 KB forward: 237 us in pieces of
-// 128 KiB, 253 in 64, 274 in 32, 244 whole; their gradient and 3474 rows of zeros: 644 us in
-// pieces of 32 KiB, 654 in 64, 668 in 128.
+// Bytes of a row that a workgroup takes.  Replayed from a graph, 4862 rows of 256 KB forward (both
+// launches): 237 us in pieces of 128 KiB, 242 in 64, 254 in 32, 240 whole; their gradient and 3474
+// rows of zeros: 648 us in pieces of 32 KiB, 654 in 64, 669 in 128.
 constexpr int64_t kSumsPiece = 128 << 10, kGradPiece = 32 << 10;
 
 size_t up256(size_t b) { return (b + 255) & ~size_t(255); }

@@ -103,7 +103,7 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
     """base[m] + scaling[a] (x[m] A[a]^T) B[a]^T for the adapter a of every row m.
 
     x: [..., K] fp32, bf16 or fp16; lora_a [n, r, K] and lora_b [n, N, r] (rounded to
-    x's dtype when they have another); scaling: fp32 [n], or one number; base: [...,
+    x's dtype when they have another, and so are their gradients); scaling: fp32 [n], or one number; base: [...,
     N] in x's dtype (None: zeros).  Sums are fp32; x A^T is passed to the second
     product in 16 bits or more and the result rounded once (fp16: x A^T up to 65504; an
     infinity in lora_b, or in a gradient's x, may come out as NaN).  Differentiable by x,
@@ -141,7 +141,10 @@ class MultiLoRALinear(nn.Module):
     """A QuantLinear with n adapters of rank r.  lora_A [n, r, in] and lora_B [n, out,
     r] are parameters (A Kaiming-uniform, B zeros, as LoRALinear's), `scaling` [n] a
     buffer.  The rows of a batch are given to forward, or set for all layers of a
-    model by set_adapter_rows."""
+    model by set_adapter_rows.  Beside 16-bit rows the parameters of all n adapters are
+    rounded to the rows' dtype at every call, and their gradients are sums in fp32 that
+    are rounded to it; parameters of the rows' dtype save the conversion.  The quantized
+    layer's kernels are called, not its forward: hooks on base_layer do not run."""
 
     def __init__(self, quant_linear: QuantLinear, n: int, r: int = 8, lora_alpha: float = 16, activation_bits: int = 16):
         if not isinstance(quant_linear, QuantLinear):

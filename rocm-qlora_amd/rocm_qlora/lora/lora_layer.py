@@ -28,7 +28,10 @@ class LoRALinear(nn.Module):
     """Wraps a QuantLinear with LoRA adapters; merge_lora folds them into an
     fp16 copy of the weight for inference.  activation_bits = 8 holds the
     adapter's input for the backward pass as an 8-bit checkpoint
-    (rocm_qlora.checkpoint): half its memory, dA and dB at the held values."""
+    (rocm_qlora.checkpoint), dA and dB at the held values: 33/32 of a byte a
+    value instead of 2 where the input is this layer's alone.  Layers that
+    share an input share it in 16 bits and hold codes of their own in 8, which
+    is more from three layers on (q, k, v)."""
 
     activation_bits = 16
 
