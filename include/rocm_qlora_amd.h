@@ -605,7 +605,7 @@ int rq_act8_dequantize(const uint8_t* codes, const uint8_t* exponents, int64_t r
  *   (average: over their number; 0 without any).
  *   D_p = beta ((logps[p] - ref[p]) - (logps[q] - ref[q])), q = S/2 + p, ref_logps [S]
  *   or NULL (zeros); loss = mean over p of -(1 - e) log sigmoid(D_p) - e log sigmoid(-D_p),
- *   e = label_smoothing.
+ *   e = label_smoothing (a side of weight 0 is left out, also where it is infinite).
  * coef [S]: d loss / d (sum of sequence i) (without loss: d logps[i] / d sum).
  * row_info: 16 bytes a row, 16-byte aligned, for the backward pass.  workspace:
  * 256-byte aligned, contents ignored.  T >= 1. */
