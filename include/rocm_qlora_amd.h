@@ -591,6 +591,36 @@ int rq_act8_dequantize(const uint8_t* codes, const uint8_t* exponents, int64_t r
                        int out_dtype, int64_t ldo, hipStream_t stream);
 
 /* ------------------------------------------------------------------------
+ * MXFP4 weights: codec, linears, experts' linears (no counterpart in the reference)
+ * ------------------------------------------------------------------------ */
+
+/* Blocks of 32 values along a row share a power of two, each value is an e2m1 code of 0, 1/2, 1, 3/2, 2, 3, 4,
+ * 6 and a sign (the OCP MX format MXFP4): with e = floor(log2 max |x|) - 2 of the block, clamped to -127 ..
+ * 127, code = rne_e2m1(x 2^-e), magnitudes past 6 become 6.  Rows are held in whole 128 values, Kp = cols rounded
+ * up to 128: codes [rows][Kp / 2], two a byte with the even value in the low bits, 16-byte aligned, zeros past
+ * cols; scales [rows][Kp / 32] bytes e + 127; 255 for a block with an infinity or a NaN, which stands for NaN. */
+int rq_mx4_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* codes, uint8_t* scales,
+                    hipStream_t stream);
+int rq_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* out, int out_dtype,
+                      int64_t ldo, hipStream_t stream);
+
+/* y[r] = x[r / shared] W[e]^T + bias[e] for r < M, e the row's expert.
+ *   codes, scales: E weights [N, K] one after another, 16- and 4-byte aligned.  plan: rq_adapter_rows' of M rows and E
+ *   experts (rows without one are zeros in y), or NULL: one weight, shared 1.  x [M / shared, K] and y
+ *   [M, N] of `dtype`; bias [E, N] of it, or NULL.  The values of W are exact beside bf16 and fp32 rows and
+ *   rounded to fp16 beside fp16 rows; sums are fp32, the result is rounded once.
+ *   act_bits: 16, or 4: x's rows quantized as above first (one weight).
+ * rq_mx4_linear_dx: dx[t] = sum over r = t shared .. of dy[r] W[e].  scratch: 256-byte aligned, contents ignored. */
+int rq_mx4_linear_scratch_size(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, int grouped,
+                               int act_bits, int dx, int64_t* bytes);
+int rq_mx4_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int64_t shared, const void* plan,
+                  int64_t plan_bytes, const uint8_t* codes, const uint8_t* scales, int64_t E, int64_t N, const void* bias,
+                  int act_bits, void* y, int64_t ldy, void* scratch, int64_t scratch_bytes, hipStream_t stream);
+int rq_mx4_linear_dx(const void* dy, int dtype, int64_t M, int64_t N, int64_t lddy, const void* plan, int64_t plan_bytes,
+                     const uint8_t* codes, const uint8_t* scales, int64_t E, int64_t K, int64_t shared, void* dx,
+                     int64_t lddx, void* scratch, int64_t scratch_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------------
  * Preference loss (no counterpart in the reference)
  * ------------------------------------------------------------------------ */
 

@@ -1,0 +1,270 @@
+// Matrix product of two MXFP4 operands: y = xq W^T + bias, xq the rows of x quantized as a
+// weight is (mx4_codec.hip), in 4 bits all the way to gfx950's scaled matrix instructions:
+// v_mfma_scale_f32_32x32x64_f8f6f4 takes 32 codes and their scale a lane and operand, which
+// is one block, and sums in fp32.
+//
+// Tile BM x 256, 128 k a step, eight waves, two a SIMD.  Rows of 64 bytes of both operands
+// come by direct-to-LDS loads into a ring of four steps, the four scales of a row and
+// step as one dword likewise.  Lane (i, q) of part e of a step takes block 2 e + q of row i:
+// 16 bytes, chunk c of row r stored at c ^ (r / 4) % 4, so that 16 consecutive rows' reads
+// of a chunk meet no bank twice; the instruction picks byte 2 e of the row's scales,
+// shifted by q bytes.  The operands of a part are read while the part before is multiplied.
+#include "rq_mx4_gemm.h"
+
+namespace rq {
+namespace {
+
+constexpr int kA4Step = 128;
+
+template <int BM_>
+struct A4Tile {
+  static constexpr int BM = BM_;
+  static constexpr int WM = BM == 64 ? 1 : 2;
+  static constexpr int WN = 8 / WM;
+  static constexpr int MB = BM / (32 * WM);
+  static constexpr int NB = 8 / WN;
+  static constexpr int BN = 256;
+  static constexpr int kRing = 4;
+  static constexpr int kXBytes = BM * 64, kWBytes = BN * 64, kSBytes = 2048;
+  static constexpr int kWOff = kXBytes, kSOff = kXBytes + kWBytes;
+  static constexpr int kStage = kXBytes + kWBytes + kSBytes;
+  static constexpr int kOutWave = 32 * MB * mx_out_pitch(NB);
+  static constexpr int kLds = kRing * kStage > 8 * kOutWave ? kRing * kStage : 8 * kOutWave;
+  static constexpr int kXLoads = BM < 128 ? 1 : BM / 128;  // of a wave and step; BM = 64: half a wave's lanes
+  static constexpr int kLoads = kXLoads + 2 + 1;
+  static_assert(kLds <= 160 * 1024, "LDS plan");
+};
+
+struct A4Args {
+  MxGemmArgs g;           // x: codes [M][pitch], codes, scales, wrows, pitch, cols, nk, splits, tiles, bias, y
+  const uint8_t* xscales; // [M][pitch / 16]
+};
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ uint32_t swz64(uint32_t r, uint32_t c) { return r * 64u + ((c ^ ((r >> 2) & 3u)) << 4); }
+
+// One direct-to-LDS load of 4 bytes a lane from an address of its own (see dma16).
+__device__ __forceinline__ void dma4(const void* p, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds_addr) : "memory", "m0");
+}
+
+template <int XT, int BM, bool OUT32>
+__global__ __launch_bounds__(kMgThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void mx4_a4_kernel(A4Args args) {
+  using T = A4Tile<BM>;
+  constexpr int MB = T::MB, NB = T::NB, BN = T::BN;
+  const MxGemmArgs& a = args.g;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
+  lds_escapes(lds);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  const int i32 = lane & 31, q = lane >> 5;
+  int rt, ct;
+  {
+    const int G = a.row_tiles * a.col_tiles;
+    int t = blockIdx.x;
+    if (G % 8 == 0) t = (t & 7) * (G / 8) + (t >> 3);
+    constexpr int GM = 4;
+    const int per = GM * a.col_tiles, grp = t / per, r = t - grp * per;
+    const int gm = a.row_tiles - grp * GM < GM ? a.row_tiles - grp * GM : GM;
+    rt = grp * GM + r % gm;
+    ct = r / gm;
+  }
+  const int64_t m0 = int64_t(BM) * rt, c0 = int64_t(BN) * ct;
+  const int count = a.rows.M - m0 < BM ? int(a.rows.M - m0) : BM;
+  const int split = blockIdx.y;
+  const int kbeg = int(int64_t(a.nk) * split / a.splits), nk = int(int64_t(a.nk) * (split + 1) / a.splits) - kbeg;
+
+  // direct-to-LDS lanes: 16 rows an instruction; wave w brings the weight's rows 32 w .. and BM / 8 w .. of x
+  const uint8_t* xbase = a.x + m0 * a.pitch;
+  const uint8_t* wbase = a.codes + c0 * a.pitch;
+  const int wrows = a.wrows - c0 < BN ? int(a.wrows - c0) : BN;
+  uint32_t xo[T::kXLoads], wo[2];
+#pragma unroll
+  for (int i = 0; i < T::kXLoads; ++i) {
+    const int r = BM / 8 * wave + 16 * i + ((lane >> 2) & (BM == 64 ? 7 : 15));
+    xo[i] = uint32_t(r < count ? r : count - 1) * uint32_t(a.pitch) + 16u * (uint32_t(lane & 3) ^ ((r >> 2) & 3u));
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 32 * wave + 16 * i + (lane >> 2);
+    wo[i] = uint32_t(r < wrows ? r : wrows - 1) * uint32_t(a.pitch) + 16u * (uint32_t(lane & 3) ^ ((r >> 2) & 3u));
+  }
+  // scales: lanes 0 .. 31 the weight's rows, the BM / 8 lanes after them x's
+  const uint8_t* sp;
+  {
+    const int64_t srow = a.pitch / 16;
+    int r = lane < 32 ? 32 * wave + lane : BM / 8 * wave + ((lane - 32) & (BM / 8 - 1));
+    const int most = lane < 32 ? wrows : count;
+    r = r < most ? r : most - 1;
+    sp = lane < 32 ? a.scales + (c0 + r) * srow : args.xscales + (m0 + r) * srow;
+  }
+  const uint32_t xdst = __builtin_amdgcn_readfirstlane(uint32_t(BM / 8 * wave) * 64u);
+  const uint32_t wdst = __builtin_amdgcn_readfirstlane(uint32_t(wave) * 2048u);
+  const uint32_t sdst = __builtin_amdgcn_readfirstlane(uint32_t(wave) * 256u);
+  auto load = [&](int j) {
+    const int kk = kbeg + (j < nk ? j : nk - 1);  // past the end: the last step again, never used
+    const uint32_t st = uint32_t(j % T::kRing) * T::kStage;
+    const int64_t k = int64_t(kk) * 64;
+    if constexpr (BM == 64) {
+      if (lane < 32) dma16(xbase + k, xo[0], st + xdst);
+    } else {
+#pragma unroll
+      for (int i = 0; i < T::kXLoads; ++i) dma16(xbase + k, xo[i], st + xdst + 1024u * i);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) dma16(wbase + k, wo[i], st + T::kWOff + wdst + 1024u * i);
+    if (lane < 32 + BM / 8) dma4(sp + int64_t(kk) * 4, st + T::kSOff + sdst);
+  };
+
+  f32x16 acc[MB][NB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[mb][nb][r] = 0.0f;
+
+  const uint32_t xrow = uint32_t(32 * MB * wm + i32), wrow = uint32_t(32 * NB * wn + i32);
+  u32x4 xf[2][MB], wf[2][NB];
+  uint32_t xs[MB], ws[NB];
+  auto read = [&](int buf, int j, int e) {
+    const uint8_t* st = lds + uint32_t(j % T::kRing) * T::kStage;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+      wf[buf][nb] = *reinterpret_cast<const u32x4*>(st + T::kWOff + swz64(wrow + 32 * nb, uint32_t(2 * e + q)));
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+      xf[buf][mb] = *reinterpret_cast<const u32x4*>(st + swz64(xrow + 32 * mb, uint32_t(2 * e + q)));
+  };
+  auto read_s = [&](int j) {
+    const uint8_t* st = lds + uint32_t(j % T::kRing) * T::kStage + T::kSOff;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const uint32_t r = wrow + 32 * nb;
+      ws[nb] = *reinterpret_cast<const uint32_t*>(st + (r >> 5) * 256 + (r & 31) * 4) >> (8 * q);
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      const uint32_t r = xrow + 32 * mb;
+      xs[mb] = *reinterpret_cast<const uint32_t*>(st + r / (BM / 8) * 256 + 128 + r % (BM / 8) * 4) >> (8 * q);
+    }
+  };
+  auto widen = [](const u32x4& v) { return i32x8{int(v.x), int(v.y), int(v.z), int(v.w), 0, 0, 0, 0}; };
+
+  load(0);
+  load(1);
+  load(2);
+  step_barrier<2 * T::kLoads>();
+  read(0, 0, 0);
+  for (int j = 0; j < nk; ++j) {
+    step_barrier<T::kLoads>();
+    load(j + 3);
+    read_s(j);
+    read(1, j, 1);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+        acc[mb][nb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(wf[0][nb]), widen(xf[0][mb]), acc[mb][nb], 4, 4, 0,
+                                                                      int(ws[nb]), 0, int(xs[mb]));
+    read(0, j + 1, 0);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+        acc[mb][nb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(wf[1][nb]), widen(xf[1][mb]), acc[mb][nb], 4, 4, 2,
+                                                                      int(ws[nb]), 2, int(xs[mb]));
+  }
+  wait_vmcnt<0>();
+  __syncthreads();
+  mx_output<XT, false, MB, NB, OUT32>(a, acc, lds + wave * T::kOutWave, lane, 0, true, split, m0, count, 32 * MB * wm,
+                                      c0 + 32 * NB * wn);
+}
+
+struct A4Plan {
+  int bm, splits;
+  int row_tiles, col_tiles;
+  int64_t ld, codes_bytes, scales_bytes, part_bytes;
+};
+
+A4Plan a4_plan(const MxCall& c, int cus) {
+  A4Plan p{};
+  const int64_t wp = mx_pad(c.wk);
+  p.bm = c.M <= 64 ? 64 : c.M <= 128 ? 128 : 256;
+  p.col_tiles = int(ceil_div(c.N, 256));
+  while (p.bm > 128 && 2 * ceil_div(c.M, p.bm) * p.col_tiles <= cus) p.bm /= 2;
+  p.row_tiles = int(ceil_div(c.M, p.bm));
+  const int64_t steps = wp / kA4Step;
+  int64_t s = cus / (int64_t(p.row_tiles) * p.col_tiles);
+  s = s < steps / 4 ? s : steps / 4;
+  s = s < 16 ? s : 16;
+  p.splits = int(s > 1 ? s : 1);
+  p.ld = (c.N + 3) / 4 * 4;
+  p.codes_bytes = up256(c.M * wp / 2);
+  p.scales_bytes = up256(c.M * wp / kMxBlock);
+  p.part_bytes = p.splits > 1 ? up256(int64_t(p.splits) * c.M * p.ld * 4) : 0;
+  return p;
+}
+
+template <int XT, int BM>
+void a4_launch(const A4Args& a, bool out32, hipStream_t stream) {
+  const dim3 grid(unsigned(a.g.row_tiles) * unsigned(a.g.col_tiles), unsigned(a.g.splits));
+  if (out32) mx4_a4_kernel<RQ_DTYPE_BF16, BM, true><<<grid, kMgThreads, 0, stream>>>(a);
+  else mx4_a4_kernel<XT, BM, false><<<grid, kMgThreads, 0, stream>>>(a);
+}
+
+template <int XT>
+void a4_launch_bm(const A4Args& a, int bm, bool out32, hipStream_t stream) {
+  if (bm == 64) a4_launch<XT, 64>(a, out32, stream);
+  else if (bm == 128) a4_launch<XT, 128>(a, out32, stream);
+  else a4_launch<XT, 256>(a, out32, stream);
+}
+
+}  // namespace
+
+int64_t mx4_a4_scratch(const MxCall& c, int cus) {
+  const A4Plan p = a4_plan(c, cus);
+  return p.codes_bytes + p.scales_bytes + p.part_bytes;
+}
+
+int mx4_a4_run(const MxCall& c) {
+  int cus = 0, dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+    return RQ_ERR_HIP;
+  const A4Plan p = a4_plan(c, cus);
+  if (int64_t(p.row_tiles) * p.col_tiles > (int64_t(1) << 22)) return RQ_ERR_UNSUPPORTED;
+  const int64_t wp = mx_pad(c.wk);
+  uint8_t* xc = static_cast<uint8_t*>(c.scratch);
+  uint8_t* xs = xc + p.codes_bytes;
+  const int st = mx4_quantize(c.x, c.dt, c.M, c.K, c.ldx, xc, xs, c.stream);
+  if (st != RQ_OK) return st;
+  A4Args a{};
+  a.xscales = xs;
+  a.g.x = xc;
+  a.g.rows = c.rows;
+  a.g.codes = c.codes;
+  a.g.scales = c.scales;
+  a.g.wrows = a.g.cols = c.N;
+  a.g.pitch = wp / 2;
+  a.g.nk = int(wp / kA4Step);
+  a.g.splits = p.splits;
+  a.g.row_tiles = p.row_tiles;
+  a.g.col_tiles = p.col_tiles;
+  a.g.bias = c.bias;
+  a.g.bias_dt = c.dt;
+  const bool partial = p.splits > 1;
+  void* part = xs + p.scales_bytes;
+  a.g.y = partial ? part : c.y;
+  a.g.ldy = partial ? p.ld : c.ldy;
+  const bool out32 = partial || c.dt == RQ_DTYPE_F32;
+  if (c.dt == RQ_DTYPE_F16) a4_launch_bm<RQ_DTYPE_F16>(a, p.bm, out32, c.stream);
+  else a4_launch_bm<RQ_DTYPE_BF16>(a, p.bm, out32, c.stream);
+  if (partial) mx4_sum(MxSumArgs{static_cast<const float*>(part), c.M, p.ld, p.splits, 1, c.M, c.N, c.y, c.ldy}, c.dt, c.stream);
+  return rq_check_launch();
+}
+
+}  // namespace rq

@@ -1,0 +1,129 @@
+// Entry points of the linears on MXFP4 weights: argument checks and the choice of kernel.
+#include "rq_mx4.h"
+
+namespace rq {
+namespace {
+
+// Whether a forward call runs on the kernel for few rows: a weight's rows fit in its tile of 64;
+// experts: where they have 16 rows each at most on average (an expert's tile reads its weight
+// once, however few its rows).
+bool few(const MxCall& c) {
+  if (c.dx) return false;
+  if (!c.rows.p) return c.M <= kTileRows;
+  return c.M <= 16 * c.E;
+}
+
+int compute_units(int* cus) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+    return RQ_ERR_HIP;
+  return RQ_OK;
+}
+
+// Sizes, whatever the pointers.  shared: rows of the product that one row of the narrower side stands for.
+int check_sizes(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, bool grouped, int act_bits) {
+  if (!valid_float_dtype(dtype)) return RQ_ERR_BAD_DTYPE;
+  if (M < 0 || K < 1 || N < 1 || E < 1 || shared < 1 || M % shared != 0) return RQ_ERR_BAD_SHAPE;
+  if (act_bits != 16 && act_bits != 4) return RQ_ERR_UNSUPPORTED;
+  if (!grouped && (E != 1 || shared != 1)) return RQ_ERR_BAD_SHAPE;
+  if (grouped && act_bits == 4) return RQ_ERR_UNSUPPORTED;
+  // 32-bit offsets within a tile's rows and a weight's scales
+  if (E > kMaxAdapters || M > (int64_t(1) << 30) || K > (int64_t(1) << 24) || N > (int64_t(1) << 30) ||
+      mx_pad(K) * ceil_div(N, 64) > (int64_t(1) << 29))
+    return RQ_ERR_UNSUPPORTED;
+  return RQ_OK;
+}
+
+int64_t scratch_of(const MxCall& c, int cus) {
+  if (c.a4) return mx4_a4_scratch(c, cus);
+  return few(c) ? 0 : mx4_gemm_scratch(c, cus);
+}
+
+MxCall call_of(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, const void* plan, int act_bits, bool dx) {
+  MxCall c{};
+  c.dt = dtype;
+  c.M = M;
+  c.E = E;
+  c.N = N;
+  c.wk = K;
+  c.K = dx ? N : K;
+  c.ldx = c.K;
+  c.xdiv = dx ? 1 : int(shared);
+  c.ysum = dx ? int(shared) : 1;
+  c.rows = rows_plan(static_cast<const int32_t*>(plan), M, E);
+  c.a4 = act_bits == 4;
+  c.dx = dx;
+  return c;
+}
+
+int run(MxCall& c, const void* x, int64_t ldx, int64_t plan_bytes, const uint8_t* codes, const uint8_t* scales,
+        const void* bias, void* y, int64_t ldy, void* scratch, int64_t scratch_bytes, hipStream_t stream) {
+  if (ldx < c.K || ldy < (c.dx ? c.wk : c.N)) return RQ_ERR_BAD_SHAPE;
+  if (c.M == 0) return RQ_OK;
+  if (!x || !codes || !scales || !y) return RQ_ERR_NULL_POINTER;
+  if (c.rows.p && plan_bytes < 4 * c.rows.words()) return RQ_ERR_WORKSPACE;
+  const size_t es = dtype_size(c.dt);
+  if (!aligned(x, es) || !aligned(y, es) || !aligned(bias, es) || !aligned(codes, 16) || !aligned(scales, 4) ||
+      !aligned(c.rows.p, 16))
+    return RQ_ERR_BAD_ALIGNMENT;
+  int cus = 0;
+  const int st = compute_units(&cus);
+  if (st != RQ_OK) return st;
+  const int64_t need = scratch_of(c, cus);
+  if (need > 0 && !scratch) return RQ_ERR_NULL_POINTER;
+  if (scratch_bytes < need) return RQ_ERR_WORKSPACE;
+  if (need > 0 && !aligned(scratch, 256)) return RQ_ERR_BAD_ALIGNMENT;
+  c.x = x;
+  c.ldx = ldx;
+  c.codes = codes;
+  c.scales = scales;
+  c.bias = bias;
+  c.y = y;
+  c.ldy = ldy;
+  c.scratch = scratch;
+  c.stream = stream;
+  if (few(c)) return mx4_few_run(c);
+  return c.a4 ? mx4_a4_run(c) : mx4_gemm_run(c);
+}
+
+}  // namespace
+}  // namespace rq
+
+extern "C" int rq_mx4_linear_scratch_size(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, int grouped,
+                                          int act_bits, int dx, int64_t* bytes) {
+  using namespace rq;
+  if (!bytes) return RQ_ERR_NULL_POINTER;
+  int cus = 0;
+  int st = check_sizes(dtype, M, K, N, E, shared, grouped != 0, act_bits);
+  if (st != RQ_OK) return st;
+  *bytes = 0;
+  if (M == 0) return RQ_OK;
+  st = compute_units(&cus);
+  if (st != RQ_OK) return st;
+  static const int32_t some = 0;  // any non-null plan: sizes alone are asked for
+  *bytes = scratch_of(call_of(dtype, M, K, N, E, shared, grouped ? &some : nullptr, act_bits, dx != 0), cus);
+  return RQ_OK;
+}
+
+extern "C" int rq_mx4_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int64_t shared, const void* plan,
+                             int64_t plan_bytes, const uint8_t* codes, const uint8_t* scales, int64_t E, int64_t N,
+                             const void* bias, int act_bits, void* y, int64_t ldy, void* scratch, int64_t scratch_bytes,
+                             hipStream_t stream) {
+  using namespace rq;
+  const int st = check_sizes(dtype, M, K, N, E, shared, plan != nullptr, act_bits);
+  if (st != RQ_OK) return st;
+  MxCall c = call_of(dtype, M, K, N, E, shared, plan, act_bits, false);
+  return run(c, x, ldx, plan_bytes, codes, scales, bias, y, ldy, scratch, scratch_bytes, stream);
+}
+
+extern "C" int rq_mx4_linear_dx(const void* dy, int dtype, int64_t M, int64_t N, int64_t lddy, const void* plan,
+                                int64_t plan_bytes, const uint8_t* codes, const uint8_t* scales, int64_t E, int64_t K,
+                                int64_t shared, void* dx, int64_t lddx, void* scratch, int64_t scratch_bytes,
+                                hipStream_t stream) {
+  using namespace rq;
+  const int st = check_sizes(dtype, M, K, N, E, shared, plan != nullptr, 16);
+  if (st != RQ_OK) return st;
+  MxCall c = call_of(dtype, M, K, N, E, shared, plan, 16, true);
+  return run(c, dy, lddy, plan_bytes, codes, scales, nullptr, dx, lddx, scratch, scratch_bytes, stream);
+}

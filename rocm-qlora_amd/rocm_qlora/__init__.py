@@ -16,6 +16,9 @@ from rocm_qlora.quantization import (  # noqa: E402
 )
 from rocm_qlora.quantization.quant_linear import QuantLinear  # noqa: E402
 from rocm_qlora.quantization.w8a8_linear import W8A8Linear  # noqa: E402
+from rocm_qlora.quantization.mxfp4 import (  # noqa: E402
+    ExpertRows, MXFP4Experts, MXFP4Linear, MXFP4Tensor, dequantize_mxfp4, mxfp4_expert_linear, mxfp4_linear, quantize_mxfp4,
+)
 from rocm_qlora.lora.lora_layer import LoRALinear  # noqa: E402
 from rocm_qlora.model.quantize_model import quantize_model, enable_all_kernels  # noqa: E402
 from rocm_qlora.optim import PagedAdamW  # noqa: E402
@@ -43,6 +46,8 @@ def __getattr__(name):
 
 __all__ = [
     "quantize_model", "QuantLinear", "LoRALinear", "W8A8Linear", "PagedAdamW",
+    "MXFP4Tensor", "quantize_mxfp4", "dequantize_mxfp4", "mxfp4_linear", "MXFP4Linear",
+    "ExpertRows", "mxfp4_expert_linear", "MXFP4Experts",
     "RocmQLoraConfig", "RocmQLoraQuantizer",
     "fused_dequant_int8_matmul", "fused_dequant_nf4_matmul",
     "get_device_info", "is_triton_available", "enable_all_kernels",

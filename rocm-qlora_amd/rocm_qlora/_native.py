@@ -125,6 +125,15 @@ SIGNATURES = {
                             _P, _I64, _P],                   # scratch, bytes, stream
     "rq_act8_quantize": [_P, _I32, _I64, _I64, _I64, _P, _P, _P],  # x, dtype, rows, cols, ldx, codes, exponents, stream
     "rq_act8_dequantize": [_P, _P, _I64, _I64, _P, _I32, _I64, _P],  # codes, exponents, rows, cols, out, dtype, ld, stream
+    "rq_mx4_quantize": [_P, _I32, _I64, _I64, _I64, _P, _P, _P],  # x, dtype, rows, cols, ldx, codes, scales, stream
+    "rq_mx4_dequantize": [_P, _P, _I64, _I64, _P, _I32, _I64, _P],  # codes, scales, rows, cols, out, dtype, ld, stream
+    "rq_mx4_linear_scratch_size": [_I32, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _P],
+    "rq_mx4_linear": [_P, _I32, _I64, _I64, _I64, _I64,      # x, dtype, M, K, ldx, shared
+                      _P, _I64, _P, _P, _I64, _I64, _P,      # plan, bytes, codes, scales, E, N, bias
+                      _I32, _P, _I64, _P, _I64, _P],         # act bits, y, ldy, scratch, bytes, stream
+    "rq_mx4_linear_dx": [_P, _I32, _I64, _I64, _I64,         # dy, dtype, M, N, lddy
+                         _P, _I64, _P, _P, _I64, _I64, _I64,  # plan, bytes, codes, scales, E, K, shared
+                         _P, _I64, _P, _I64, _P],            # dx, lddx, scratch, bytes, stream
     "rq_preference_workspace_size": [_I32, _I64, _I64, _I64, _P],
     "rq_preference_forward": [_P, _I32, _I64, _I64, _I64, _I64, _I64,  # logits, dtype, T, V, ld, period, outer
                               _P, _P, _I64, _I64,            # labels, offsets, S, ignore index

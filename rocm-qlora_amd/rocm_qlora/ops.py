@@ -1020,3 +1020,139 @@ def preference_backward(logits: torch.Tensor, state, grad: Optional[torch.Tensor
         nat.call("rq_preference_backward", z.data_ptr(), nat.dtype_code(z.dtype), T, V, ld, period, outer, info, info + 16 * T,
                  nat.ptr(grad), int(grad is not None and grad.dim() > 0), dz.data_ptr(), V, nat.stream_handle(dev))
     return dz
+
+
+# ---- MXFP4 weights: codec, linears, experts' linears -------------------------------------
+MX4_BLOCK = 32    # values that share a scale (kMxBlock in csrc/rq_mx4.h)
+MX4_WHOLE = 128   # values that a row is held in multiples of (kMxWhole)
+
+
+def mx4_pad(K: int) -> int:
+    """Values that a row of K is held in."""
+    return -(-K // MX4_WHOLE) * MX4_WHOLE
+
+
+def mx4_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The MXFP4 codes [..., Kp / 2] and scales [..., Kp / 32] (uint8; Kp = K rounded up to 128)
+    of x's rows ([..., K] fp32/bf16/fp16)."""
+    dev = nat.require_gpu(x)
+    code = nat.dtype_code(x.dtype)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise RuntimeError(f"rows expected, got shape {tuple(x.shape)}")
+    K = x.shape[-1]
+    with on(dev):
+        x2, ldx = _rows(x, K)
+        M = x2.shape[0]
+        pitch = mx4_pad(K)
+        codes = torch.empty((*x.shape[:-1], pitch // 2), dtype=torch.uint8, device=dev)
+        scales = torch.empty((*x.shape[:-1], pitch // MX4_BLOCK), dtype=torch.uint8, device=dev)
+        nat.call("rq_mx4_quantize", x2.data_ptr(), code, M, K, ldx, codes.data_ptr(), scales.data_ptr(), nat.stream_handle(dev))
+    return codes, scales
+
+
+def _check_mx4(codes: torch.Tensor, scales: torch.Tensor, K: int) -> None:
+    pitch = mx4_pad(K)
+    if K < 1 or codes.dim() < 1 or codes.shape[-1] * 2 != pitch or scales.shape[-1:] != (pitch // MX4_BLOCK,) or \
+            codes.shape[:-1] != scales.shape[:-1]:
+        raise RuntimeError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not MXFP4 rows of {K} values: "
+                           f"{pitch // 2} and {pitch // MX4_BLOCK} bytes a row expected")
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise TypeError(f"MXFP4 codes and scales must be uint8, got {codes.dtype} and {scales.dtype}")
+    if not codes.is_contiguous() or not scales.is_contiguous():
+        raise RuntimeError("MXFP4 codes and scales must be contiguous")
+
+
+def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, K: int, dtype: torch.dtype) -> torch.Tensor:
+    """The values [..., K] that mx4_quantize's codes stand for."""
+    dev = nat.require_gpu(codes, scales)
+    code = nat.dtype_code(dtype)
+    _check_mx4(codes, scales, K)
+    with on(dev):
+        out = torch.empty((*codes.shape[:-1], K), dtype=dtype, device=dev)
+        rows = out.numel() // K
+        nat.call("rq_mx4_dequantize", codes.data_ptr(), scales.data_ptr(), rows, K, out.data_ptr(), code, K,
+                 nat.stream_handle(dev))
+    return out
+
+
+def _mx4_weight(codes: torch.Tensor, plan: Optional[torch.Tensor]) -> Tuple[int, int]:
+    """Experts and rows of a weight: [N, Kp / 2] without a plan, [E, N, Kp / 2] with one."""
+    if plan is None:
+        if codes.dim() != 2:
+            raise RuntimeError(f"a weight's codes are [N, Kp / 2], got {tuple(codes.shape)}")
+        return 1, codes.shape[0]
+    if codes.dim() != 3:
+        raise RuntimeError(f"experts' codes are [E, N, Kp / 2], got {tuple(codes.shape)}")
+    return codes.shape[0], codes.shape[1]
+
+
+def _mx4_bias(bias: Optional[torch.Tensor], dtype: torch.dtype, E: int, N: int, grouped: bool) -> Optional[torch.Tensor]:
+    if bias is None:
+        return None
+    if bias.shape != ((E, N) if grouped else (N,)):
+        raise RuntimeError(f"bias must be {(E, N) if grouped else (N,)}, got {tuple(bias.shape)}")
+    return bias.detach().to(dtype).contiguous()
+
+
+def mx4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, K: int, bias: Optional[torch.Tensor] = None, *,
+               activation_bits: int = 16, plan: Optional[torch.Tensor] = None, M: Optional[int] = None) -> torch.Tensor:
+    """y[r] = x[r / shared] W[e]^T + bias[e] on MXFP4 weights.  x: rows [R, K] fp32/bf16/fp16.
+    Without a plan codes are [N, Kp / 2] and y is [R, N]; with one (adapter_rows of M rows and E
+    experts) codes are [E, N, Kp / 2], y is [M, N], and M / R rows of it read one row of x."""
+    dev = nat.require_gpu(x, codes, scales, bias, plan)
+    code = nat.dtype_code(x.dtype)
+    _check_mx4(codes, scales, K)
+    E, N = _mx4_weight(codes, plan)
+    if x.dim() != 2 or x.shape[1] != K:
+        raise RuntimeError(f"x must be rows of {K}, got {tuple(x.shape)}")
+    if activation_bits not in (4, 16):
+        raise ValueError(f"activation_bits must be 4 or 16, got {activation_bits}")
+    R = x.shape[0]
+    M = R if plan is None or M is None else M
+    if plan is not None and activation_bits != 16:
+        raise RuntimeError("experts' rows are multiplied in 16 bits or more")
+    if M != R and (R == 0 or M % R):
+        raise RuntimeError(f"{M} rows do not share {R} rows of x evenly")
+    bias = _mx4_bias(bias, x.dtype, E, N, plan is not None)
+    with on(dev):
+        if plan is not None and plan.numel() != _bytes("rq_adapter_rows_size", dev.index, M, E):
+            raise RuntimeError(f"the rows by expert are not those of {M} rows and {E} experts")
+        y = torch.empty((M, N), dtype=x.dtype, device=dev)
+        if M == 0 or N == 0:
+            return y
+        x, ldx = _rows(x, K)
+        shared = M // R
+        scratch = _scratch("rq_mx4_linear_scratch_size", dev, code, M, K, N, E, shared, int(plan is not None), activation_bits, 0)
+        nat.call("rq_mx4_linear", x.data_ptr(), code, M, K, ldx, shared, nat.ptr(plan), plan.numel() if plan is not None else 0,
+                 codes.data_ptr(), scales.data_ptr(), E, N, nat.ptr(bias), activation_bits, y.data_ptr(), N,
+                 nat.ptr(scratch), scratch.numel() if scratch is not None else 0, nat.stream_handle(dev))
+    return y
+
+
+def mx4_linear_dx(dy: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, K: int, *, plan: Optional[torch.Tensor] = None,
+                  shared: int = 1) -> torch.Tensor:
+    """dx[t] = sum of dy[r] W[e] over the `shared` rows r of t: mx4_linear's gradient by x.
+    dy [M, N]; dx [M / shared, K] in its dtype."""
+    dev = nat.require_gpu(dy, codes, scales, plan)
+    code = nat.dtype_code(dy.dtype)
+    _check_mx4(codes, scales, K)
+    E, N = _mx4_weight(codes, plan)
+    if dy.dim() != 2 or dy.shape[1] != N:
+        raise RuntimeError(f"dY must be rows of {N}, got {tuple(dy.shape)}")
+    M = dy.shape[0]
+    if shared < 1 or M % shared:
+        raise RuntimeError(f"{M} rows are not {shared} for each row of x")
+    with on(dev):
+        if plan is not None and plan.numel() != _bytes("rq_adapter_rows_size", dev.index, M, E):
+            raise RuntimeError(f"the rows by expert are not those of {M} rows and {E} experts")
+        dx = torch.empty((M // shared, K), dtype=dy.dtype, device=dev)
+        if M == 0:
+            return dx
+        if N == 0:
+            return dx.zero_()
+        dy, lddy = _rows(dy, N)
+        scratch = _scratch("rq_mx4_linear_scratch_size", dev, code, M, K, N, E, shared, int(plan is not None), 16, 1)
+        nat.call("rq_mx4_linear_dx", dy.data_ptr(), code, M, N, lddy, nat.ptr(plan), plan.numel() if plan is not None else 0,
+                 codes.data_ptr(), scales.data_ptr(), E, K, shared, dx.data_ptr(), K,
+                 nat.ptr(scratch), scratch.numel() if scratch is not None else 0, nat.stream_handle(dev))
+    return dx
