@@ -39,6 +39,7 @@ __device__ __forceinline__ int wave_excl(int v, int& carry) {
 __global__ __launch_bounds__(kArThreads) void adapter_rows_kernel(const int32_t* ids, RowsPlan P, int32_t* plan) {
   __shared__ int hist[kArWaves][kMaxAdapters + 1];  // counts, then this wave's next place among the adapter's rows
   __shared__ int first[kMaxAdapters + 2];           // first tile of each adapter
+  __shared__ int first_big[kBigTables][kMaxAdapters + 1];
   __shared__ int total[kMaxAdapters + 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = P.n;
@@ -79,6 +80,15 @@ __global__ __launch_bounds__(kArThreads) void adapter_rows_kernel(const int32_t*
       if (a <= n) first[a] = e;
     }
     if (lane == 0) first[n + 1] = carry;
+  } else if (wave <= kBigTables) {  // likewise, their big tiles
+    int carry = 0;
+    const int tiles = big_tiles(wave - 1);
+    for (int a0 = 0; a0 <= n; a0 += 64) {
+      const int a = a0 + lane;
+      const int e = wave_excl(a <= n ? ((total[a] + kTileRows - 1) / kTileRows + tiles - 1) / tiles : 0, carry);
+      if (a <= n) first_big[wave - 1][a] = e;
+    }
+    if (lane == 0) plan[kChunkTables + wave] = carry;
   }
   __syncthreads();
   const int tiles = first[n + 1];
@@ -111,7 +121,7 @@ __global__ __launch_bounds__(kArThreads) void adapter_rows_kernel(const int32_t*
     }
     if (lane == 0) plan[1 + k] = chunks;
   }
-  if (tid < 16 && (tid == 0 || tid > kChunkTables)) plan[tid] = tid == 0 ? tiles : 0;
+  if (tid < 16 && (tid == 0 || tid > kChunkTables + kBigTables)) plan[tid] = tid == 0 ? tiles : 0;
   for (int t = tid; t < tiles; t += kArThreads) {
     int lo = 0, hi = n;  // the last adapter whose first tile is at most t
     while (lo < hi) {
@@ -122,6 +132,13 @@ __global__ __launch_bounds__(kArThreads) void adapter_rows_kernel(const int32_t*
     const int left = total[lo] - kTileRows * (t - first[lo]);
     plan[16 + 2 * t] = lo < n ? lo : -1;
     plan[16 + 2 * t + 1] = left < kTileRows ? left : kTileRows;
+    const int at = t - first[lo];
+    int64_t off = P.off_big();
+#pragma unroll
+    for (int k = 0; k < kBigTables; ++k) {
+      if (at % big_tiles(k) == 0) plan[off + first_big[k][lo] + at / big_tiles(k)] = t;
+      off += P.bigs(k);
+    }
   }
   for (int a = wave; a <= n; a += kArWaves) {  // the slots after the last row of an adapter
     const int left = total[a] % kTileRows;

@@ -10,6 +10,7 @@
 // of a chunk meet no bank twice; the instruction picks byte 2 e of the row's scales,
 // shifted by q bytes.  The operands of a part are read while the part before is multiplied.
 #include "rq_mx4_gemm.h"
+#include <stdlib.h>
 
 namespace rq {
 namespace {
@@ -28,7 +29,7 @@ struct A4Tile {
   static constexpr int kXBytes = BM * 64, kWBytes = BN * 64, kSBytes = 2048;
   static constexpr int kWOff = kXBytes, kSOff = kXBytes + kWBytes;
   static constexpr int kStage = kXBytes + kWBytes + kSBytes;
-  static constexpr int kOutWave = 32 * MB * mx_out_pitch(NB);
+  static constexpr int kOutWave = mx_out_wave(MB, NB);
   static constexpr int kLds = kRing * kStage > 8 * kOutWave ? kRing * kStage : 8 * kOutWave;
   static constexpr int kXLoads = BM < 128 ? 1 : BM / 128;  // of a wave and step; BM = 64: half a wave's lanes
   static constexpr int kLoads = kXLoads + 2 + 1;
@@ -47,6 +48,13 @@ __device__ __forceinline__ uint32_t swz64(uint32_t r, uint32_t c) { return r * 6
 // One direct-to-LDS load of 4 bytes a lane from an address of its own (see dma16).
 __device__ __forceinline__ void dma4(const void* p, uint32_t lds_addr) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds_addr) : "memory", "m0");
+}
+
+// A wave-uniform value in scalar registers (the compiler may keep one that a masked load uses in vector registers).
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  return reinterpret_cast<const uint8_t*>(uint64_t(uniform(uint32_t(v >> 32))) << 32 | uniform(uint32_t(v)));
 }
 
 template <int XT, int BM, bool OUT32>
@@ -104,19 +112,27 @@ void mx4_a4_kernel(A4Args args) {
   const uint32_t xdst = __builtin_amdgcn_readfirstlane(uint32_t(BM / 8 * wave) * 64u);
   const uint32_t wdst = __builtin_amdgcn_readfirstlane(uint32_t(wave) * 2048u);
   const uint32_t sdst = __builtin_amdgcn_readfirstlane(uint32_t(wave) * 256u);
-  auto load = [&](int j) {
-    const int kk = kbeg + (j < nk ? j : nk - 1);  // past the end: the last step again, never used
+  auto step_at = [&](int j) { return kbeg + (j < nk ? j : nk - 1); };  // past the end: the last step again, never used
+  auto load_x = [&](int j) {
     const uint32_t st = uint32_t(j % T::kRing) * T::kStage;
-    const int64_t k = int64_t(kk) * 64;
+    const int64_t k = int64_t(step_at(j)) * 64;
     if constexpr (BM == 64) {
-      if (lane < 32) dma16(xbase + k, xo[0], st + xdst);
+      const uint8_t* p = uniform(xbase + k);
+      const uint32_t to = uniform(st + xdst);
+      if (lane < 32) dma16(p, xo[0], to);
     } else {
 #pragma unroll
-      for (int i = 0; i < T::kXLoads; ++i) dma16(xbase + k, xo[i], st + xdst + 1024u * i);
+      for (int i = 0; i < T::kXLoads; ++i) dma16(uniform(xbase + k), xo[i], uniform(st + xdst + 1024u * i));
     }
+  };
+  auto load_w = [&](int j) {
+    const uint32_t st = uint32_t(j % T::kRing) * T::kStage;
+    const int kk = step_at(j);
+    const int64_t k = int64_t(kk) * 64;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) dma16(wbase + k, wo[i], st + T::kWOff + wdst + 1024u * i);
-    if (lane < 32 + BM / 8) dma4(sp + int64_t(kk) * 4, st + T::kSOff + sdst);
+    for (int i = 0; i < 2; ++i) dma16(uniform(wbase + k), wo[i], uniform(st + T::kWOff + wdst + 1024u * i));
+    const uint32_t to = uniform(st + T::kSOff + sdst);
+    if (lane < 32 + BM / 8) dma4(sp + int64_t(kk) * 4, to);
   };
 
   f32x16 acc[MB][NB];
@@ -154,30 +170,37 @@ void mx4_a4_kernel(A4Args args) {
   };
   auto widen = [](const u32x4& v) { return i32x8{int(v.x), int(v.y), int(v.z), int(v.w), 0, 0, 0, 0}; };
 
-  load(0);
-  load(1);
-  load(2);
+#define RQ_A4_PRODUCTS(BUF, N0, N1, BYTE)                                                                                      \
+  _Pragma("unroll") for (int nb = N0; nb < N1; ++nb)                                                                           \
+  _Pragma("unroll") for (int mb = 0; mb < MB; ++mb)                                                                            \
+    acc[mb][nb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(wf[BUF][nb]), widen(xf[BUF][mb]), acc[mb][nb], 4, 4,   \
+                                                                  BYTE, int(ws[nb]), BYTE, int(xs[mb]))
+  load_x(0), load_w(0);
+  load_x(1), load_w(1);
+  load_x(2), load_w(2);
   step_barrier<2 * T::kLoads>();
   read(0, 0, 0);
+  read_s(0);
   for (int j = 0; j < nk; ++j) {
+    // the loads of step j + 3 are issued between products (together after the barrier they kept all waves
+    // from their first product while the addresses went out)
     step_barrier<T::kLoads>();
-    load(j + 3);
-    read_s(j);
     read(1, j, 1);
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-        acc[mb][nb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(wf[0][nb]), widen(xf[0][mb]), acc[mb][nb], 4, 4, 0,
-                                                                      int(ws[nb]), 0, int(xs[mb]));
+    __builtin_amdgcn_sched_barrier(0);
+    RQ_A4_PRODUCTS(0, 0, 1, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_x(j + 3);
+    __builtin_amdgcn_sched_barrier(0);
+    RQ_A4_PRODUCTS(0, 1, NB, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_w(j + 3);
     read(0, j + 1, 0);
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-        acc[mb][nb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(wf[1][nb]), widen(xf[1][mb]), acc[mb][nb], 4, 4, 2,
-                                                                      int(ws[nb]), 2, int(xs[mb]));
+    __builtin_amdgcn_sched_barrier(0);
+    RQ_A4_PRODUCTS(1, 0, NB, 2);
+    __builtin_amdgcn_sched_barrier(0);
+    read_s(j + 1);
   }
+#undef RQ_A4_PRODUCTS
   wait_vmcnt<0>();
   __syncthreads();
   mx_output<XT, false, MB, NB, OUT32>(a, acc, lds + wave * T::kOutWave, lane, 0, true, split, m0, count, 32 * MB * wm,
@@ -196,11 +219,13 @@ A4Plan a4_plan(const MxCall& c, int cus) {
   p.bm = c.M <= 64 ? 64 : c.M <= 128 ? 128 : 256;
   p.col_tiles = int(ceil_div(c.N, 256));
   while (p.bm > 128 && 2 * ceil_div(c.M, p.bm) * p.col_tiles <= cus) p.bm /= 2;
+  if (getenv("BM")) p.bm = atoi(getenv("BM"));
   p.row_tiles = int(ceil_div(c.M, p.bm));
   const int64_t steps = wp / kA4Step;
   int64_t s = cus / (int64_t(p.row_tiles) * p.col_tiles);
   s = s < steps / 4 ? s : steps / 4;
   s = s < 16 ? s : 16;
+  if (getenv("SP")) s = atoi(getenv("SP"));
   p.splits = int(s > 1 ? s : 1);
   p.ld = (c.N + 3) / 4 * 4;
   p.codes_bytes = up256(c.M * wp / 2);

@@ -1,34 +1,34 @@
 // Few rows beside an MXFP4 weight (decoding): y = x W^T + bias, rows grouped by expert
 // or all of one weight.
 //
-// A workgroup takes 16 rows of the weight and a tile of at most 64 rows of x (rq_rows.h),
-// its eight waves every eighth step of 128 k.  Lane (i, g) = (l % 16, l / 16) holds block
-// g of the step of weight row n0 + i: 16 bytes of codes, one scale, 32 values, which are
-// four operands of v_mfma_f32_16x16x32 (the k order within a step is free as long as both
-// operands have the same: operand s is values 8 s .. of each block).  x comes straight
-// from memory in that order.  A weight is read and decoded once for all 64 rows.  The waves'
-// sums meet in LDS and are added in wave order, 16 rows of x to a wave.
+// A workgroup takes 16 NB rows of the weight and a tile of at most 64 rows of x (rq_rows.h),
+// its eight waves chunks of four steps of 128 k in turn.  Lane (i, g) = (l % 16, l / 16)
+// loads block g of a step of weight row i, 16 bytes; the 4 x 4 dwords of four lane groups
+// are turned by four lane swaps, so that operand s of v_mfma_f32_16x16x32 is k = 32 s +
+// 8 g .. and a wave reads x in whole 64-byte pieces of its rows (in the order of the
+// blocks each 16-byte piece was a line of its own: 16 rows beside 14336 x 4096 took
+// 26 us).  A chunk's loads, x's among them, are issued before its first product; a weight
+// is read and decoded once for all 64 rows.  The waves' sums meet in LDS and are added in
+// wave order, 16 rows of x to a wave.
 //
 // fp32 rows: x = hi + mid + lo in bf16 (exact, rq_mx4.h), three products a value, all
 // into the same fp32 sum.  Activations in 4 bits: x's codes and scales instead of values,
 // one v_mfma_scale_f32_16x16x128_f8f6f4 a step, nothing decoded.
 #include "rq_mx4.h"
+#include <stdlib.h>
 
 namespace rq {
 namespace {
 
 constexpr int kFwWaves = 8;
 constexpr int kFwThreads = 64 * kFwWaves;
-constexpr int kFwCols = 16;   // weight rows of a workgroup
-constexpr int kFwDepth = 4;   // steps of a wave in flight
 
 struct FewArgs {
-  const void* x;
+  const void* x;           // rows 16-byte aligned, within 32-bit offsets
   const uint8_t* xscales;  // 4 bits: [rows][wp / 32]
   int64_t ldx;             // elements (4 bits: bytes)
-  int64_t K, wp;           // x's columns, the weight's padded ones
+  int64_t wp;              // columns of x and of the weight, whole steps
   int xdiv;
-  bool vec;                // rows of x are 16-byte aligned and whole steps
   RowsPlan rows;
   const uint8_t* codes;
   const uint8_t* scales;
@@ -40,150 +40,309 @@ struct FewArgs {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// XT: x's and y's dtype.  A4: activations in 4 bits.  CH: chunks of 16 rows, at most.
-template <int XT, bool A4, int CH>
-__global__ __launch_bounds__(kFwThreads) void mx4_few_kernel(FewArgs a) {
+// dword d of lane group g <-> dword g of lane group d
+__device__ __forceinline__ void turn4(u32x4& v) {
+  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+  u2 p = __builtin_amdgcn_permlane32_swap(v.x, v.z, false, false);
+  u2 r = __builtin_amdgcn_permlane32_swap(v.y, v.w, false, false);
+  u2 a = __builtin_amdgcn_permlane16_swap(p.x, r.x, false, false);
+  u2 b = __builtin_amdgcn_permlane16_swap(p.y, r.y, false, false);
+  v = u32x4{a.x, a.y, b.x, b.y};
+}
+
+// Steps of a batch, as registers allow.  One chunk of rows: a wave's whole share of a contraction of 4096
+// or, for 16 columns, 8192 is asked for at once (each batch waits for memory: 1.5 to 2 us).  More
+// chunks: two batches are in flight.
+constexpr int few_depth(bool a4, bool f32, int ch, int nb, bool deep) {
+  int d = ch == 1 ? (deep ? 8 : 4) : nb == 1 ? (a4 ? 4 : 2) : nb == 2 ? 2 : 1;
+  return f32 && d > 1 ? d / 2 : d;
+}
+
+// XT: x's and y's dtype.  A4: activations in 4 bits.  CH: chunks of 16 rows of x in one pass.
+// DEEP: longer batches (one chunk of rows, NB = 1).
+template <int XT, bool A4, int CH, int NB, bool DEEP>
+__global__ __launch_bounds__(kFwThreads) __attribute__((amdgpu_waves_per_eu(2)))
+void mx4_few_kernel(FewArgs a) {
+  typedef typename Elem<XT>::T T;
+  constexpr int ES = int(sizeof(T));
   constexpr int OT = XT == RQ_DTYPE_F16 ? RQ_DTYPE_F16 : RQ_DTYPE_BF16;  // operand type
-  __shared__ f32x4 red[kFwWaves][CH][64];
+  constexpr int V = Elem<XT>::kVec, P = A4 ? 1 : 8 / V;  // pieces of 16 bytes of an operand
+  constexpr int D = few_depth(A4, XT == RQ_DTYPE_F32, CH, NB, DEEP);
+  constexpr int kX = A4 ? 1 : 4 * P;  // 16-byte pieces of x of a lane and step
+  __shared__ f32x4 red[kFwWaves][CH][NB][64];
   const Tile tile = plan_tile(a.rows, blockIdx.y);
   if (tile.count == 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
   const int i = lane & 15, g = lane >> 4;
-  const int64_t n0 = int64_t(blockIdx.x) * kFwCols;
-  const int expert = tile.adapter < 0 ? 0 : tile.adapter;
+  const int64_t n0 = int64_t(blockIdx.x) * (16 * NB);
+  const int64_t expert = __builtin_amdgcn_readfirstlane(tile.adapter < 0 ? 0 : tile.adapter);
   const int64_t slot0 = int64_t(kTileRows) * blockIdx.y;
+  const int steps = __builtin_amdgcn_readfirstlane(tile.adapter < 0 ? 0 : int(a.wp / kMxWhole));
 
-  // this lane's row of x in each chunk (a live row where there is none: its result is not stored)
-  int row[CH];
-  const uint8_t* xp[CH];
-  const uint8_t* xs[CH];
+  // Loads go by buffers without a branch around them: a lane without a row, a row past the last and a step
+  // past the last read zeros at an offset out of bounds, and the waits count what is in flight.
+  const int64_t left = a.N - n0 < 16 * NB ? a.N - n0 : 16 * NB;
+  const uint32_t pitch = uint32_t(a.wp / 2), spitch = uint32_t(a.wp / kMxBlock);
+  const __amdgpu_buffer_rsrc_t wr = buffer_rsrc(a.codes + (expert * a.N + n0) * pitch, uint32_t(left) * pitch);
+  const __amdgpu_buffer_rsrc_t sr = buffer_rsrc(a.scales + (expert * a.N + n0) * spitch, uint32_t(left) * spitch);
+  const __amdgpu_buffer_rsrc_t xr = buffer_rsrc(a.x, kMxFewBytes), xsr = buffer_rsrc(A4 ? a.xscales : a.scales, kMxFewBytes);
+  // a wave's steps: two adjacent ones of every sixteen
+  const int batches = (2 * ((steps + 15) / 16) + D - 1) / D;
+  auto step_of = [&](int b, int d) { return 16 * ((b * D + d) / 2) + 2 * wave + ((b * D + d) & 1); };
+  struct W {
+    u32x4 c[D][NB];
+    uint32_t s[D][NB];
+  };
+  auto load_w = [&](W& w, int b) {
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const int at = 16 * c + i;
-    row[c] = at < tile.count ? plan_row(a.rows, slot0 + at) : -1;
-    const int64_t r = (row[c] < 0 ? plan_row(a.rows, slot0) : row[c]) / a.xdiv;
-    if constexpr (A4) {
-      xp[c] = static_cast<const uint8_t*>(a.x) + r * a.ldx + 16 * g;
-      xs[c] = a.xscales + r * (a.wp / kMxBlock) + g;
-    } else {
-      xp[c] = static_cast<const uint8_t*>(a.x) + r * a.ldx * int64_t(sizeof(typename Elem<XT>::T));
-    }
-  }
-  f32x4 acc[CH];
+    for (int d = 0; d < D; ++d) {
+      const int st = step_of(b, d);
+      const uint32_t off = uint32_t(i) * pitch + 16u * g + 64u * uint32_t(st);
+      const uint32_t soff = uint32_t(i) * spitch + 4u * uint32_t(st) + (A4 ? g : 0);
 #pragma unroll
-  for (int c = 0; c < CH; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  const int steps = tile.adapter < 0 ? 0 : int(a.wp / kMxWhole);
-  const int64_t n = n0 + i < a.N ? n0 + i : a.N - 1;  // past the last: a live row again, not stored
-  const uint8_t* wc = a.codes + (int64_t(expert) * a.N + n) * (a.wp / 2) + 16 * g;
-  const uint8_t* ws = a.scales + (int64_t(expert) * a.N + n) * (a.wp / kMxBlock) + g;
-  for (int s0 = wave; s0 < steps; s0 += kFwWaves * kFwDepth) {
-    u32x4 w[kFwDepth];
-    uint32_t sc[kFwDepth];
-#pragma unroll
-    for (int d = 0; d < kFwDepth; ++d) {
-      const int st = s0 + kFwWaves * d < steps ? s0 + kFwWaves * d : s0;
-      w[d] = *reinterpret_cast<const u32x4*>(wc + int64_t(st) * 64);
-      sc[d] = ws[int64_t(st) * 4];
-    }
-#pragma unroll
-    for (int d = 0; d < kFwDepth; ++d) {
-      const int st = s0 + kFwWaves * d;
-      if (st >= steps) break;
-      if constexpr (A4) {
-        const i32x8 wa = {int(w[d].x), int(w[d].y), int(w[d].z), int(w[d].w), 0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          if (16 * c >= tile.count) break;
-          const u32x4 v = *reinterpret_cast<const u32x4*>(xp[c] + int64_t(st) * 64);
-          const i32x8 xa = {int(v.x), int(v.y), int(v.z), int(v.w), 0, 0, 0, 0};
-          acc[c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xa, acc[c], 4, 4, 0, int(sc[d]), 0,
-                                                                    int(xs[c][int64_t(st) * 4]));
-        }
-      } else {
-        const float scale = mx_scale(sc[d]);
-        u32x4 wv[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) wv[s] = mx_decode8<OT>(w[d][s], scale);
-        const int64_t k = int64_t(st) * kMxWhole + 32 * g;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          if (16 * c >= tile.count) break;
-          const typename Elem<XT>::T* p = reinterpret_cast<const typename Elem<XT>::T*>(xp[c]) + k;
-#pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            constexpr int V = Elem<XT>::kVec, P = 8 / V;
-            u32x4 v[P];
-#pragma unroll
-            for (int j = 0; j < P; ++j) {
-              const int64_t left = a.K - k - 8 * s - V * j;
-              if (a.vec) v[j] = *reinterpret_cast<const u32x4*>(p + 8 * s + V * j);
-              else v[j] = left > 0 ? load16_part<XT>(p + 8 * s + V * j, left) : u32x4{0u, 0u, 0u, 0u};
-            }
-            if constexpr (XT == RQ_DTYPE_F32) {
-              u32x4 h, m, l;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const Split3 e = mx_split(u2f(v[j >> 1][2 * (j & 1)])), o = mx_split(u2f(v[j >> 1][2 * (j & 1) + 1]));
-                h[j] = e.hi >> 16 | o.hi;
-                m[j] = e.mid >> 16 | o.mid;
-                l[j] = e.lo >> 16 | o.lo;
-              }
-              acc[c] = mfma16x16x32<OT>(wv[s], l, acc[c]);
-              acc[c] = mfma16x16x32<OT>(wv[s], m, acc[c]);
-              acc[c] = mfma16x16x32<OT>(wv[s], h, acc[c]);
-            } else {
-              acc[c] = mfma16x16x32<OT>(wv[s], v[0], acc[c]);
-            }
-          }
+      for (int nb = 0; nb < NB; ++nb) {
+        w.c[d][nb] = buf_load16(wr, st < steps ? off + 16u * nb * pitch : kOobOffset);
+        const uint32_t at = st < steps ? soff + 16u * nb * spitch : kOobOffset;
+        if constexpr (A4) {
+          w.s[d][nb] = __builtin_amdgcn_raw_buffer_load_b8(sr, at, 0, 0);
+        } else if constexpr (D == 1) {
+          w.s[d][nb] = buf_load4(sr, at);
+        } else if (d % 2 == 0) {  // two steps' (a 4-byte load of 16 rows costs as much as a 16-byte one)
+          const u32x2 two = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(sr, at, 0, 0));
+          w.s[d][nb] = two.x;
+          w.s[d + 1][nb] = st + 1 < steps ? two.y : 0u;  // (not another row's: 255 times a code of zero is a NaN)
         }
       }
     }
+  };
+  uint32_t bias[NB][4];  // as loaded; without one zeros
+  {
+    const bool on = a.bias && tile.adapter >= 0;
+    const __amdgpu_buffer_rsrc_t br =
+        buffer_rsrc(static_cast<const uint8_t*>(a.bias) + (on ? (expert * a.N + n0) * ES : 0), on ? uint32_t(left) * ES : 0u);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t off = uint32_t(ES) * (16 * nb + 4 * g + r);
+        if constexpr (XT == RQ_DTYPE_F32) bias[nb][r] = buf_load4(br, off);
+        else bias[nb][r] = buf_load2(br, off);
+      }
   }
+
+  // 16 CH rows of the tile at a time (one pass, but for an expert with more than its share)
+  for (int at0 = 0; at0 < tile.count; at0 += 16 * CH) {
+    int row[CH];       // this lane's row of x in each chunk
+    uint32_t xo[CH];   // its offset
+    uint32_t xso[CH];
 #pragma unroll
-  for (int c = 0; c < CH; ++c) red[wave][c][lane] = acc[c];
-  __syncthreads();
-  // wave c: chunk c; lane (i, g): row of x i, columns n0 + 4 g .. + 3
-#pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    if (c != wave || row[c] < 0) continue;
-    f32x4 sum = red[0][c][lane];
-#pragma unroll
-    for (int w = 1; w < kFwWaves; ++w)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) sum[r] = __fadd_rn(sum[r], red[w][c][lane][r]);
-    typename Elem<XT>::T* yp = static_cast<typename Elem<XT>::T*>(a.y) + int64_t(row[c]) * a.ldy;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t no = n0 + 4 * g + r;
-      if (no >= a.N) break;
-      float v = sum[r];
-      if (a.bias && tile.adapter >= 0) v = __fadd_rn(v, load_as_f32(a.bias, int64_t(expert) * a.N + no, XT));
-      yp[no] = from_f32<XT>(v);
+    for (int c = 0; c < CH; ++c) {
+      const int at = at0 + 16 * c + i;
+      row[c] = at < tile.count ? plan_row(a.rows, slot0 + at) : -1;
+      const uint32_t r = uint32_t(row[c] < 0 ? 0 : row[c]) / uint32_t(a.xdiv);
+      xo[c] = r * uint32_t(a.ldx * (A4 ? 1 : ES)) + (A4 ? 16u * g : uint32_t(8 * ES) * g);
+      xso[c] = A4 ? r * spitch + g : 0u;
     }
+    struct X {
+      u32x4 v[D][kX];
+      uint32_t s[D];
+    };
+    // operand s of step d in pieces P s ..; past a row's end zeros
+    auto load_x = [&](X& x, int b, int c) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        const int st = step_of(b, d);
+        const bool on = row[c] >= 0 && st < steps;
+        if constexpr (A4) {
+          x.v[d][0] = buf_load16(xr, on ? xo[c] + 64u * uint32_t(st) : kOobOffset);
+          x.s[d] = __builtin_amdgcn_raw_buffer_load_b8(xsr, on ? xso[c] + 4u * uint32_t(st) : kOobOffset, 0, 0);
+        } else {
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+              x.v[d][P * s + j] = buf_load16(xr, on ? xo[c] + uint32_t(ES) * (128u * uint32_t(st) + 32u * s + V * j) : kOobOffset);
+            }
+        }
+      }
+    };
+    f32x4 acc[CH][NB];
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) acc[c][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto products = [&](int c, const u32x4 (&wv)[NB][A4 ? 1 : 4], const uint32_t (&wsc)[NB], const u32x4 (&x)[kX], uint32_t xsc) {
+      if constexpr (A4) {
+        const i32x8 xa = {int(x[0].x), int(x[0].y), int(x[0].z), int(x[0].w), 0, 0, 0, 0};
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const u32x4& v = wv[nb][0];
+          const i32x8 wa = {int(v.x), int(v.y), int(v.z), int(v.w), 0, 0, 0, 0};
+          acc[c][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xa, acc[c][nb], 4, 4, 0, int(wsc[nb]), 0, int(xsc));
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          if constexpr (XT == RQ_DTYPE_F32) {
+            u32x4 h, m, l;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const u32x4& v = x[2 * s + (j >> 1)];
+              const Split3 e = mx_split(u2f(v[2 * (j & 1)])), o = mx_split(u2f(v[2 * (j & 1) + 1]));
+              h[j] = e.hi >> 16 | o.hi;
+              m[j] = e.mid >> 16 | o.mid;
+              l[j] = e.lo >> 16 | o.lo;
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              acc[c][nb] = mfma16x16x32<OT>(wv[nb][s], l, acc[c][nb]);
+              acc[c][nb] = mfma16x16x32<OT>(wv[nb][s], m, acc[c][nb]);
+              acc[c][nb] = mfma16x16x32<OT>(wv[nb][s], h, acc[c][nb]);
+            }
+          } else {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) acc[c][nb] = mfma16x16x32<OT>(wv[nb][s], x[s], acc[c][nb]);
+          }
+        }
+      }
+    };
+    auto decode = [&](W& w, int d, u32x4 (&wv)[NB][A4 ? 1 : 4]) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        if constexpr (A4) {
+          wv[nb][0] = w.c[d][nb];
+        } else {
+          turn4(w.c[d][nb]);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) wv[nb][s] = mx_decode8<OT>(w.c[d][nb][s], mx_scale(w.s[d][nb] >> (8 * s) & 255u));
+        }
+      }
+    };
+
+    if constexpr (CH == 1) {
+      for (int b = 0; b < batches; ++b) {
+        W w;
+        X x;
+        load_w(w, b);
+        load_x(x, b, 0);
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+          u32x4 wv[NB][A4 ? 1 : 4];
+          decode(w, d, wv);
+          products(0, wv, w.s[d], x.v[d], x.s[d]);
+        }
+      }
+    } else {
+      W wb[2];
+      X xb[2];
+      // a batch: the next one's weight and the next chunk's rows (or the next batch's) are asked for, then
+      // this one's are multiplied
+      auto batch = [&](int b, W& w, W& next) {
+        load_w(next, b + 1);
+        u32x4 wv[D][NB][A4 ? 1 : 4];  // for all chunks
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          if (c + 1 < CH) load_x(xb[(c + 1) & 1], b, c + 1);
+          else load_x(xb[0], b + 1, 0);
+#pragma unroll
+          for (int d = 0; d < D; ++d) {
+            if (c == 0) decode(w, d, wv[d]);
+            products(c, wv[d], w.s[d], xb[c & 1].v[d], xb[c & 1].s[d]);
+          }
+        }
+      };
+      load_w(wb[0], 0);
+      load_x(xb[0], 0, 0);
+      for (int b = 0; b < batches; b += 2) {  // (an odd count's last one multiplies zeros)
+        batch(b, wb[0], wb[1]);
+        batch(b + 1, wb[1], wb[0]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) red[wave][c][nb][lane] = acc[c][nb];
+    __syncthreads();
+    // chunk c and block nb to wave (c + CH nb) % 8; lane (i, g): row of x i, columns 4 g .. + 3
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        if ((c + CH * nb) % kFwWaves != wave || row[c] < 0) continue;
+        f32x4 sum = red[0][c][nb][lane];
+#pragma unroll
+        for (int w = 1; w < kFwWaves; ++w) {
+          const f32x4 v = red[w][c][nb][lane];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum[r] = __fadd_rn(sum[r], v[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (XT == RQ_DTYPE_F32) sum[r] = __fadd_rn(sum[r], u2f(bias[nb][r]));
+          else sum[r] = __fadd_rn(sum[r], from_x16<XT>(bias[nb][r]));
+        }
+        const int64_t no = n0 + 16 * nb + 4 * g;
+        T* yp = static_cast<T*>(a.y) + int64_t(row[c]) * a.ldy + no;
+        if (no + 4 <= a.N) {
+          if constexpr (XT == RQ_DTYPE_F32) store16_any(yp, u32x4{f2u(sum[0]), f2u(sum[1]), f2u(sum[2]), f2u(sum[3])});
+          else *reinterpret_cast<u32x2_any*>(yp) = u32x2_any{cvt_pk<XT>(sum[0], sum[1]), cvt_pk<XT>(sum[2], sum[3])};
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (no + r < a.N) yp[r] = from_f32<XT>(sum[r]);
+        }
+      }
+    __syncthreads();
   }
+}
+
+template <int XT, bool A4, int CH, int NB>
+void few_launch(const FewArgs& a, hipStream_t stream) {
+  const dim3 grid(unsigned(ceil_div(a.N, 16 * NB)), unsigned(a.rows.T));
+  if (CH == 1 && NB == 1 && a.wp > 4096) mx4_few_kernel<XT, A4, CH, NB, CH == 1 && NB == 1><<<grid, kFwThreads, 0, stream>>>(a);
+  else mx4_few_kernel<XT, A4, CH, NB, false><<<grid, kFwThreads, 0, stream>>>(a);
+}
+
+template <int XT, bool A4, int CH>
+void few_launch(const FewArgs& a, int nb, hipStream_t stream) {
+  if (nb == 1) few_launch<XT, A4, CH, 1>(a, stream);
+  else if (nb == 2) few_launch<XT, A4, CH, 2>(a, stream);
+  else few_launch<XT, A4, CH, 4>(a, stream);
 }
 
 template <int XT, bool A4>
 int few_launch(const FewArgs& a, int most, hipStream_t stream) {
-  const dim3 grid(unsigned(ceil_div(a.N, kFwCols)), unsigned(a.rows.T));
-  if (most <= 16) mx4_few_kernel<XT, A4, 1><<<grid, kFwThreads, 0, stream>>>(a);
-  else if (most <= 32) mx4_few_kernel<XT, A4, 2><<<grid, kFwThreads, 0, stream>>>(a);
-  else mx4_few_kernel<XT, A4, 4><<<grid, kFwThreads, 0, stream>>>(a);
+  // blocks of a workgroup: as many as still leave a workgroup or so for each compute unit (14336 columns beside
+  // 16 rows: 25, 18 and 16 us with 1, 2 and 4; 4096 columns: 9, 11 and 14)
+  const int64_t blocks = ceil_div(a.N, 16) * a.rows.T;
+  int nb = blocks > 768 ? 4 : blocks > 384 ? 2 : 1;
+  if (getenv("NB")) nb = atoi(getenv("NB"));
+  if (most <= 16) few_launch<XT, A4, 1>(a, nb, stream);
+  else if (!A4 || most <= 32) few_launch<XT, A4, 2>(a, nb, stream);
+  else few_launch<XT, A4, A4 ? 4 : 2>(a, nb, stream);
   return rq_check_launch();
 }
 
 }  // namespace
 
+// Codes of x, or a copy of rows that the kernel does not read as they are.
+static bool few_copies(const MxCall& c) {
+  return !c.aligned16 || c.K != mx_pad(c.wk) || ceil_div(c.M, c.xdiv) * c.ldx * int64_t(dtype_size(c.dt)) > int64_t(kMxFewBytes);
+}
+
+int64_t mx4_few_scratch(const MxCall& c) {
+  const int64_t rows = ceil_div(c.M, c.xdiv), wp = mx_pad(c.wk);
+  if (c.a4) return up256(rows * wp / 2) + up256(rows * wp / kMxBlock);
+  return few_copies(c) ? up256(rows * wp * int64_t(dtype_size(c.dt))) : 0;
+}
+
 int mx4_few_run(const MxCall& c) {
   FewArgs a{};
-  const int es = int(dtype_size(c.dt));
+  const int64_t rows = ceil_div(c.M, c.xdiv);
   a.x = c.x;
   a.ldx = c.ldx;
-  a.K = c.K;
   a.wp = mx_pad(c.wk);
   a.xdiv = c.xdiv;
-  a.vec = c.K == a.wp && aligned(c.x, 16) && c.ldx * es % 16 == 0;
   a.rows = c.rows;
   a.codes = c.codes;
   a.scales = c.scales;
@@ -193,15 +352,19 @@ int mx4_few_run(const MxCall& c) {
   a.ldy = c.ldy;
   const int most = int(c.M < kTileRows ? c.M : kTileRows);
   if (c.a4) {
-    const int64_t rows = ceil_div(c.M, c.xdiv);
     uint8_t* xc = static_cast<uint8_t*>(c.scratch);
-    uint8_t* xs = xc + rows * (a.wp / 2);
+    uint8_t* xs = xc + up256(rows * a.wp / 2);
     const int st = mx4_quantize(c.x, c.dt, rows, c.K, c.ldx, xc, xs, c.stream);
     if (st != RQ_OK) return st;
     a.x = xc;
     a.ldx = a.wp / 2;
     a.xscales = xs;
     RQ_DISPATCH_DT(c.dt, XT, return few_launch<XT, true>(a, most, c.stream));
+  }
+  if (few_copies(c)) {
+    mx4_rows_whole(c.x, c.dt, rows, c.K, c.ldx, c.scratch, a.wp, c.stream);
+    a.x = c.scratch;
+    a.ldx = a.wp;
   }
   RQ_DISPATCH_DT(c.dt, XT, return few_launch<XT, false>(a, most, c.stream));
   return RQ_OK;

@@ -28,6 +28,7 @@
 // columns 4 i + b, so that the four blocks' results of a lane are four adjacent outputs.  The
 // scales, transposed and as bf16 once a call (1 / 16 of the codes), come by the same ring.
 #include "rq_mx4_gemm.h"
+#include <stdlib.h>
 
 namespace rq {
 namespace {
@@ -49,7 +50,7 @@ struct MgTile {
   static constexpr int kWOff = kXRing * kXBytes;
   static constexpr int kSOff = kWOff + kWRing * kWBytes;
   static constexpr int kRing = kSOff + kWRing * kSBytes;
-  static constexpr int kOutWave = 32 * MB * mx_out_pitch(NB);   // a wave's staged outputs
+  static constexpr int kOutWave = mx_out_wave(MB, NB);
   static constexpr int kLds = kRing > 8 * kOutWave ? kRing : 8 * kOutWave;
   static constexpr int kXLoads = BM / 64, kWLoads = kWBytes / 8192;
   static constexpr int kLoads = kXLoads + kWLoads + (DX ? 1 : 0);  // of a wave and step
@@ -70,48 +71,41 @@ void mx4_gemm_kernel(MxGemmArgs a) {
   const int wm = wave / T::WN, wn = wave % T::WN;
   const int i32 = lane & 31, q = lane >> 5;
 
-  // tile of this workgroup: an XCD (workgroup % 8) takes a run of tiles, groups of row tiles
+  // tile of this workgroup: an XCD (workgroup % 8) takes a run of tiles, groups of four row tiles
   // walked column by column
   int rt, ct;
   {
-    const int G = a.row_tiles * a.col_tiles;
+    int rows = a.row_tiles;  // a plan's: those in use
+    if (a.rows.p) rows = a.rows.p[BM == 64 ? 0 : BM == 128 ? 3 : 4];
+    const int G = rows * a.col_tiles, each = G / 8;
     int t = blockIdx.x;
-    if (G % 8 == 0) t = (t & 7) * (G / 8) + (t >> 3);
-    const int GM = a.rows.p ? 4 * (BM / kTileRows) : 4;
+    if (t >= G) return;
+    if (t < 8 * each) t = (t & 7) * each + (t >> 3);
+    constexpr int GM = 4;
     const int per = GM * a.col_tiles, grp = t / per, r = t - grp * per;
-    const int gm = a.row_tiles - grp * GM < GM ? a.row_tiles - grp * GM : GM;
+    const int gm = rows - grp * GM < GM ? rows - grp * GM : GM;
     rt = grp * GM + r % gm;
     ct = r / gm;
   }
-  // its rows: slots slot0 .. + count - 1.  Of a plan's 64-row tiles, every BM / 64th of an
-  // expert begins a tile here; the others' workgroups end.
+  // its rows: slots slot0 .. + count - 1
   int expert, count;
   int64_t slot0;
   if (a.rows.p) {
-    const Tile first = plan_tile(a.rows, rt);
-    if (first.count == 0) return;
-    expert = __builtin_amdgcn_readfirstlane(first.adapter);
-    count = __builtin_amdgcn_readfirstlane(first.count);
-    slot0 = int64_t(kTileRows) * rt;
-    if constexpr (BM > kTileRows) {
-      int before = 0;  // tiles of this expert before this one
-      for (int b = rt - 1; b >= 0; b -= 64) {
-        const int at = b - lane;
-        const bool same = at >= 0 && plan_tile(a.rows, at).adapter == expert;
-        const unsigned long long other = ~__ballot(same);
-        const int run = other ? __builtin_ctzll(other) : 64;
-        before += run;
-        if (run < 64) break;
-      }
-      if (before % (BM / kTileRows) != 0) return;
+    int first = rt;  // 64-row tile
+    if constexpr (BM > kTileRows) first = a.rows.p[a.rows.off_big() + (BM == 256 ? a.rows.bigs(0) : 0) + rt];
+    slot0 = int64_t(kTileRows) * first;
+    const Tile tile = plan_tile(a.rows, first);
+    expert = tile.adapter;
+    count = tile.count;
 #pragma unroll
-      for (int j = 1; j < BM / kTileRows; ++j) {
-        if (rt + j >= a.rows.T) break;
-        const Tile next = plan_tile(a.rows, rt + j);
-        if (next.adapter != expert || next.count == 0) break;
-        count += __builtin_amdgcn_readfirstlane(next.count);
-      }
+    for (int j = 1; j < BM / kTileRows; ++j) {
+      if (first + j >= a.rows.T) break;
+      const Tile next = plan_tile(a.rows, first + j);
+      if (next.adapter != expert) break;
+      count += next.count;
     }
+    expert = __builtin_amdgcn_readfirstlane(expert);
+    count = __builtin_amdgcn_readfirstlane(count);
   } else {
     expert = 0;
     slot0 = int64_t(BM) * rt;
@@ -191,14 +185,19 @@ void mx4_gemm_kernel(MxGemmArgs a) {
       plane = a.planes == 1 ? 0 : t / a.nk;
       kk = t - plane * a.nk;
     };
-    auto load_x = [&](int j) {
+    auto load_x_part = [&](int j, int i0, int i1) {
       int plane, kk;
       place(j, plane, kk);
       const uint8_t* p = xbase + plane * a.plane + int64_t(kk) * 128;
       const uint32_t dst = uint32_t(j % T::kXRing) * T::kXBytes + xdst;
 #pragma unroll
-      for (int i = 0; i < T::kXLoads; ++i) dma16(p, xo[i], dst + 1024u * i);
+      for (int i = 0; i < T::kXLoads; ++i)
+        if (i >= i0 && i < i1) dma16(p, xo[i], dst + 1024u * i);
     };
+    auto load_x = [&](int j) { load_x_part(j, 0, T::kXLoads); };
+    // The loads of a step go out between its products, a part after each of the first three quarters (together
+    // after the barrier they kept all waves from their first product while the addresses went out).
+    constexpr int kHalfX = (T::kXLoads + 1) / 2;
     auto load_w = [&](int j) {
       int plane, kk;
       place(j, plane, kk);
@@ -288,8 +287,6 @@ void mx4_gemm_kernel(MxGemmArgs a) {
           }
           load_s(scn, kk + 8 < a.nk ? kk + 8 : 0);
         }
-        load_x(j + 3);
-        load_w(j + 3);
         float scale[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) scale[nb] = mx_scale((sc[nb].x >> (16 * (kk & 1))) & 255u);
@@ -310,7 +307,12 @@ void mx4_gemm_kernel(MxGemmArgs a) {
             read_x(xf[0], j + 1, 0);
             read_w(j + 1);
           }
+          __builtin_amdgcn_sched_barrier(0);
           mma(w, xf[s & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+          if (s == 0) load_x_part(j + 3, 0, kHalfX);
+          if (s == 1) load_x_part(j + 3, kHalfX, T::kXLoads);
+          if (s == 2) load_w(j + 3);
         }
       }
     } else {
@@ -335,8 +337,6 @@ void mx4_gemm_kernel(MxGemmArgs a) {
       read_x(xf[0], 0, 0);
       for (int j = 0; j < nk; ++j) {
         step_barrier<T::kLoads>();
-        load_w(j + 2);
-        load_x(j + 3);
         const uint32_t wb = uint32_t(j % T::kWRing) * T::kWBytes, sb = uint32_t(j % T::kWRing) * T::kSBytes;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
@@ -361,7 +361,12 @@ void mx4_gemm_kernel(MxGemmArgs a) {
           }
           if (s < 3) read_x(xf[(s + 1) & 1], j, s + 1);
           else read_x(xf[0], j + 1, 0);
+          __builtin_amdgcn_sched_barrier(0);
           mma(w, xf[s & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+          if (s == 0) load_w(j + 2);
+          if (s == 1) load_x_part(j + 3, 0, kHalfX);
+          if (s == 2) load_x_part(j + 3, kHalfX, T::kXLoads);
         }
       }
     }
@@ -388,7 +393,8 @@ struct MxRowsArgs {
   uint16_t* out;
 };
 
-template <int XT>
+// SPLIT: fp32 rows as three planes, else as they are.
+template <int XT, bool SPLIT>
 __global__ __launch_bounds__(256) void mx4_rows_kernel(MxRowsArgs a) {
   typedef typename Elem<XT>::T T;
   constexpr int V = Elem<XT>::kVec, P = 8 / V;
@@ -408,8 +414,9 @@ __global__ __launch_bounds__(256) void mx4_rows_kernel(MxRowsArgs a) {
       const int64_t left = a.cols - 8 * c8 - V * j;
       v[j] = left > 0 ? load16_part<XT>(p + V * j, left) : u32x4{0u, 0u, 0u, 0u};
     }
-    uint16_t* o = a.out + r * a.pitch + 8 * c8;
-    if constexpr (XT == RQ_DTYPE_F32) {
+    T* whole = reinterpret_cast<T*>(a.out) + r * a.pitch + 8 * c8;
+    if constexpr (XT == RQ_DTYPE_F32 && SPLIT) {
+      uint16_t* o = a.out + r * a.pitch + 8 * c8;
       u32x4 h, m, l;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -422,7 +429,8 @@ __global__ __launch_bounds__(256) void mx4_rows_kernel(MxRowsArgs a) {
       *reinterpret_cast<u32x4*>(o + a.plane) = m;
       *reinterpret_cast<u32x4*>(o + 2 * a.plane) = h;
     } else {
-      *reinterpret_cast<u32x4*>(o) = v[0];
+#pragma unroll
+      for (int j = 0; j < P; ++j) *reinterpret_cast<u32x4*>(whole + V * j) = v[j];
     }
   }
 }
@@ -478,9 +486,8 @@ struct MgPlan {
   int row_tiles, col_tiles;
 };
 
-// What a call runs as: a function of its sizes, dtype, strides' and pointers' alignment (any_alignment:
-// with the memory that the worst of these takes).
-MgPlan mg_plan(const MxCall& c, int cus, bool any_alignment) {
+// What a call runs as: a function of its sizes, dtype, row stride and its rows' alignment.
+MgPlan mg_plan(const MxCall& c, int cus) {
   MgPlan p{};
   const int64_t wp = mx_pad(c.wk);
   const int64_t cols = c.dx ? c.wk : c.N;
@@ -493,7 +500,7 @@ MgPlan mg_plan(const MxCall& c, int cus, bool any_alignment) {
   // plan's rows: of the first) row; else a copy, in the plan's order where that is too large as well
   const int64_t far = int64_t(1) << 32;
   auto near = [&](int64_t ld) { return (shared ? xrows : 256) * ld * 2 < far; };
-  p.copy = any_alignment || p.planes > 1 || c.K != p.xpitch || !aligned(c.x, 16) || c.ldx % 8 != 0 || !near(c.ldx);
+  p.copy = p.planes > 1 || c.K != p.xpitch || !c.aligned16 || !near(c.ldx);
   p.by_slot = !shared || (p.copy && !near(p.xpitch));
   p.xrows = shared && p.by_slot ? c.rows.slots() : xrows;
   p.x_bytes = p.copy ? up256(p.planes * p.xrows * p.xpitch * 2) : 0;
@@ -513,14 +520,16 @@ MgPlan mg_plan(const MxCall& c, int cus, bool any_alignment) {
     p.bm /= 2;
     t = tiles(p.bm);
   }
+  if (getenv("BM")) p.bm = atoi(getenv("BM"));
   t = tiles(p.bm);
   // splits of the contraction where the tiles leave compute units idle, 8 steps each at least
   const int64_t steps = p.planes * steps64;
   int64_t s = cus / (t > 0 ? t : 1);
   s = s < steps / 8 ? s : steps / 8;
   s = s < 16 ? s : 16;
+  if (getenv("SP")) s = atoi(getenv("SP"));
   p.splits = int(s > 1 ? s : 1);
-  p.row_tiles = int(shared ? c.rows.T : ceil_div(c.M, p.bm));
+  p.row_tiles = int(!shared ? ceil_div(c.M, p.bm) : p.bm == 64 ? c.rows.T : c.rows.bigs(p.bm == 128 ? 0 : 1));
   p.partial = p.splits > 1 || c.ysum > 1;
   p.ld = (cols + 3) / 4 * 4;
   p.part_bytes = p.partial ? up256(int64_t(p.splits) * c.M * p.ld * 4) : 0;
@@ -541,7 +550,16 @@ void mg_launch_bm(const MxGemmArgs& a, int bm, bool out32, hipStream_t stream) {
   else mg_launch<XT, DX, 256>(a, out32, stream);
 }
 
+dim3 rows_grid(int64_t rows, int64_t pitch) {
+  return dim3(unsigned(ceil_div(pitch / 8, 256)), unsigned(rows < 32768 ? rows : 32768));
+}
+
 }  // namespace
+
+void mx4_rows_whole(const void* x, int dt, int64_t rows, int64_t cols, int64_t ld, void* out, int64_t pitch, hipStream_t stream) {
+  const MxRowsArgs r{x, ld, cols, rows, pitch, 0, RowsPlan{}, 1, false, static_cast<uint16_t*>(out)};
+  RQ_DISPATCH_DT(dt, XT, mx4_rows_kernel<XT, false><<<rows_grid(rows, pitch), 256, 0, stream>>>(r));
+}
 
 void mx4_sum(const MxSumArgs& s, int dt, hipStream_t stream) {
   const dim3 grid(unsigned(ceil_div(s.ld / 4, 256)), unsigned(s.out_rows < 32768 ? s.out_rows : 32768));
@@ -549,7 +567,7 @@ void mx4_sum(const MxSumArgs& s, int dt, hipStream_t stream) {
 }
 
 int64_t mx4_gemm_scratch(const MxCall& c, int cus) {
-  const MgPlan p = mg_plan(c, cus, true);
+  const MgPlan p = mg_plan(c, cus);
   return p.x_bytes + p.s_bytes + p.part_bytes;
 }
 
@@ -558,7 +576,7 @@ int mx4_gemm_run(const MxCall& c) {
   if (hipGetDevice(&dev) != hipSuccess ||
       hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
     return RQ_ERR_HIP;
-  const MgPlan p = mg_plan(c, cus, false);
+  const MgPlan p = mg_plan(c, cus);
   if (int64_t(p.row_tiles) * p.col_tiles > (int64_t(1) << 22)) return RQ_ERR_UNSUPPORTED;
   uint8_t* ws = static_cast<uint8_t*>(c.scratch);
   const int64_t wp = mx_pad(c.wk);
@@ -572,8 +590,7 @@ int mx4_gemm_run(const MxCall& c) {
   if (p.copy) {
     MxRowsArgs r{c.x, c.ldx, c.K, p.xrows, p.xpitch, p.xrows * p.xpitch, c.rows, c.xdiv, c.rows.p && p.by_slot,
                  reinterpret_cast<uint16_t*>(ws)};
-    const dim3 grid(unsigned(ceil_div(p.xpitch / 8, 256)), unsigned(p.xrows < 32768 ? p.xrows : 32768));
-    RQ_DISPATCH_DT(c.dt, XT, mx4_rows_kernel<XT><<<grid, 256, 0, c.stream>>>(r));
+    RQ_DISPATCH_DT(c.dt, XT, mx4_rows_kernel<XT, true><<<rows_grid(p.xrows, p.xpitch), 256, 0, c.stream>>>(r));
     a.x = ws;
     a.ldx = p.xpitch * 2;
     a.plane = p.xrows * p.xpitch * 2;

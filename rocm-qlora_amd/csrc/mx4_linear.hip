@@ -1,5 +1,6 @@
 // Entry points of the linears on MXFP4 weights: argument checks and the choice of kernel.
 #include "rq_mx4.h"
+#include <stdlib.h>
 
 namespace rq {
 namespace {
@@ -8,7 +9,8 @@ namespace {
 // experts: where they have 16 rows each at most on average (an expert's tile reads its weight
 // once, however few its rows).
 bool few(const MxCall& c) {
-  if (c.dx) return false;
+  if (c.dx || ceil_div(c.M, c.xdiv) * mx_pad(c.wk) * int64_t(dtype_size(c.dt)) > int64_t(kMxFewBytes)) return false;
+  if (getenv("FEWM")) return c.M <= atoi(getenv("FEWM"));
   if (!c.rows.p) return c.M <= kTileRows;
   return c.M <= 16 * c.E;
 }
@@ -36,11 +38,12 @@ int check_sizes(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t s
 }
 
 int64_t scratch_of(const MxCall& c, int cus) {
-  if (c.a4) return mx4_a4_scratch(c, cus);
-  return few(c) ? 0 : mx4_gemm_scratch(c, cus);
+  if (few(c)) return mx4_few_scratch(c);
+  return c.a4 ? mx4_a4_scratch(c, cus) : mx4_gemm_scratch(c, cus);
 }
 
-MxCall call_of(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, const void* plan, int act_bits, bool dx) {
+MxCall call_of(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, const void* plan, int act_bits, bool dx,
+               int64_t ldx, bool aligned16) {
   MxCall c{};
   c.dt = dtype;
   c.M = M;
@@ -48,7 +51,8 @@ MxCall call_of(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t sh
   c.N = N;
   c.wk = K;
   c.K = dx ? N : K;
-  c.ldx = c.K;
+  c.ldx = ldx;
+  c.aligned16 = aligned16 && ldx * int64_t(dtype_size(dtype)) % 16 == 0;
   c.xdiv = dx ? 1 : int(shared);
   c.ysum = dx ? int(shared) : 1;
   c.rows = rows_plan(static_cast<const int32_t*>(plan), M, E);
@@ -57,9 +61,9 @@ MxCall call_of(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t sh
   return c;
 }
 
-int run(MxCall& c, const void* x, int64_t ldx, int64_t plan_bytes, const uint8_t* codes, const uint8_t* scales,
+int run(MxCall& c, const void* x, int64_t plan_bytes, const uint8_t* codes, const uint8_t* scales,
         const void* bias, void* y, int64_t ldy, void* scratch, int64_t scratch_bytes, hipStream_t stream) {
-  if (ldx < c.K || ldy < (c.dx ? c.wk : c.N)) return RQ_ERR_BAD_SHAPE;
+  if (c.ldx < c.K || ldy < (c.dx ? c.wk : c.N)) return RQ_ERR_BAD_SHAPE;
   if (c.M == 0) return RQ_OK;
   if (!x || !codes || !scales || !y) return RQ_ERR_NULL_POINTER;
   if (c.rows.p && plan_bytes < 4 * c.rows.words()) return RQ_ERR_WORKSPACE;
@@ -75,7 +79,6 @@ int run(MxCall& c, const void* x, int64_t ldx, int64_t plan_bytes, const uint8_t
   if (scratch_bytes < need) return RQ_ERR_WORKSPACE;
   if (need > 0 && !aligned(scratch, 256)) return RQ_ERR_BAD_ALIGNMENT;
   c.x = x;
-  c.ldx = ldx;
   c.codes = codes;
   c.scales = scales;
   c.bias = bias;
@@ -91,18 +94,19 @@ int run(MxCall& c, const void* x, int64_t ldx, int64_t plan_bytes, const uint8_t
 }  // namespace rq
 
 extern "C" int rq_mx4_linear_scratch_size(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, int grouped,
-                                          int act_bits, int dx, int64_t* bytes) {
+                                          int act_bits, int dx, int64_t ldx, int aligned16, int64_t* bytes) {
   using namespace rq;
   if (!bytes) return RQ_ERR_NULL_POINTER;
   int cus = 0;
   int st = check_sizes(dtype, M, K, N, E, shared, grouped != 0, act_bits);
   if (st != RQ_OK) return st;
+  if (ldx < (dx ? N : K)) return RQ_ERR_BAD_SHAPE;
   *bytes = 0;
   if (M == 0) return RQ_OK;
   st = compute_units(&cus);
   if (st != RQ_OK) return st;
   static const int32_t some = 0;  // any non-null plan: sizes alone are asked for
-  *bytes = scratch_of(call_of(dtype, M, K, N, E, shared, grouped ? &some : nullptr, act_bits, dx != 0), cus);
+  *bytes = scratch_of(call_of(dtype, M, K, N, E, shared, grouped ? &some : nullptr, act_bits, dx != 0, ldx, aligned16 != 0), cus);
   return RQ_OK;
 }
 
@@ -113,8 +117,8 @@ extern "C" int rq_mx4_linear(const void* x, int dtype, int64_t M, int64_t K, int
   using namespace rq;
   const int st = check_sizes(dtype, M, K, N, E, shared, plan != nullptr, act_bits);
   if (st != RQ_OK) return st;
-  MxCall c = call_of(dtype, M, K, N, E, shared, plan, act_bits, false);
-  return run(c, x, ldx, plan_bytes, codes, scales, bias, y, ldy, scratch, scratch_bytes, stream);
+  MxCall c = call_of(dtype, M, K, N, E, shared, plan, act_bits, false, ldx, aligned(x, 16));
+  return run(c, x, plan_bytes, codes, scales, bias, y, ldy, scratch, scratch_bytes, stream);
 }
 
 extern "C" int rq_mx4_linear_dx(const void* dy, int dtype, int64_t M, int64_t N, int64_t lddy, const void* plan,
@@ -124,6 +128,6 @@ extern "C" int rq_mx4_linear_dx(const void* dy, int dtype, int64_t M, int64_t N,
   using namespace rq;
   const int st = check_sizes(dtype, M, K, N, E, shared, plan != nullptr, 16);
   if (st != RQ_OK) return st;
-  MxCall c = call_of(dtype, M, K, N, E, shared, plan, 16, true);
-  return run(c, dy, lddy, plan_bytes, codes, scales, nullptr, dx, lddx, scratch, scratch_bytes, stream);
+  MxCall c = call_of(dtype, M, K, N, E, shared, plan, 16, true, lddy, aligned(dy, 16));
+  return run(c, dy, plan_bytes, codes, scales, nullptr, dx, lddx, scratch, scratch_bytes, stream);
 }

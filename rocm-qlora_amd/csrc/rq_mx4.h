@@ -73,6 +73,7 @@ struct MxCall {
   const void* x;
   int dt;
   int64_t M, K, ldx;  // rows of the product, x's columns
+  bool aligned16;     // x's rows are 16-byte aligned
   int xdiv;           // product rows that read one row of x
   RowsPlan rows;
   const uint8_t* codes;   // [E][N][Kp / 2]
@@ -87,9 +88,15 @@ struct MxCall {
   hipStream_t stream;
 };
 
+inline int64_t up256(int64_t n) { return (n + 255) & ~int64_t(255); }
+
 int mx4_quantize(const void* x, int dt, int64_t rows, int64_t cols, int64_t ld, uint8_t* codes, uint8_t* scales,
                  hipStream_t stream);
-// M rows a tile at most: the kernel for few rows (mx4_few.hip).
+// A copy of rows, zeros up to `pitch` values (a multiple of 8).
+void mx4_rows_whole(const void* x, int dt, int64_t rows, int64_t cols, int64_t ld, void* out, int64_t pitch, hipStream_t stream);
+// The kernel for few rows (mx4_few.hip): x's rows in whole steps take at most kMxFewBytes.
+constexpr uint32_t kMxFewBytes = 0xFFFFFFE0u;  // (kOobOffset is past them)
+int64_t mx4_few_scratch(const MxCall& c);
 int mx4_few_run(const MxCall& c);
 int mx4_gemm_run(const MxCall& c);
 int64_t mx4_gemm_scratch(const MxCall& c, int cus);

@@ -38,79 +38,78 @@ __device__ __forceinline__ void lds_escapes(uint8_t* lds) {
   asm volatile("" ::"v"((__attribute__((address_space(3))) uint8_t*)lds) : "memory");
 }
 
-// Bytes of a wave's staged row of 32 NB 16-bit outputs.
-__host__ __device__ constexpr int mx_out_pitch(int NB) { return 64 * NB + 16; }
+// Bytes of a wave's staged row of 32 NB outputs, and of what it stages at once: its 32 MB rows, of fp32 results 32.
+__host__ __device__ constexpr int mx_out_pitch(int NB, bool out32) { return (out32 ? 128 : 64) * NB + 16; }
+__host__ __device__ constexpr int mx_out_wave(int MB, int NB) {
+  const int a = 32 * MB * mx_out_pitch(NB, false), b = 32 * mx_out_pitch(NB, true);
+  return a > b ? a : b;
+}
 
-// The results of a wave: 32 MB rows from slot0 + rw, columns cw ...  `stage`: 32 MB mx_out_pitch(NB) bytes of
-// LDS of its own (16-bit results).
-//
-// Output.  Block (mb, nb): lane (i32, q) holds row 32 mb + i32 of the wave's, and in register r the
-// A operand's row 8 (r / 4) + 4 q + r % 4: forward column 32 nb + that, dX 4 that + nb.  Four values
-// v of adjacent columns: forward registers 4 h .. of block nb, dX register r of the four blocks.
+// The results of a wave: 32 MB rows from slot0 + rw, columns cw ...  `stage`: mx_out_wave(MB, NB) bytes of
+// LDS of its own.  Block (mb, nb): lane (i32, q) holds row 32 mb + i32 of the wave's, and in register r the
+// A operand's row 8 (r / 4) + 4 q + r % 4: forward column 32 nb + that, dX 4 that + nb; so four values of
+// adjacent columns are forward registers 4 h .. of block nb, dX register r of the four blocks.  (fp32 results
+// stored straight from registers, 16 bytes a row, took twice the time.)
 template <int XT, bool DX, int MB, int NB, bool OUT32>
 __device__ __forceinline__ void mx_output(const MxGemmArgs& a, const f32x16 (&acc)[MB][NB], uint8_t* stage, int lane, int64_t e,
                                           bool live, int split, int64_t slot0, int count, int rw, int64_t cw) {
-  constexpr int kOutPitch = mx_out_pitch(NB);
+  constexpr int kPitch = mx_out_pitch(NB, OUT32);
   const int i32 = lane & 31, q = lane >> 5;
+  // (never with dX; past the columns zeros)
+  const bool biased = !DX && a.bias && live && split == 0 && cw < a.cols;
+  const int bs = a.bias_dt == RQ_DTYPE_F32 ? 4 : 2;
+  const __amdgpu_buffer_rsrc_t br =
+      buffer_rsrc(static_cast<const uint8_t*>(a.bias) + (biased ? (e * a.cols + cw) * bs : 0),
+                  biased ? uint32_t((a.cols - cw < 32 * NB ? a.cols - cw : 32 * NB) * bs) : 0u);
   constexpr int kQuads = DX ? 16 : 4 * NB;
-  auto quad = [&](int mb, int k, float (&v)[4]) -> int {  // returns the first column, of the wave's
-    if constexpr (DX) {
+  constexpr int ES = OUT32 ? 4 : 2, V = 16 / ES;
+  constexpr int kOnce = OUT32 ? 1 : MB;  // 32-row blocks staged at a time
 #pragma unroll
-      for (int c = 0; c < 4; ++c) v[c] = acc[mb][c][k];
-      return 4 * (8 * (k / 4) + 4 * q + k % 4);
-    } else {
+  for (int m0 = 0; m0 < MB; m0 += kOnce) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) v[c] = acc[mb][k / 4][4 * (k % 4) + c];
-      return 32 * (k / 4) + 8 * (k % 4) + 4 * q;
-    }
-  };
-  const bool biased = a.bias && live && split == 0;
-#pragma unroll
-  for (int k = 0; k < kQuads; ++k) {
-    float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (biased) {
-      const int64_t col = cw + (DX ? 0 : 32 * (k / 4) + 8 * (k % 4) + 4 * q);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (col + c < a.cols) bias[c] = load_as_f32(a.bias, e * a.cols + col + c, a.bias_dt);
-    }
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      float v[4];
-      const int col = quad(mb, k, v);
+    for (int k = 0; k < kQuads; ++k) {
+      const int col = DX ? 4 * (8 * (k / 4) + 4 * q + k % 4) : 32 * (k / 4) + 8 * (k % 4) + 4 * q;  // the quad's first
+      float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       if (biased) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = __fadd_rn(v[c], bias[c]);
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t at = uint32_t(col + c);
+          if (a.bias_dt == RQ_DTYPE_F32) bias[c] = u2f(buf_load4(br, 4 * at));
+          else if (a.bias_dt == RQ_DTYPE_BF16) bias[c] = bf16_to_f32(uint16_t(buf_load2(br, 2 * at)));
+          else bias[c] = f16_to_f32(uint16_t(buf_load2(br, 2 * at)));
+        }
       }
-      const int r = rw + 32 * mb + i32;
-      if constexpr (OUT32) {
-        if (r >= count) continue;
-        float* p = static_cast<float*>(a.y) + (int64_t(split) * a.rows.M + plan_row(a.rows, slot0 + r)) * a.ldy + cw + col;
-        const int64_t left = a.cols - cw - col;
-        if (left >= 4) store16_any(p, u32x4{f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])});
-        else
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (c < left) p[c] = v[c];
-      } else {
-        *reinterpret_cast<u32x2*>(stage + (32 * mb + i32) * kOutPitch + 2 * col) =
-            u32x2{cvt_pk<XT>(v[0], v[1]), cvt_pk<XT>(v[2], v[3])};
+      for (int m = 0; m < kOnce; ++m) {
+        float v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if constexpr (DX) v[c] = acc[m0 + m][c][k];
+          else v[c] = __fadd_rn(acc[m0 + m][k / 4][4 * (k % 4) + c], bias[c]);
+        }
+        uint8_t* o = stage + (32 * m + i32) * kPitch + ES * col;
+        if constexpr (OUT32) *reinterpret_cast<u32x4*>(o) = u32x4{f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])};
+        else *reinterpret_cast<u32x2*>(o) = u32x2{cvt_pk<XT>(v[0], v[1]), cvt_pk<XT>(v[2], v[3])};
       }
     }
-  }
-  if constexpr (!OUT32) {
     // the wave reads back its own rows, 16 bytes a lane
-    constexpr int kLanes = 4 * NB;  // of a row
+    constexpr int kLanes = 32 * NB / V;  // of a row
 #pragma unroll 4
-    for (int it = 0; it < 32 * MB * kLanes / 64; ++it) {
-      const int r = it * (64 / kLanes) + lane / kLanes, c = lane % kLanes;
-      if (rw + r >= count) continue;
-      const u32x4 v = *reinterpret_cast<const u32x4*>(stage + r * kOutPitch + 16 * c);
-      const int64_t col = cw + 8 * c, row = plan_row(a.rows, slot0 + rw + r);
-      uint16_t* p = static_cast<uint16_t*>(a.y) + row * a.ldy + col;
+    for (int it = 0; it < 32 * kOnce * kLanes / 64; ++it) {
+      const int at = it * 64 + lane, r = at / kLanes, c = at % kLanes;
+      if (rw + 32 * m0 + r >= count) continue;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(stage + r * kPitch + 16 * c);
+      const int64_t col = cw + V * c, row = plan_row(a.rows, slot0 + rw + 32 * m0 + r);
       const int64_t left = a.cols - col;
-      if (left >= 8) store16_any(p, v);
-      else if (left > 0) store_edge<XT>(p, v, int(left));
+      if constexpr (OUT32) {
+        float* p = static_cast<float*>(a.y) + (int64_t(split) * a.rows.M + row) * a.ldy + col;
+        if (left >= 4) store16_any(p, v);
+        else if (left > 0) store_edge<RQ_DTYPE_F32>(p, v, int(left));
+      } else {
+        uint16_t* p = static_cast<uint16_t*>(a.y) + row * a.ldy + col;
+        if (left >= 8) store16_any(p, v);
+        else if (left > 0) store_edge<XT>(p, v, int(left));
+      }
     }
   }
 }
@@ -125,7 +124,5 @@ struct MxSumArgs {
   int64_t ldy;
 };
 void mx4_sum(const MxSumArgs& s, int dt, hipStream_t stream);
-
-inline int64_t up256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
 }  // namespace rq

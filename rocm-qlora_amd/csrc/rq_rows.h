@@ -10,11 +10,14 @@
 // 16 tiles at least: few columns take the finer one.
 //
 // The plan is int32 device memory:
-//   [0] tiles in use, [1], [2] chunks in use of the two tables, [3..15] zero
+//   [0] tiles in use, [1], [2] chunks in use of the two tables, [3], [4] big tiles in use of the two
+//   tables, [5..15] zero
 //   tile[T][2]                        (adapter, -1: rows without one; rows, 0: not in use)
 //   slot_row[64 T]                    (-1: padding; of tiles in use)
 //   chunk[2][C][4]                    (adapter, first tile, end tile, partial slot or -1)
 //   part[2][n][2]                     (chunks of the adapter, its first partial slot)
+//   big[2][S]                         (first tile of each two, four adjacent tiles of an adapter, or what
+//                                      is left of its tiles; rows without one last)
 // A null plan stands for M rows of adapter 0 in their own order.
 #pragma once
 
@@ -31,6 +34,8 @@ constexpr int kRowChunks = 16;
 constexpr int kChunkTables = 2;
 __host__ __device__ constexpr int chunk_least(int table) { return table == 0 ? 4 : 16; }
 constexpr int kMaxParts = 2 * kRowChunks;
+constexpr int kBigTables = 2;
+__host__ __device__ constexpr int big_tiles(int table) { return 2 << table; }  // tiles of a big one
 
 struct RowsPlan {
   const int32_t* p;  // device, or nullptr
@@ -42,7 +47,13 @@ struct RowsPlan {
   __host__ __device__ int64_t off_rows() const { return 16 + ((2 * int64_t(T) + 3) & ~int64_t(3)); }
   __host__ __device__ int64_t off_chunks() const { return off_rows() + int64_t(kTileRows) * T; }
   __host__ __device__ int64_t off_part() const { return off_chunks() + kChunkTables * 4 * int64_t(C); }
-  __host__ __device__ int64_t words() const { return off_part() + kChunkTables * 2 * int64_t(n); }
+  __host__ __device__ int64_t off_big() const { return off_part() + kChunkTables * 2 * int64_t(n); }
+  // big tiles of a table, at most: whole ones and an end of each adapter's
+  __host__ __device__ int64_t bigs(int table) const {
+    const int64_t some = int64_t(n) + 1 < T ? int64_t(n) + 1 : T;
+    return T / big_tiles(table) + some;
+  }
+  __host__ __device__ int64_t words() const { return off_big() + bigs(0) + bigs(1); }
   __host__ __device__ int64_t slots() const { return int64_t(kTileRows) * T; }
 
   // tiles per chunk when `tiles` are in use

@@ -1099,31 +1099,44 @@ def mx4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, K: in
     """y[r] = x[r / shared] W[e]^T + bias[e] on MXFP4 weights.  x: rows [R, K] fp32/bf16/fp16.
     Without a plan codes are [N, Kp / 2] and y is [R, N]; with one (adapter_rows of M rows and E
     experts) codes are [E, N, Kp / 2], y is [M, N], and M / R rows of it read one row of x."""
+    _check_mx4(codes, scales, K)
+    return _mx4_linear(x, codes, scales, K, bias, activation_bits, plan, M)
+
+
+def _mx4_linear(x, codes, scales, K, bias, activation_bits, plan, M):
+    """mx4_linear on codes and scales that fit."""
     dev = nat.require_gpu(x, codes, scales, bias, plan)
     code = nat.dtype_code(x.dtype)
-    _check_mx4(codes, scales, K)
     E, N = _mx4_weight(codes, plan)
     if x.dim() != 2 or x.shape[1] != K:
         raise RuntimeError(f"x must be rows of {K}, got {tuple(x.shape)}")
-    if activation_bits not in (4, 16):
+    if activation_bits != 16 and activation_bits != 4:
         raise ValueError(f"activation_bits must be 4 or 16, got {activation_bits}")
     R = x.shape[0]
-    M = R if plan is None or M is None else M
-    if plan is not None and activation_bits != 16:
-        raise RuntimeError("experts' rows are multiplied in 16 bits or more")
-    if M != R and (R == 0 or M % R):
-        raise RuntimeError(f"{M} rows do not share {R} rows of x evenly")
-    bias = _mx4_bias(bias, x.dtype, E, N, plan is not None)
+    grouped = shared = plan_bytes = 0
+    if plan is None:
+        M = R
+    else:
+        M = R if M is None else M
+        grouped, plan_bytes = 1, plan.numel()
+        if activation_bits != 16:
+            raise RuntimeError("experts' rows are multiplied in 16 bits or more")
+        if M != R and (R == 0 or M % R):
+            raise RuntimeError(f"{M} rows do not share {R} rows of x evenly")
+    if bias is not None:
+        bias = _mx4_bias(bias, x.dtype, E, N, plan is not None)
     with on(dev):
-        if plan is not None and plan.numel() != _bytes("rq_adapter_rows_size", dev.index, M, E):
+        if grouped and plan_bytes != _bytes("rq_adapter_rows_size", dev.index, M, E):
             raise RuntimeError(f"the rows by expert are not those of {M} rows and {E} experts")
         y = torch.empty((M, N), dtype=x.dtype, device=dev)
         if M == 0 or N == 0:
             return y
         x, ldx = _rows(x, K)
         shared = M // R
-        scratch = _scratch("rq_mx4_linear_scratch_size", dev, code, M, K, N, E, shared, int(plan is not None), activation_bits, 0)
-        nat.call("rq_mx4_linear", x.data_ptr(), code, M, K, ldx, shared, nat.ptr(plan), plan.numel() if plan is not None else 0,
+        xp = x.data_ptr()
+        scratch = _scratch("rq_mx4_linear_scratch_size", dev, code, M, K, N, E, shared, grouped, activation_bits, 0, ldx,
+                           xp % 16 == 0)
+        nat.call("rq_mx4_linear", xp, code, M, K, ldx, shared, nat.ptr(plan), plan_bytes,
                  codes.data_ptr(), scales.data_ptr(), E, N, nat.ptr(bias), activation_bits, y.data_ptr(), N,
                  nat.ptr(scratch), scratch.numel() if scratch is not None else 0, nat.stream_handle(dev))
     return y
@@ -1133,26 +1146,35 @@ def mx4_linear_dx(dy: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, K
                   shared: int = 1) -> torch.Tensor:
     """dx[t] = sum of dy[r] W[e] over the `shared` rows r of t: mx4_linear's gradient by x.
     dy [M, N]; dx [M / shared, K] in its dtype."""
+    _check_mx4(codes, scales, K)
+    return _mx4_linear_dx(dy, codes, scales, K, plan, shared)
+
+
+def _mx4_linear_dx(dy, codes, scales, K, plan, shared):
+    """mx4_linear_dx on codes and scales that fit."""
     dev = nat.require_gpu(dy, codes, scales, plan)
     code = nat.dtype_code(dy.dtype)
-    _check_mx4(codes, scales, K)
     E, N = _mx4_weight(codes, plan)
     if dy.dim() != 2 or dy.shape[1] != N:
         raise RuntimeError(f"dY must be rows of {N}, got {tuple(dy.shape)}")
     M = dy.shape[0]
-    if shared < 1 or M % shared:
+    if shared < 1 or M % shared or (plan is None and shared != 1):
         raise RuntimeError(f"{M} rows are not {shared} for each row of x")
+    grouped = plan_bytes = 0
     with on(dev):
-        if plan is not None and plan.numel() != _bytes("rq_adapter_rows_size", dev.index, M, E):
-            raise RuntimeError(f"the rows by expert are not those of {M} rows and {E} experts")
+        if plan is not None:
+            grouped, plan_bytes = 1, plan.numel()
+            if plan_bytes != _bytes("rq_adapter_rows_size", dev.index, M, E):
+                raise RuntimeError(f"the rows by expert are not those of {M} rows and {E} experts")
         dx = torch.empty((M // shared, K), dtype=dy.dtype, device=dev)
         if M == 0:
             return dx
         if N == 0:
             return dx.zero_()
         dy, lddy = _rows(dy, N)
-        scratch = _scratch("rq_mx4_linear_scratch_size", dev, code, M, K, N, E, shared, int(plan is not None), 16, 1)
-        nat.call("rq_mx4_linear_dx", dy.data_ptr(), code, M, N, lddy, nat.ptr(plan), plan.numel() if plan is not None else 0,
+        dp = dy.data_ptr()
+        scratch = _scratch("rq_mx4_linear_scratch_size", dev, code, M, K, N, E, shared, grouped, 16, 1, lddy, dp % 16 == 0)
+        nat.call("rq_mx4_linear_dx", dp, code, M, N, lddy, nat.ptr(plan), plan_bytes,
                  codes.data_ptr(), scales.data_ptr(), E, K, shared, dx.data_ptr(), K,
                  nat.ptr(scratch), scratch.numel() if scratch is not None else 0, nat.stream_handle(dev))
     return dx

@@ -97,14 +97,14 @@ class _MXFP4Linear(torch.autograd.Function):
         if rows is not None:
             plan, M = rows.plan, rows.M
         ctx.args = (K, plan, 1 if M is None or x.shape[0] == 0 else M // x.shape[0])
-        return ops.mx4_linear(x, codes, scales, K, bias, activation_bits=bits, plan=plan, M=M)
+        return ops._mx4_linear(x, codes, scales, K, bias, bits, plan, M)
 
     @staticmethod
     @first_order
     def backward(ctx, dy):
         codes, scales = ctx.saved_tensors
         K, plan, shared = ctx.args
-        return ops.mx4_linear_dx(dy, codes, scales, K, plan=plan, shared=shared), None, None, None, None, None, None
+        return ops._mx4_linear_dx(dy, codes, scales, K, plan, shared), None, None, None, None, None, None
 
 
 def _refuse_bias_gradient(bias: Optional[torch.Tensor], name: str) -> None:
@@ -115,7 +115,7 @@ def _refuse_bias_gradient(bias: Optional[torch.Tensor], name: str) -> None:
 def _linear(x, codes, scales, K, bias, bits):
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if dm._nothing_recorded_eagerly(x):
-        y = ops.mx4_linear(x2, codes, scales, K, bias, activation_bits=bits)
+        y = ops._mx4_linear(x2, codes, scales, K, bias, bits, None, None)
     else:
         y = _MXFP4Linear.apply(x2, codes, scales, K, bias, bits, None)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[-1])
@@ -145,7 +145,7 @@ def _expert_linear(x, codes, scales, K, rows, bias):
     if codes.dim() != 3 or codes.shape[0] != rows.n:
         raise RuntimeError(f"weights of {rows.n} experts expected, got codes {tuple(codes.shape)}")
     if dm._nothing_recorded_eagerly(x):
-        return ops.mx4_linear(x, codes, scales, K, bias, plan=rows.plan, M=rows.M)
+        return ops._mx4_linear(x, codes, scales, K, bias, 16, rows.plan, rows.M)
     return _MXFP4Linear.apply(x, codes, scales, K, bias, 16, rows)
 
 
@@ -191,6 +191,7 @@ class MXFP4Linear(nn.Module):
     @eager_only
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         _refuse_bias_gradient(self.bias, "MXFP4Linear")
+        ops._check_mx4(self.weight_quant, self.weight_scales, self.in_features)
         if x.dim() == 0 or x.shape[-1] != self.in_features:
             raise RuntimeError(f"x must be rows of {self.in_features}, got {tuple(x.shape)}")
         return _linear(x, self.weight_quant, self.weight_scales, self.in_features, self.bias, self.activation_bits)
@@ -244,6 +245,7 @@ class MXFP4Experts(nn.Module):
     @eager_only
     def forward(self, x: torch.Tensor, rows: ExpertRows) -> torch.Tensor:
         _refuse_bias_gradient(self.bias, "MXFP4Experts")
+        ops._check_mx4(self.weight_quant, self.weight_scales, self.in_features)
         return _expert_linear(x, self.weight_quant, self.weight_scales, self.in_features, rows, self.bias)
 
     def extra_repr(self) -> str:
