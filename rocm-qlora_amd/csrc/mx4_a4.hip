@@ -38,7 +38,8 @@ struct A4Tile {
 
 struct A4Args {
   MxGemmArgs g;           // x: codes [M][pitch], codes, scales, wrows, pitch, cols, nk, splits, tiles, bias, y
-  const uint8_t* xscales; // [M][pitch / 16]
+  const uint8_t* xscales; // [M][xpitch / 16]
+  int64_t xpitch;         // bytes of a row of x's codes
 };
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -48,6 +49,11 @@ __device__ __forceinline__ uint32_t swz64(uint32_t r, uint32_t c) { return r * 6
 // One direct-to-LDS load of 4 bytes a lane from an address of its own (see dma16).
 __device__ __forceinline__ void dma4(const void* p, uint32_t lds_addr) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds_addr) : "memory", "m0");
+}
+
+// 16 bytes a lane, likewise.
+__device__ __forceinline__ void dma16_at(const void* p, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds_addr) : "memory", "m0");
 }
 
 // A wave-uniform value in scalar registers (the compiler may keep one that a masked load uses in vector registers).
@@ -207,8 +213,255 @@ void mx4_a4_kernel(A4Args args) {
                                       c0 + 32 * NB * wn);
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: 256 x 256 tiles, 256 k a step.  A cache line of a row's codes is 256 k, and what bounds the kernel above
+// with many tiles is the number of lines it asks the L2 for (half a line of codes, and one more for
+// four bytes of scales, a row and step: 0.73 requests a channel and cycle, the matrix units busy 36 %); here a step
+// takes whole lines, and 16 bytes of a row's scales are asked for every second step.
+//
+// Wave (wr, wc) = (wave / 4, wave % 4) owns rows 64 wr .. + 63 and columns 32 wc .. + 31 of each 128 x 128
+// quadrant, two blocks of 32 x 32.  A phase is a quadrant's eight products (256 cycles) behind the phase's
+// LDS reads and one half tile's loads (128 rows, 16 KiB); waves 4 - 7 run one phase slot behind waves 0 - 3, so
+// that of the two waves of a SIMD one reads while the other multiplies.  A half tile is refilled in the phase after its
+// last reads, two steps ahead of its next use, and the waits leave the youngest six in flight.
+// ---------------------------------------------------------------------------
+constexpr int kBgHalf = 128 * 128;                    // bytes of a half tile
+constexpr int kBgStep = 4 * kBgHalf;                  // X0 X1 W0 W1
+constexpr int kBgScales = 512 * 16;                   // two steps' scales: 256 rows of x, then the weight's
+constexpr int kBgSOff = 2 * kBgStep;
+constexpr int kBgRing = kBgSOff + 3 * kBgScales;
+constexpr int kBgPitch = 256 * 2 + 16;                // the staged output tile's rows
+constexpr int kBgLds = kBgRing > 256 * kBgPitch ? kBgRing : 256 * kBgPitch;
+static_assert(kBgLds <= 160 * 1024, "LDS plan");
+
+template <int XT>
+__global__ __launch_bounds__(kMgThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void mx4_a4_big_kernel(A4Args args) {
+  const MxGemmArgs& a = args.g;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kBgLds];
+  lds_escapes(lds);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave >> 2, wc = wave & 3;
+  const int i32 = lane & 31, q = lane >> 5;
+  int rt, ct;
+  {
+    const int G = a.row_tiles * a.col_tiles, each = G / 8;
+    int t = blockIdx.x;
+    if (t < 8 * each) t = (t & 7) * each + (t >> 3);
+    constexpr int GM = 4;
+    const int per = GM * a.col_tiles, grp = t / per, r = t - grp * per;
+    const int gm = a.row_tiles - grp * GM < GM ? a.row_tiles - grp * GM : GM;
+    rt = grp * GM + r % gm;
+    ct = r / gm;
+  }
+  const int64_t m0 = int64_t(256) * rt, c0 = int64_t(256) * ct;
+  const int xrows = a.rows.M - m0 < 256 ? int(a.rows.M - m0) : 256;
+  const int wrows = a.wrows - c0 < 256 ? int(a.wrows - c0) : 256;
+  const int nk = a.nk;  // steps; the weight's last may be half of one (x has zeros there)
+
+  // direct-to-LDS lanes: half tile h: rows 128 h + 16 wave + 8 i + lane / 8, chunk swizzled.  Where the weight's last
+  // step is half of one, its second half's chunks are the first's again and their scales 2^-127.
+  const uint8_t* xbase = a.x + m0 * args.xpitch;
+  const uint8_t* wbase = a.codes + c0 * a.pitch;
+  uint32_t xo[2][2], wo[2][2], back[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * wave + 8 * i + (lane >> 3);
+    const uint32_t c = uint32_t(lane & 7) ^ ((r >> 1) & 7);
+    back[i] = c >= 4 ? 64u : 0u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int rx = 128 * h + r < xrows ? 128 * h + r : xrows - 1, rw = 128 * h + r < wrows ? 128 * h + r : wrows - 1;
+      xo[h][i] = uint32_t(rx) * uint32_t(args.xpitch) + 16u * c;
+      wo[h][i] = uint32_t(rw) * uint32_t(a.pitch) + 16u * c;
+    }
+  }
+  const bool half = a.pitch % 128 != 0;
+  const uint32_t dst0 = __builtin_amdgcn_readfirstlane(uint32_t(wave) * 2048u);
+  auto load_x = [&](int h, int step, uint32_t at) {
+    const uint8_t* p = xbase + int64_t(step < nk ? step : nk - 1) * 128;  // past the end: the last step again, never used
+    dma16(p, xo[h][0], dst0 + at);
+    dma16(p, xo[h][1], dst0 + at + 1024u);
+  };
+  auto load_w = [&](int h, int step, uint32_t at) {
+    const int st = step < nk ? step : nk - 1;
+    const uint8_t* p = wbase + int64_t(st) * 128;
+    const bool cut = half && st == nk - 1;
+    dma16(p, wo[h][0] - (cut ? back[0] : 0u), dst0 + at);
+    dma16(p, wo[h][1] - (cut ? back[1] : 0u), dst0 + at + 1024u);
+  };
+  // scales of steps 2 g, 2 g + 1: 16 bytes of row (tid) of x or of the weight; near a row's end its last 16 bytes
+  const int xrow = int(args.xpitch / 16), wrow = int(a.pitch / 16);
+  const uint8_t* sbase;
+  {
+    const int r = tid & 255, most = tid < 256 ? xrows : wrows;
+    const int rr = r < most ? r : most - 1;
+    sbase = tid < 256 ? args.xscales + (m0 + rr) * xrow : a.scales + (c0 + rr) * wrow;
+  }
+  auto group_at = [](int g, int row) { return 16 * g < row - 16 ? 16 * g : row - 16; };
+  auto load_scales = [&](int g) {
+    const int last = (nk - 1) / 2, gg = g < last ? g : last;
+    const uint32_t to = __builtin_amdgcn_readfirstlane(uint32_t(kBgSOff + g % 3 * kBgScales) + 1024u * uint32_t(wave));
+    dma16_at(sbase + (wave < 4 ? group_at(gg, xrow) : group_at(gg, wrow)), to);
+  };
+  auto xoff = [](int b, int h) { return uint32_t(b * kBgStep + h * kBgHalf); };
+  auto woff = [](int b, int h) { return uint32_t(b * kBgStep + (2 + h) * kBgHalf); };
+  // operand reads: chunk 2 s + q of the lane's row is its block of product s
+  uint32_t xr[4], wrd[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    xr[s] = swz(uint32_t(64 * wr + i32), uint32_t(2 * s + q));
+    wrd[s] = swz(uint32_t(32 * wc + i32), uint32_t(2 * s + q));
+  }
+  f32x16 acc[2][2][2];  // quadrant (hm, hn), block mb
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i >> 2][(i >> 1) & 1][i & 1][r] = 0.0f;
+  u32x4 xa[2][4], w[2][4];
+  uint32_t xs[2][2], ws[2][2];  // scales of a row: products 0 and 1 in bytes 0 and 2 of the first, 2 and 3 of the second
+  // a step's scales: in its group's buffer, at the step's place in the row's 16 bytes
+  const uint32_t sx = uint32_t(kBgSOff + 16 * (64 * wr + i32)), sw = uint32_t(kBgSOff + 16 * (256 + 32 * wc + i32));
+  auto read_x = [&](int t, int b, int h) {
+    const uint32_t at = sx + uint32_t(t / 2 % 3 * kBgScales + 8 * t - group_at(t / 2, xrow));
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) xa[mb][s] = *reinterpret_cast<const u32x4*>(lds + xoff(b, h) + mb * 4096 + xr[s]);
+#pragma unroll
+      for (int d = 0; d < 2; ++d) xs[mb][d] = *reinterpret_cast<const uint32_t*>(lds + at + 16 * (128 * h + 32 * mb) + 4 * d) >> (8 * q);
+    }
+  };
+  auto read_w = [&](u32x4 (&o)[4], uint32_t (&so)[2], int step, int b, int h) {
+    const int t = step < nk ? step : nk - 1;
+    const uint32_t at = sw + uint32_t(t / 2 % 3 * kBgScales + 8 * t - group_at(t / 2, wrow));
+#pragma unroll
+    for (int s = 0; s < 4; ++s) o[s] = *reinterpret_cast<const u32x4*>(lds + woff(b, h) + wrd[s]);
+#pragma unroll
+    for (int d = 0; d < 2; ++d) so[d] = *reinterpret_cast<const uint32_t*>(lds + at + 16 * 128 * h + 4 * d) >> (8 * q);
+    if (half && t == nk - 1) so[1] = 0;
+  };
+  auto widen = [](const u32x4& v) { return i32x8{int(v.x), int(v.y), int(v.z), int(v.w), 0, 0, 0, 0}; };
+#define RQ_BG_MEM_END()                                                                 \
+  do {                                                                                  \
+    __builtin_amdgcn_sched_barrier(0);                                                  \
+    asm volatile("s_waitcnt vmcnt(12) lgkmcnt(0)\n\ts_barrier" ::: "memory");          \
+    __builtin_amdgcn_sched_barrier(0);                                                  \
+  } while (0)
+#define RQ_BG_MMA_END()                          \
+  do {                                           \
+    __builtin_amdgcn_sched_barrier(0);           \
+    asm volatile("s_barrier" ::: "memory");      \
+    __builtin_amdgcn_sched_barrier(0);           \
+  } while (0)
+#define RQ_BG_MMA1(C, W, WS, S)                                                                                             \
+  _Pragma("unroll") for (int mb = 0; mb < 2; ++mb) C[mb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                  \
+      widen(W[S]), widen(xa[mb][S]), C[mb], 4, 4, (S & 1) * 2, int(WS[S / 2]), (S & 1) * 2, int(xs[mb][S / 2]))
+#define RQ_BG_MMA(C, W, WS)         \
+  do {                              \
+    __builtin_amdgcn_s_setprio(1);  \
+    RQ_BG_MMA1(C, W, WS, 0);        \
+    RQ_BG_MMA1(C, W, WS, 1);        \
+    RQ_BG_MMA1(C, W, WS, 2);        \
+    RQ_BG_MMA1(C, W, WS, 3);        \
+    __builtin_amdgcn_s_setprio(0);  \
+  } while (0)
+  // step t in buffer F = t % 2, which is also the weight half it starts with, so that a step's first can be read
+  // while the step before multiplies by its other
+#define RQ_BG_STEP(t, F)                                             \
+  do {                                                               \
+    read_x(t, F, 0);                                                 \
+    load_w(F, (t) + 2, woff(F, F));                                  \
+    if ((F) == 0) load_scales((t) / 2 + 2);                          \
+    RQ_BG_MEM_END();                                                 \
+    RQ_BG_MMA(acc[0][F], w[F], ws[F]);                               \
+    RQ_BG_MMA_END();                                                 \
+    read_w(w[1 - (F)], ws[1 - (F)], t, F, 1 - (F));                  \
+    load_x(0, (t) + 2, xoff(F, 0));                                  \
+    RQ_BG_MEM_END();                                                 \
+    RQ_BG_MMA(acc[0][1 - (F)], w[1 - (F)], ws[1 - (F)]);             \
+    RQ_BG_MMA_END();                                                 \
+    read_x(t, F, 1);                                                 \
+    load_w(1 - (F), (t) + 2, woff(F, 1 - (F)));                      \
+    RQ_BG_MEM_END();                                                 \
+    RQ_BG_MMA(acc[1][1 - (F)], w[1 - (F)], ws[1 - (F)]);             \
+    RQ_BG_MMA_END();                                                 \
+    read_w(w[1 - (F)], ws[1 - (F)], (t) + 1, 1 - (F), 1 - (F));      \
+    load_x(1, (t) + 2, xoff(F, 1));                                  \
+    RQ_BG_MEM_END();                                                 \
+    RQ_BG_MMA(acc[1][F], w[F], ws[F]);                               \
+    RQ_BG_MMA_END();                                                 \
+  } while (0)
+  load_scales(0);
+  load_scales(1);
+  load_w(0, 0, woff(0, 0));
+  load_x(0, 0, xoff(0, 0));
+  load_w(1, 0, woff(0, 1));
+  load_x(1, 0, xoff(0, 1));
+  load_w(1, 1, woff(1, 1));
+  load_x(0, 1, xoff(1, 0));
+  load_w(0, 1, woff(1, 0));
+  load_x(1, 1, xoff(1, 1));
+  RQ_BG_MEM_END();
+  read_w(w[0], ws[0], 0, 0, 0);
+  RQ_BG_MEM_END();
+  if (wr == 1) RQ_BG_MMA_END();  // waves 4 - 7 run one slot behind
+  int t = 0;
+  for (; t + 2 <= nk; t += 2) {
+    RQ_BG_STEP(t, 0);
+    RQ_BG_STEP(t + 1, 1);
+  }
+  if (t < nk) RQ_BG_STEP(t, 0);
+  if (wr == 0) asm volatile("s_barrier" ::: "memory");
+  step_barrier<0>();
+#undef RQ_BG_STEP
+#undef RQ_BG_MMA
+#undef RQ_BG_MMA1
+#undef RQ_BG_MMA_END
+#undef RQ_BG_MEM_END
+
+  // Output: lane (i32, q) holds row i32 of a block, columns 8 h + 4 q .. + 3 in registers 4 h ..; the tile is
+  // staged in LDS and stored 512 bytes a row.
+  const int64_t left = a.cols - c0 < 256 ? a.cols - c0 : 256;
+  const __amdgpu_buffer_rsrc_t br =
+      buffer_rsrc(static_cast<const uint8_t*>(a.bias) + (a.bias ? c0 * 2 : 0), a.bias ? uint32_t(left * 2) : 0u);
+#pragma unroll
+  for (int hn = 0; hn < 2; ++hn)
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const int col = 128 * hn + 32 * wc + 8 * h + 4 * q;
+      float bias[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) bias[c] = from_x16<XT>(buf_load2(br, 2u * uint32_t(col + c)));
+#pragma unroll
+      for (int hm = 0; hm < 2; ++hm)
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+          float v[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] = __fadd_rn(acc[hm][hn][mb][4 * h + c], bias[c]);
+          *reinterpret_cast<u32x2*>(lds + (128 * hm + 64 * wr + 32 * mb + i32) * kBgPitch + 2 * col) =
+              u32x2{cvt_pk<XT>(v[0], v[1]), cvt_pk<XT>(v[2], v[3])};
+        }
+    }
+  __syncthreads();
+#pragma unroll 4
+  for (int it = 0; it < 16; ++it) {
+    const int r = 32 * wave + 2 * it + (lane >> 5);
+    if (r >= xrows) continue;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(lds + r * kBgPitch + 16 * (lane & 31));
+    const int64_t col = c0 + 8 * (lane & 31);
+    uint16_t* p = static_cast<uint16_t*>(a.y) + (m0 + r) * a.ldy + col;
+    if (col + 8 <= a.cols) store16_any(p, v);
+    else if (col < a.cols) store_edge<XT>(p, v, int(a.cols - col));
+  }
+}
+
 struct A4Plan {
   int bm, splits;
+  bool big;
+  int64_t xp;  // values of a row of x's codes
   int row_tiles, col_tiles;
   int64_t ld, codes_bytes, scales_bytes, part_bytes;
 };
@@ -227,9 +480,12 @@ A4Plan a4_plan(const MxCall& c, int cus) {
   s = s < 16 ? s : 16;
   if (getenv("SP")) s = atoi(getenv("SP"));
   p.splits = int(s > 1 ? s : 1);
+  p.big = p.bm == 256 && p.splits == 1 && c.dt != RQ_DTYPE_F32 && wp >= 512;
+  if (getenv("BIG")) p.big = p.big && atoi(getenv("BIG"));
   p.ld = (c.N + 3) / 4 * 4;
-  p.codes_bytes = up256(c.M * wp / 2);
-  p.scales_bytes = up256(c.M * wp / kMxBlock);
+  p.xp = p.big ? ceil_div(wp, 256) * 256 : wp;
+  p.codes_bytes = up256(c.M * p.xp / 2);
+  p.scales_bytes = up256(c.M * p.xp / kMxBlock);
   p.part_bytes = p.splits > 1 ? up256(int64_t(p.splits) * c.M * p.ld * 4) : 0;
   return p;
 }
@@ -265,9 +521,10 @@ int mx4_a4_run(const MxCall& c) {
   const int64_t wp = mx_pad(c.wk);
   uint8_t* xc = static_cast<uint8_t*>(c.scratch);
   uint8_t* xs = xc + p.codes_bytes;
-  const int st = mx4_quantize(c.x, c.dt, c.M, c.K, c.ldx, xc, xs, c.stream);
+  const int st = mx4_quantize(c.x, c.dt, c.M, c.K, c.ldx, xc, xs, p.xp, c.stream);
   if (st != RQ_OK) return st;
   A4Args a{};
+  a.xpitch = p.xp / 2;
   a.xscales = xs;
   a.g.x = xc;
   a.g.rows = c.rows;
@@ -286,6 +543,13 @@ int mx4_a4_run(const MxCall& c) {
   a.g.y = partial ? part : c.y;
   a.g.ldy = partial ? p.ld : c.ldy;
   const bool out32 = partial || c.dt == RQ_DTYPE_F32;
+  if (p.big) {
+    a.g.nk = int(ceil_div(wp, 256));
+    const unsigned grid = unsigned(p.row_tiles) * unsigned(p.col_tiles);
+    if (c.dt == RQ_DTYPE_F16) mx4_a4_big_kernel<RQ_DTYPE_F16><<<grid, kMgThreads, 0, c.stream>>>(a);
+    else mx4_a4_big_kernel<RQ_DTYPE_BF16><<<grid, kMgThreads, 0, c.stream>>>(a);
+    return rq_check_launch();
+  }
   if (c.dt == RQ_DTYPE_F16) a4_launch_bm<RQ_DTYPE_F16>(a, p.bm, out32, c.stream);
   else a4_launch_bm<RQ_DTYPE_BF16>(a, p.bm, out32, c.stream);
   if (partial) mx4_sum(MxSumArgs{static_cast<const float*>(part), c.M, p.ld, p.splits, 1, c.M, c.N, c.y, c.ldy}, c.dt, c.stream);

@@ -131,15 +131,16 @@ __global__ __launch_bounds__(kMxThreads) void mx4_dequantize_kernel(MxCodecArgs 
 }
 
 // Rows that lie end to end and are whole are one long row.
-int codec_args(int64_t rows, int64_t cols, int64_t ld, MxCodecArgs* a, dim3* grid, unsigned* threads) {
+int codec_args(int64_t rows, int64_t cols, int64_t ld, int64_t pitch, MxCodecArgs* a, dim3* grid, unsigned* threads) {
   if (rows < 0 || cols < 1 || ld < cols || cols > (int64_t(1) << 40) || rows > (int64_t(1) << 40)) return RQ_ERR_BAD_SHAPE;
   if (rows > 0 && cols > (int64_t(1) << 40) / rows) return RQ_ERR_UNSUPPORTED;
   *a = MxCodecArgs{rows, cols, ld, 0};
-  if (cols % kMxWhole == 0 && ld == cols && rows > 1) {
+  a->groups = pitch / kMxVals;
+  if (pitch == cols && ld == cols && rows > 1) {
     a->cols = a->ld = rows * cols;
+    a->groups *= rows;
     a->rows = 1;
   }
-  a->groups = mx_pad(a->cols) / kMxVals;
   *threads = a->groups <= 64 * kMxDepth ? 64 : a->groups <= 128 * kMxDepth ? 128 : kMxThreads;
   const int64_t blocks = ceil_div(a->groups, int64_t(*threads) * kMxDepth);
   if (blocks * *threads > kMaxThreads1D) return RQ_ERR_UNSUPPORTED;
@@ -150,11 +151,11 @@ int codec_args(int64_t rows, int64_t cols, int64_t ld, MxCodecArgs* a, dim3* gri
 }  // namespace
 
 int mx4_quantize(const void* x, int dt, int64_t rows, int64_t cols, int64_t ld, uint8_t* codes, uint8_t* scales,
-                 hipStream_t stream) {
+                 int64_t pitch, hipStream_t stream) {
   MxCodecArgs a{};
   dim3 grid;
   unsigned threads = 0;
-  const int st = codec_args(rows, cols, ld, &a, &grid, &threads);
+  const int st = codec_args(rows, cols, ld, pitch, &a, &grid, &threads);
   if (st != RQ_OK || rows == 0) return st;
   RQ_DISPATCH_DT(dt, XT, mx4_quantize_kernel<XT><<<grid, threads, 0, stream>>>(a, x, reinterpret_cast<uint32_t*>(codes), scales));
   return rq_check_launch();
@@ -168,7 +169,7 @@ extern "C" int rq_mx4_quantize(const void* x, int x_dtype, int64_t rows, int64_t
   if (!valid_float_dtype(x_dtype)) return RQ_ERR_BAD_DTYPE;
   if (rows > 0 && (!x || !codes || !scales)) return RQ_ERR_NULL_POINTER;
   if (!aligned(x, dtype_size(x_dtype)) || !aligned(codes, 16)) return RQ_ERR_BAD_ALIGNMENT;
-  return mx4_quantize(x, x_dtype, rows, cols, ldx, codes, scales, stream);
+  return mx4_quantize(x, x_dtype, rows, cols, ldx, codes, scales, mx_pad(cols), stream);
 }
 
 extern "C" int rq_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* out,
@@ -178,7 +179,7 @@ extern "C" int rq_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, in
   MxCodecArgs a{};
   dim3 grid;
   unsigned threads = 0;
-  const int st = codec_args(rows, cols, ldo, &a, &grid, &threads);
+  const int st = codec_args(rows, cols, ldo, mx_pad(cols), &a, &grid, &threads);
   if (st != RQ_OK || rows == 0) return st;
   if (!codes || !scales || !out) return RQ_ERR_NULL_POINTER;
   if (!aligned(out, dtype_size(out_dtype)) || !aligned(codes, 16)) return RQ_ERR_BAD_ALIGNMENT;

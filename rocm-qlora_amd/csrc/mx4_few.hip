@@ -354,7 +354,7 @@ int mx4_few_run(const MxCall& c) {
   if (c.a4) {
     uint8_t* xc = static_cast<uint8_t*>(c.scratch);
     uint8_t* xs = xc + up256(rows * a.wp / 2);
-    const int st = mx4_quantize(c.x, c.dt, rows, c.K, c.ldx, xc, xs, c.stream);
+    const int st = mx4_quantize(c.x, c.dt, rows, c.K, c.ldx, xc, xs, a.wp, c.stream);
     if (st != RQ_OK) return st;
     a.x = xc;
     a.ldx = a.wp / 2;

@@ -90,7 +90,8 @@ struct MxCall {
 
 inline int64_t up256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
-int mx4_quantize(const void* x, int dt, int64_t rows, int64_t cols, int64_t ld, uint8_t* codes, uint8_t* scales,
+// `pitch`: values of a row of codes, whole 128.
+int mx4_quantize(const void* x, int dt, int64_t rows, int64_t cols, int64_t ld, uint8_t* codes, uint8_t* scales, int64_t pitch,
                  hipStream_t stream);
 // A copy of rows, zeros up to `pitch` values (a multiple of 8).
 void mx4_rows_whole(const void* x, int dt, int64_t rows, int64_t cols, int64_t ld, void* out, int64_t pitch, hipStream_t stream);
