@@ -10,7 +10,6 @@
 // of a chunk meet no bank twice; the instruction picks byte 2 e of the row's scales,
 // shifted by q bytes.  The operands of a part are read while the part before is multiplied.
 #include "rq_mx4_gemm.h"
-#include <stdlib.h>
 
 namespace rq {
 namespace {
@@ -472,16 +471,13 @@ A4Plan a4_plan(const MxCall& c, int cus) {
   p.bm = c.M <= 64 ? 64 : c.M <= 128 ? 128 : 256;
   p.col_tiles = int(ceil_div(c.N, 256));
   while (p.bm > 128 && 2 * ceil_div(c.M, p.bm) * p.col_tiles <= cus) p.bm /= 2;
-  if (getenv("BM")) p.bm = atoi(getenv("BM"));
   p.row_tiles = int(ceil_div(c.M, p.bm));
   const int64_t steps = wp / kA4Step;
   int64_t s = cus / (int64_t(p.row_tiles) * p.col_tiles);
   s = s < steps / 4 ? s : steps / 4;
   s = s < 16 ? s : 16;
-  if (getenv("SP")) s = atoi(getenv("SP"));
   p.splits = int(s > 1 ? s : 1);
   p.big = p.bm == 256 && p.splits == 1 && c.dt != RQ_DTYPE_F32 && wp >= 512;
-  if (getenv("BIG")) p.big = p.big && atoi(getenv("BIG"));
   p.ld = (c.N + 3) / 4 * 4;
   p.xp = p.big ? ceil_div(wp, 256) * 256 : wp;
   p.codes_bytes = up256(c.M * p.xp / 2);
@@ -511,11 +507,7 @@ int64_t mx4_a4_scratch(const MxCall& c, int cus) {
   return p.codes_bytes + p.scales_bytes + p.part_bytes;
 }
 
-int mx4_a4_run(const MxCall& c) {
-  int cus = 0, dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
-    return RQ_ERR_HIP;
+int mx4_a4_run(const MxCall& c, int cus) {
   const A4Plan p = a4_plan(c, cus);
   if (int64_t(p.row_tiles) * p.col_tiles > (int64_t(1) << 22)) return RQ_ERR_UNSUPPORTED;
   const int64_t wp = mx_pad(c.wk);

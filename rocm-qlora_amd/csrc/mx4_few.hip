@@ -15,7 +15,6 @@
 // into the same fp32 sum.  Activations in 4 bits: x's codes and scales instead of values,
 // one v_mfma_scale_f32_16x16x128_f8f6f4 a step, nothing decoded.
 #include "rq_mx4.h"
-#include <stdlib.h>
 
 namespace rq {
 namespace {
@@ -315,8 +314,7 @@ int few_launch(const FewArgs& a, int most, hipStream_t stream) {
   // blocks of a workgroup: as many as still leave a workgroup or so for each compute unit (14336 columns beside
   // 16 rows: 25, 18 and 16 us with 1, 2 and 4; 4096 columns: 9, 11 and 14)
   const int64_t blocks = ceil_div(a.N, 16) * a.rows.T;
-  int nb = blocks > 768 ? 4 : blocks > 384 ? 2 : 1;
-  if (getenv("NB")) nb = atoi(getenv("NB"));
+  const int nb = blocks > 768 ? 4 : blocks > 384 ? 2 : 1;
   if (most <= 16) few_launch<XT, A4, 1>(a, nb, stream);
   else if (!A4 || most <= 32) few_launch<XT, A4, 2>(a, nb, stream);
   else few_launch<XT, A4, A4 ? 4 : 2>(a, nb, stream);

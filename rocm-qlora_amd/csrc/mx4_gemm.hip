@@ -28,17 +28,22 @@
 // columns 4 i + b, so that the four blocks' results of a lane are four adjacent outputs.  The
 // scales, transposed and as bf16 once a call (1 / 16 of the codes), come by the same ring.
 #include "rq_mx4_gemm.h"
-#include <stdlib.h>
 
 namespace rq {
 namespace {
 
 // WM x WN waves of 32 MB x 32 NB outputs each.
+//
+// 64 rows.  Forward: a step's products of a wave take 256 cycles, so a barrier is passed every second step only
+// and loads run six steps ahead (64 x 256 tiles, a step: 0.45 us with one step a barrier, three ahead).  dX: the two
+// waves of a column block would decode the same weights for half the rows each; instead each takes all rows and
+// half the quarters of every step (kShare), and they exchange half their sums at the end.
 template <bool DX, int BM_>
 struct MgTile {
   static constexpr int BM = BM_;
-  static constexpr int WM = DX ? (BM == 256 ? 4 : 2) : (BM == 64 ? 1 : 2);
-  static constexpr int WN = 8 / WM;
+  static constexpr int kShare = DX && BM == 64 ? 2 : 1;  // waves that share a block's contraction
+  static constexpr int WM = DX ? (BM == 256 ? 4 : BM == 128 ? 2 : 1) : (BM == 64 ? 1 : 2);
+  static constexpr int WN = 8 / (WM * kShare);
   static constexpr int MB = BM / (32 * WM);
   static constexpr int NB = DX ? 4 : (BM == 64 ? 1 : 2);
   static constexpr int BN = 32 * NB * WN;
@@ -46,12 +51,16 @@ struct MgTile {
   static constexpr int kWRow = DX ? BN / 2 : 32;               // bytes of a tile row of codes
   static constexpr int kWBytes = DX ? kMgStep * kWRow : BN * kWRow;
   static constexpr int kSBytes = DX ? BN / 32 * 128 : 0;       // scales of a step
-  static constexpr int kXRing = 4, kWRing = DX ? 3 : 4;
+  static constexpr int kSteps = !DX && BM == 64 ? 2 : 1;       // steps a barrier (forward)
+  static constexpr int kXRing = 4 * kSteps, kWRing = DX ? 3 : 4 * kSteps;
+  static constexpr int kAhead = kXRing - kSteps;               // steps that a step's loads are ahead of it
   static constexpr int kWOff = kXRing * kXBytes;
   static constexpr int kSOff = kWOff + kWRing * kWBytes;
   static constexpr int kRing = kSOff + kWRing * kSBytes;
-  static constexpr int kOutWave = mx_out_wave(MB, NB);
-  static constexpr int kLds = kRing > 8 * kOutWave ? kRing : 8 * kOutWave;
+  static constexpr int kOutWave = mx_out_wave(MB / kShare, NB);
+  static constexpr int kSwapWave = kShare == 2 ? 64 * 4 * 16 * NB : 0;  // bytes a wave hands to the one it shares with
+  static constexpr int kEnd = 8 * (kOutWave > kSwapWave ? kOutWave : kSwapWave);
+  static constexpr int kLds = kRing > kEnd ? kRing : kEnd;
   static constexpr int kXLoads = BM / 64, kWLoads = kWBytes / 8192;
   static constexpr int kLoads = kXLoads + kWLoads + (DX ? 1 : 0);  // of a wave and step
   static_assert(kLds <= 160 * 1024 && BN >= 256, "LDS plan");
@@ -68,7 +77,8 @@ void mx4_gemm_kernel(MxGemmArgs a) {
   lds_escapes(lds);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / T::WN, wn = wave % T::WN;
+  const int part = wave / (T::WM * T::WN);  // of a shared contraction
+  const int wm = wave / T::WN % T::WM, wn = wave % T::WN;
   const int i32 = lane & 31, q = lane >> 5;
 
   // tile of this workgroup: an XCD (workgroup % 8) takes a run of tiles, groups of four row tiles
@@ -195,8 +205,7 @@ void mx4_gemm_kernel(MxGemmArgs a) {
         if (i >= i0 && i < i1) dma16(p, xo[i], dst + 1024u * i);
     };
     auto load_x = [&](int j) { load_x_part(j, 0, T::kXLoads); };
-    // The loads of a step go out between its products, a part after each of the first three quarters (together
-    // after the barrier they kept all waves from their first product while the addresses went out).
+    // the loads of a step go out in parts, between its products
     constexpr int kHalfX = (T::kXLoads + 1) / 2;
     auto load_w = [&](int j) {
       int plane, kk;
@@ -226,7 +235,8 @@ void mx4_gemm_kernel(MxGemmArgs a) {
     auto read_x = [&](u32x4 (&o)[MB], int j, int s) {
       const uint8_t* p = lds + (j % T::kXRing) * T::kXBytes;
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) o[mb] = *reinterpret_cast<const u32x4*>(p + xr[s] + 4096 * mb);
+      for (int mb = 0; mb < MB; ++mb)
+        o[mb] = *reinterpret_cast<const u32x4*>(p + (T::kShare == 1 ? xr[s] : swz(uint32_t(i32), uint32_t(4 * q + s))) + 4096 * mb);
     };
     auto mma = [&](const u32x4 (&w)[NB], const u32x4 (&x)[MB]) {
 #pragma unroll
@@ -269,50 +279,60 @@ void mx4_gemm_kernel(MxGemmArgs a) {
       load_s(scn, kk + 8 < a.nk ? kk + 8 : 0);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) sc[nb] = u32x4{sc[nb].x >> 8 * q, sc[nb].y >> 8 * q, sc[nb].z >> 8 * q, sc[nb].w >> 8 * q};
-      load_x(1), load_w(1);
-      load_x(2), load_w(2);
-      step_barrier<2 * T::kLoads>();
+#pragma unroll
+      for (int p = 1; p < T::kAhead; ++p) {
+        load_x(p);
+        load_w(p);
+      }
+      step_barrier<(T::kAhead - 1) * T::kLoads>();
       read_x(xf[0], 0, 0);
       read_w(0);
       int left = (a.nk - kk < 8 ? a.nk - kk : 8);  // steps that sc is good for
-      for (int j = 0; j < nk; ++j) {
-        step_barrier<T::kLoads>();
-        if (left == 0) {
-          // the waits on these loads, 8 steps old, come before the step's own loads
-          left = a.nk - kk < 8 ? a.nk - kk : 8;
+      for (int j0 = 0; j0 < nk; j0 += T::kSteps) {  // (a split's steps are even in number)
+        // the steps up to the next barrier's first have landed
+        step_barrier<(T::kAhead - T::kSteps - 1) * T::kLoads>();
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            sc[nb] = u32x4{scn[nb].x >> 8 * q, scn[nb].y >> 8 * q, scn[nb].z >> 8 * q, scn[nb].w >> 8 * q};
-            asm volatile("" : "+v"(sc[nb].x), "+v"(sc[nb].y), "+v"(sc[nb].z), "+v"(sc[nb].w));
+        for (int u = 0; u < T::kSteps; ++u) {
+          const int j = j0 + u;
+          if (left == 0) {
+            // the waits on these loads, 8 steps old, come before the step's own loads
+            left = a.nk - kk < 8 ? a.nk - kk : 8;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              sc[nb] = u32x4{scn[nb].x >> 8 * q, scn[nb].y >> 8 * q, scn[nb].z >> 8 * q, scn[nb].w >> 8 * q};
+              asm volatile("" : "+v"(sc[nb].x), "+v"(sc[nb].y), "+v"(sc[nb].z), "+v"(sc[nb].w));
+            }
+            load_s(scn, kk + 8 < a.nk ? kk + 8 : 0);
           }
-          load_s(scn, kk + 8 < a.nk ? kk + 8 : 0);
-        }
-        float scale[NB];
+          float scale[NB];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) scale[nb] = mx_scale((sc[nb].x >> (16 * (kk & 1))) & 255u);
-        --left;
-        if (kk & 1) {
+          for (int nb = 0; nb < NB; ++nb) scale[nb] = mx_scale((sc[nb].x >> (16 * (kk & 1))) & 255u);
+          --left;
+          if (kk & 1) {
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) sc[nb] = u32x4{sc[nb].y, sc[nb].z, sc[nb].w, 0u};
-        }
-        if (++kk == a.nk) kk = 0;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          u32x4 w[NB];
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) w[nb] = mx_decode8<XT>(wraw[nb][s], scale[nb]);
-          if (s < 3) {
-            read_x(xf[(s + 1) & 1], j, s + 1);
-          } else {
-            read_x(xf[0], j + 1, 0);
-            read_w(j + 1);
+            for (int nb = 0; nb < NB; ++nb) sc[nb] = u32x4{sc[nb].y, sc[nb].z, sc[nb].w, 0u};
           }
-          __builtin_amdgcn_sched_barrier(0);
-          mma(w, xf[s & 1]);
-          __builtin_amdgcn_sched_barrier(0);
-          if (s == 0) load_x_part(j + 3, 0, kHalfX);
-          if (s == 1) load_x_part(j + 3, kHalfX, T::kXLoads);
-          if (s == 2) load_w(j + 3);
+          if (++kk == a.nk) kk = 0;
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            u32x4 w[NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) w[nb] = mx_decode8<XT>(wraw[nb][s], scale[nb]);
+            if (s < 3) {
+              read_x(xf[(s + 1) & 1], j, s + 1);
+            } else {
+              read_x(xf[0], j + 1, 0);
+              read_w(j + 1);
+            }
+            // (as it is written, but for 64 rows: 0.65 us a step of 128 x 256 so, 0.73 as the compiler mixes it; of 64
+            // rows 0.41 as the compiler mixes it)
+            if constexpr (BM > 64) __builtin_amdgcn_sched_barrier(0);
+            mma(w, xf[s & 1]);
+            if constexpr (BM > 64) __builtin_amdgcn_sched_barrier(0);
+            if (s == 0) load_x_part(j + T::kAhead, 0, kHalfX);
+            if (s == 1) load_x_part(j + T::kAhead, kHalfX, T::kXLoads);
+            if (s == 2) load_w(j + T::kAhead);
+          }
         }
       }
     } else {
@@ -334,18 +354,20 @@ void mx4_gemm_kernel(MxGemmArgs a) {
       load_w(1);
       load_x(2);
       step_barrier<T::kLoads>();
-      read_x(xf[0], 0, 0);
+      read_x(xf[0], 0, T::kShare == 1 ? 0 : 2 * part);
       for (int j = 0; j < nk; ++j) {
         step_barrier<T::kLoads>();
         const uint32_t wb = uint32_t(j % T::kWRing) * T::kWBytes, sb = uint32_t(j % T::kWRing) * T::kSBytes;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+        for (int g = 0; g < 4 / T::kShare; ++g) {
+          const int s = T::kShare == 1 ? g : 2 * part + g;  // the quarter
           const u32x4 sv = *reinterpret_cast<const u32x4*>(lds + sb + sr + 16 * s);
           u32x4 w[NB];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const s16x4 t4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(lds + wb + tr[s][h]));
+            const uint32_t at = T::kShare == 1 ? tr[s][h] : tr[g][h] + 2u * 8u * uint32_t(T::kWRow * part);
+            const s16x4 t4 =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + wb + at));
             const u32x2 v = __builtin_bit_cast(u32x2, t4);
 #pragma unroll
             for (int p = 0; p < 2; ++p) {  // rows 4 h + 2 p, + 1
@@ -359,14 +381,15 @@ void mx4_gemm_kernel(MxGemmArgs a) {
               w[3][2 * h + p] = __builtin_amdgcn_perm(b23, a23, 0x07060302u);
             }
           }
-          if (s < 3) read_x(xf[(s + 1) & 1], j, s + 1);
-          else read_x(xf[0], j + 1, 0);
+          constexpr int kLast = 4 / T::kShare - 1;
+          if (g < kLast) read_x(xf[(g + 1) & 1], j, s + 1);
+          else read_x(xf[0], j + 1, T::kShare == 1 ? 0 : 2 * part);
           __builtin_amdgcn_sched_barrier(0);
-          mma(w, xf[s & 1]);
+          mma(w, xf[g & 1]);
           __builtin_amdgcn_sched_barrier(0);
-          if (s == 0) load_w(j + 2);
-          if (s == 1) load_x_part(j + 3, 0, kHalfX);
-          if (s == 2) load_x_part(j + 3, kHalfX, T::kXLoads);
+          if (g == 0) load_w(j + 2);
+          if (g == (kLast > 0)) load_x_part(j + 3, 0, kHalfX);
+          if (g == (kLast > 1 ? 2 : kLast)) load_x_part(j + 3, kHalfX, T::kXLoads);
         }
       }
     }
@@ -374,8 +397,41 @@ void mx4_gemm_kernel(MxGemmArgs a) {
   }
   __syncthreads();
 
-  mx_output<XT, DX, MB, NB, OUT32>(a, acc, lds + wave * T::kOutWave, lane, e, live, split, slot0, count, 32 * MB * wm,
-                                   c0 + 32 * NB * wn);
+  if constexpr (T::kShare == 2) {
+    // block 1 - part of this wave's sums to its partner, whose own are added: wave `part` ends with block `part`
+    const int other = wave ^ (8 / T::kShare);
+    f32x4* to = reinterpret_cast<f32x4*>(lds + wave * T::kSwapWave);
+    const f32x4* from = reinterpret_cast<const f32x4*>(lds + other * T::kSwapWave);
+    f32x16 sum[1][NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum[0][nb][r] = part ? acc[1][nb][r] : acc[0][nb][r];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        f32x4 v;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = part ? acc[0][nb][4 * r + c] : acc[1][nb][4 * r + c];
+        to[64 * (4 * nb + r) + lane] = v;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 v = from[64 * (4 * nb + r) + lane];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[0][nb][4 * r + c] = __fadd_rn(sum[0][nb][4 * r + c], v[c]);
+      }
+    __syncthreads();
+    mx_output<XT, DX, 1, NB, OUT32>(a, sum, lds + wave * T::kOutWave, lane, e, live, split, slot0, count, 32 * part,
+                                    c0 + 32 * NB * wn);
+  } else {
+    mx_output<XT, DX, MB, NB, OUT32>(a, acc, lds + wave * T::kOutWave, lane, e, live, split, slot0, count, 32 * MB * wm,
+                                     c0 + 32 * NB * wn);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -506,29 +562,38 @@ MgPlan mg_plan(const MxCall& c, int cus) {
   p.x_bytes = p.copy ? up256(p.planes * p.xrows * p.xpitch * 2) : 0;
   p.np = ceil_div(c.N, kMgStep) * kMgStep;
   p.s_bytes = c.dx ? up256(c.E * (wp / kMxBlock) * p.np * 2) : 0;
-  // rows of a tile
+  // Rows of a tile, and splits of the contraction where the tiles leave compute units idle: the least of an
+  // estimate from measured times (us, each within 15 %): a launch, a step, a step's lengthening when all units
+  // work; a split's partial sums written and read at 4 TB/s by one more launch.  Forward 128 x 4096 -> 4096: 34,
+  // 26, 21 us with 64 rows and 1, 2, 4 splits, 48, 35, 27 with 128, 86, 55, 39 with 256.
   const int64_t groups = shared ? (c.E < c.M ? c.E : c.M) : 1;
-  const int64_t each = ceil_div(c.M, groups);
-  p.bm = each <= 64 ? 64 : each <= 192 ? 128 : 256;
-  auto tiles = [&](int bm) {
-    const int bn = c.dx ? (bm == 256 ? 256 : 512) : 256;
-    p.col_tiles = int(ceil_div(cols, bn));
-    return (shared ? ceil_div(c.M, bm) + groups / 2 : ceil_div(c.M, bm)) * p.col_tiles;
-  };
-  int64_t t = tiles(p.bm);
-  while (p.bm > 64 && t * 2 <= cus && p.bm / 2 >= each / 2) {
-    p.bm /= 2;
-    t = tiles(p.bm);
-  }
-  if (getenv("BM")) p.bm = atoi(getenv("BM"));
-  t = tiles(p.bm);
-  // splits of the contraction where the tiles leave compute units idle, 8 steps each at least
   const int64_t steps = p.planes * steps64;
-  int64_t s = cus / (t > 0 ? t : 1);
-  s = s < steps / 8 ? s : steps / 8;
-  s = s < 16 ? s : 16;
-  if (getenv("SP")) s = atoi(getenv("SP"));
-  p.splits = int(s > 1 ? s : 1);
+  double best = 0.0;
+  p.bm = 64;
+  p.splits = 1;
+  p.col_tiles = int(ceil_div(cols, c.dx ? 512 : 256));
+  for (int bm = 64; bm <= 256; bm *= 2) {
+    const double launch = c.dx ? 10.0 : bm == 64 ? 5.0 : bm == 128 ? 7.0 : 8.0;
+    const double step = c.dx ? (bm == 64 ? 0.92 : 1.43) : bm == 64 ? 0.41 : bm == 128 ? 0.65 : 1.2;
+    const double busy = c.dx || bm == 256 ? 0.25 : bm == 128 ? 0.35 : 0.4;
+    const int64_t bn = c.dx && bm < 256 ? 512 : 256;
+    // experts: about half a tile more each, a whole one for each that has fewer rows than a tile
+    const double each = double(c.M) / double(groups);
+    const double ends = shared ? double(groups) * (each >= bm ? 0.5 : 1.0 - 0.5 * each / bm) : 0.0;
+    const int64_t ct = ceil_div(cols, bn), tiles = (ceil_div(c.M, bm) + int64_t(ends)) * ct;
+    for (int s = 1; s <= 16 && (s == 1 || steps / s >= 4); s *= 2) {
+      const int64_t units = tiles * s;
+      const double full = units < cus ? double(units) / cus : 1.0;
+      const double sums = s > 1 || c.ysum > 1 ? 4.0 + double(s) * double(c.M) * double(cols) * 8.0 / 4e6 : 0.0;
+      const double t = launch + double(ceil_div(units, cus)) * double(ceil_div(steps, s)) * step * (1.0 + busy * full) + sums;
+      if (best == 0.0 || t < best) {
+        best = t;
+        p.bm = bm;
+        p.splits = s;
+        p.col_tiles = int(ct);
+      }
+    }
+  }
   p.row_tiles = int(!shared ? ceil_div(c.M, p.bm) : p.bm == 64 ? c.rows.T : c.rows.bigs(p.bm == 128 ? 0 : 1));
   p.partial = p.splits > 1 || c.ysum > 1;
   p.ld = (cols + 3) / 4 * 4;
@@ -571,11 +636,7 @@ int64_t mx4_gemm_scratch(const MxCall& c, int cus) {
   return p.x_bytes + p.s_bytes + p.part_bytes;
 }
 
-int mx4_gemm_run(const MxCall& c) {
-  int cus = 0, dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
-    return RQ_ERR_HIP;
+int mx4_gemm_run(const MxCall& c, int cus) {
   const MgPlan p = mg_plan(c, cus);
   if (int64_t(p.row_tiles) * p.col_tiles > (int64_t(1) << 22)) return RQ_ERR_UNSUPPORTED;
   uint8_t* ws = static_cast<uint8_t*>(c.scratch);

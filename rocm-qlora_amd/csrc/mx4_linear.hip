@@ -1,26 +1,21 @@
 // Entry points of the linears on MXFP4 weights: argument checks and the choice of kernel.
 #include "rq_mx4.h"
-#include <stdlib.h>
 
 namespace rq {
+
+int mx4_compute_units(int* cus);
+
 namespace {
 
-// Whether a forward call runs on the kernel for few rows: a weight's rows fit in its tile of 64;
-// experts: where they have 16 rows each at most on average (an expert's tile reads its weight
-// once, however few its rows).
+// Whether a forward call runs on the kernel for few rows.  One weight: up to 16 rows, or 32 where the contraction is
+// not long (us, this kernel and the tiles': 4096 -> 4096 with 16 rows 8 and 16, with 32 12 and 16; 8192 -> 2048 with
+// 24 rows 18 and 18, with 32 21 and 18; 14336 -> 4096 with 16 rows 22 and 21, with 24 30 and 22); 4-bit activations: up
+// to 64 (4096 -> 14336 with 48 rows 21 and 21, with 64 23 and 23; 4096 -> 4096 16 and 18, 17 and 20).  Experts: up to 4
+// rows each on average (8 of 4096 -> 14336 with 16 rows 67 and 106, with 32 98 and 111, with 64 103 and 86).
 bool few(const MxCall& c) {
   if (c.dx || ceil_div(c.M, c.xdiv) * mx_pad(c.wk) * int64_t(dtype_size(c.dt)) > int64_t(kMxFewBytes)) return false;
-  if (getenv("FEWM")) return c.M <= atoi(getenv("FEWM"));
-  if (!c.rows.p) return c.M <= kTileRows;
-  return c.M <= 16 * c.E;
-}
-
-int compute_units(int* cus) {
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
-    return RQ_ERR_HIP;
-  return RQ_OK;
+  if (c.rows.p) return c.M <= 4 * c.E;
+  return c.a4 ? c.M <= kTileRows : c.M <= 32 && c.M * mx_pad(c.wk) <= 24 * 8192;
 }
 
 // Sizes, whatever the pointers.  shared: rows of the product that one row of the narrower side stands for.
@@ -72,7 +67,7 @@ int run(MxCall& c, const void* x, int64_t plan_bytes, const uint8_t* codes, cons
       !aligned(c.rows.p, 16))
     return RQ_ERR_BAD_ALIGNMENT;
   int cus = 0;
-  const int st = compute_units(&cus);
+  const int st = mx4_compute_units(&cus);
   if (st != RQ_OK) return st;
   const int64_t need = scratch_of(c, cus);
   if (need > 0 && !scratch) return RQ_ERR_NULL_POINTER;
@@ -87,10 +82,25 @@ int run(MxCall& c, const void* x, int64_t plan_bytes, const uint8_t* codes, cons
   c.scratch = scratch;
   c.stream = stream;
   if (few(c)) return mx4_few_run(c);
-  return c.a4 ? mx4_a4_run(c) : mx4_gemm_run(c);
+  return c.a4 ? mx4_a4_run(c, cus) : mx4_gemm_run(c, cus);
 }
 
 }  // namespace
+
+// Of the current device, asked for once.
+int mx4_compute_units(int* cus) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return RQ_ERR_HIP;
+  if (dev < 64) {
+    *cus = known[dev].load(std::memory_order_relaxed);
+    if (*cus > 0) return RQ_OK;
+  }
+  if (hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return RQ_ERR_HIP;
+  if (dev < 64) known[dev].store(*cus, std::memory_order_relaxed);
+  return RQ_OK;
+}
+
 }  // namespace rq
 
 extern "C" int rq_mx4_linear_scratch_size(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, int grouped,
@@ -103,7 +113,7 @@ extern "C" int rq_mx4_linear_scratch_size(int dtype, int64_t M, int64_t K, int64
   if (ldx < (dx ? N : K)) return RQ_ERR_BAD_SHAPE;
   *bytes = 0;
   if (M == 0) return RQ_OK;
-  st = compute_units(&cus);
+  st = mx4_compute_units(&cus);
   if (st != RQ_OK) return st;
   static const int32_t some = 0;  // any non-null plan: sizes alone are asked for
   *bytes = scratch_of(call_of(dtype, M, K, N, E, shared, grouped ? &some : nullptr, act_bits, dx != 0, ldx, aligned16 != 0), cus);

@@ -99,9 +99,9 @@ void mx4_rows_whole(const void* x, int dt, int64_t rows, int64_t cols, int64_t l
 constexpr uint32_t kMxFewBytes = 0xFFFFFFE0u;  // (kOobOffset is past them)
 int64_t mx4_few_scratch(const MxCall& c);
 int mx4_few_run(const MxCall& c);
-int mx4_gemm_run(const MxCall& c);
+int mx4_gemm_run(const MxCall& c, int cus);
 int64_t mx4_gemm_scratch(const MxCall& c, int cus);
-int mx4_a4_run(const MxCall& c);
+int mx4_a4_run(const MxCall& c, int cus);
 int64_t mx4_a4_scratch(const MxCall& c, int cus);
 
 }  // namespace rq

@@ -1037,15 +1037,16 @@ def mx4_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     of x's rows ([..., K] fp32/bf16/fp16)."""
     dev = nat.require_gpu(x)
     code = nat.dtype_code(x.dtype)
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise RuntimeError(f"rows expected, got shape {tuple(x.shape)}")
-    K = x.shape[-1]
+    shape = x.shape
+    if len(shape) == 0 or shape[-1] == 0:
+        raise RuntimeError(f"rows expected, got shape {tuple(shape)}")
+    K = shape[-1]
     with on(dev):
         x2, ldx = _rows(x, K)
         M = x2.shape[0]
         pitch = mx4_pad(K)
-        codes = torch.empty((*x.shape[:-1], pitch // 2), dtype=torch.uint8, device=dev)
-        scales = torch.empty((*x.shape[:-1], pitch // MX4_BLOCK), dtype=torch.uint8, device=dev)
+        codes = torch.empty((*shape[:-1], pitch // 2), dtype=torch.uint8, device=dev)
+        scales = torch.empty((*shape[:-1], pitch // MX4_BLOCK), dtype=torch.uint8, device=dev)
         nat.call("rq_mx4_quantize", x2.data_ptr(), code, M, K, ldx, codes.data_ptr(), scales.data_ptr(), nat.stream_handle(dev))
     return codes, scales
 
@@ -1064,9 +1065,14 @@ def _check_mx4(codes: torch.Tensor, scales: torch.Tensor, K: int) -> None:
 
 def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, K: int, dtype: torch.dtype) -> torch.Tensor:
     """The values [..., K] that mx4_quantize's codes stand for."""
+    _check_mx4(codes, scales, K)
+    return _mx4_dequantize(codes, scales, K, dtype)
+
+
+def _mx4_dequantize(codes, scales, K, dtype):
+    """mx4_dequantize of codes and scales that fit."""
     dev = nat.require_gpu(codes, scales)
     code = nat.dtype_code(dtype)
-    _check_mx4(codes, scales, K)
     with on(dev):
         out = torch.empty((*codes.shape[:-1], K), dtype=dtype, device=dev)
         rows = out.numel() // K
@@ -1077,13 +1083,14 @@ def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, K: int, dtype: tor
 
 def _mx4_weight(codes: torch.Tensor, plan: Optional[torch.Tensor]) -> Tuple[int, int]:
     """Experts and rows of a weight: [N, Kp / 2] without a plan, [E, N, Kp / 2] with one."""
+    shape = codes.shape
     if plan is None:
-        if codes.dim() != 2:
-            raise RuntimeError(f"a weight's codes are [N, Kp / 2], got {tuple(codes.shape)}")
-        return 1, codes.shape[0]
-    if codes.dim() != 3:
-        raise RuntimeError(f"experts' codes are [E, N, Kp / 2], got {tuple(codes.shape)}")
-    return codes.shape[0], codes.shape[1]
+        if len(shape) != 2:
+            raise RuntimeError(f"a weight's codes are [N, Kp / 2], got {tuple(shape)}")
+        return 1, shape[0]
+    if len(shape) != 3:
+        raise RuntimeError(f"experts' codes are [E, N, Kp / 2], got {tuple(shape)}")
+    return shape[0], shape[1]
 
 
 def _mx4_bias(bias: Optional[torch.Tensor], dtype: torch.dtype, E: int, N: int, grouped: bool) -> Optional[torch.Tensor]:
@@ -1091,7 +1098,7 @@ def _mx4_bias(bias: Optional[torch.Tensor], dtype: torch.dtype, E: int, N: int, 
         return None
     if bias.shape != ((E, N) if grouped else (N,)):
         raise RuntimeError(f"bias must be {(E, N) if grouped else (N,)}, got {tuple(bias.shape)}")
-    return bias.detach().to(dtype).contiguous()
+    return bias if bias.dtype == dtype and bias.is_contiguous() else bias.detach().to(dtype).contiguous()
 
 
 def mx4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, K: int, bias: Optional[torch.Tensor] = None, *,
@@ -1106,14 +1113,16 @@ def mx4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, K: in
 def _mx4_linear(x, codes, scales, K, bias, activation_bits, plan, M):
     """mx4_linear on codes and scales that fit."""
     dev = nat.require_gpu(x, codes, scales, bias, plan)
-    code = nat.dtype_code(x.dtype)
+    dtype, shape = x.dtype, x.shape
+    code = nat.dtype_code(dtype)
     E, N = _mx4_weight(codes, plan)
-    if x.dim() != 2 or x.shape[1] != K:
-        raise RuntimeError(f"x must be rows of {K}, got {tuple(x.shape)}")
+    if len(shape) != 2 or shape[1] != K:
+        raise RuntimeError(f"x must be rows of {K}, got {tuple(shape)}")
     if activation_bits != 16 and activation_bits != 4:
         raise ValueError(f"activation_bits must be 4 or 16, got {activation_bits}")
-    R = x.shape[0]
-    grouped = shared = plan_bytes = 0
+    R = shape[0]
+    grouped = plan_bytes = 0
+    shared = 1
     if plan is None:
         M = R
     else:
@@ -1121,24 +1130,26 @@ def _mx4_linear(x, codes, scales, K, bias, activation_bits, plan, M):
         grouped, plan_bytes = 1, plan.numel()
         if activation_bits != 16:
             raise RuntimeError("experts' rows are multiplied in 16 bits or more")
-        if M != R and (R == 0 or M % R):
-            raise RuntimeError(f"{M} rows do not share {R} rows of x evenly")
+        if M != R:
+            if R == 0 or M % R:
+                raise RuntimeError(f"{M} rows do not share {R} rows of x evenly")
+            shared = M // R
     if bias is not None:
-        bias = _mx4_bias(bias, x.dtype, E, N, plan is not None)
+        bias = _mx4_bias(bias, dtype, E, N, plan is not None)
     with on(dev):
         if grouped and plan_bytes != _bytes("rq_adapter_rows_size", dev.index, M, E):
             raise RuntimeError(f"the rows by expert are not those of {M} rows and {E} experts")
-        y = torch.empty((M, N), dtype=x.dtype, device=dev)
+        y = x.new_empty((M, N))
         if M == 0 or N == 0:
             return y
         x, ldx = _rows(x, K)
-        shared = M // R
         xp = x.data_ptr()
         scratch = _scratch("rq_mx4_linear_scratch_size", dev, code, M, K, N, E, shared, grouped, activation_bits, 0, ldx,
                            xp % 16 == 0)
-        nat.call("rq_mx4_linear", xp, code, M, K, ldx, shared, nat.ptr(plan), plan_bytes,
-                 codes.data_ptr(), scales.data_ptr(), E, N, nat.ptr(bias), activation_bits, y.data_ptr(), N,
-                 nat.ptr(scratch), scratch.numel() if scratch is not None else 0, nat.stream_handle(dev))
+        nat.call("rq_mx4_linear", xp, code, M, K, ldx, shared, None if plan is None else plan.data_ptr(), plan_bytes,
+                 codes.data_ptr(), scales.data_ptr(), E, N, None if bias is None else bias.data_ptr(), activation_bits,
+                 y.data_ptr(), N, None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel(),
+                 nat.stream_handle(dev))
     return y
 
 

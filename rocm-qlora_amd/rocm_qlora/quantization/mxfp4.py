@@ -35,6 +35,13 @@ class MXFP4Tensor:
         ops._check_mx4(codes, scales, K)
         self.codes, self.scales, self.K = codes, scales, int(K)
 
+    @classmethod
+    def _of(cls, codes: torch.Tensor, scales: torch.Tensor, K: int) -> "MXFP4Tensor":
+        """Of codes and scales that fit."""
+        t = cls.__new__(cls)
+        t.codes, t.scales, t.K = codes, scales, K
+        return t
+
     @property
     def shape(self) -> torch.Size:
         return torch.Size((*self.codes.shape[:-1], self.K))
@@ -57,21 +64,21 @@ class MXFP4Tensor:
 def quantize_mxfp4(tensor: torch.Tensor) -> MXFP4Tensor:
     """tensor ([..., K] fp32/bf16/fp16) in MXFP4 blocks along its last dimension.  A CPU tensor
     is staged through the GPU and its codes are returned on the CPU, as quantize_int4's."""
-    if tensor.dim() == 0 or tensor.shape[-1] == 0:
-        raise RuntimeError(f"rows expected, got shape {tuple(tensor.shape)}")
-    src, home = to_gpu(tensor.detach())
-    codes, scales = ops.mx4_quantize(src)
-    if home != src.device:
-        codes, scales = codes.to(home), scales.to(home)
-    return MXFP4Tensor(codes, scales, tensor.shape[-1])
+    if tensor.is_cuda:
+        codes, scales = ops.mx4_quantize(tensor)
+    else:
+        src, home = to_gpu(tensor.detach())
+        codes, scales = (t.to(home) for t in ops.mx4_quantize(src))
+    return MXFP4Tensor._of(codes, scales, tensor.shape[-1])
 
 
 @eager_only
 def dequantize_mxfp4(t: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of t in `dtype` (exact in bf16 and fp32; in fp16 where it holds them)."""
+    if t.codes.is_cuda:
+        return ops._mx4_dequantize(t.codes, t.scales, t.K, dtype)
     codes, home = to_gpu(t.codes)
-    out = ops.mx4_dequantize(codes, t.scales.to(codes.device), t.K, dtype)
-    return out if home == codes.device else out.to(home)
+    return ops._mx4_dequantize(codes, t.scales.to(codes.device), t.K, dtype).to(home)
 
 
 class ExpertRows:
@@ -113,12 +120,13 @@ def _refuse_bias_gradient(bias: Optional[torch.Tensor], name: str) -> None:
 
 
 def _linear(x, codes, scales, K, bias, bits):
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    flat = x.dim() == 2
+    x2 = x if flat else x.reshape(-1, x.shape[-1])
     if dm._nothing_recorded_eagerly(x):
         y = ops._mx4_linear(x2, codes, scales, K, bias, bits, None, None)
     else:
         y = _MXFP4Linear.apply(x2, codes, scales, K, bias, bits, None)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[-1])
+    return y if flat else y.view(*x.shape[:-1], y.shape[-1])
 
 
 @eager_only
@@ -131,11 +139,11 @@ def mxfp4_linear(x: torch.Tensor, w: MXFP4Tensor, bias: Optional[torch.Tensor] =
     are multiplied as three bf16 parts each, which hold all their bits.
     activation_bits=4: x's rows are quantized as quantize_mxfp4 does first, and codes multiplied by codes.
     Differentiable by x: dX = dY w (activation_bits=4: as if x had not been rounded), once."""
-    _refuse_bias_gradient(bias, "mxfp4_linear")
-    if w.codes.dim() != 2:
-        raise RuntimeError(f"a weight [N, K] expected, got {w!r} (experts': mxfp4_expert_linear)")
-    if x.dim() == 0 or x.shape[-1] != w.K:
-        raise RuntimeError(f"x must be rows of {w.K}, got {tuple(x.shape)}")
+    if bias is not None:
+        _refuse_bias_gradient(bias, "mxfp4_linear")
+    shape = x.shape
+    if len(shape) == 0 or shape[-1] != w.K:
+        raise RuntimeError(f"x must be rows of {w.K}, got {tuple(shape)}")
     return _linear(x, w.codes, w.scales, w.K, bias, activation_bits)
 
 
