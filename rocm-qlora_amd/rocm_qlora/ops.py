@@ -1163,29 +1163,35 @@ def mx4_linear_dx(dy: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, K
 
 def _mx4_linear_dx(dy, codes, scales, K, plan, shared):
     """mx4_linear_dx on codes and scales that fit."""
-    dev = nat.require_gpu(dy, codes, scales, plan)
-    code = nat.dtype_code(dy.dtype)
+    nat.require_gpu(dy, codes, scales, plan)
     E, N = _mx4_weight(codes, plan)
     if dy.dim() != 2 or dy.shape[1] != N:
         raise RuntimeError(f"dY must be rows of {N}, got {tuple(dy.shape)}")
     M = dy.shape[0]
     if shared < 1 or M % shared or (plan is None and shared != 1):
         raise RuntimeError(f"{M} rows are not {shared} for each row of x")
-    grouped = plan_bytes = 0
-    with on(dev):
-        if plan is not None:
-            grouped, plan_bytes = 1, plan.numel()
-            if plan_bytes != _bytes("rq_adapter_rows_size", dev.index, M, E):
+    if plan is not None:
+        with on(dy.device):
+            if plan.numel() != _bytes("rq_adapter_rows_size", dy.device.index, M, E):
                 raise RuntimeError(f"the rows by expert are not those of {M} rows and {E} experts")
-        dx = torch.empty((M // shared, K), dtype=dy.dtype, device=dev)
+    return _mx4_dx(dy, codes, scales, K, E, N, plan, shared)
+
+
+def _mx4_dx(dy, codes, scales, K, E, N, plan, shared):
+    """mx4_linear_dx of operands that are known to fit (a backward pass's, which autograd has checked)."""
+    dev = dy.device
+    code = nat.dtype_code(dy.dtype)
+    M = dy.shape[0]
+    with on(dev):
+        dx = dy.new_empty((M // shared, K))
         if M == 0:
             return dx
         if N == 0:
             return dx.zero_()
         dy, lddy = _rows(dy, N)
         dp = dy.data_ptr()
-        scratch = _scratch("rq_mx4_linear_scratch_size", dev, code, M, K, N, E, shared, grouped, 16, 1, lddy, dp % 16 == 0)
-        nat.call("rq_mx4_linear_dx", dp, code, M, N, lddy, nat.ptr(plan), plan_bytes,
-                 codes.data_ptr(), scales.data_ptr(), E, K, shared, dx.data_ptr(), K,
-                 nat.ptr(scratch), scratch.numel() if scratch is not None else 0, nat.stream_handle(dev))
+        scratch = _scratch("rq_mx4_linear_scratch_size", dev, code, M, K, N, E, shared, plan is not None, 16, 1, lddy, dp % 16 == 0)
+        nat.call("rq_mx4_linear_dx", dp, code, M, N, lddy, None if plan is None else plan.data_ptr(),
+                 0 if plan is None else plan.numel(), codes.data_ptr(), scales.data_ptr(), E, K, shared, dx.data_ptr(), K,
+                 scratch.data_ptr(), scratch.numel(), nat.stream_handle(dev))
     return dx

@@ -97,21 +97,22 @@ class ExpertRows:
 
 
 class _MXFP4Linear(torch.autograd.Function):
+    """y by the linears' kernels, dX in the backward pass.  w: a weight's (codes, scales, K), frozen."""
+
     @staticmethod
-    def forward(ctx, x, codes, scales, K, bias, bits, rows):
-        ctx.save_for_backward(codes, scales)
-        plan = M = None
-        if rows is not None:
-            plan, M = rows.plan, rows.M
-        ctx.args = (K, plan, 1 if M is None or x.shape[0] == 0 else M // x.shape[0])
-        return ops._mx4_linear(x, codes, scales, K, bias, bits, plan, M)
+    def forward(ctx, x, w, bias, bits, rows):
+        codes, scales, K = w
+        if rows is None:
+            ctx.args = (codes, scales, K, 1, codes.shape[0], None, 1)
+            return ops._mx4_linear(x, codes, scales, K, bias, bits, None, None)
+        R = x.shape[0]
+        ctx.args = (codes, scales, K, codes.shape[0], codes.shape[1], rows.plan, rows.M // R if R else 1)
+        return ops._mx4_linear(x, codes, scales, K, bias, bits, rows.plan, rows.M)
 
     @staticmethod
     @first_order
     def backward(ctx, dy):
-        codes, scales = ctx.saved_tensors
-        K, plan, shared = ctx.args
-        return ops._mx4_linear_dx(dy, codes, scales, K, plan, shared), None, None, None, None, None, None
+        return ops._mx4_dx(dy, *ctx.args), None, None, None, None
 
 
 def _refuse_bias_gradient(bias: Optional[torch.Tensor], name: str) -> None:
@@ -125,7 +126,7 @@ def _linear(x, codes, scales, K, bias, bits):
     if dm._nothing_recorded_eagerly(x):
         y = ops._mx4_linear(x2, codes, scales, K, bias, bits, None, None)
     else:
-        y = _MXFP4Linear.apply(x2, codes, scales, K, bias, bits, None)
+        y = _MXFP4Linear.apply(x2, (codes, scales, K), bias, bits, None)
     return y if flat else y.view(*x.shape[:-1], y.shape[-1])
 
 
@@ -154,7 +155,7 @@ def _expert_linear(x, codes, scales, K, rows, bias):
         raise RuntimeError(f"weights of {rows.n} experts expected, got codes {tuple(codes.shape)}")
     if dm._nothing_recorded_eagerly(x):
         return ops._mx4_linear(x, codes, scales, K, bias, 16, rows.plan, rows.M)
-    return _MXFP4Linear.apply(x, codes, scales, K, bias, 16, rows)
+    return _MXFP4Linear.apply(x, (codes, scales, K), bias, 16, rows)
 
 
 @eager_only
