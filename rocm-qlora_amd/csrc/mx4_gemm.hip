@@ -42,7 +42,7 @@ template <bool DX, int BM_>
 struct MgTile {
   static constexpr int BM = BM_;
   static constexpr int kShare = DX && BM == 64 ? 2 : 1;  // waves that share a block's contraction
-  static constexpr int WM = DX ? (BM == 256 ? 4 : BM == 128 ? 2 : 1) : (BM == 64 ? 1 : 2);
+  static constexpr int WM = BM == 64 ? 1 : 2;
   static constexpr int WN = 8 / (WM * kShare);
   static constexpr int MB = BM / (32 * WM);
   static constexpr int NB = DX ? 4 : (BM == 64 ? 1 : 2);
@@ -68,59 +68,43 @@ struct MgTile {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+// The rows of row tile rt: slots slot0 .. + count - 1 of one expert (-1: none).
+struct MgRows {
+  int expert, count;
+  int64_t slot0;
+};
+template <int BM>
+__device__ __forceinline__ MgRows mg_rows(const MxGemmArgs& a, int rt) {
+  if (!a.rows.p) {
+    const int64_t slot0 = int64_t(BM) * rt;
+    return MgRows{0, a.rows.M - slot0 < BM ? int(a.rows.M - slot0) : BM, slot0};
+  }
+  int first = rt;  // 64-row tile
+  if constexpr (BM > kTileRows) first = a.rows.p[a.rows.off_big() + (BM == 256 ? a.rows.bigs(0) : 0) + rt];
+  const Tile tile = plan_tile(a.rows, first);
+  int count = tile.count;
+#pragma unroll
+  for (int j = 1; j < BM / kTileRows; ++j) {
+    if (first + j >= a.rows.T) break;
+    const Tile next = plan_tile(a.rows, first + j);
+    if (next.adapter != tile.adapter) break;
+    count += next.count;
+  }
+  return MgRows{__builtin_amdgcn_readfirstlane(tile.adapter), __builtin_amdgcn_readfirstlane(count), int64_t(kTileRows) * first};
+}
+
+// One tile: rows R, columns of column tile ct.
 template <int XT, bool DX, int BM, bool OUT32>
-__global__ __launch_bounds__(kMgThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void mx4_gemm_kernel(MxGemmArgs a) {
+__device__ __forceinline__ void mg_tile(const MxGemmArgs& a, uint8_t* lds, const MgRows& R, int ct) {
   using T = MgTile<DX, BM>;
   constexpr int MB = T::MB, NB = T::NB, BN = T::BN;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
-  lds_escapes(lds);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int part = wave / (T::WM * T::WN);  // of a shared contraction
   const int wm = wave / T::WN % T::WM, wn = wave % T::WN;
   const int i32 = lane & 31, q = lane >> 5;
-
-  // tile of this workgroup: an XCD (workgroup % 8) takes a run of tiles, groups of four row tiles
-  // walked column by column
-  int rt, ct;
-  {
-    int rows = a.row_tiles;  // a plan's: those in use
-    if (a.rows.p) rows = a.rows.p[BM == 64 ? 0 : BM == 128 ? 3 : 4];
-    const int G = rows * a.col_tiles, each = G / 8;
-    int t = blockIdx.x;
-    if (t >= G) return;
-    if (t < 8 * each) t = (t & 7) * each + (t >> 3);
-    constexpr int GM = 4;
-    const int per = GM * a.col_tiles, grp = t / per, r = t - grp * per;
-    const int gm = rows - grp * GM < GM ? rows - grp * GM : GM;
-    rt = grp * GM + r % gm;
-    ct = r / gm;
-  }
-  // its rows: slots slot0 .. + count - 1
-  int expert, count;
-  int64_t slot0;
-  if (a.rows.p) {
-    int first = rt;  // 64-row tile
-    if constexpr (BM > kTileRows) first = a.rows.p[a.rows.off_big() + (BM == 256 ? a.rows.bigs(0) : 0) + rt];
-    slot0 = int64_t(kTileRows) * first;
-    const Tile tile = plan_tile(a.rows, first);
-    expert = tile.adapter;
-    count = tile.count;
-#pragma unroll
-    for (int j = 1; j < BM / kTileRows; ++j) {
-      if (first + j >= a.rows.T) break;
-      const Tile next = plan_tile(a.rows, first + j);
-      if (next.adapter != expert) break;
-      count += next.count;
-    }
-    expert = __builtin_amdgcn_readfirstlane(expert);
-    count = __builtin_amdgcn_readfirstlane(count);
-  } else {
-    expert = 0;
-    slot0 = int64_t(BM) * rt;
-    count = a.rows.M - slot0 < BM ? int(a.rows.M - slot0) : BM;
-  }
+  const int expert = R.expert, count = R.count;
+  const int64_t slot0 = R.slot0;
   const bool live = expert >= 0;  // rows without an expert are zeros
   const int64_t e = live ? expert : 0;
   const int64_t c0 = int64_t(BN) * ct;  // first output column
@@ -434,6 +418,53 @@ void mx4_gemm_kernel(MxGemmArgs a) {
   }
 }
 
+// TAIL: no splits; tiles past the last whole round of compute units run as halves of their rows where these take
+// one round (a half tile's step takes 0.55 of a whole one's).
+template <int XT, bool DX, int BM, bool OUT32, bool TAIL>
+__global__ __launch_bounds__(kMgThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void mx4_gemm_kernel(MxGemmArgs a) {
+  static_assert(!TAIL || MgTile<DX, BM>::BN == MgTile<DX, BM / 2>::BN, "halves have the tile's columns");
+  constexpr int kLds = TAIL && MgTile<DX, BM / 2>::kLds > MgTile<DX, BM>::kLds ? MgTile<DX, BM / 2>::kLds : MgTile<DX, BM>::kLds;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
+  lds_escapes(lds);
+  int rows = a.row_tiles;  // a plan's: those in use
+  if (a.rows.p) rows = a.rows.p[BM == 64 ? 0 : BM == 128 ? 3 : 4];
+  const int G = rows * a.col_tiles;
+  // An XCD (workgroup % 8) takes a run of tiles, groups of four row tiles walked column by column.
+  auto run = [](int t, int n) { return t < n / 8 * 8 ? (t & 7) * (n / 8) + (t >> 3) : t; };
+  int t = blockIdx.x, half = -1;
+  const int rest = G % a.cus;
+  if (TAIL && 2 * rest <= a.cus) {
+    if (t >= G + rest) return;
+    if (t < G - rest) {
+      t = run(t, G - rest);
+    } else {
+      const int v = run(t - (G - rest), 2 * rest);
+      t = G - rest + (v >> 1);
+      half = v & 1;
+    }
+  } else {
+    if (t >= G) return;
+    t = run(t, G);
+  }
+  constexpr int GM = 4;
+  const int per = GM * a.col_tiles, grp = t / per, r = t - grp * per;
+  const int gm = rows - grp * GM < GM ? rows - grp * GM : GM;
+  MgRows R = mg_rows<BM>(a, grp * GM + r % gm);
+  const int ct = r / gm;
+  if constexpr (TAIL) {
+    if (half >= 0) {
+      R.slot0 += half * (BM / 2);
+      R.count -= half * (BM / 2);
+      if (R.count <= 0) return;
+      if (R.count > BM / 2) R.count = BM / 2;
+      mg_tile<XT, DX, BM / 2, OUT32>(a, lds, R, ct);
+      return;
+    }
+  }
+  mg_tile<XT, DX, BM, OUT32>(a, lds, R, ct);
+}
+
 // ---------------------------------------------------------------------------
 // Rows as the kernel reads them: 16 bits, 16-byte aligned, zeros up to `pitch` values;
 // fp32 rows in three planes of bf16 parts (least first).  by_slot: in the plan's order.
@@ -572,25 +603,28 @@ MgPlan mg_plan(const MxCall& c, int cus) {
   p.bm = 64;
   p.splits = 1;
   p.col_tiles = int(ceil_div(cols, c.dx ? 512 : 256));
-  for (int bm = 64; bm <= 256; bm *= 2) {
+  for (int bm = 64; bm <= (c.dx ? 128 : 256); bm *= 2) {
     const double launch = c.dx ? 10.0 : bm == 64 ? 5.0 : bm == 128 ? 7.0 : 8.0;
-    const double step = c.dx ? (bm == 64 ? 0.92 : 1.43) : bm == 64 ? 0.41 : bm == 128 ? 0.65 : 1.2;
-    const double busy = c.dx || bm == 256 ? 0.25 : bm == 128 ? 0.35 : 0.4;
-    const int64_t bn = c.dx && bm < 256 ? 512 : 256;
+    // a step of `units` workgroups on the compute units
+    auto step = [&](int b, int64_t units) {
+      const double alone = c.dx ? (b == 64 ? 0.92 : 1.43) : b == 64 ? 0.41 : b == 128 ? 0.65 : 1.2;
+      const double busy = c.dx || b == 256 ? 0.25 : b == 128 ? 0.35 : 0.4;
+      return alone * (1.0 + busy * (units < cus ? double(units) / cus : 1.0));
+    };
     // experts: about half a tile more each, a whole one for each that has fewer rows than a tile
     const double each = double(c.M) / double(groups);
     const double ends = shared ? double(groups) * (each >= bm ? 0.5 : 1.0 - 0.5 * each / bm) : 0.0;
-    const int64_t ct = ceil_div(cols, bn), tiles = (ceil_div(c.M, bm) + int64_t(ends)) * ct;
+    const int64_t ct = ceil_div(cols, c.dx ? 512 : 256), tiles = (ceil_div(c.M, bm) + int64_t(ends)) * ct;
     for (int s = 1; s <= 16 && (s == 1 || steps / s >= 4); s *= 2) {
-      const int64_t units = tiles * s;
-      const double full = units < cus ? double(units) / cus : 1.0;
+      const int64_t units = tiles * s, rest = units % cus;
+      double rounds = double(units / cus) * step(bm, cus);
+      if (rest > 0) rounds += s == 1 && bm > 64 && 2 * rest <= cus ? step(bm / 2, 2 * rest) : step(bm, units);
       const double sums = s > 1 || c.ysum > 1 ? 4.0 + double(s) * double(c.M) * double(cols) * 8.0 / 4e6 : 0.0;
-      const double t = launch + double(ceil_div(units, cus)) * double(ceil_div(steps, s)) * step * (1.0 + busy * full) + sums;
+      const double t = launch + rounds * double(ceil_div(steps, s)) + sums;
       if (best == 0.0 || t < best) {
         best = t;
         p.bm = bm;
         p.splits = s;
-        p.col_tiles = int(ct);
       }
     }
   }
@@ -603,16 +637,33 @@ MgPlan mg_plan(const MxCall& c, int cus) {
 
 template <int XT, bool DX, int BM>
 void mg_launch(const MxGemmArgs& a, bool out32, hipStream_t stream) {
-  const dim3 grid(unsigned(a.row_tiles) * unsigned(a.col_tiles), unsigned(a.splits));
-  if (out32) mx4_gemm_kernel<XT, DX, BM, true><<<grid, kMgThreads, 0, stream>>>(a);
-  else mx4_gemm_kernel<XT, DX, BM, false><<<grid, kMgThreads, 0, stream>>>(a);
+  const unsigned tiles = unsigned(a.row_tiles) * unsigned(a.col_tiles);
+  const dim3 grid(tiles, unsigned(a.splits));
+  if constexpr (BM > 64) {
+    if (a.splits == 1) {
+      // a tile's halves are two workgroups
+      const dim3 all(tiles + unsigned(a.cus));
+      if (out32) mx4_gemm_kernel<XT, DX, BM, true, true><<<all, kMgThreads, 0, stream>>>(a);
+      else mx4_gemm_kernel<XT, DX, BM, false, true><<<all, kMgThreads, 0, stream>>>(a);
+    } else {
+      mx4_gemm_kernel<XT, DX, BM, true, false><<<grid, kMgThreads, 0, stream>>>(a);  // partial sums
+    }
+  } else {
+    if (out32) mx4_gemm_kernel<XT, DX, BM, true, false><<<grid, kMgThreads, 0, stream>>>(a);
+    else mx4_gemm_kernel<XT, DX, BM, false, false><<<grid, kMgThreads, 0, stream>>>(a);
+  }
 }
 
-template <int XT, bool DX>
-void mg_launch_bm(const MxGemmArgs& a, int bm, bool out32, hipStream_t stream) {
-  if (bm == 64) mg_launch<XT, DX, 64>(a, out32, stream);
-  else if (bm == 128) mg_launch<XT, DX, 128>(a, out32, stream);
-  else mg_launch<XT, DX, 256>(a, out32, stream);
+template <int XT>
+void mg_launch(const MxGemmArgs& a, bool dx, int bm, bool out32, hipStream_t stream) {
+  if (dx) {
+    if (bm == 64) mg_launch<XT, true, 64>(a, out32, stream);
+    else mg_launch<XT, true, 128>(a, out32, stream);
+  } else {
+    if (bm == 64) mg_launch<XT, false, 64>(a, out32, stream);
+    else if (bm == 128) mg_launch<XT, false, 128>(a, out32, stream);
+    else mg_launch<XT, false, 256>(a, out32, stream);
+  }
 }
 
 dim3 rows_grid(int64_t rows, int64_t pitch) {
@@ -672,6 +723,7 @@ int mx4_gemm_run(const MxCall& c, int cus) {
   a.cols = c.dx ? c.wk : c.N;
   a.nk = int(p.xpitch / kMgStep);
   a.splits = p.splits;
+  a.cus = cus;
   a.row_tiles = p.row_tiles;
   a.col_tiles = p.col_tiles;
   a.bias = c.bias;
@@ -679,13 +731,8 @@ int mx4_gemm_run(const MxCall& c, int cus) {
   const bool out32 = p.partial || c.dt == RQ_DTYPE_F32;
   a.y = p.partial ? ws : c.y;
   a.ldy = p.partial ? p.ld : c.ldy;
-  if (c.dt == RQ_DTYPE_F16) {
-    if (c.dx) mg_launch_bm<RQ_DTYPE_F16, true>(a, p.bm, out32, c.stream);
-    else mg_launch_bm<RQ_DTYPE_F16, false>(a, p.bm, out32, c.stream);
-  } else {
-    if (c.dx) mg_launch_bm<RQ_DTYPE_BF16, true>(a, p.bm, out32, c.stream);
-    else mg_launch_bm<RQ_DTYPE_BF16, false>(a, p.bm, out32, c.stream);
-  }
+  if (c.dt == RQ_DTYPE_F16) mg_launch<RQ_DTYPE_F16>(a, c.dx, p.bm, out32, c.stream);
+  else mg_launch<RQ_DTYPE_BF16>(a, c.dx, p.bm, out32, c.stream);
   if (p.partial) {
     mx4_sum(MxSumArgs{reinterpret_cast<const float*>(ws), c.M, p.ld, p.splits, c.ysum, c.M / c.ysum, a.cols, c.y, c.ldy}, c.dt,
             c.stream);

@@ -25,6 +25,7 @@ struct MxGemmArgs {
   int64_t cols;           // of the output
   int nk;                 // steps of a plane
   int splits;
+  int cus;             // compute units
   int row_tiles, col_tiles;
   const void* bias;    // [E][cols]
   int bias_dt;
