@@ -23,6 +23,8 @@ def _export_dequant_layer(lora_linear: nn.Module) -> torch.Tensor:
     """[out, in] fp16 merged weight of one LoRALinear (gguf_export.py:30-79)."""
     if not isinstance(lora_linear, LoRALinear):
         raise TypeError(f"Expected LoRALinear, got {type(lora_linear)}")
+    if not hasattr(lora_linear.base_layer, "merged_weight"):
+        raise TypeError(f"a LoRALinear on a {type(lora_linear.base_layer).__name__} has no merged weight to export")
     return lora_linear.base_layer.merged_weight(lora_linear.lora_A, lora_linear.lora_B, lora_linear.scaling,
                                                 "round_then_sum", torch.float16)
 

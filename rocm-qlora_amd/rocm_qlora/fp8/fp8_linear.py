@@ -23,6 +23,7 @@ from rocm_qlora import torch_ops
 from rocm_qlora.fp8.fp8_config import detect_fp8_support, FP8Config
 from rocm_qlora.kernels import dequant_matmul as dm
 from rocm_qlora.lora.lora_layer import LoRALinear
+from rocm_qlora.quantization.mxfp4 import MXFP4Linear
 
 _FNUZ_MAX = 240.0
 
@@ -88,6 +89,9 @@ class FP8LinearWrapper(nn.Module):
         self.fp8_info = detect_fp8_support()
         if self.config.enabled and self.fp8_info["fp8_supported"] and self.fp8_info["fp8_dtypes_available"]:
             self.backend = "native"
+            held = getattr(base_lora_linear, "base_layer", None)
+            if isinstance(held, MXFP4Linear):
+                raise TypeError("an MXFP4Linear's weight is not multiplied in FP8: leave its LoRALinear unwrapped")
         else:
             self.backend = "bf16"
         self._cache_key = None

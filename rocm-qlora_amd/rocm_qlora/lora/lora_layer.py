@@ -87,6 +87,8 @@ class LoRALinear(nn.Module):
         unmerge_lora cannot restore the adapted layer; here it does)."""
         if self.merged:
             raise RuntimeError("LoRA already merged")
+        if not hasattr(self.base_layer, "merged_weight"):
+            raise TypeError(f"adapters merge into a QuantLinear, not into a {type(self.base_layer).__name__}")
         # one kernel: RND_fp16(W_deq + RND(RND(B @ A) * s)) from the quantized
         # buffers (double quantization included)
         merged = self.base_layer.merged_weight(self.lora_A, self.lora_B, self.scaling, "sum_then_round",

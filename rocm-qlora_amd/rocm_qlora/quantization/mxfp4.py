@@ -91,6 +91,8 @@ class ExpertRows:
     def __init__(self, ids: torch.Tensor, n: int):
         if ids.dim() not in (1, 2):
             raise RuntimeError(f"ids are [tokens] or [tokens, experts of a token], got {tuple(ids.shape)}")
+        if ids.dim() == 2 and ids.shape[1] == 0:
+            raise RuntimeError("ids name at least one expert a token")
         self.M, self.n = ids.numel(), int(n)
         self.k = 1 if ids.dim() == 1 else ids.shape[1]
         self.plan = ops.adapter_rows(ids.reshape(-1), self.n)
@@ -227,20 +229,21 @@ class MXFP4Experts(nn.Module):
     def from_weights(cls, weights: Union[torch.Tensor, nn.ModuleList, list], bias: Optional[torch.Tensor] = None) -> "MXFP4Experts":
         """From stacked weights [n, out, in] (and bias [n, out]), or a list of nn.Linear layers of one
         shape, quantized one expert at a time."""
+        layers = None
         if not isinstance(weights, torch.Tensor):
             layers = list(weights)
-            if not layers:
-                raise ValueError("no experts given")
-            if bias is None and any(m.bias is not None for m in layers):
-                if any(m.bias is None for m in layers):
-                    raise ValueError("all experts have a bias, or none")
-                bias = torch.stack([m.bias.detach() for m in layers])
             weights = [m.weight for m in layers]
         elif weights.dim() != 3:
             raise RuntimeError(f"weights must be [experts, out, in], got {tuple(weights.shape)}")
+        if len(weights) == 0:
+            raise ValueError("no experts given")
         out, cols = weights[0].shape
         if any(tuple(w.shape) != (out, cols) for w in weights):
             raise ValueError("experts' weights differ in shape")
+        if layers and bias is None and any(m.bias is not None for m in layers):
+            if any(m.bias is None for m in layers):
+                raise ValueError("all experts have a bias, or none")
+            bias = torch.stack([m.bias.detach() for m in layers])
         m = cls(len(weights), cols, out, bias is not None)
         held = [quantize_mxfp4(w) for w in weights]
         m.weight_quant = torch.stack([t.codes for t in held])
