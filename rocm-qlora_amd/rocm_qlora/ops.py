@@ -746,6 +746,7 @@ def adapter_rows(ids: torch.Tensor, n: int) -> torch.Tensor:
         ids = ids.contiguous()
         plan = _scratch("rq_adapter_rows_size", dev, M, n)
         nat.call("rq_adapter_rows", ids.data_ptr(), M, n, plan.data_ptr(), plan.numel(), nat.stream_handle(dev))
+    plan.grouped = (M, n)  # what it holds rows for: plans of other batches can have its size
     return plan
 
 
@@ -1093,6 +1094,12 @@ def _mx4_weight(codes: torch.Tensor, plan: Optional[torch.Tensor]) -> Tuple[int,
     return shape[0], shape[1]
 
 
+def _mx4_plan(plan: torch.Tensor, M: int, E: int) -> None:
+    """Refuses a plan of other rows, whose entries would lie outside the operands."""
+    if getattr(plan, "grouped", None) != (M, E):
+        raise RuntimeError(f"the rows by expert are not those of {M} rows and {E} experts, as adapter_rows returned them")
+
+
 def _mx4_bias(bias: Optional[torch.Tensor], dtype: torch.dtype, E: int, N: int, grouped: bool) -> Optional[torch.Tensor]:
     if bias is None:
         return None
@@ -1136,9 +1143,9 @@ def _mx4_linear(x, codes, scales, K, bias, activation_bits, plan, M):
             shared = M // R
     if bias is not None:
         bias = _mx4_bias(bias, dtype, E, N, plan is not None)
+    if grouped:
+        _mx4_plan(plan, M, E)
     with on(dev):
-        if grouped and plan_bytes != _bytes("rq_adapter_rows_size", dev.index, M, E):
-            raise RuntimeError(f"the rows by expert are not those of {M} rows and {E} experts")
         y = x.new_empty((M, N))
         if M == 0 or N == 0:
             return y
@@ -1171,9 +1178,7 @@ def _mx4_linear_dx(dy, codes, scales, K, plan, shared):
     if shared < 1 or M % shared or (plan is None and shared != 1):
         raise RuntimeError(f"{M} rows are not {shared} for each row of x")
     if plan is not None:
-        with on(dy.device):
-            if plan.numel() != _bytes("rq_adapter_rows_size", dy.device.index, M, E):
-                raise RuntimeError(f"the rows by expert are not those of {M} rows and {E} experts")
+        _mx4_plan(plan, M, E)
     return _mx4_dx(dy, codes, scales, K, E, N, plan, shared)
 
 

@@ -183,6 +183,16 @@ def test_calls_that_do_not_fit_are_refused():
             mxfp4_expert_linear(x, bad, rows)
 
 
+def test_plans_of_other_rows_are_refused():
+    """Also where the sizes are the same."""
+    plan = torch.zeros(16, dtype=torch.uint8)
+    plan.grouped = (16, 3)
+    ops._mx4_plan(plan, 16, 3)
+    for p, M, E in ((plan, 8, 3), (plan, 16, 4), (plan.clone(), 16, 3)):
+        with pytest.raises(RuntimeError, match="by expert"):
+            ops._mx4_plan(p, M, E)
+
+
 def test_the_oracle_against_the_format():
     """Every code and many scales by hand: the oracle's values are what the format defines, and quantizing them
     again gives them back."""

@@ -314,8 +314,7 @@ def test_rows_past_4_gib(dev):
     we, _ = weight(N, K, dev, lead=(3,))
     r = ExpertRows(routes(M, 2, 3, 1).to(dev), 3)
     assert torch.equal(mxfp4_expert_linear(x, we, r), mxfp4_expert_linear(near, we, r))
-    assert torch.equal(ops.mx4_linear_dx(far[:, :N], w.codes, w.scales, K), ops.mx4_linear_dx(far[:, :N].contiguous(), w.codes, w.scales, K)) \
-        if bool(far[:, :N].isfinite().all()) else True
+    assert torch.equal(ops.mx4_linear_dx(far[:, :N], w.codes, w.scales, K), ops.mx4_linear_dx(near[:, :N], w.codes, w.scales, K))
 
 
 # ---- layers, gradients against differences, streams, graphs -----------------------------
