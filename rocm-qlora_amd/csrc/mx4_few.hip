@@ -1,15 +1,17 @@
 // Few rows beside an MXFP4 weight (decoding): y = x W^T + bias, rows grouped by expert
 // or all of one weight.
 //
-// A workgroup takes 16 NB rows of the weight and a tile of at most 64 rows of x (rq_rows.h),
-// its eight waves chunks of four steps of 128 k in turn.  Lane (i, g) = (l % 16, l / 16)
-// loads block g of a step of weight row i, 16 bytes; the 4 x 4 dwords of four lane groups
-// are turned by four lane swaps, so that operand s of v_mfma_f32_16x16x32 is k = 32 s +
-// 8 g .. and a wave reads x in whole 64-byte pieces of its rows (in the order of the
-// blocks each 16-byte piece was a line of its own: 16 rows beside 14336 x 4096 took
-// 26 us).  A chunk's loads, x's among them, are issued before its first product; a weight
-// is read and decoded once for all 64 rows.  The waves' sums meet in LDS and are added in
-// wave order, 16 rows of x to a wave.
+// A workgroup takes 16 NB rows of the weight and a tile of at most 64 rows of x (rq_rows.h), its eight waves
+// two adjacent steps of 128 k of every sixteen each.  Lane (i, g) = (l % 16, l / 16) loads block g of a step of
+// weight row i, 16 bytes; the 4 x 4 dwords of four lane groups are turned by four lane swaps, so that operand s of
+// v_mfma_f32_16x16x32 is k = 32 s + 8 g .. and a wave reads x in whole 64-byte pieces of its rows (in the order of
+// the blocks each 16-byte piece was a line of its own: 16 rows beside 14336 x 4096 took 26 us).  A batch of steps'
+// loads, x's among them, are issued before its first product; a weight is read and decoded once for all rows of a
+// pass.  The waves' sums meet in LDS and are added in wave order, 16 rows of x to a wave.
+//
+// Bound by memory latency and by x, which every workgroup reads from the L2: 4096 -> 4096 with 1, 16 and 32 bf16 rows
+// 5.5, 8.1 and 12.9 us (1.6 TB/s of weight with 1), 4096 -> 14336 with 16 rows 12.8 us (2.4 TB/s), 64 experts'
+// 4096 -> 2048 with 64 rows 47 us (3.7 TB/s).
 //
 // fp32 rows: x = hi + mid + lo in bf16 (exact, rq_mx4.h), three products a value, all
 // into the same fp32 sum.  Activations in 4 bits: x's codes and scales instead of values,
@@ -51,9 +53,9 @@ __device__ __forceinline__ void turn4(u32x4& v) {
 
 // Steps of a batch, as registers allow.  One chunk of rows: a wave's whole share of a contraction of 4096
 // or, for 16 columns, 8192 is asked for at once (each batch waits for memory: 1.5 to 2 us).  More
-// chunks: two batches are in flight.
+// chunks: two batches are in flight, rows of all chunks among them.
 constexpr int few_depth(bool a4, bool f32, int ch, int nb, bool deep) {
-  int d = ch == 1 ? (deep ? 8 : 4) : nb == 1 ? (a4 ? 4 : 2) : nb == 2 ? 2 : 1;
+  int d = ch == 1 ? (deep ? 8 : 4) : nb == 1 ? (a4 && ch == 2 ? 4 : 2) : nb == 2 ? 2 : 1;
   return f32 && d > 1 ? d / 2 : d;
 }
 
@@ -97,14 +99,12 @@ void mx4_few_kernel(FewArgs a) {
     for (int d = 0; d < D; ++d) {
       const int st = step_of(b, d);
       const uint32_t off = uint32_t(i) * pitch + 16u * g + 64u * uint32_t(st);
-      const uint32_t soff = uint32_t(i) * spitch + 4u * uint32_t(st) + (A4 ? g : 0);
+      const uint32_t soff = uint32_t(i) * spitch + 4u * uint32_t(st);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         w.c[d][nb] = buf_load16(wr, st < steps ? off + 16u * nb * pitch : kOobOffset);
         const uint32_t at = st < steps ? soff + 16u * nb * spitch : kOobOffset;
-        if constexpr (A4) {
-          w.s[d][nb] = __builtin_amdgcn_raw_buffer_load_b8(sr, at, 0, 0);
-        } else if constexpr (D == 1) {
+        if constexpr (D == 1) {
           w.s[d][nb] = buf_load4(sr, at);
         } else if (d % 2 == 0) {  // two steps' (a 4-byte load of 16 rows costs as much as a 16-byte one)
           const u32x2 two = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(sr, at, 0, 0));
@@ -140,7 +140,7 @@ void mx4_few_kernel(FewArgs a) {
       row[c] = at < tile.count ? plan_row(a.rows, slot0 + at) : -1;
       const uint32_t r = uint32_t(row[c] < 0 ? 0 : row[c]) / uint32_t(a.xdiv);
       xo[c] = r * uint32_t(a.ldx * (A4 ? 1 : ES)) + (A4 ? 16u * g : uint32_t(8 * ES) * g);
-      xso[c] = A4 ? r * spitch + g : 0u;
+      xso[c] = A4 ? r * spitch : 0u;
     }
     struct X {
       u32x4 v[D][kX];
@@ -154,7 +154,14 @@ void mx4_few_kernel(FewArgs a) {
         const bool on = row[c] >= 0 && st < steps;
         if constexpr (A4) {
           x.v[d][0] = buf_load16(xr, on ? xo[c] + 64u * uint32_t(st) : kOobOffset);
-          x.s[d] = __builtin_amdgcn_raw_buffer_load_b8(xsr, on ? xso[c] + 4u * uint32_t(st) : kOobOffset, 0, 0);
+          const uint32_t at = on ? xso[c] + 4u * uint32_t(st) : kOobOffset;
+          if constexpr (D == 1) {
+            x.s[d] = buf_load4(xsr, at);
+          } else if (d % 2 == 0) {
+            const u32x2 two = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(xsr, at, 0, 0));
+            x.s[d] = two.x;
+            x.s[d + 1] = st + 1 < steps ? two.y : 0u;
+          }
         } else {
 #pragma unroll
           for (int s = 0; s < 4; ++s)
@@ -177,7 +184,8 @@ void mx4_few_kernel(FewArgs a) {
         for (int nb = 0; nb < NB; ++nb) {
           const u32x4& v = wv[nb][0];
           const i32x8 wa = {int(v.x), int(v.y), int(v.z), int(v.w), 0, 0, 0, 0};
-          acc[c][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xa, acc[c][nb], 4, 4, 0, int(wsc[nb]), 0, int(xsc));
+          acc[c][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xa, acc[c][nb], 4, 4, 0, int(wsc[nb] >> (8 * g)), 0,
+                                                                       int(xsc >> (8 * g)));
         }
       } else {
 #pragma unroll
@@ -232,30 +240,31 @@ void mx4_few_kernel(FewArgs a) {
         }
       }
     } else {
+      // a batch: the next one's weight and rows are asked for, then this one's are multiplied
       W wb[2];
-      X xb[2];
-      // a batch: the next one's weight and the next chunk's rows (or the next batch's) are asked for, then
-      // this one's are multiplied
-      auto batch = [&](int b, W& w, W& next) {
-        load_w(next, b + 1);
-        u32x4 wv[D][NB][A4 ? 1 : 4];  // for all chunks
+      X xb[2][CH];
+      auto load = [&](W& w, X (&x)[CH], int b) {
+        load_w(w, b);
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          if (c + 1 < CH) load_x(xb[(c + 1) & 1], b, c + 1);
-          else load_x(xb[0], b + 1, 0);
+        for (int c = 0; c < CH; ++c) load_x(x[c], b, c);
+      };
+      auto batch = [&](W& w, X (&x)[CH]) {
 #pragma unroll
-          for (int d = 0; d < D; ++d) {
-            if (c == 0) decode(w, d, wv[d]);
-            products(c, wv[d], w.s[d], xb[c & 1].v[d], xb[c & 1].s[d]);
-          }
+        for (int d = 0; d < D; ++d) {
+          u32x4 wv[NB][A4 ? 1 : 4];  // for all chunks
+          decode(w, d, wv);
+#pragma unroll
+          for (int c = 0; c < CH; ++c) products(c, wv, w.s[d], x[c].v[d], x[c].s[d]);
         }
       };
-      load_w(wb[0], 0);
-      load_x(xb[0], 0, 0);
-      for (int b = 0; b < batches; b += 2) {  // (an odd count's last one multiplies zeros)
-        batch(b, wb[0], wb[1]);
-        batch(b + 1, wb[1], wb[0]);
+      load(wb[0], xb[0], 0);
+      for (int b = 0; b + 2 <= batches; b += 2) {
+        load(wb[1], xb[1], b + 1);
+        batch(wb[0], xb[0]);
+        load(wb[0], xb[0], b + 2);
+        batch(wb[1], xb[1]);
       }
+      if (batches & 1) batch(wb[0], xb[0]);
     }
 #pragma unroll
     for (int c = 0; c < CH; ++c)
@@ -310,14 +319,26 @@ void few_launch(const FewArgs& a, int nb, hipStream_t stream) {
 }
 
 template <int XT, bool A4>
-int few_launch(const FewArgs& a, int most, hipStream_t stream) {
-  // blocks of a workgroup: as many as still leave a workgroup or so for each compute unit (14336 columns beside
-  // 16 rows: 25, 18 and 16 us with 1, 2 and 4; 4096 columns: 9, 11 and 14)
+int few_launch(const FewArgs& a, hipStream_t stream) {
+  // Blocks of a workgroup: as many as still leave a workgroup or so for each compute unit (14336 columns beside
+  // 16 rows: 25, 18 and 16 us with 1, 2 and 4; 4096 columns: 9, 11 and 14; 16 experts' 1024 columns of 2048 - 10 us with 2, 11
+  // with 4 - and 32's 13 and 15; their 2048 of 4096 21 and 20).
+  const bool grouped = a.rows.p != nullptr;
   const int64_t blocks = ceil_div(a.N, 16) * a.rows.T;
-  const int nb = blocks > 768 ? 4 : blocks > 384 ? 2 : 1;
-  if (most <= 16) few_launch<XT, A4, 1>(a, nb, stream);
-  else if (!A4 || most <= 32) few_launch<XT, A4, 2>(a, nb, stream);
-  else few_launch<XT, A4, A4 ? 4 : 2>(a, nb, stream);
+  const int nb = blocks > (grouped ? 1024 : 768) ? 4 : blocks > 384 ? 2 : 1;
+  // Chunks of a pass: all of one weight's rows (fp32 rows: at most 16 come here).  An expert has few rows: a chunk, and a
+  // pass more where it has more (64 experts' 2048 columns of 4096 beside 64 rows: 47 us, with two chunks a pass 66).
+  if constexpr (XT != RQ_DTYPE_F32 || A4) {
+    if (!grouped && a.rows.M > 32 && A4) {
+      few_launch<XT, A4, A4 ? 4 : 1>(a, nb, stream);
+      return rq_check_launch();
+    }
+    if (!grouped && a.rows.M > 16) {
+      few_launch<XT, A4, 2>(a, nb, stream);
+      return rq_check_launch();
+    }
+  }
+  few_launch<XT, A4, 1>(a, nb, stream);
   return rq_check_launch();
 }
 
@@ -348,7 +369,6 @@ int mx4_few_run(const MxCall& c) {
   a.bias = c.bias;
   a.y = c.y;
   a.ldy = c.ldy;
-  const int most = int(c.M < kTileRows ? c.M : kTileRows);
   if (c.a4) {
     uint8_t* xc = static_cast<uint8_t*>(c.scratch);
     uint8_t* xs = xc + up256(rows * a.wp / 2);
@@ -357,14 +377,14 @@ int mx4_few_run(const MxCall& c) {
     a.x = xc;
     a.ldx = a.wp / 2;
     a.xscales = xs;
-    RQ_DISPATCH_DT(c.dt, XT, return few_launch<XT, true>(a, most, c.stream));
+    RQ_DISPATCH_DT(c.dt, XT, return few_launch<XT, true>(a, c.stream));
   }
   if (few_copies(c)) {
     mx4_rows_whole(c.x, c.dt, rows, c.K, c.ldx, c.scratch, a.wp, c.stream);
     a.x = c.scratch;
     a.ldx = a.wp;
   }
-  RQ_DISPATCH_DT(c.dt, XT, return few_launch<XT, false>(a, most, c.stream));
+  RQ_DISPATCH_DT(c.dt, XT, return few_launch<XT, false>(a, c.stream));
   return RQ_OK;
 }
 

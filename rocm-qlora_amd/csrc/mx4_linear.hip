@@ -7,15 +7,16 @@ int mx4_compute_units(int* cus);
 
 namespace {
 
-// Whether a forward call runs on the kernel for few rows.  One weight: up to 16 rows, or 32 where the contraction is
-// not long (us, this kernel and the tiles': 4096 -> 4096 with 16 rows 8 and 16, with 32 12 and 16; 8192 -> 2048 with
-// 24 rows 18 and 18, with 32 21 and 18; 14336 -> 4096 with 16 rows 22 and 21, with 24 30 and 22); 4-bit activations: up
-// to 64 (4096 -> 14336 with 48 rows 21 and 21, with 64 23 and 23; 4096 -> 4096 16 and 18, 17 and 20).  Experts: up to 4
-// rows each on average (8 of 4096 -> 14336 with 16 rows 67 and 106, with 32 98 and 111, with 64 103 and 86).
+// Whether a forward call runs on the kernel for few rows (us, it and the tiles).  One weight: up to 32 rows where the
+// contraction is not long (4096 -> 4096 with 16 rows 8 and 16, with 32 13 and 16; 8192 -> 2048 with 24 rows 18 and 18, with 32
+// 21 and 18; 11008 -> 4096 with 16 rows 20 and 21, with 24 24 and 22); fp32 rows up to 16 (4096 -> 14336 with 16 rows 21 and 41,
+// with 24 54 and 42); 4-bit activations up to 64 (4096 -> 14336 with 33 rows 20 and 20, with 64 23 and 23; 4096 -> 4096 12
+// and 17, 14 and 20).  Experts: up to 8 rows each on average, fp32 rows 16 (16 of 4096 -> 2048 with 128 rows 24 and 44, with 256
+// 44 and 36; 64 of 4096 -> 8192 with 512 328 and 347, with 768 387 and 351; fp32 16 of 4096 -> 2048 with 256 rows 68 and 90).
 bool few(const MxCall& c) {
   if (c.dx || ceil_div(c.M, c.xdiv) * mx_pad(c.wk) * int64_t(dtype_size(c.dt)) > int64_t(kMxFewBytes)) return false;
-  if (c.rows.p) return c.M <= 4 * c.E;
-  return c.a4 ? c.M <= kTileRows : c.M <= 32 && c.M * mx_pad(c.wk) <= 24 * 8192;
+  if (c.rows.p) return c.M <= (c.dt == RQ_DTYPE_F32 ? 16 : 8) * c.E;
+  return c.a4 ? c.M <= kTileRows : c.M <= (c.dt == RQ_DTYPE_F32 ? 16 : 32) && c.M * mx_pad(c.wk) <= 24 * 8192;
 }
 
 // Sizes, whatever the pointers.  shared: rows of the product that one row of the narrower side stands for.
