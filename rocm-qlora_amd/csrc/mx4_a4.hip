@@ -9,6 +9,7 @@
 // 16 bytes, chunk c of row r stored at c ^ (r / 4) % 4, so that 16 consecutive rows' reads
 // of a chunk meet no bank twice; the instruction picks byte 2 e of the row's scales,
 // shifted by q bytes.  The operands of a part are read while the part before is multiplied.
+// Products of many tiles run on the second kernel below.  4096 x 4096 x 14336: 143 us (3.4 PFLOP/s), 10 more for x's codes.
 #include "rq_mx4_gemm.h"
 
 namespace rq {
@@ -62,43 +63,27 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
   return reinterpret_cast<const uint8_t*>(uint64_t(uniform(uint32_t(v >> 32))) << 32 | uniform(uint32_t(v)));
 }
 
+// Rows m0 .. + count - 1, 256 columns from c0, nk steps from kbeg.
 template <int XT, int BM, bool OUT32>
-__global__ __launch_bounds__(kMgThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void mx4_a4_kernel(A4Args args) {
+__device__ __forceinline__ void a4_tile(const A4Args& args, uint8_t* lds, int64_t m0, int count, int64_t c0, int split, int kbeg,
+                                        int nk) {
   using T = A4Tile<BM>;
   constexpr int MB = T::MB, NB = T::NB, BN = T::BN;
   const MxGemmArgs& a = args.g;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
-  lds_escapes(lds);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
   const int i32 = lane & 31, q = lane >> 5;
-  int rt, ct;
-  {
-    const int G = a.row_tiles * a.col_tiles;
-    int t = blockIdx.x;
-    if (G % 8 == 0) t = (t & 7) * (G / 8) + (t >> 3);
-    constexpr int GM = 4;
-    const int per = GM * a.col_tiles, grp = t / per, r = t - grp * per;
-    const int gm = a.row_tiles - grp * GM < GM ? a.row_tiles - grp * GM : GM;
-    rt = grp * GM + r % gm;
-    ct = r / gm;
-  }
-  const int64_t m0 = int64_t(BM) * rt, c0 = int64_t(BN) * ct;
-  const int count = a.rows.M - m0 < BM ? int(a.rows.M - m0) : BM;
-  const int split = blockIdx.y;
-  const int kbeg = int(int64_t(a.nk) * split / a.splits), nk = int(int64_t(a.nk) * (split + 1) / a.splits) - kbeg;
 
   // direct-to-LDS lanes: 16 rows an instruction; wave w brings the weight's rows 32 w .. and BM / 8 w .. of x
-  const uint8_t* xbase = a.x + m0 * a.pitch;
+  const uint8_t* xbase = a.x + m0 * args.xpitch;
   const uint8_t* wbase = a.codes + c0 * a.pitch;
   const int wrows = a.wrows - c0 < BN ? int(a.wrows - c0) : BN;
   uint32_t xo[T::kXLoads], wo[2];
 #pragma unroll
   for (int i = 0; i < T::kXLoads; ++i) {
     const int r = BM / 8 * wave + 16 * i + ((lane >> 2) & (BM == 64 ? 7 : 15));
-    xo[i] = uint32_t(r < count ? r : count - 1) * uint32_t(a.pitch) + 16u * (uint32_t(lane & 3) ^ ((r >> 2) & 3u));
+    xo[i] = uint32_t(r < count ? r : count - 1) * uint32_t(args.xpitch) + 16u * (uint32_t(lane & 3) ^ ((r >> 2) & 3u));
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -108,7 +93,7 @@ void mx4_a4_kernel(A4Args args) {
   // scales: lanes 0 .. 31 the weight's rows, the BM / 8 lanes after them x's
   const uint8_t* sp;
   {
-    const int64_t srow = a.pitch / 16;
+    const int64_t srow = lane < 32 ? a.pitch / 16 : args.xpitch / 16;
     int r = lane < 32 ? 32 * wave + lane : BM / 8 * wave + ((lane - 32) & (BM / 8 - 1));
     const int most = lane < 32 ? wrows : count;
     r = r < most ? r : most - 1;
@@ -212,6 +197,32 @@ void mx4_a4_kernel(A4Args args) {
                                       c0 + 32 * NB * wn);
 }
 
+// Tile t of n in order: an XCD (workgroup % 8) takes a run of tiles.
+__device__ __forceinline__ int a4_run(int t, int n) { return t < n / 8 * 8 ? (t & 7) * (n / 8) + (t >> 3) : t; }
+
+// Row and column tile of tile t: groups of four row tiles walked column by column.
+__device__ __forceinline__ void a4_place(const MxGemmArgs& a, int t, int& rt, int& ct) {
+  constexpr int GM = 4;
+  const int per = GM * a.col_tiles, grp = t / per, r = t - grp * per;
+  const int gm = a.row_tiles - grp * GM < GM ? a.row_tiles - grp * GM : GM;
+  rt = grp * GM + r % gm;
+  ct = r / gm;
+}
+
+template <int XT, int BM, bool OUT32>
+__global__ __launch_bounds__(kMgThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void mx4_a4_kernel(A4Args args) {
+  const MxGemmArgs& a = args.g;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[A4Tile<BM>::kLds];
+  lds_escapes(lds);
+  int rt, ct;
+  a4_place(a, a4_run(blockIdx.x, a.row_tiles * a.col_tiles), rt, ct);
+  const int64_t m0 = int64_t(BM) * rt;
+  const int split = blockIdx.y;
+  const int kbeg = int(int64_t(a.nk) * split / a.splits), nk = int(int64_t(a.nk) * (split + 1) / a.splits) - kbeg;
+  a4_tile<XT, BM, OUT32>(args, lds, m0, a.rows.M - m0 < BM ? int(a.rows.M - m0) : BM, int64_t(256) * ct, split, kbeg, nk);
+}
+
 // ---------------------------------------------------------------------------
 // Many rows: 256 x 256 tiles, 256 k a step.  A cache line of a row's codes is 256 k, and what bounds the kernel above
 // with many tiles is the number of lines it asks the L2 for (half a line of codes, and one more for
@@ -223,6 +234,10 @@ void mx4_a4_kernel(A4Args args) {
 // LDS reads and one half tile's loads (128 rows, 16 KiB); waves 4 - 7 run one phase slot behind waves 0 - 3, so
 // that of the two waves of a SIMD one reads while the other multiplies.  A half tile is refilled in the phase after its
 // last reads, two steps ahead of its next use, and the waits leave the youngest six in flight.
+//
+// Bound by what the L2 gives: 4096 x 8192 x 8192 at 3.7 PFLOP/s reads 1.7 GB from it in 138 us (12.4 TB/s), the matrix units
+// busy 49 to 55 %.  Four waves of 128 x 128 outputs, which read two thirds as much from LDS, took the same time to 3 %, and
+// bringing lines to the L2 four steps ahead took 6 % more.
 // ---------------------------------------------------------------------------
 constexpr int kBgHalf = 128 * 128;                    // bytes of a half tile
 constexpr int kBgStep = 4 * kBgHalf;                  // X0 X1 W0 W1
@@ -231,7 +246,7 @@ constexpr int kBgSOff = 2 * kBgStep;
 constexpr int kBgRing = kBgSOff + 3 * kBgScales;
 constexpr int kBgPitch = 256 * 2 + 16;                // the staged output tile's rows
 constexpr int kBgLds = kBgRing > 256 * kBgPitch ? kBgRing : 256 * kBgPitch;
-static_assert(kBgLds <= 160 * 1024, "LDS plan");
+static_assert(kBgLds <= 160 * 1024 && A4Tile<128>::kLds <= kBgLds, "LDS plan");
 
 template <int XT>
 __global__ __launch_bounds__(kMgThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -245,14 +260,18 @@ void mx4_a4_big_kernel(A4Args args) {
   const int i32 = lane & 31, q = lane >> 5;
   int rt, ct;
   {
-    const int G = a.row_tiles * a.col_tiles, each = G / 8;
-    int t = blockIdx.x;
-    if (t < 8 * each) t = (t & 7) * each + (t >> 3);
-    constexpr int GM = 4;
-    const int per = GM * a.col_tiles, grp = t / per, r = t - grp * per;
-    const int gm = a.row_tiles - grp * GM < GM ? a.row_tiles - grp * GM : GM;
-    rt = grp * GM + r % gm;
-    ct = r / gm;
+    // Tiles past the last whole round of compute units run as halves of their rows where these take one round, by the
+    // kernel above's steps (896 tiles of 4096 x 4096 x 14336: 146 -> 143 us).
+    const int G = a.row_tiles * a.col_tiles, rest = 2 * (G % a.cus) <= a.cus ? G % a.cus : 0, t = blockIdx.x;
+    if (t >= G - rest) {
+      const int v = a4_run(t - (G - rest), 2 * rest);
+      a4_place(a, G - rest + (v >> 1), rt, ct);
+      const int64_t m0 = int64_t(256) * rt + 128 * (v & 1);
+      const int count = a.rows.M - m0 < 128 ? int(a.rows.M - m0) : 128;
+      if (count > 0) a4_tile<XT, 128, false>(args, lds, m0, count, int64_t(256) * ct, 0, 0, int(a.pitch / 64));
+      return;
+    }
+    a4_place(a, a4_run(t, G - rest), rt, ct);
   }
   const int64_t m0 = int64_t(256) * rt, c0 = int64_t(256) * ct;
   const int xrows = a.rows.M - m0 < 256 ? int(a.rows.M - m0) : 256;
@@ -537,7 +556,9 @@ int mx4_a4_run(const MxCall& c, int cus) {
   const bool out32 = partial || c.dt == RQ_DTYPE_F32;
   if (p.big) {
     a.g.nk = int(ceil_div(wp, 256));
-    const unsigned grid = unsigned(p.row_tiles) * unsigned(p.col_tiles);
+    a.g.cus = cus;
+    const int tiles = p.row_tiles * p.col_tiles, rest = tiles % cus;
+    const unsigned grid = unsigned(tiles + (2 * rest <= cus ? rest : 0));
     if (c.dt == RQ_DTYPE_F16) mx4_a4_big_kernel<RQ_DTYPE_F16><<<grid, kMgThreads, 0, c.stream>>>(a);
     else mx4_a4_big_kernel<RQ_DTYPE_BF16><<<grid, kMgThreads, 0, c.stream>>>(a);
     return rq_check_launch();

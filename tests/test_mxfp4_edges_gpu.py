@@ -20,6 +20,14 @@ def test_tiles_past_the_last_whole_round(dev, M, K, N, dtype):
     check_linear(rows(M, K, dtype, dev), w, vals, rows(1, N, dtype, dev)[0])
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("M,K,N", [(4096, 512, 4100), (2300, 1100, 7700), (3900, 640, 4200)])
+def test_tiles_past_the_last_whole_round_4_bit_activations(dev, M, K, N, dtype):
+    """The same for both operands in 4 bits; lengths of half a step among them."""
+    w, vals = weight(N, K, dev)
+    check_linear(rows(M, K, dtype, dev), w, vals, rows(1, N, dtype, dev)[0], bits=4)
+
+
 @pytest.mark.parametrize("M,K,N", [(2048, 8500, 100), (2000, 8704, 130)])
 def test_gradient_tiles_past_the_last_whole_round(dev, M, K, N):
     w, vals = weight(N, K, dev)
