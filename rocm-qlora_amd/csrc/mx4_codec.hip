@@ -2,6 +2,7 @@
 // share a block, a lane holds 8 values of it (16 bytes of 16-bit values, one
 // instruction's 1 KiB a wave), the block's largest |x| is found by lane swaps, and
 // gfx950's own conversions, which take the power of two with them, round and pack.
+// 14336 x 4096 in bf16: 25.4 us to codes (5.9 TB/s), 22.7 back (6.5 TB/s; part of the codes still in the cache).
 #include "rq_mx4.h"
 
 namespace rq {
