@@ -71,10 +71,15 @@ void mx4_few_kernel(FewArgs a) {
   constexpr int D = few_depth(A4, XT == RQ_DTYPE_F32, CH, NB, DEEP);
   constexpr int kX = A4 ? 1 : 4 * P;  // 16-byte pieces of x of a lane and step
   __shared__ f32x4 red[kFwWaves][CH][NB][64];
-  const Tile tile = plan_tile(a.rows, blockIdx.y);
-  if (tile.count == 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
   const int i = lane & 15, g = lane >> 4;
+  // An expert's rows of the first pass, asked for beside the tile (of slots not in use: anything).  Not with NB = 4, whose
+  // 127 registers let two workgroups share a compute unit (64 experts' 2048 columns of 4096 beside 64 rows: 47 us, with
+  // registers for one 55).
+  constexpr bool kEarly = CH == 1 && NB < 4;
+  const int first = kEarly ? plan_row(a.rows, int64_t(kTileRows) * blockIdx.y + i) : 0;
+  const Tile tile = plan_tile(a.rows, blockIdx.y);
+  if (tile.count == 0) return;
   const int64_t n0 = int64_t(blockIdx.x) * (16 * NB);
   const int64_t expert = __builtin_amdgcn_readfirstlane(tile.adapter < 0 ? 0 : tile.adapter);
   const int64_t slot0 = int64_t(kTileRows) * blockIdx.y;
@@ -137,7 +142,7 @@ void mx4_few_kernel(FewArgs a) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int at = at0 + 16 * c + i;
-      row[c] = at < tile.count ? plan_row(a.rows, slot0 + at) : -1;
+      row[c] = at < tile.count ? (kEarly && at0 == 0 ? first : plan_row(a.rows, slot0 + at)) : -1;
       const uint32_t r = uint32_t(row[c] < 0 ? 0 : row[c]) / uint32_t(a.xdiv);
       xo[c] = r * uint32_t(a.ldx * (A4 ? 1 : ES)) + (A4 ? 16u * g : uint32_t(8 * ES) * g);
       xso[c] = A4 ? r * spitch : 0u;
