@@ -423,7 +423,9 @@ __device__ __forceinline__ void mg_tile(const MxGemmArgs& a, uint8_t* lds, const
 }
 
 // TAIL: no splits; tiles past the last whole round of compute units run as halves of their rows where these take
-// one round (a half tile's step takes 0.55 of a whole one's; 896 tiles of 4096 x 4096 x 14336: 3 % less, 2048 tokens' experts 5).
+// one round (a half tile's step takes 0.55 of a whole one's; 896 tiles of 4096 x 4096 x 14336: 3 % less, 2048 tokens' experts 5).  Tiles
+// of at most half their rows run as one half (experts 1 to 5 % less; one weight's dX, where it is one tile of each column,
+// 0 to 5 % more: not there).
 template <int XT, bool DX, int BM, bool OUT32, bool TAIL>
 __global__ __launch_bounds__(kMgThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void mx4_gemm_kernel(MxGemmArgs a) {
@@ -462,6 +464,8 @@ void mx4_gemm_kernel(MxGemmArgs a) {
       R.count -= half * (BM / 2);
       if (R.count <= 0) return;
       if (R.count > BM / 2) R.count = BM / 2;
+    }
+    if (half >= 0 || (R.count <= BM / 2 && (!DX || a.rows.p))) {
       mg_tile<XT, DX, BM / 2, OUT32>(a, lds, R, ct);
       return;
     }
