@@ -1,5 +1,7 @@
 """MXFP4 linears at their edges: outputs within larger rows, tiles that are split, long contractions, many experts,
 gradients of every layout, refusals, graphs side by side, and a block of routed experts that trains and serves."""
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
@@ -190,6 +192,67 @@ def test_two_graphs_at_once(dev):
         for _, held, work in sets:
             got = [t.clone() for t in held]
             assert all(torch.equal(a, b) for a, b in zip(got, work())), i
+
+
+def test_a_captured_backward_pass(dev):
+    """Forward and backward pass by autograd in one graph, its leaf made within it, replayed on other inputs."""
+    K, N, n, T = 384, 300, 4, 140
+    w, _ = weight(N, K, dev)
+    we, _ = weight(N, K, dev, lead=(n,))
+    x, dy = rows(T, K, BF16, dev), rows(2 * T, N, BF16, dev)
+    ids = routes(T, 2, n, 1).to(dev).to(torch.int32)
+
+    def step():
+        leaf = x.detach().requires_grad_(True)
+        y, z = mxfp4_linear(leaf, w), mxfp4_expert_linear(leaf, we, ExpertRows(ids, n))
+        (dx,) = torch.autograd.grad((y, z), leaf, (dy[:T], dy))
+        return y.detach(), z.detach(), dx
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        held = step()
+    for i in range(3):
+        x.copy_(rows(T, K, BF16, dev, 60 + i))
+        dy.copy_(rows(2 * T, N, BF16, dev, 70 + i))
+        ids.copy_(routes(T, 2, n, 80 + i).to(dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        assert all(torch.equal(a, b) for a, b in zip(got, step())), i
+
+
+def test_threads_at_once(dev):
+    """Calls and backward passes of three threads on streams of their own, the weights shared."""
+    K, N, n, T = 384, 300, 4, 130
+    w, _ = weight(N, K, dev)
+    we, _ = weight(N, K, dev, lead=(n,))
+
+    def work(seed):
+        x = rows(T, K, BF16, dev, seed).requires_grad_(True)
+        ids = routes(T, 2, n, seed).to(dev)
+        outs = []
+        for _ in range(10):
+            y, z = mxfp4_linear(x, w), mxfp4_expert_linear(x, we, ExpertRows(ids, n))
+            outs = [y, z, *torch.autograd.grad((y, z), x, (torch.ones_like(y), torch.ones_like(z)))]
+        return [t.detach() for t in outs]
+
+    want = [work(s) for s in range(3)]
+    torch.cuda.synchronize()
+
+    def on_own_stream(seed):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = work(seed)
+        torch.cuda.synchronize()
+        return got
+
+    with ThreadPoolExecutor(3) as pool:
+        for a, b in zip(want, pool.map(on_own_stream, range(3))):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
 # ---- a block of routed experts ----------------------------------------------------------
