@@ -488,19 +488,19 @@ struct MxRowsArgs {
   uint16_t* out;
 };
 
-// SPLIT: fp32 rows as three planes, else as they are.
+// SPLIT: fp32 rows as three planes, else as they are.  256 threads, workgroup (bx, by) of by_all rows of workgroups.
 template <int XT, bool SPLIT>
-__global__ __launch_bounds__(256) void mx4_rows_kernel(MxRowsArgs a) {
+__device__ __forceinline__ void mx4_rows(const MxRowsArgs& a, unsigned bx, unsigned by, unsigned by_all) {
   typedef typename Elem<XT>::T T;
   constexpr int V = Elem<XT>::kVec, P = 8 / V;
   const int64_t per = a.pitch / 8;
-  for (int64_t r = blockIdx.y; r < a.out_rows; r += gridDim.y) {
+  for (int64_t r = by; r < a.out_rows; r += by_all) {
     int64_t row = r;
     if (a.by_slot) {
       if (a.rows.p && plan_tile(a.rows, int(r / kTileRows)).count <= r % kTileRows) continue;
       row = plan_row(a.rows, r) / a.xdiv;
     }
-    const int64_t c8 = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t c8 = int64_t(bx) * 256 + threadIdx.x;
     if (c8 >= per) continue;
     const T* p = static_cast<const T*>(a.x) + row * a.ld + 8 * c8;
     u32x4 v[P];
@@ -530,21 +530,48 @@ __global__ __launch_bounds__(256) void mx4_rows_kernel(MxRowsArgs a) {
   }
 }
 
-// Scales for dX: bytes [E][N][nb] to bf16 [E][nb][np], 1.0 past N.
-__global__ __launch_bounds__(256) void mx4_scales_kernel(const uint8_t* in, uint16_t* out, int64_t N, int64_t nb, int64_t np) {
+template <int XT, bool SPLIT>
+__global__ __launch_bounds__(256) void mx4_rows_kernel(MxRowsArgs a) {
+  mx4_rows<XT, SPLIT>(a, blockIdx.x, blockIdx.y, gridDim.y);
+}
+
+// Scales for dX: bytes [E][N][nb] to bf16 [E][nb][np], 1.0 past N, 64 x 64 a workgroup.
+struct MxScalesArgs {
+  const uint8_t* in;
+  uint16_t* out;
+  int64_t N, nb, np;
+  unsigned gx, gy, all;  // pieces along n and the blocks, and in all
+};
+__device__ __forceinline__ void mx4_scales(const MxScalesArgs& a, unsigned first, unsigned step) {
   __shared__ uint8_t t[64][68];
-  const int64_t n0 = int64_t(blockIdx.x) * 64, b0 = int64_t(blockIdx.y) * 64, e = blockIdx.z;
-  for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-    const int r = i / 16, c = 4 * (i % 16);  // nb is a multiple of 4
-    uint32_t v = 0x7F7F7F7Fu;
-    if (n0 + r < N && b0 + c < nb) v = *reinterpret_cast<const uint32_t*>(in + (e * N + n0 + r) * nb + b0 + c);
-    *reinterpret_cast<uint32_t*>(&t[r][c]) = v;
+  for (unsigned piece = first; piece < a.all; piece += step) {
+    const int64_t n0 = int64_t(piece % a.gx) * 64, b0 = int64_t(piece / a.gx % a.gy) * 64, e = piece / a.gx / a.gy;
+    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+      const int r = i / 16, c = 4 * (i % 16);  // nb is a multiple of 4
+      uint32_t v = 0x7F7F7F7Fu;
+      if (n0 + r < a.N && b0 + c < a.nb) v = *reinterpret_cast<const uint32_t*>(a.in + (e * a.N + n0 + r) * a.nb + b0 + c);
+      *reinterpret_cast<uint32_t*>(&t[r][c]) = v;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
+      const int b = i / 32, r = 2 * (i % 32);
+      if (b0 + b >= a.nb || n0 + r >= a.np) continue;  // np is a multiple of 64
+      *reinterpret_cast<uint32_t*>(a.out + (e * a.nb + b0 + b) * a.np + n0 + r) = uint32_t(t[r][b]) << 7 | uint32_t(t[r + 1][b]) << 23;
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-    const int b = i / 32, r = 2 * (i % 32);
-    if (b0 + b >= nb || n0 + r >= np) continue;  // np is a multiple of 64
-    *reinterpret_cast<uint32_t*>(out + (e * nb + b0 + b) * np + n0 + r) = uint32_t(t[r][b]) << 7 | uint32_t(t[r + 1][b]) << 23;
+}
+
+__global__ __launch_bounds__(256) void mx4_scales_kernel(MxScalesArgs a) { mx4_scales(a, blockIdx.x, gridDim.x); }
+
+// Both, in one launch (4 us of a small call's time): workgroups 0 .. scales - 1, then the rows'.
+template <int XT>
+__global__ __launch_bounds__(256) void mx4_scales_rows_kernel(MxScalesArgs s, MxRowsArgs r, unsigned scales, unsigned gx, unsigned gy) {
+  if (blockIdx.x < scales) {
+    mx4_scales(s, blockIdx.x, scales);
+  } else {
+    const unsigned b = blockIdx.x - scales;
+    mx4_rows<XT, true>(r, b % gx, b / gx, gy);
   }
 }
 
@@ -707,14 +734,16 @@ int mx4_gemm_run(const MxCall& c, int cus) {
   a.xdiv = c.xdiv;
   a.by_slot = p.by_slot;
   a.rows = c.rows;
+  MxRowsArgs r{};
+  const dim3 rgrid = rows_grid(p.xrows, p.xpitch);
   if (p.copy) {
-    MxRowsArgs r{c.x, c.ldx, c.K, p.xrows, p.xpitch, p.xrows * p.xpitch, c.rows, c.xdiv, c.rows.p && p.by_slot,
-                 reinterpret_cast<uint16_t*>(ws)};
-    RQ_DISPATCH_DT(c.dt, XT, mx4_rows_kernel<XT, true><<<rows_grid(p.xrows, p.xpitch), 256, 0, c.stream>>>(r));
+    r = MxRowsArgs{c.x, c.ldx, c.K, p.xrows, p.xpitch, p.xrows * p.xpitch, c.rows, c.xdiv, c.rows.p && p.by_slot,
+                   reinterpret_cast<uint16_t*>(ws)};
     a.x = ws;
     a.ldx = p.xpitch * 2;
     a.plane = p.xrows * p.xpitch * 2;
     ws += p.x_bytes;
+    if (!c.dx) RQ_DISPATCH_DT(c.dt, XT, mx4_rows_kernel<XT, true><<<rgrid, 256, 0, c.stream>>>(r));
   }
   a.codes = c.codes;
   a.scales = c.scales;
@@ -723,8 +752,14 @@ int mx4_gemm_run(const MxCall& c, int cus) {
   a.np = p.np;
   if (c.dx) {
     const int64_t nb = wp / kMxBlock;
-    const dim3 grid(unsigned(p.np / 64), unsigned(ceil_div(nb, 64)), unsigned(c.E));
-    mx4_scales_kernel<<<grid, 256, 0, c.stream>>>(c.scales, reinterpret_cast<uint16_t*>(ws), c.N, nb, p.np);
+    const MxScalesArgs s{c.scales, reinterpret_cast<uint16_t*>(ws), c.N, nb, p.np, unsigned(p.np / 64), unsigned(ceil_div(nb, 64)),
+                         unsigned(p.np / 64 * ceil_div(nb, 64) * c.E)};
+    constexpr unsigned kMost = 1u << 22;  // workgroups of either
+    const unsigned scales = s.all < kMost ? s.all : kMost, gy = rgrid.y < kMost / rgrid.x ? rgrid.y : kMost / rgrid.x;
+    if (!p.copy) mx4_scales_kernel<<<scales, 256, 0, c.stream>>>(s);
+    else
+      RQ_DISPATCH_DT(c.dt, XT,
+                     mx4_scales_rows_kernel<XT><<<scales + rgrid.x * gy, 256, 0, c.stream>>>(s, r, scales, rgrid.x, gy));
     a.scales = ws;
     ws += p.s_bytes;
   }
