@@ -733,7 +733,7 @@ MAX_ADAPTERS = 1024  # kMaxAdapters in csrc/rq_rows.h
 def adapter_rows(ids: torch.Tensor, n: int) -> torch.Tensor:
     """The rows of a batch grouped by adapter: ids [M] int32 or int64 on the GPU, 0 ..
     n - 1 or, for a row without an adapter, anything else.  The result is what
-    multi_lora takes as `plan`."""
+    multi_lora and, for experts, mx4_linear take as `plan`."""
     dev = nat.require_gpu(ids)
     if ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"adapter ids must be int32 or int64, got {ids.dtype}")
