@@ -610,10 +610,16 @@ int rq_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows,
  *   [M, N] of `dtype`; bias [E, N] of it, or NULL.  The values of W are exact beside bf16 and fp32 rows and
  *   rounded to fp16 beside fp16 rows; sums are fp32, the result is rounded once.
  *   act_bits: 16, or 4: x's rows quantized as above first (one weight).
+ *   Sizes: K at most 2^24, K rounded up to 128 times N / 64 at most 2^29; dx: rows of dy past 2^25 values where there
+ *   are 64 of them or more (fewer rows: 2^31 values in all) are refused as unsupported.
  * rq_mx4_linear_dx: dx[t] = sum over r = t shared .. of dy[r] W[e].  scratch: 256-byte aligned, contents ignored; its
  * size is for rows of x (dx: of dy) of stride ldx whose first element is 16-byte aligned (aligned16) or not. */
 int rq_mx4_linear_scratch_size(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, int grouped,
                                int act_bits, int dx, int64_t ldx, int aligned16, int64_t* bytes);
+/* What the sizes run as: out[0..2] = rows of a tile (0: the kernel for few rows), splits of the contraction, whether
+ * the rows are copied first; for 256 compute units where there is no GPU. */
+int rq_mx4_tile_plan(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, int grouped, int act_bits, int dx,
+                     int64_t ldx, int aligned16, int32_t* out);
 int rq_mx4_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int64_t shared, const void* plan,
                   int64_t plan_bytes, const uint8_t* codes, const uint8_t* scales, int64_t E, int64_t N, const void* bias,
                   int act_bits, void* y, int64_t ldy, void* scratch, int64_t scratch_bytes, hipStream_t stream);

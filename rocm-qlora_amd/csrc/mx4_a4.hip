@@ -526,6 +526,13 @@ int64_t mx4_a4_scratch(const MxCall& c, int cus) {
   return p.codes_bytes + p.scales_bytes + p.part_bytes;
 }
 
+void mx4_a4_tiles(const MxCall& c, int cus, int32_t* out) {
+  const A4Plan p = a4_plan(c, cus);
+  out[0] = p.bm;
+  out[1] = p.splits;
+  out[2] = 1;
+}
+
 int mx4_a4_run(const MxCall& c, int cus) {
   const A4Plan p = a4_plan(c, cus);
   if (int64_t(p.row_tiles) * p.col_tiles > (int64_t(1) << 22)) return RQ_ERR_UNSUPPORTED;

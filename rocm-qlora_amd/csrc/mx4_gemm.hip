@@ -139,7 +139,7 @@ __device__ __forceinline__ void mg_tile(const MxGemmArgs& a, uint8_t* lds, const
       const int rr = r < count ? r : count - 1;  // a live row again where there is none
       const uint32_t c = uint32_t(16 * ((lane & 7) ^ ((r >> 1) & 7)));
       const uint32_t row = a.by_slot ? uint32_t(rr) : uint32_t(plan_row(a.rows, slot0 + rr)) / uint32_t(a.xdiv);
-      xo[i] = row * uint32_t(a.ldx) + c;  // the host keeps it under 4 GiB
+      xo[i] = row * uint32_t(a.ldx) + c;  // (mg_plan takes no more rows than keep it under 4 GiB)
     }
     const uint32_t xdst = __builtin_amdgcn_readfirstlane(uint32_t(BM / 8 * wave) * 128u);
     // Codes.  Forward: rows of 32 bytes, wave w rows 32 w .. (+ 256 an instruction), chunk c of
@@ -628,6 +628,9 @@ MgPlan mg_plan(const MxCall& c, int cus) {
   p.x_bytes = p.copy ? up256(p.planes * p.xrows * p.xpitch * 2) : 0;
   p.np = ceil_div(c.N, kMgStep) * kMgStep;
   p.s_bytes = c.dx ? up256(c.E * (wp / kMxBlock) * p.np * 2) : 0;
+  // A copy that is read by slot is as long as its rows: the tile's rows are those that 32-bit offsets reach
+  // (64 always are, mx4_row_tiles_fit).
+  auto reached = [&](int bm) { return !p.copy || !p.by_slot || (c.M < bm ? c.M : bm) * p.xpitch * 2 <= far; };
   // Rows of a tile, and splits of the contraction where the tiles leave compute units idle: the least of an
   // estimate from measured times (us, each within 15 %): a launch, a step, a step's lengthening when all units
   // work; a split's partial sums written and read at 4 TB/s by one more launch.  Forward 128 x 4096 -> 4096: 34,
@@ -638,7 +641,7 @@ MgPlan mg_plan(const MxCall& c, int cus) {
   p.bm = 64;
   p.splits = 1;
   p.col_tiles = int(ceil_div(cols, c.dx ? 512 : 256));
-  for (int bm = 64; bm <= (c.dx ? 128 : 256); bm *= 2) {
+  for (int bm = 64; bm <= (c.dx ? 128 : 256) && (bm == 64 || reached(bm)); bm *= 2) {
     const double launch = c.dx ? 10.0 : bm == 64 ? 5.0 : bm == 128 ? 7.0 : 8.0;
     // a step of `units` workgroups on the compute units
     auto step = [&](int b, int64_t units) {
@@ -720,6 +723,13 @@ void mx4_sum(const MxSumArgs& s, int dt, hipStream_t stream) {
 int64_t mx4_gemm_scratch(const MxCall& c, int cus) {
   const MgPlan p = mg_plan(c, cus);
   return p.x_bytes + p.s_bytes + p.part_bytes;
+}
+
+void mx4_gemm_tiles(const MxCall& c, int cus, int32_t* out) {
+  const MgPlan p = mg_plan(c, cus);
+  out[0] = p.bm;
+  out[1] = p.splits;
+  out[2] = p.copy;
 }
 
 int mx4_gemm_run(const MxCall& c, int cus) {

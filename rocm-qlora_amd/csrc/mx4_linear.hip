@@ -19,16 +19,22 @@ bool few(const MxCall& c) {
   return c.a4 ? c.M <= kTileRows : c.M <= (c.dt == RQ_DTYPE_F32 ? 16 : 32) && c.M * mx_pad(c.wk) <= 24 * 8192;
 }
 
+// Whether a tile of 64 rows of dY, or of all there are, lies within 32-bit offsets of its first (rows of x always do: K
+// is at most 2^24).
+bool mx4_row_tiles_fit(int64_t M, int64_t N) {
+  return (M < kTileRows ? M : kTileRows) * ceil_div(N, 64) * 64 <= int64_t(1) << 31;
+}
+
 // Sizes, whatever the pointers.  shared: rows of the product that one row of the narrower side stands for.
-int check_sizes(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, bool grouped, int act_bits) {
+int check_sizes(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, bool grouped, int act_bits, bool dx) {
   if (!valid_float_dtype(dtype)) return RQ_ERR_BAD_DTYPE;
   if (M < 0 || K < 1 || N < 1 || E < 1 || shared < 1 || M % shared != 0) return RQ_ERR_BAD_SHAPE;
   if (act_bits != 16 && act_bits != 4) return RQ_ERR_UNSUPPORTED;
   if (!grouped && (E != 1 || shared != 1)) return RQ_ERR_BAD_SHAPE;
   if (grouped && act_bits == 4) return RQ_ERR_UNSUPPORTED;
-  // 32-bit offsets within a tile's rows and a weight's scales
+  // 32-bit offsets within 64 rows of a tile (mg_plan: taller tiles) and a weight's scales
   if (E > kMaxAdapters || M > (int64_t(1) << 30) || K > (int64_t(1) << 24) || N > (int64_t(1) << 30) ||
-      mx_pad(K) * ceil_div(N, 64) > (int64_t(1) << 29))
+      mx_pad(K) * ceil_div(N, 64) > (int64_t(1) << 29) || (dx && !mx4_row_tiles_fit(M, N)))
     return RQ_ERR_UNSUPPORTED;
   return RQ_OK;
 }
@@ -109,7 +115,7 @@ extern "C" int rq_mx4_linear_scratch_size(int dtype, int64_t M, int64_t K, int64
   using namespace rq;
   if (!bytes) return RQ_ERR_NULL_POINTER;
   int cus = 0;
-  int st = check_sizes(dtype, M, K, N, E, shared, grouped != 0, act_bits);
+  int st = check_sizes(dtype, M, K, N, E, shared, grouped != 0, act_bits, dx != 0);
   if (st != RQ_OK) return st;
   if (ldx < (dx ? N : K)) return RQ_ERR_BAD_SHAPE;
   *bytes = 0;
@@ -121,12 +127,29 @@ extern "C" int rq_mx4_linear_scratch_size(int dtype, int64_t M, int64_t K, int64
   return RQ_OK;
 }
 
+extern "C" int rq_mx4_tile_plan(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, int grouped, int act_bits,
+                                int dx, int64_t ldx, int aligned16, int32_t* out) {
+  using namespace rq;
+  if (!out) return RQ_ERR_NULL_POINTER;
+  const int st = check_sizes(dtype, M, K, N, E, shared, grouped != 0, act_bits, dx != 0);
+  if (st != RQ_OK) return st;
+  if (M < 1 || ldx < (dx ? N : K)) return RQ_ERR_BAD_SHAPE;
+  int cus = 0;
+  if (mx4_compute_units(&cus) != RQ_OK) cus = 256;
+  static const int32_t some = 0;  // any non-null plan: sizes alone are asked for
+  const MxCall c = call_of(dtype, M, K, N, E, shared, grouped ? &some : nullptr, act_bits, dx != 0, ldx, aligned16 != 0);
+  out[0] = out[1] = out[2] = 0;
+  if (few(c)) return RQ_OK;
+  c.a4 ? mx4_a4_tiles(c, cus, out) : mx4_gemm_tiles(c, cus, out);
+  return RQ_OK;
+}
+
 extern "C" int rq_mx4_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int64_t shared, const void* plan,
                              int64_t plan_bytes, const uint8_t* codes, const uint8_t* scales, int64_t E, int64_t N,
                              const void* bias, int act_bits, void* y, int64_t ldy, void* scratch, int64_t scratch_bytes,
                              hipStream_t stream) {
   using namespace rq;
-  const int st = check_sizes(dtype, M, K, N, E, shared, plan != nullptr, act_bits);
+  const int st = check_sizes(dtype, M, K, N, E, shared, plan != nullptr, act_bits, false);
   if (st != RQ_OK) return st;
   MxCall c = call_of(dtype, M, K, N, E, shared, plan, act_bits, false, ldx, aligned(x, 16));
   return run(c, x, plan_bytes, codes, scales, bias, y, ldy, scratch, scratch_bytes, stream);
@@ -137,7 +160,7 @@ extern "C" int rq_mx4_linear_dx(const void* dy, int dtype, int64_t M, int64_t N,
                                 int64_t shared, void* dx, int64_t lddx, void* scratch, int64_t scratch_bytes,
                                 hipStream_t stream) {
   using namespace rq;
-  const int st = check_sizes(dtype, M, K, N, E, shared, plan != nullptr, 16);
+  const int st = check_sizes(dtype, M, K, N, E, shared, plan != nullptr, 16, true);
   if (st != RQ_OK) return st;
   MxCall c = call_of(dtype, M, K, N, E, shared, plan, 16, true, lddy, aligned(dy, 16));
   return run(c, dy, plan_bytes, codes, scales, nullptr, dx, lddx, scratch, scratch_bytes, stream);

@@ -103,5 +103,8 @@ int mx4_gemm_run(const MxCall& c, int cus);
 int64_t mx4_gemm_scratch(const MxCall& c, int cus);
 int mx4_a4_run(const MxCall& c, int cus);
 int64_t mx4_a4_scratch(const MxCall& c, int cus);
+// Rows of a tile, splits of the contraction, whether the rows are copied (or quantized) first.
+void mx4_gemm_tiles(const MxCall& c, int cus, int32_t* out);
+void mx4_a4_tiles(const MxCall& c, int cus, int32_t* out);
 
 }  // namespace rq

@@ -128,6 +128,7 @@ SIGNATURES = {
     "rq_mx4_quantize": [_P, _I32, _I64, _I64, _I64, _P, _P, _P],  # x, dtype, rows, cols, ldx, codes, scales, stream
     "rq_mx4_dequantize": [_P, _P, _I64, _I64, _P, _I32, _I64, _P],  # codes, scales, rows, cols, out, dtype, ld, stream
     "rq_mx4_linear_scratch_size": [_I32, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _I64, _I32, _P],
+    "rq_mx4_tile_plan": [_I32, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _I64, _I32, _P],
     "rq_mx4_linear": [_P, _I32, _I64, _I64, _I64, _I64,      # x, dtype, M, K, ldx, shared
                       _P, _I64, _P, _P, _I64, _I64, _P,      # plan, bytes, codes, scales, E, N, bias
                       _I32, _P, _I64, _P, _I64, _P],         # act bits, y, ldy, scratch, bytes, stream
