@@ -27,6 +27,7 @@ constexpr int kFwThreads = 64 * kFwWaves;
 struct FewArgs {
   const void* x;           // rows 16-byte aligned, within 32-bit offsets
   const uint8_t* xscales;  // 4 bits: [rows][wp / 32]
+  uint32_t xsbytes;        // of them all: the last row's last step may be the first of a load of two
   int64_t ldx;             // elements (4 bits: bytes)
   int64_t wp;              // columns of x and of the weight, whole steps
   int xdiv;
@@ -91,7 +92,7 @@ void mx4_few_kernel(FewArgs a) {
   const uint32_t pitch = uint32_t(a.wp / 2), spitch = uint32_t(a.wp / kMxBlock);
   const __amdgpu_buffer_rsrc_t wr = buffer_rsrc(a.codes + (expert * a.N + n0) * pitch, uint32_t(left) * pitch);
   const __amdgpu_buffer_rsrc_t sr = buffer_rsrc(a.scales + (expert * a.N + n0) * spitch, uint32_t(left) * spitch);
-  const __amdgpu_buffer_rsrc_t xr = buffer_rsrc(a.x, kMxFewBytes), xsr = buffer_rsrc(A4 ? a.xscales : a.scales, kMxFewBytes);
+  const __amdgpu_buffer_rsrc_t xr = buffer_rsrc(a.x, kMxFewBytes), xsr = buffer_rsrc(A4 ? a.xscales : a.scales, A4 ? a.xsbytes : 0u);
   // a wave's steps: two adjacent ones of every sixteen
   const int batches = (2 * ((steps + 15) / 16) + D - 1) / D;
   auto step_of = [&](int b, int d) { return 16 * ((b * D + d) / 2) + 2 * wave + ((b * D + d) & 1); };
@@ -382,6 +383,7 @@ int mx4_few_run(const MxCall& c) {
     a.x = xc;
     a.ldx = a.wp / 2;
     a.xscales = xs;
+    a.xsbytes = uint32_t(rows * (a.wp / kMxBlock));
     RQ_DISPATCH_DT(c.dt, XT, return few_launch<XT, true>(a, c.stream));
   }
   if (few_copies(c)) {

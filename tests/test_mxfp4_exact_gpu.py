@@ -1,10 +1,13 @@
 """MXFP4 linears on operands whose products and sums are exact: small whole numbers beside every code at scales of 1/2, 1
 and 2, so that a sum in any order is the same, as long as it stays under 2^22.  Results are equal, whatever the length."""
+import ctypes
+
 import pytest
 import torch
 
 import mxfp4_oracle as oracle
 from rocm_qlora import MXFP4Tensor, dequantize_mxfp4, mxfp4_linear, ops
+from rocm_qlora import _native as nat
 
 pytestmark = pytest.mark.gpu
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -46,3 +49,24 @@ def test_rows_past_4_gib_in_a_copied_tile(dev):
     # the same rows 64 at a time
     for m in range(0, M, 64):
         assert torch.equal(y[m:m + 64], mxfp4_linear(x[m:m + 64], w)), m
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("M,K,N", [(64, 1408, 4096), (64, 128, 100), (64, 1152, 8192), (64, 640, 14336), (32, 1408, 512), (16, 384, 512)])
+def test_scratch_of_its_size_alone(dev, M, K, N, dtype):
+    """4-bit activations, an odd number of 128-value steps: their codes and scales fill the scratch memory to its last
+    byte where M is 64, and nothing behind it is asked for (it holds what would be NaN scales)."""
+    w = exact_weight(N, K, dev, 3)
+    x = whole(M, K, dtype, dev, 4)
+    xq = torch.from_numpy(oracle.quantize(x)[2])[:, :K]
+    want = xq.double() @ oracle.held(w.codes, w.scales, K).t()
+    code = nat.dtype_code(dtype)
+    n = ctypes.c_int64(0)
+    nat.call("rq_mx4_linear_scratch_size", code, M, K, N, 1, 1, 0, 4, 0, K, 1, ctypes.byref(n))
+    area = torch.full((n.value + 512,), 255, dtype=torch.uint8, device=dev)
+    assert area.data_ptr() % 256 == 0
+    y = torch.empty(M, N, dtype=dtype, device=dev)
+    nat.call("rq_mx4_linear", x.data_ptr(), code, M, K, K, 1, None, 0, w.codes.data_ptr(), w.scales.data_ptr(), 1, N, None, 4,
+             y.data_ptr(), N, area.data_ptr(), n.value, nat.stream_handle(dev))
+    assert torch.equal(y.cpu(), want.to(dtype))
+    assert bool((area[n.value:] == 255).all())
