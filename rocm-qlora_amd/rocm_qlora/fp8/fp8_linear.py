@@ -73,6 +73,11 @@ class _FP8LinearFunc(torch.autograd.Function):
         return _stored_dx(grad_output, ctx.qw), None, None, None, None
 
 
+def _refuse_mxfp4(lora: nn.Module, name: str = "") -> None:
+    if isinstance(getattr(lora, "base_layer", None), MXFP4Linear):
+        raise TypeError(f"{name and name + ': '}an MXFP4Linear's weight is not multiplied in FP8: leave its LoRALinear unwrapped")
+
+
 class FP8LinearWrapper(nn.Module):
     """Runs a LoRALinear's base matmul in FP8 (fp8_linear.py:69-118).  Backend
     'native' (this package's FP8 kernels) when FP8 is supported and enabled,
@@ -89,9 +94,7 @@ class FP8LinearWrapper(nn.Module):
         self.fp8_info = detect_fp8_support()
         if self.config.enabled and self.fp8_info["fp8_supported"] and self.fp8_info["fp8_dtypes_available"]:
             self.backend = "native"
-            held = getattr(base_lora_linear, "base_layer", None)
-            if isinstance(held, MXFP4Linear):
-                raise TypeError("an MXFP4Linear's weight is not multiplied in FP8: leave its LoRALinear unwrapped")
+            _refuse_mxfp4(base_lora_linear)
         else:
             self.backend = "bf16"
         self._cache_key = None
@@ -143,13 +146,19 @@ class FP8LinearWrapper(nn.Module):
 def wrap_model_for_fp8(model: nn.Module, config: Optional[FP8Config] = None) -> Tuple[nn.Module, Dict[str, Any]]:
     """Wrap every LoRALinear in an FP8LinearWrapper (fp8_linear.py:120-160).
     Unlike the reference, no environment variables are set: the FP8 kernels
-    need no NCCL stream priority or hardware-queue settings."""
+    need no NCCL stream priority or hardware-queue settings.  A model with a
+    LoRALinear that cannot be wrapped is refused before any layer is changed,
+    and what a native wrapper holds already is not wrapped again."""
     config = config if config is not None else FP8Config()
     info = detect_fp8_support()
     status = {"enabled": False, "backend": "bf16", "layers_wrapped": 0, "reason": info["reason"]}
     if not info["fp8_supported"] and config.enabled:
         return model, status
-    targets = [(n, m) for n, m in model.named_modules() if isinstance(m, LoRALinear)]
+    held = {m.base for m in model.modules() if isinstance(m, FP8LinearWrapper) and m.backend == "native"}
+    targets = [(n, m) for n, m in model.named_modules() if isinstance(m, LoRALinear) and m not in held]
+    if config.enabled and info["fp8_dtypes_available"]:
+        for name, module in targets:
+            _refuse_mxfp4(module, name)
     for name, module in targets:
         parent_name, _, child = name.rpartition(".")
         parent = model.get_submodule(parent_name) if parent_name else model
