@@ -70,8 +70,20 @@ class LoRALinear(nn.Module):
             base_out = base(x.to(base.weight.dtype))
         else:
             base_out = base(x)
-        lora_out = self.lora_dropout(x) @ self.lora_A.to(x.dtype).T @ self.lora_B.to(x.dtype).T * self.scaling
+        if self.activation_bits == 8 and torch.is_grad_enabled():
+            lora_out = self._term_saved_in_8_bits(x)
+        else:
+            lora_out = self._term(x)
         return base_out + lora_out.to(base_out.dtype)
+
+    def _term(self, x: torch.Tensor) -> torch.Tensor:
+        return self.lora_dropout(x) @ self.lora_A.to(x.dtype).T @ self.lora_B.to(x.dtype).T * self.scaling
+
+    @eager_only
+    def _term_saved_in_8_bits(self, x: torch.Tensor) -> torch.Tensor:
+        # (the base layer's own saved tensors, its weight among them, stay as they are)
+        with inputs_saved_in_8_bits(x, self.lora_A, self.lora_B):
+            return self._term(x)
 
     @eager_only
     def _forward_saved_in_8_bits(self, x: torch.Tensor, p: float) -> torch.Tensor:
