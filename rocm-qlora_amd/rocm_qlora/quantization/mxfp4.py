@@ -98,12 +98,20 @@ class ExpertRows:
         self.plan = ops.adapter_rows(ids.reshape(-1), self.n)
 
 
+def _versions(codes: torch.Tensor, scales: torch.Tensor):
+    """How often each has been written to in place (inference tensors do not count that)."""
+    return tuple(None if t.is_inference() else t._version for t in (codes, scales))
+
+
 class _MXFP4Linear(torch.autograd.Function):
-    """y by the linears' kernels, dX in the backward pass.  w: a weight's (codes, scales, K), frozen."""
+    """y by the linears' kernels, dX in the backward pass.  w: a weight's (codes, scales, K), frozen: kept as
+    it is, not among autograd's saved tensors, whose hooks (8-bit checkpoints, offloading) are for activations.  As
+    for those, a write to it in between is refused."""
 
     @staticmethod
     def forward(ctx, x, w, bias, bits, rows):
         codes, scales, K = w
+        ctx.versions = _versions(codes, scales)
         if rows is None:
             ctx.args = (codes, scales, K, 1, codes.shape[0], None, 1)
             return ops._mx4_linear(x, codes, scales, K, bias, bits, None, None)
@@ -114,6 +122,9 @@ class _MXFP4Linear(torch.autograd.Function):
     @staticmethod
     @first_order
     def backward(ctx, dy):
+        if _versions(*ctx.args[:2]) != ctx.versions:
+            raise RuntimeError("the MXFP4 weight needed for gradient computation has been modified by an inplace operation "
+                               "since the forward pass")
         return ops._mx4_dx(dy, *ctx.args), None, None, None, None
 
 
