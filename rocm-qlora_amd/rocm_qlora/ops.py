@@ -733,7 +733,8 @@ MAX_ADAPTERS = 1024  # kMaxAdapters in csrc/rq_rows.h
 def adapter_rows(ids: torch.Tensor, n: int) -> torch.Tensor:
     """The rows of a batch grouped by adapter: ids [M] int32 or int64 on the GPU, 0 ..
     n - 1 or, for a row without an adapter, anything else.  The result is what
-    multi_lora and, for experts, mx4_linear take as `plan`."""
+    multi_lora and, for experts, mx4_linear take as `plan`, for M rows and n adapters alone: it
+    carries both numbers, which a copy of its bytes (clone, to) does not."""
     dev = nat.require_gpu(ids)
     if ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"adapter ids must be int32 or int64, got {ids.dtype}")
@@ -778,12 +779,13 @@ def _check_rows(t: torch.Tensor, M: int, cols: int, dtype: torch.dtype, name: st
                        f"of strides {t.stride()}")
 
 
-def _check_plan(plan: Optional[torch.Tensor], dev, M: int, n: int) -> None:
+def _check_plan(plan: Optional[torch.Tensor], M: int, n: int) -> None:
+    """Refuses a plan of other rows, whose entries would lie outside the operands (its size can be the same)."""
     if plan is None:
         if n != 1:
             raise RuntimeError(f"{n} adapters without the batch's rows by adapter")
-    elif plan.numel() != _bytes("rq_adapter_rows_size", dev.index, M, n):
-        raise RuntimeError(f"the rows by adapter are not those of {M} rows and {n} adapters")
+    elif getattr(plan, "grouped", None) != (M, n):
+        raise RuntimeError(f"the rows by adapter are not those of {M} rows and {n} adapters, as adapter_rows returned them")
 
 
 def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: torch.Tensor,
@@ -808,7 +810,7 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
         else:
             base, ld_base = _rows(base, N)
     with on(dev):
-        _check_plan(plan, dev, M, n)
+        _check_plan(plan, M, n)
         grouped = 0 if plan is None else 1
         if out is None:
             out = x.new_empty((M, N))
@@ -854,7 +856,7 @@ def multi_lora_grads(x, dy: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Te
     if dx is not None:
         _check_rows(dx, M, K, dy.dtype, "dx")
     with on(dev):
-        _check_plan(plan, dev, M, n)
+        _check_plan(plan, M, n)
         if need_b and (u is None or u.dtype != torch.uint8 or not u.is_contiguous() or
                        u.numel() != _bytes("rq_multi_lora_u_size", dev.index, M, n, rank, 0 if plan is None else 1)):
             raise RuntimeError("u is not multi_lora's of these rows and factors")
