@@ -17,6 +17,7 @@ import torch
 import torch.nn as nn
 
 from rocm_qlora.lora.lora_layer import LoRALinear
+from rocm_qlora.quantization.mxfp4 import MXFP4Experts, MXFP4Linear
 
 
 def _export_dequant_layer(lora_linear: nn.Module) -> torch.Tensor:
@@ -32,7 +33,10 @@ def _export_dequant_layer(lora_linear: nn.Module) -> torch.Tensor:
 def _build_export_state_dict(model: nn.Module) -> Dict[str, torch.Tensor]:
     """fp16 state dict with merged LoRA weights under the layers' own keys
     ('<layer>.weight', '<layer>.bias') and no adapter keys
-    (gguf_export.py:82-125)."""
+    (gguf_export.py:82-125).  An MXFP4 layer's weight is no parameter, and would be missing: refused."""
+    for name, module in model.named_modules():
+        if isinstance(module, (MXFP4Linear, MXFP4Experts)):
+            raise TypeError(f"{name or 'the model'}: the weight of an {type(module).__name__} is not exported")
     state_dict: Dict[str, torch.Tensor] = {}
     for name, param in model.named_parameters():
         if "lora_A" not in name and "lora_B" not in name:
