@@ -1133,6 +1133,8 @@ def _mx4_linear(x, codes, scales, K, bias, activation_bits, plan, M):
     grouped = plan_bytes = 0
     shared = 1
     if plan is None:
+        if M is not None and M != R:
+            raise RuntimeError(f"{M} rows of one weight's, got {R}: without a plan no rows are shared")
         M = R
     else:
         M = R if M is None else M
