@@ -3,9 +3,11 @@
 // counts its own stretch of the rows, the counts are summed over waves and
 // adapters, and each wave then places its stretch 64 rows at a time, rows of the
 // same adapter found by a ballot for each bit of its number.  Bound by latency, the chain of
-// loads, counts and sums: 3.6 us for 8 rows, 4.9 for 256 rows of 64 adapters, 7.4 for 4096 of
-// 4, 35 for 4096 of 1024 (one of two tables after the other, sums by lane shuffles, padding a
-// tile a thread: 6.6, 7.5, 10 and 63; a graph's replays).
+// loads, counts and sums: 3.2 us for 8 rows of one adapter, 4.8 for 256 rows of 64, 7.3 for 4096
+// of 4, 35 for 4096 of 1024 (one of two tables after the other, sums by lane shuffles, padding a
+// tile a thread: 6.6, 7.5, 10 and 63; a graph's replays).  The tables of larger tiles, which experts' products
+// read and adapters' do not, are 0.1 to 0.3 us of it (half in their sums, half in their stores; a shift for the sums'
+// division gained nothing).
 // It runs once for a batch, for all the projections of all its layers.
 #include "rq_launch.h"
 #include "rq_rows.h"

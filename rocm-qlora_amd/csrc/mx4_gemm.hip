@@ -7,8 +7,7 @@
 // tile issues 8 of them (dX: 16 and 16 byte permutes) beside 8 v_mfma_f32_32x32x16 of 32
 // cycles each, and a second wave of the SIMD multiplies meanwhile: a loop of 8 products
 // and 16 conversions takes the time of the products, with 16 permutes more 13 % longer.
-// So nothing is gained by decoding the weight once into memory, and 4-bit tiles take a
-// quarter of the LDS, of its reads and of the traffic to it.
+// 4-bit tiles take a quarter of the LDS, of its reads and of the traffic to it.
 //
 // Tile BM x BN, 64 k a step, eight waves, two a SIMD; the weight is the products' A operand,
 // so that a lane's results lie along an output row.  Rows come by direct-to-LDS loads into
@@ -16,9 +15,11 @@
 // of a step are issued two to three steps before its products, one barrier a step, and the operands of
 // the next quarter step are read from LDS while this one's are multiplied.
 //
-// Bound by the matrix units and the power they take: 4096 x 4096 x 14336 in bf16 forward 415 us (1.16 PFLOP/s), dX
-// 453 (1.06), a library's product of decoded weights 401 without the decoding.  Experts: 2048 tokens' two of 8 of 4096 -> 14336
-// 500 us (0.96 PFLOP/s of live rows: tiles' ends).
+// 4096 x 4096 x 14336 in bf16, replayed for seconds: forward 392 us (1.23 PFLOP/s), dX 411 (1.17); a library's products of the
+// decoded weight 313 and 325, decoding it 23 more.  Bound by the loop's waits and by the clock: the matrix units are busy in 59 %
+// of the cycles (dX 52, experts 54), LDS in 18 (20), the L2 gives 11.4 of the 33 TB/s that reads alone reach, and waves wait for
+// 45 % of theirs (34); power takes the clock from 2.4 to 1.9 GHz (the same instructions on zeros: 312 us).  Experts: 2048 tokens'
+// two of 8 of 4096 -> 14336 486 us (0.99 PFLOP/s of live rows: tiles' ends).
 //
 // Forward: lane (i, q) (i = l % 32, q = l / 32) of a 32-column block holds a whole block
 // of 32 k of its weight row: one 16-byte LDS read and one scale a step; its quarter s

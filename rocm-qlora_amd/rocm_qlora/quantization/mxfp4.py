@@ -100,7 +100,7 @@ class ExpertRows:
 
 def _versions(codes: torch.Tensor, scales: torch.Tensor):
     """How often each has been written to in place (inference tensors do not count that)."""
-    return tuple(None if t.is_inference() else t._version for t in (codes, scales))
+    return -1 if codes.is_inference() else codes._version, -1 if scales.is_inference() else scales._version
 
 
 class _MXFP4Linear(torch.autograd.Function):
