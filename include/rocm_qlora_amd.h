@@ -610,8 +610,8 @@ int rq_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows,
  *   [M, N] of `dtype`; bias [E, N] of it, or NULL.  The values of W are exact beside bf16 and fp32 rows and
  *   rounded to fp16 beside fp16 rows; sums are fp32, the result is rounded once.
  *   act_bits: 16, or 4: x's rows quantized as above first (one weight).
- *   Sizes: K at most 2^24, K rounded up to 128 times N / 64 at most 2^29; dx: rows of dy past 2^25 values where there
- *   are 64 of them or more (fewer rows: 2^31 values in all) are refused as unsupported.
+ *   Sizes: K at most 2^24, K rounded up to 128 times N / 64 at most 2^29; dx: 63 rows of dy, or all
+ *   but one, of N rounded up to 64 take less than 4 GiB in 16 bits (N to 34087040 from 64 rows on).  Else unsupported.
  * rq_mx4_linear_dx: dx[t] = sum over r = t shared .. of dy[r] W[e].  scratch: 256-byte aligned, contents ignored; its
  * size is for rows of x (dx: of dy) of stride ldx whose first element is 16-byte aligned (aligned16) or not. */
 int rq_mx4_linear_scratch_size(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, int grouped,

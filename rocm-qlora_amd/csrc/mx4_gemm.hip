@@ -630,8 +630,8 @@ MgPlan mg_plan(const MxCall& c, int cus) {
   p.np = ceil_div(c.N, kMgStep) * kMgStep;
   p.s_bytes = c.dx ? up256(c.E * (wp / kMxBlock) * p.np * 2) : 0;
   // A copy that is read by slot is as long as its rows: the tile's rows are those that 32-bit offsets reach
-  // (64 always are, mx4_row_tiles_fit).
-  auto reached = [&](int bm) { return !p.copy || !p.by_slot || (c.M < bm ? c.M : bm) * p.xpitch * 2 <= far; };
+  // (64 always are, check_sizes).
+  auto reached = [&](int bm) { return !p.copy || !p.by_slot || mx_rows_reached(c.M < bm ? c.M : bm, p.xpitch); };
   // Rows of a tile, and splits of the contraction where the tiles leave compute units idle: the least of an
   // estimate from measured times (us, each within 15 %): a launch, a step, a step's lengthening when all units
   // work; a split's partial sums written and read at 4 TB/s by one more launch.  Forward 128 x 4096 -> 4096: 34,

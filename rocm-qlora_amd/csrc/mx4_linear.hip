@@ -19,12 +19,6 @@ bool few(const MxCall& c) {
   return c.a4 ? c.M <= kTileRows : c.M <= (c.dt == RQ_DTYPE_F32 ? 16 : 32) && c.M * mx_pad(c.wk) <= 24 * 8192;
 }
 
-// Whether a tile of 64 rows of dY, or of all there are, lies within 32-bit offsets of its first (rows of x always do: K
-// is at most 2^24).
-bool mx4_row_tiles_fit(int64_t M, int64_t N) {
-  return (M < kTileRows ? M : kTileRows) * ceil_div(N, 64) * 64 <= int64_t(1) << 31;
-}
-
 // Sizes, whatever the pointers.  shared: rows of the product that one row of the narrower side stands for.
 int check_sizes(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t shared, bool grouped, int act_bits, bool dx) {
   if (!valid_float_dtype(dtype)) return RQ_ERR_BAD_DTYPE;
@@ -32,9 +26,10 @@ int check_sizes(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t s
   if (act_bits != 16 && act_bits != 4) return RQ_ERR_UNSUPPORTED;
   if (!grouped && (E != 1 || shared != 1)) return RQ_ERR_BAD_SHAPE;
   if (grouped && act_bits == 4) return RQ_ERR_UNSUPPORTED;
-  // 32-bit offsets within 64 rows of a tile (mg_plan: taller tiles) and a weight's scales
+  // 32-bit offsets within 64 rows of a tile (mg_plan: taller tiles; rows of x, of at most 2^24, need no check) and a
+  // weight's scales
   if (E > kMaxAdapters || M > (int64_t(1) << 30) || K > (int64_t(1) << 24) || N > (int64_t(1) << 30) ||
-      mx_pad(K) * ceil_div(N, 64) > (int64_t(1) << 29) || (dx && !mx4_row_tiles_fit(M, N)))
+      mx_pad(K) * ceil_div(N, 64) > (int64_t(1) << 29) || (dx && !mx_rows_reached(M < kTileRows ? M : kTileRows, ceil_div(N, 64) * 64)))
     return RQ_ERR_UNSUPPORTED;
   return RQ_OK;
 }

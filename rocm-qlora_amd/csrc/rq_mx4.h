@@ -23,6 +23,11 @@ constexpr int kMxWhole = 128;
 
 __host__ __device__ constexpr int64_t mx_pad(int64_t K) { return (K + kMxWhole - 1) / kMxWhole * kMxWhole; }
 
+// Whether all of `rows` rows of `pitch` 16-bit values lie within 32-bit offsets of the first, read 128 bytes a step.
+__host__ __device__ constexpr bool mx_rows_reached(int64_t rows, int64_t pitch) {
+  return (rows - 1) * pitch * 2 + 128 <= int64_t(1) << 32;
+}
+
 // Scale byte of a block whose largest |x| has the fp32 bits `absmax` (an exponent field
 // of 0 is a zero or below 2^-126: the least scale).
 __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t absmax) {

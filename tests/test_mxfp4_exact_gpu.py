@@ -32,9 +32,9 @@ def whole(M, K, dtype, dev, seed=1, most=2):
 
 
 def test_rows_past_4_gib_in_a_copied_tile(dev):
-    """512 rows of 16 MiB: the rows are copied, and the copy's tiles hold no more of them than 32-bit offsets reach."""
-    M, K, N = 512, (1 << 23) + 128, 2048
-    print("rows of 16 MiB", M, K, N, flush=True)
+    """512 rows of 18 MB: the rows are copied, and the copy's tiles hold no more of them than 32-bit offsets reach."""
+    M, K, N = 512, 9_000_064, 2048
+    print("rows of 18 MB", M, K, N, flush=True)
     w = exact_weight(N, K, dev, 1, (127, 128))
     x = whole(M, K, BF16, dev, 2, 1)
     y = mxfp4_linear(x, w)
