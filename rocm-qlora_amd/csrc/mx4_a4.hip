@@ -237,9 +237,9 @@ void mx4_a4_kernel(A4Args args) {
 //
 // No unit is near its limit: 4096 x 8192 x 8192 at 3.7 PFLOP/s reads 1.7 GB from the L2 in 138 us (12.4 of the 33 TB/s that reads
 // alone reach), the matrix units busy 49 to 55 % (4096 x 4096 x 14336: 15.5 TB/s and 41 %, LDS 25 %); waves wait for 39 % of
-// their cycles (there are eight barriers a step; which of the waits it is was not resolved).  Power takes the clock from 2.4 to 1.9 GHz (8192 x 8192 x 8192 291 us, on
-// zeros 230).  Four waves of 128 x 128 outputs, which read two thirds as much from LDS, took the same time to 3 %, and bringing
-// lines to the L2 four steps ahead took 6 % more.
+// their cycles (there are eight barriers a step; which of the waits it is was not resolved).  Power takes the clock from 2.4 to
+// 1.9 GHz (8192 x 8192 x 8192 291 us, on zeros 230).  Four waves of 128 x 128 outputs, which read two thirds as much from LDS,
+// took the same time to 3 %, and bringing lines to the L2 four steps ahead took 6 % more.
 // ---------------------------------------------------------------------------
 constexpr int kBgHalf = 128 * 128;                    // bytes of a half tile
 constexpr int kBgStep = 4 * kBgHalf;                  // X0 X1 W0 W1

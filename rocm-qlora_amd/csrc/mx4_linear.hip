@@ -29,7 +29,8 @@ int check_sizes(int dtype, int64_t M, int64_t K, int64_t N, int64_t E, int64_t s
   // 32-bit offsets within 64 rows of a tile (mg_plan: taller tiles; rows of x, of at most 2^24, need no check) and a
   // weight's scales
   if (E > kMaxAdapters || M > (int64_t(1) << 30) || K > (int64_t(1) << 24) || N > (int64_t(1) << 30) ||
-      mx_pad(K) * ceil_div(N, 64) > (int64_t(1) << 29) || (dx && !mx_rows_reached(M < kTileRows ? M : kTileRows, ceil_div(N, 64) * 64)))
+      mx_pad(K) * ceil_div(N, 64) > (int64_t(1) << 29) ||
+      (dx && !mx_rows_reached(M < kTileRows ? M : kTileRows, ceil_div(N, 64) * 64)))
     return RQ_ERR_UNSUPPORTED;
   return RQ_OK;
 }
